@@ -11,7 +11,9 @@ only re-exports, so the two import names always run the same code.
     >>> C = bsk._C.sparse_mm_bsr(rp, ci, vals, brp, bci, bvals, M, N, K, 256, 128, 32)
 """
 from periodicdent42_b200 import __version__
-from periodicdent42_b200.ops import attention_forward, gemm, gemm_fp8, quantize_e4m3, sparse_mm, sparse_mm_benchmark
+from periodicdent42_b200.ops import (attention_forward, attention_paged, attention_varlen, gemm, gemm_fp8,
+                                     kv_cache_append, kv_cache_gather, quantize_e4m3, rotary_embedding,
+                                     rotary_frequencies, sparse_mm, sparse_mm_benchmark)
 from periodicdent42_b200.utils import convert_to_bsr, estimate_speedup, get_optimal_block_size, validate_sparse_matrix
 
 from . import ops, utils  # noqa: E402  (the reference's submodules: bsk.ops, bsk.utils)

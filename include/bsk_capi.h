@@ -349,6 +349,84 @@ void launch_attention_backward(const void* grad_out, const void* Q, const void* 
                                bool causal, void* stream);
 
 /*
+ * Rotary positions of Q [tokens, heads, dim] and K [tokens, kv_heads, dim] in one launch (dtype 0 = bf16, 1 = f16,
+ * 2 = f32). With t = position * inv_freq[i], pair i of a head -- elements (2i, 2i+1) when `interleaved`, else
+ * (i, i + rotary_dim/2) -- becomes  scale * (a cos t - b sin t, a sin t + b cos t);  elements from rotary_dim on are
+ * copied. `backward` turns by -t (the gradient with respect to the input, given the output's).
+ *   Q, K      : rows of dim elements at token and head strides given in elements (either may have 0 heads);
+ *               Q_out, K_out contiguous, not overlapping the inputs
+ *   positions : int32 or int64 [tokens] (position_bytes 4 or 8); angles are reduced in 64 bits
+ *   dim       : even, at most 512; rotary_dim even, 2..dim; inv_freq fp32 [rotary_dim/2], device memory
+ * No reference counterpart.
+ */
+int bsk_rotary(int dtype, const void* Q, int64_t q_token_stride, int64_t q_head_stride, void* Q_out, int heads,
+               const void* K, int64_t k_token_stride, int64_t k_head_stride, void* K_out, int kv_heads,
+               const void* positions, int position_bytes, const float* inv_freq, int tokens, int dim, int rotary_dim,
+               int interleaved, float scale, int backward, void* stream);
+
+/*
+ * Paged key/value cache: caches [pages, page size, kv_heads, dim] (dim 64 or 128) of the rows' type (dtype 0 = bf16,
+ * 1 = f16) or, with cache_e4m3, of e4m3 codes with fp32 scales [pages, page size, kv_heads].
+ * append writes row t of K and V [tokens, kv_heads, dim] (16-byte aligned rows, strides in elements) to flat slot
+ * slots[t] = page * page size + offset: copied, or quantised with scale = max|x| / 448 and code = e4m3(x / scale) per
+ * row (a row of zeros: scale 0). Non-negative slots of one call must differ. gather reads rows back into contiguous
+ * K and V (codes times scale, rounded once). slots: int32 or int64 (slot_bytes 4 or 8); a negative slot is padding
+ * (nothing written; zeros read), a slot >= num_slots (= pages * page size) is treated as padding and sets the device
+ * error word. No reference counterpart.
+ */
+int bsk_kv_cache_append(int dtype, const void* K, int64_t k_token_stride, int64_t k_head_stride, const void* V,
+                        int64_t v_token_stride, int64_t v_head_stride, void* k_cache, void* v_cache, int cache_e4m3,
+                        float* k_scale, float* v_scale, const void* slots, int slot_bytes, int tokens, int kv_heads,
+                        int dim, int64_t num_slots, void* stream);
+int bsk_kv_cache_gather(int dtype, const void* k_cache, const void* v_cache, int cache_e4m3, const float* k_scale,
+                        const float* v_scale, const void* slots, int slot_bytes, void* K, void* V, int tokens, int kv_heads,
+                        int dim, int64_t num_slots, void* stream);
+
+/*
+ * Attention of new tokens over a paged cache, causal, heads grouped over kv heads (dtype 0 = bf16, 1 = f16; dim 64 or
+ * 128; at most 128 heads per kv head). Sequence i has the n_i = cu_seqlens[i+1] - cu_seqlens[i] new tokens (n_i >= 0)
+ * in rows cu_seqlens[i].. of Q [tokens, heads, dim] (16-byte aligned rows, strides in elements), and its first
+ * kv_lens[i] cached tokens are its keys, the new tokens' own keys the last n_i of them (append before attending). New
+ * token t sees the keys at positions <= kv_lens[i] - n_i + t. The key at position p is in page
+ * block_table[i * table_stride + p / page_size] at offset p % page_size; the rest of the last page is never used.
+ * O [tokens, heads, dim] is contiguous; a row that sees no key, and rows behind the last sequence, are zero.
+ *   caches as in bsk_kv_cache_append; page_size a power of two, 8..1024; pages x page_size below 2^31
+ *   cu_seqlens int32 [batch + 1], cu_seqlens[0] = 0, non-decreasing, at most `tokens`; kv_lens int32 [batch],
+ *   at most table_width * page_size; entries outside their range are clamped, a page outside [0, num_pages) reads as
+ *   zeros, and either sets the device error word.
+ * No reference counterpart.
+ */
+int bsk_attention_paged(int dtype, const void* Q, int64_t q_token_stride, int64_t q_head_stride, const void* k_cache,
+                        const void* v_cache, int cache_e4m3, const float* k_scale, const float* v_scale,
+                        const int32_t* block_table, int64_t table_stride, int table_width, const int32_t* kv_lens,
+                        const int32_t* cu_seqlens, void* O, int tokens, int batch, int heads, int kv_heads, int dim,
+                        int num_pages, int page_size, float scale, void* stream);
+
+/*
+ * Attention over packed sequences of different lengths, heads grouped over kv heads (types, dims and cu_seqlens as in
+ * bsk_attention_paged): Q [tokens, heads, dim], K and V [tokens, kv_heads, dim] with 16-byte aligned rows (strides in
+ * elements); each sequence attends to itself, causally when `causal`. O [tokens, heads, dim] contiguous; lse
+ * [tokens, heads] (optional): natural-log log-sum-exp of the row's scaled scores. The backward takes the forward's O and
+ * lse and writes contiguous dQ, dK, dV:
+ *   dV = P^T dO,  dS = P * (dO V^T - rowsum(dO * O)),  dQ = scale * dS K,  dK = scale * dS^T Q
+ * with dK, dV summed over the heads of a group, in a fixed order (no atomics). Rows behind the last sequence are zero.
+ * workspace: device memory of bsk_attention_varlen_workspace_bytes(...) bytes, 16-byte aligned, not shared by calls
+ * that may run at the same time. No reference counterpart.
+ */
+int64_t bsk_attention_varlen_workspace_bytes(int tokens, int batch, int heads, int kv_heads, int dim, int backward);
+int bsk_attention_varlen_fwd(int dtype, const void* Q, int64_t q_token_stride, int64_t q_head_stride, const void* K,
+                             int64_t k_token_stride, int64_t k_head_stride, const void* V, int64_t v_token_stride,
+                             int64_t v_head_stride, const int32_t* cu_seqlens, void* O, float* lse, int tokens, int batch,
+                             int heads, int kv_heads, int dim, float scale, int causal, void* workspace,
+                             int64_t workspace_bytes, void* stream);
+int bsk_attention_varlen_bwd(int dtype, const void* dO, int64_t do_token_stride, int64_t do_head_stride, const void* Q,
+                             int64_t q_token_stride, int64_t q_head_stride, const void* K, int64_t k_token_stride,
+                             int64_t k_head_stride, const void* V, int64_t v_token_stride, int64_t v_head_stride,
+                             const void* O, const float* lse, const int32_t* cu_seqlens, void* dQ, void* dK, void* dV,
+                             int tokens, int batch, int heads, int kv_heads, int dim, float scale, int causal,
+                             void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
  * Drop-in for the reference's launcher signature (BlackwellSparseK/src/kernel_launch.cu:33-61).
  * A is BSR with blocks of (M/A_M_blocks) x (K/A_K_blocks). A B with every block present is read as the dense
  * row-major [K, N] matrix the reference Python layer passes (BlackwellSparseK/python/ops.py:104-107); a B with

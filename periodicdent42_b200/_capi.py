@@ -78,6 +78,19 @@ SIGNATURES = {
     "bsk_bsattn_mask_transpose": (_i32, [_vp, _vp, _i32, _i32, _vp, _vp, _vp, _i64, _vp]),
     "bsk_bsattn_bwd": (_i32, [_i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32,
                               _i32, _i32, _f32, _i32, _vp, _vp]),
+    "bsk_rotary": (_i32, [_i32, _vp, _i64, _i64, _vp, _i32, _vp, _i64, _i64, _vp, _i32, _vp, _i32, _vp, _i32, _i32,
+                          _i32, _i32, _f32, _i32, _vp]),
+    "bsk_kv_cache_append": (_i32, [_i32, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i32, _vp, _vp, _vp, _i32, _i32,
+                                   _i32, _i32, _i64, _vp]),
+    "bsk_kv_cache_gather": (_i32, [_i32, _vp, _vp, _i32, _vp, _vp, _vp, _i32, _vp, _vp, _i32, _i32, _i32, _i64, _vp]),
+    "bsk_attention_paged": (_i32, [_i32, _vp, _i64, _i64, _vp, _vp, _i32, _vp, _vp, _vp, _i64, _i32, _vp, _vp, _vp, _i32,
+                                   _i32, _i32, _i32, _i32, _i32, _i32, _f32, _vp]),
+    "bsk_attention_varlen_workspace_bytes": (_i64, [_i32, _i32, _i32, _i32, _i32, _i32]),
+    "bsk_attention_varlen_fwd": (_i32, [_i32, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _i32, _i32,
+                                        _i32, _i32, _i32, _f32, _i32, _vp, _i64, _vp]),
+    "bsk_attention_varlen_bwd": (_i32, [_i32, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp,
+                                        _vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _f32, _i32, _vp, _i64,
+                                        _vp]),
     "launch_attention_forward": (None, [_vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _f32, ctypes.c_bool, _vp]),
     "launch_attention_backward": (None, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _f32,
                                          ctypes.c_bool, _vp]),

@@ -162,6 +162,283 @@ torch::Tensor bsattn_fwd(torch::Tensor Q, torch::Tensor K, torch::Tensor V, torc
   return O;
 }
 
+// ------------------------------------------------------------------ rotary, paged cache, packed and paged attention
+// Argument errors of these operators are ValueErrors (TORCH_CHECK_VALUE), as in the Python layer.
+using OptTensor = std::optional<torch::Tensor>;
+
+void check_cuda(const torch::Tensor& t, const torch::Tensor& like, const char* op, const char* name) {
+  TORCH_CHECK_VALUE(t.is_cuda(), op, ": CUDA tensors required (CPU not supported), ", name, " is not one");
+  TORCH_CHECK_VALUE(t.device() == like.device(), op, ": ", name, " is on another device");
+}
+
+int dtype_code(const torch::Tensor& t, const char* op, bool f32_ok = false) {
+  const auto dt = t.scalar_type();
+  if (dt == torch::kBFloat16) return 0;
+  if (dt == torch::kFloat16) return 1;
+  TORCH_CHECK_VALUE(f32_ok && dt == torch::kFloat32, op, ": tensors must be float16 or bfloat16", f32_ok ? " or float32" : "");
+  return 2;
+}
+
+// [tokens, heads, D] rows that the kernels can read in 16-byte pieces at a token and a head stride; a tensor with
+// another inner stride, other alignment or broadcast (stride 0) rows is copied once.
+struct Rows {
+  torch::Tensor t;
+  int64_t ts, hs;
+  const void* p() const { return t.data_ptr(); }
+};
+
+Rows as_rows(const torch::Tensor& x, bool any_alignment = false) {
+  const int64_t T = x.size(0), H = x.size(1), D = x.size(2), e = x.element_size();
+  const auto fits = [&](const torch::Tensor& t) {
+    if (D > 1 && t.stride(2) != 1) return false;
+    const int64_t ts = T > 1 ? t.stride(0) : H * D, hs = H > 1 ? t.stride(1) : D;
+    if (any_alignment) return true;
+    return ts > 0 && hs > 0 && ts * e % 16 == 0 && hs * e % 16 == 0 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+  };
+  torch::Tensor t = fits(x) ? x : x.clone(at::MemoryFormat::Contiguous);
+  return {t, T > 1 ? t.stride(0) : H * D, H > 1 ? t.stride(1) : D};
+}
+
+// 1-D (or 2-D) int32 index tensor on `like`'s device; int64 is narrowed.
+torch::Tensor as_index(const torch::Tensor& t, const torch::Tensor& like, const char* op, const char* name, int64_t dim) {
+  check_cuda(t, like, op, name);
+  TORCH_CHECK_VALUE(t.dim() == dim, op, ": ", name, " must have ", dim, " dimension(s)");
+  TORCH_CHECK_VALUE(t.scalar_type() == torch::kInt32 || t.scalar_type() == torch::kInt64, op, ": ", name, " must be int32 or int64");
+  return t.to(torch::kInt32).contiguous();
+}
+
+int narrow(int64_t v, const char* op, const char* name) {
+  TORCH_CHECK_VALUE(v >= 0 && v < (int64_t{1} << 31), op, ": ", name, " (", v, ") out of range");
+  return static_cast<int>(v);
+}
+
+std::tuple<torch::Tensor, OptTensor> rotary(torch::Tensor Q, OptTensor K, torch::Tensor positions, torch::Tensor inv_freq,
+                                            bool interleaved, double scale, bool backward) {
+  const char* op = "rotary_embedding";
+  check_cuda(Q, Q, op, "Q");
+  TORCH_CHECK_VALUE(Q.dim() == 3, op, ": Q must be [tokens, heads, dim]");
+  const int code = dtype_code(Q, op, true);
+  const int64_t T = Q.size(0), D = Q.size(2);
+  if (K) {
+    check_cuda(*K, Q, op, "K");
+    TORCH_CHECK_VALUE(K->dim() == 3 && K->size(0) == T && K->size(2) == D, op, ": K must be [tokens, kv_heads, dim] like Q");
+    TORCH_CHECK_VALUE(K->scalar_type() == Q.scalar_type(), op, ": K and Q must have one dtype");
+  }
+  check_cuda(positions, Q, op, "positions");
+  TORCH_CHECK_VALUE(positions.dim() == 1 && positions.size(0) == T, op, ": positions must be [tokens]");
+  TORCH_CHECK_VALUE(positions.scalar_type() == torch::kInt32 || positions.scalar_type() == torch::kInt64, op,
+                    ": positions must be int32 or int64");
+  check_cuda(inv_freq, Q, op, "inv_freq");
+  TORCH_CHECK_VALUE(inv_freq.dim() == 1 && inv_freq.scalar_type() == torch::kFloat32, op, ": inv_freq must be 1-D float32");
+  TORCH_CHECK_VALUE(inv_freq.size(0) >= 1 && 2 * inv_freq.size(0) <= D, op, ": inv_freq must hold 1 to dim / 2 frequencies");
+  TORCH_CHECK_VALUE(D % 2 == 0 && D <= 512, op, ": the head dimension must be even and at most 512, got ", D);
+  const at::cuda::CUDAGuard guard(Q.device());
+  const auto pos = positions.contiguous(), freq = inv_freq.contiguous();
+  const Rows q = as_rows(Q, true);
+  auto qo = torch::empty({T, Q.size(1), D}, Q.options());
+  Rows k{};
+  OptTensor ko;
+  if (K) {
+    k = as_rows(*K, true);
+    ko = torch::empty({T, K->size(1), D}, K->options());
+  }
+  check_rc(bsk_rotary(code, q.p(), q.ts, q.hs, qo.data_ptr(), narrow(Q.size(1), op, "heads"), K ? k.p() : nullptr, k.ts,
+                      k.hs, K ? ko->data_ptr() : nullptr, K ? narrow(K->size(1), op, "kv_heads") : 0, pos.data_ptr(),
+                      static_cast<int>(pos.element_size()), freq.data_ptr<float>(), narrow(T, op, "tokens"),
+                      static_cast<int>(D), static_cast<int>(2 * freq.size(0)), interleaved, static_cast<float>(scale),
+                      backward, stream_of(Q)),
+           "bsk_rotary");
+  return {qo, ko};
+}
+
+// The caches' checks shared by append, gather and attention: returns whether they hold e4m3 codes.
+bool check_caches(const char* op, const torch::Tensor& like, const torch::Tensor& kc, const torch::Tensor& vc,
+                  const OptTensor& ks, const OptTensor& vs, at::ScalarType dtype) {
+  check_cuda(kc, like, op, "k_cache");
+  check_cuda(vc, like, op, "v_cache");
+  TORCH_CHECK_VALUE(kc.dim() == 4 && vc.sizes() == kc.sizes(), op, ": caches must be [pages, page size, kv_heads, dim] of one shape");
+  TORCH_CHECK_VALUE(kc.is_contiguous() && vc.is_contiguous(), op, ": caches must be contiguous");
+  TORCH_CHECK_VALUE(kc.scalar_type() == vc.scalar_type(), op, ": caches must have one dtype");
+  TORCH_CHECK_VALUE(kc.size(3) == 64 || kc.size(3) == 128, op, ": head dimension must be 64 or 128, got ", kc.size(3));
+  if (kc.scalar_type() != at::kFloat8_e4m3fn) {
+    TORCH_CHECK_VALUE(kc.scalar_type() == dtype, op, ": the caches must be float8_e4m3fn or of the rows' dtype");
+    TORCH_CHECK_VALUE(!ks && !vs, op, ": k_scale and v_scale go with float8_e4m3fn caches only");
+    return false;
+  }
+  TORCH_CHECK_VALUE(ks && vs, op, ": float8_e4m3fn caches need k_scale and v_scale");
+  for (const auto* s : {&*ks, &*vs}) {
+    check_cuda(*s, like, op, "k_scale / v_scale");
+    TORCH_CHECK_VALUE(s->scalar_type() == torch::kFloat32 && s->is_contiguous() && s->dim() == 3 && s->size(0) == kc.size(0) &&
+                          s->size(1) == kc.size(1) && s->size(2) == kc.size(2),
+                      op, ": scales must be contiguous float32 [pages, page size, kv_heads]");
+  }
+  return true;
+}
+
+float* scale_ptr(const OptTensor& s) { return s ? s->data_ptr<float>() : nullptr; }
+
+torch::Tensor check_slots(const char* op, const torch::Tensor& slots, const torch::Tensor& like) {
+  check_cuda(slots, like, op, "slots");
+  TORCH_CHECK_VALUE(slots.dim() == 1 && (slots.scalar_type() == torch::kInt32 || slots.scalar_type() == torch::kInt64), op,
+                    ": slots must be 1-D int32 or int64");
+  return slots.contiguous();
+}
+
+void kv_cache_append(torch::Tensor K, torch::Tensor V, torch::Tensor k_cache, torch::Tensor v_cache, torch::Tensor slots,
+                     OptTensor k_scale, OptTensor v_scale) {
+  const char* op = "kv_cache_append";
+  check_cuda(K, K, op, "K");
+  check_cuda(V, K, op, "V");
+  TORCH_CHECK_VALUE(K.dim() == 3 && V.sizes() == K.sizes(), op, ": K and V must be [tokens, kv_heads, dim] of one shape");
+  const int code = dtype_code(K, op);
+  TORCH_CHECK_VALUE(V.scalar_type() == K.scalar_type(), op, ": K and V must have one dtype");
+  const bool e4m3 = check_caches(op, K, k_cache, v_cache, k_scale, v_scale, K.scalar_type());
+  TORCH_CHECK_VALUE(K.size(1) == k_cache.size(2) && K.size(2) == k_cache.size(3), op, ": K and the caches differ in kv_heads or dim");
+  const at::cuda::CUDAGuard guard(K.device());
+  const auto at = check_slots(op, slots, K);
+  TORCH_CHECK_VALUE(at.size(0) == K.size(0), op, ": slots must be [tokens]");
+  const Rows k = as_rows(K), v = as_rows(V);
+  check_rc(bsk_kv_cache_append(code, k.p(), k.ts, k.hs, v.p(), v.ts, v.hs, k_cache.data_ptr(), v_cache.data_ptr(), e4m3,
+                               scale_ptr(k_scale), scale_ptr(v_scale), at.data_ptr(), static_cast<int>(at.element_size()),
+                               narrow(K.size(0), op, "tokens"), narrow(K.size(1), op, "kv_heads"),
+                               static_cast<int>(K.size(2)), k_cache.size(0) * k_cache.size(1), stream_of(K)),
+           "bsk_kv_cache_append");
+  for (const auto& t : {k_cache, v_cache})  // written in place: autograd's version counters notice
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+  for (const auto& t : {k_scale, v_scale})
+    if (t && !t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+}
+
+std::tuple<torch::Tensor, torch::Tensor> kv_cache_gather(torch::Tensor k_cache, torch::Tensor v_cache, torch::Tensor slots,
+                                                         bool f16, OptTensor k_scale, OptTensor v_scale) {
+  const char* op = "kv_cache_gather";
+  const auto dtype = f16 ? torch::kFloat16 : torch::kBFloat16;
+  const bool e4m3 = check_caches(op, k_cache, k_cache, v_cache, k_scale, v_scale, dtype);
+  const at::cuda::CUDAGuard guard(k_cache.device());
+  const auto at = check_slots(op, slots, k_cache);
+  auto K = torch::empty({at.size(0), k_cache.size(2), k_cache.size(3)}, k_cache.options().dtype(dtype));
+  auto V = torch::empty_like(K);
+  check_rc(bsk_kv_cache_gather(f16, k_cache.data_ptr(), v_cache.data_ptr(), e4m3, scale_ptr(k_scale), scale_ptr(v_scale),
+                               at.data_ptr(), static_cast<int>(at.element_size()), K.data_ptr(), V.data_ptr(),
+                               narrow(K.size(0), op, "tokens"), narrow(K.size(1), op, "kv_heads"),
+                               static_cast<int>(K.size(2)), k_cache.size(0) * k_cache.size(1), stream_of(K)),
+           "bsk_kv_cache_gather");
+  return {K, V};
+}
+
+void check_heads(const char* op, const torch::Tensor& Q, int64_t kv_heads, double scale) {
+  TORCH_CHECK_VALUE(Q.size(2) == 64 || Q.size(2) == 128, op, ": head dimension must be 64 or 128, got ", Q.size(2));
+  TORCH_CHECK_VALUE(kv_heads > 0 && Q.size(1) > 0 && Q.size(1) % kv_heads == 0, op, ": heads (", Q.size(1),
+                    ") must be a positive multiple of kv_heads (", kv_heads, ")");
+  TORCH_CHECK_VALUE(Q.size(1) / kv_heads <= 128, op, ": at most 128 heads per kv head");
+  TORCH_CHECK_VALUE(scale > 0.0 && scale < 1e30, op, ": scale must be positive and finite");
+}
+
+torch::Tensor attention_paged(torch::Tensor Q, torch::Tensor k_cache, torch::Tensor v_cache, torch::Tensor block_table,
+                              torch::Tensor kv_lens, torch::Tensor cu_seqlens, double scale, OptTensor k_scale,
+                              OptTensor v_scale) {
+  const char* op = "attention_paged";
+  check_cuda(Q, Q, op, "Q");
+  TORCH_CHECK_VALUE(Q.dim() == 3, op, ": Q must be [tokens, heads, dim]");
+  const int code = dtype_code(Q, op);
+  const bool e4m3 = check_caches(op, Q, k_cache, v_cache, k_scale, v_scale, Q.scalar_type());
+  TORCH_CHECK_VALUE(Q.size(2) == k_cache.size(3), op, ": Q and the caches differ in the head dimension");
+  check_heads(op, Q, k_cache.size(2), scale);
+  const int64_t page = k_cache.size(1);
+  TORCH_CHECK_VALUE(page >= 8 && page <= 1024 && (page & (page - 1)) == 0, op, ": the page size must be a power of two from 8 to 1024");
+  const at::cuda::CUDAGuard guard(Q.device());
+  const auto table = as_index(block_table, Q, op, "block_table", 2), lens = as_index(kv_lens, Q, op, "kv_lens", 1),
+             cu = as_index(cu_seqlens, Q, op, "cu_seqlens", 1);
+  TORCH_CHECK_VALUE(cu.size(0) == lens.size(0) + 1 && table.size(0) == lens.size(0), op,
+                    ": block_table [batch, width], kv_lens [batch] and cu_seqlens [batch + 1] differ in the batch");
+  const Rows q = as_rows(Q);
+  auto O = torch::empty({Q.size(0), Q.size(1), Q.size(2)}, Q.options());
+  check_rc(bsk_attention_paged(code, q.p(), q.ts, q.hs, k_cache.data_ptr(), v_cache.data_ptr(), e4m3, scale_ptr(k_scale),
+                               scale_ptr(v_scale), table.data_ptr<int32_t>(), table.size(1),
+                               narrow(table.size(1), op, "table width"), lens.data_ptr<int32_t>(), cu.data_ptr<int32_t>(),
+                               O.data_ptr(), narrow(Q.size(0), op, "tokens"), narrow(lens.size(0), op, "batch"),
+                               static_cast<int>(Q.size(1)), static_cast<int>(k_cache.size(2)), static_cast<int>(Q.size(2)),
+                               narrow(k_cache.size(0), op, "pages"), static_cast<int>(page), static_cast<float>(scale),
+                               stream_of(Q)),
+           "bsk_attention_paged");
+  return O;
+}
+
+torch::Tensor varlen_workspace(const torch::Tensor& Q, int64_t batch, int64_t kv_heads, bool backward) {
+  const int64_t n = bsk_attention_varlen_workspace_bytes(static_cast<int>(Q.size(0)), static_cast<int>(batch),
+                                                         static_cast<int>(Q.size(1)), static_cast<int>(kv_heads),
+                                                         static_cast<int>(Q.size(2)), backward);
+  TORCH_CHECK(n >= 0, "bsk_attention_varlen_workspace_bytes failed: ", bsk_last_error());
+  return torch::empty({n}, Q.options().dtype(torch::kUInt8));
+}
+
+void check_varlen(const char* op, const torch::Tensor& Q, const torch::Tensor& K, const torch::Tensor& V, double scale) {
+  check_cuda(Q, Q, op, "Q");
+  check_cuda(K, Q, op, "K");
+  check_cuda(V, Q, op, "V");
+  TORCH_CHECK_VALUE(Q.dim() == 3 && K.dim() == 3 && V.sizes() == K.sizes() && K.size(0) == Q.size(0) && K.size(2) == Q.size(2), op,
+                    ": Q must be [tokens, heads, dim], K and V [tokens, kv_heads, dim]");
+  TORCH_CHECK_VALUE(K.scalar_type() == Q.scalar_type() && V.scalar_type() == Q.scalar_type(), op, ": Q, K and V must have one dtype");
+  check_heads(op, Q, K.size(1), scale);
+  narrow(Q.size(0), op, "tokens");
+}
+
+// (O, LSE): the log-sum-exp [tokens, heads] only when asked for (else an empty tensor).
+std::tuple<torch::Tensor, torch::Tensor> attention_varlen_fwd(torch::Tensor Q, torch::Tensor K, torch::Tensor V,
+                                                              torch::Tensor cu_seqlens, double scale, bool causal,
+                                                              bool want_lse) {
+  const char* op = "attention_varlen";
+  check_varlen(op, Q, K, V, scale);
+  const int code = dtype_code(Q, op);
+  const at::cuda::CUDAGuard guard(Q.device());
+  const auto cu = as_index(cu_seqlens, Q, op, "cu_seqlens", 1);
+  TORCH_CHECK_VALUE(cu.size(0) >= 1, op, ": cu_seqlens must be [batch + 1]");
+  const int64_t batch = cu.size(0) - 1;
+  const Rows q = as_rows(Q), k = as_rows(K), v = as_rows(V);
+  auto O = torch::empty({Q.size(0), Q.size(1), Q.size(2)}, Q.options());
+  auto lse = torch::empty({want_lse ? Q.size(0) : 0, Q.size(1)}, Q.options().dtype(torch::kFloat32));
+  auto ws = varlen_workspace(Q, batch, K.size(1), false);
+  check_rc(bsk_attention_varlen_fwd(code, q.p(), q.ts, q.hs, k.p(), k.ts, k.hs, v.p(), v.ts, v.hs, cu.data_ptr<int32_t>(),
+                                    O.data_ptr(), want_lse ? lse.data_ptr<float>() : nullptr, static_cast<int>(Q.size(0)),
+                                    narrow(batch, op, "batch"), static_cast<int>(Q.size(1)), static_cast<int>(K.size(1)),
+                                    static_cast<int>(Q.size(2)), static_cast<float>(scale), causal, ws.data_ptr(),
+                                    ws.numel(), stream_of(Q)),
+           "bsk_attention_varlen_fwd");
+  return {O, lse};
+}
+
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> attention_varlen_bwd(torch::Tensor dO, torch::Tensor Q, torch::Tensor K,
+                                                                             torch::Tensor V, torch::Tensor O, torch::Tensor lse,
+                                                                             torch::Tensor cu_seqlens, double scale, bool causal) {
+  const char* op = "attention_varlen backward";
+  check_varlen(op, Q, K, V, scale);
+  const int code = dtype_code(Q, op);
+  check_cuda(dO, Q, op, "dO");
+  check_cuda(O, Q, op, "O");
+  check_cuda(lse, Q, op, "lse");
+  TORCH_CHECK_VALUE(dO.sizes() == Q.sizes() && O.sizes() == Q.sizes() && dO.scalar_type() == Q.scalar_type() &&
+                        O.scalar_type() == Q.scalar_type() && O.is_contiguous(),
+                    op, ": dO and O must be like Q, O contiguous");
+  TORCH_CHECK_VALUE(lse.scalar_type() == torch::kFloat32 && lse.is_contiguous() && lse.numel() == Q.size(0) * Q.size(1), op,
+                    ": lse must be float32 [tokens, heads]");
+  const at::cuda::CUDAGuard guard(Q.device());
+  const auto cu = as_index(cu_seqlens, Q, op, "cu_seqlens", 1);
+  TORCH_CHECK_VALUE(cu.size(0) >= 1, op, ": cu_seqlens must be [batch + 1]");
+  const int64_t batch = cu.size(0) - 1;
+  const Rows g = as_rows(dO), q = as_rows(Q), k = as_rows(K), v = as_rows(V);
+  auto dQ = torch::empty({Q.size(0), Q.size(1), Q.size(2)}, Q.options());
+  auto dK = torch::empty({K.size(0), K.size(1), K.size(2)}, K.options());
+  auto dV = torch::empty_like(dK);
+  auto ws = varlen_workspace(Q, batch, K.size(1), true);
+  check_rc(bsk_attention_varlen_bwd(code, g.p(), g.ts, g.hs, q.p(), q.ts, q.hs, k.p(), k.ts, k.hs, v.p(), v.ts, v.hs,
+                                    O.data_ptr(), lse.data_ptr<float>(), cu.data_ptr<int32_t>(), dQ.data_ptr(),
+                                    dK.data_ptr(), dV.data_ptr(), static_cast<int>(Q.size(0)), narrow(batch, op, "batch"),
+                                    static_cast<int>(Q.size(1)), static_cast<int>(K.size(1)), static_cast<int>(Q.size(2)),
+                                    static_cast<float>(scale), causal, ws.data_ptr(), ws.numel(), stream_of(Q)),
+           "bsk_attention_varlen_bwd");
+  return {dQ, dK, dV};
+}
+
 int64_t device_error() {
   uint32_t w = 0;
   check_rc(bsk_device_error(&w), "bsk_device_error");
@@ -182,5 +459,21 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("Bqt"), py::arg("scale_a"), py::arg("scale_b"));
   m.def("bsattn_fwd", &bsattn_fwd, "block-sparse attention forward (sm_100a)", py::arg("Q"), py::arg("K"),
         py::arg("V"), py::arg("row_ptr"), py::arg("col_idx"), py::arg("scale"), py::arg("causal_diag") = true);
+  m.def("rotary", &rotary, "rotary positions of Q and K (sm_100a)", py::arg("Q"), py::arg("K"), py::arg("positions"),
+        py::arg("inv_freq"), py::arg("interleaved") = false, py::arg("scale") = 1.0, py::arg("backward") = false);
+  m.def("kv_cache_append", &kv_cache_append, "write rows to a paged key/value cache (sm_100a)", py::arg("K"), py::arg("V"),
+        py::arg("k_cache"), py::arg("v_cache"), py::arg("slots"), py::arg("k_scale") = py::none(),
+        py::arg("v_scale") = py::none());
+  m.def("kv_cache_gather", &kv_cache_gather, "read rows of a paged key/value cache (sm_100a)", py::arg("k_cache"),
+        py::arg("v_cache"), py::arg("slots"), py::arg("f16"), py::arg("k_scale") = py::none(),
+        py::arg("v_scale") = py::none());
+  m.def("attention_paged", &attention_paged, "attention of new tokens over a paged cache (sm_100a)", py::arg("Q"),
+        py::arg("k_cache"), py::arg("v_cache"), py::arg("block_table"), py::arg("kv_lens"), py::arg("cu_seqlens"),
+        py::arg("scale"), py::arg("k_scale") = py::none(), py::arg("v_scale") = py::none());
+  m.def("attention_varlen_fwd", &attention_varlen_fwd, "attention over packed sequences (sm_100a)", py::arg("Q"),
+        py::arg("K"), py::arg("V"), py::arg("cu_seqlens"), py::arg("scale"), py::arg("causal") = true,
+        py::arg("want_lse") = false);
+  m.def("attention_varlen_bwd", &attention_varlen_bwd, "its gradients (sm_100a)", py::arg("dO"), py::arg("Q"), py::arg("K"),
+        py::arg("V"), py::arg("O"), py::arg("lse"), py::arg("cu_seqlens"), py::arg("scale"), py::arg("causal") = true);
   m.def("device_error", &device_error, "read and clear the device error word");
 }

@@ -20,6 +20,10 @@
 #include "bsattn_sm100.cuh"
 #include "bsr_convert.cuh"
 #include "bsattn_bwd_sm100.cuh"
+#include "rotary.cuh"
+#include "kv_cache.cuh"
+#include "paged_decode_sm100.cuh"
+#include "varlen_simple.cuh"
 
 namespace {
 
@@ -52,6 +56,7 @@ struct DeviceState {
   int sm_count = 0;
   int pair_clusters = 0;       // co-resident 2-CTA clusters of the pair GEMM kernels (all share one footprint)
   int bsr_pair_clusters = 0;   // co-resident 2-CTA clusters of the pair BSR SpMM kernel (0: not used)
+  int paged_max_cluster = 8;   // CTAs per cluster of the paged decode kernel (16 where the device can place them)
   uint32_t* err_word = nullptr;
 };
 DeviceState g_devices[kMaxDevices];
@@ -62,6 +67,14 @@ PFN_cuTensorMapEncodeTiled_v12000 g_encode = nullptr;
 template <class K>
 cudaError_t allow_smem(K kernel, int bytes) {
   return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+}
+
+// Shared memory and the 16-CTA clusters of one instantiation of the paged decode kernel.
+template <bool kF16, int kD, bool kFp8>
+cudaError_t allow_paged() {
+  const auto k = bsk::paged_decode_kernel<kF16, kD, kFp8>;
+  const cudaError_t e = allow_smem(k, bsk::PagedShape<kF16, kD, kFp8>::kSmemBytes);
+  return e != cudaSuccess ? e : cudaFuncSetAttribute(k, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
 }
 
 // How many 2-CTA clusters of `kernel` can be resident at once (persistent grids are sized to this).
@@ -159,6 +172,9 @@ void init_device(DeviceState& st, int dev) {
       allow_smem(gemm_pair_sm100_kernel<2, Epi::F32PeerRows, 2>, kPairWideSmemBytes),
       allow_smem(gemm_pair_sm100_kernel<1, Epi::BF16Scaled, 2>, kPairWideSmemBytes),
       allow_smem(spmm_bsr_pair_sm100_kernel, kBsrPairSmemBytes),
+      allow_paged<false, 128, false>(), allow_paged<false, 128, true>(), allow_paged<false, 64, false>(),
+      allow_paged<false, 64, true>(),   allow_paged<true, 128, false>(), allow_paged<true, 128, true>(),
+      allow_paged<true, 64, false>(),   allow_paged<true, 64, true>(),
   };
   for (cudaError_t x : errs) {
     if (x != cudaSuccess) {
@@ -176,6 +192,23 @@ void init_device(DeviceState& st, int dev) {
     for (int i = 1; i < 4; ++i) st.pair_clusters = c[i] < st.pair_clusters ? c[i] : st.pair_clusters;
   }
   st.bsr_pair_clusters = max_clusters(spmm_bsr_pair_sm100_kernel, kPairThreads, kBsrPairSmemBytes);
+  {
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 16;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.gridDim = dim3(16, 1, 1);
+    cfg.blockDim = dim3(kPagedThreads, 1, 1);
+    cfg.dynamicSmemBytes = PagedShape<false, 64, true>::kSmemBytes;  // the largest of the instantiations
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int n = 0;
+    const cudaError_t x =
+        cudaOccupancyMaxActiveClusters(&n, reinterpret_cast<const void*>(paged_decode_kernel<false, 64, true>), &cfg);
+    if (x == cudaSuccess && n > 0) st.paged_max_cluster = 16;
+    else cudaGetLastError();
+  }
   if (st.pair_clusters <= 0) {
     st.status = BSK_ERR_CUDA;
     st.init_error = "cudaOccupancyMaxActiveClusters reports no co-resident CTA pair";
@@ -1827,6 +1860,367 @@ int bsk_selftest_exp2(const float* x, float* y, int n, int fma_pipe, void* strea
   const int grid = blocks_needed < 4 * st->sm_count ? blocks_needed : 4 * st->sm_count;
   bsk::exp2_probe_kernel<<<grid, 256, 0, static_cast<cudaStream_t>(stream)>>>(x, y, n, fma_pipe);
   return launch_status("selftest_exp2 launch");
+}
+
+}  // extern "C"
+
+// ------------------------------------------------------------------------------------------------ rotary positions
+namespace {
+
+// Rows of `heads` heads of `dim` 16-bit (or, for rotary, wider) elements: strides in elements, head rows 16-byte aligned.
+bool rows_aligned(const void* p, int64_t token_stride, int64_t head_stride, int elem_bytes) {
+  return aligned16(p) && (token_stride * elem_bytes) % 16 == 0 && (head_stride * elem_bytes) % 16 == 0;
+}
+
+template <class T, int kVec, bool kInter>
+int rotary_launch(const bsk::RotaryArgs& a, const DeviceState& st, cudaStream_t s) {
+  // Few tokens: one per block, so that the rows spread over the SMs. Many: up to 4, so that a block's threads all take
+  // part in the angles (rotary_dim / 2 of them per token).
+  const int tpb = a.tokens <= 8 * st.sm_count ? 1 : 4;
+  const int64_t grid = ((int64_t)a.tokens + tpb - 1) / tpb;
+  const int smem = tpb * (a.rotary_dim / 2) * (int)sizeof(float2);
+  bsk::rotary_kernel<T, kVec, kInter><<<(unsigned)grid, bsk::kRotaryThreads, smem, s>>>(a, tpb);
+  return launch_status("rotary launch");
+}
+
+template <class T>
+int rotary_pick(const bsk::RotaryArgs& a, bool inter, const DeviceState& st, cudaStream_t s) {
+  constexpr int kVec = 16 / sizeof(T);
+  bool wide = (a.dim - a.rotary_dim) % (2 * kVec) == 0 &&
+              (inter ? a.rotary_dim % (2 * kVec) == 0 : (a.rotary_dim / 2) % kVec == 0);
+  for (int w = 0; w < 2; ++w)
+    if (a.heads[w])
+      wide = wide && aligned16(a.y[w]) && rows_aligned(a.x[w], a.token_stride[w], a.head_stride[w], sizeof(T));
+  if (wide) return inter ? rotary_launch<T, kVec, true>(a, st, s) : rotary_launch<T, kVec, false>(a, st, s);
+  return inter ? rotary_launch<T, 1, true>(a, st, s) : rotary_launch<T, 1, false>(a, st, s);
+}
+
+}  // namespace
+
+extern "C" {
+
+int bsk_rotary(int dtype, const void* Q, int64_t q_token_stride, int64_t q_head_stride, void* Q_out, int heads,
+               const void* K, int64_t k_token_stride, int64_t k_head_stride, void* K_out, int kv_heads,
+               const void* positions, int position_bytes, const float* inv_freq, int tokens, int dim, int rotary_dim,
+               int interleaved, float scale, int backward, void* stream) {
+  const char* what = "rotary";
+  if (dtype < 0 || dtype > 2) return set_error(BSK_ERR_INVALID_ARG, "%s: dtype must be 0 (bf16), 1 (f16) or 2 (f32)", what);
+  if (tokens < 0 || heads < 0 || kv_heads < 0) return set_error(BSK_ERR_INVALID_ARG, "%s: negative extent", what);
+  if (dim <= 0 || dim % 2 || dim > bsk::kRotaryMaxDim)
+    return set_error(BSK_ERR_UNSUPPORTED, "%s: head dim %d unsupported (even, at most %d)", what, dim, bsk::kRotaryMaxDim);
+  if (rotary_dim < 2 || rotary_dim % 2 || rotary_dim > dim)
+    return set_error(BSK_ERR_INVALID_ARG, "%s: rotary dim %d must be even and within [2, %d]", what, rotary_dim, dim);
+  if (position_bytes != 4 && position_bytes != 8)
+    return set_error(BSK_ERR_INVALID_ARG, "%s: positions must be 4- or 8-byte integers", what);
+  if (!(scale > -1e30f && scale < 1e30f)) return set_error(BSK_ERR_INVALID_ARG, "%s: scale must be finite", what);
+  DeviceState* st;
+  if (tokens == 0 || (heads == 0 && kv_heads == 0)) return device_state(&st);
+  if (!positions || !inv_freq || (heads && (!Q || !Q_out)) || (kv_heads && (!K || !K_out)))
+    return set_error(BSK_ERR_INVALID_ARG, "%s: null pointer", what);
+  if (int rc = device_state(&st)) return rc;
+  bsk::RotaryArgs a{};
+  a.x[0] = Q; a.x[1] = K;
+  a.y[0] = Q_out; a.y[1] = K_out;
+  a.token_stride[0] = q_token_stride; a.token_stride[1] = k_token_stride;
+  a.head_stride[0] = q_head_stride; a.head_stride[1] = k_head_stride;
+  a.heads[0] = heads; a.heads[1] = kv_heads;
+  a.positions = positions;
+  a.positions64 = position_bytes == 8;
+  a.inv_freq = inv_freq;
+  a.tokens = tokens;
+  a.dim = dim;
+  a.rotary_dim = rotary_dim;
+  a.scale = scale;
+  a.sign = backward ? -1.0f : 1.0f;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (dtype == 0) return rotary_pick<__nv_bfloat16>(a, interleaved != 0, *st, s);
+  if (dtype == 1) return rotary_pick<__half>(a, interleaved != 0, *st, s);
+  return rotary_pick<float>(a, interleaved != 0, *st, s);
+}
+
+}  // extern "C"
+
+// ------------------------------------------------------------------------------------------------ paged cache
+namespace {
+
+int cache_checks(const char* what, int dtype, int cache_e4m3, const void* slots, int slot_bytes, int tokens, int kv_heads,
+                 int dim, int64_t num_slots, const void* k_cache, const void* v_cache, const float* k_scale,
+                 const float* v_scale) {
+  if (dtype != 0 && dtype != 1) return set_error(BSK_ERR_INVALID_ARG, "%s: dtype must be 0 (bf16) or 1 (f16)", what);
+  if (dim != 64 && dim != 128) return set_error(BSK_ERR_UNSUPPORTED, "%s: head dim %d unsupported (64 or 128)", what, dim);
+  if (tokens < 0 || kv_heads < 0 || num_slots < 0) return set_error(BSK_ERR_INVALID_ARG, "%s: negative extent", what);
+  if ((int64_t)tokens * kv_heads >= (int64_t)1 << 31)
+    return set_error(BSK_ERR_UNSUPPORTED, "%s: tokens x kv_heads must stay below 2^31", what);
+  if (slot_bytes != 4 && slot_bytes != 8) return set_error(BSK_ERR_INVALID_ARG, "%s: slots must be 4- or 8-byte integers", what);
+  if (tokens == 0 || kv_heads == 0) return BSK_OK;
+  if (!slots || (num_slots > 0 && (!k_cache || !v_cache || (cache_e4m3 && (!k_scale || !v_scale)))))
+    return set_error(BSK_ERR_INVALID_ARG, "%s: null pointer", what);
+  if (!aligned16(k_cache) || !aligned16(v_cache)) return set_error(BSK_ERR_INVALID_ARG, "%s: caches must be 16-byte aligned", what);
+  return BSK_OK;
+}
+
+void cache_args(bsk::KvCacheArgs& a, const DeviceState& st, const void* k_cache, const void* v_cache, const float* k_scale,
+                const float* v_scale, const void* slots, int slot_bytes, int tokens, int kv_heads, int64_t num_slots) {
+  a.cache[0] = const_cast<void*>(k_cache);
+  a.cache[1] = const_cast<void*>(v_cache);
+  a.scale[0] = const_cast<float*>(k_scale);
+  a.scale[1] = const_cast<float*>(v_scale);
+  a.slots = slots;
+  a.slots64 = slot_bytes == 8;
+  a.tokens = tokens;
+  a.heads = kv_heads;
+  a.num_slots = num_slots;
+  a.err = st.err_word;
+}
+
+// Instantiation by element type, head dim and cache type.
+#define BSK_BY_TYPE(KERNEL, f16, dim, fp8, ...)                             \
+  do {                                                                      \
+    if (f16) {                                                              \
+      if (dim == 128) { if (fp8) KERNEL<true, 128, true> __VA_ARGS__; else KERNEL<true, 128, false> __VA_ARGS__; } \
+      else            { if (fp8) KERNEL<true, 64, true> __VA_ARGS__; else KERNEL<true, 64, false> __VA_ARGS__; }   \
+    } else {                                                                \
+      if (dim == 128) { if (fp8) KERNEL<false, 128, true> __VA_ARGS__; else KERNEL<false, 128, false> __VA_ARGS__; } \
+      else            { if (fp8) KERNEL<false, 64, true> __VA_ARGS__; else KERNEL<false, 64, false> __VA_ARGS__; }   \
+    }                                                                       \
+  } while (0)
+
+}  // namespace
+
+extern "C" {
+
+int bsk_kv_cache_append(int dtype, const void* K, int64_t k_token_stride, int64_t k_head_stride, const void* V,
+                        int64_t v_token_stride, int64_t v_head_stride, void* k_cache, void* v_cache, int cache_e4m3,
+                        float* k_scale, float* v_scale, const void* slots, int slot_bytes, int tokens, int kv_heads,
+                        int dim, int64_t num_slots, void* stream) {
+  const char* what = "kv_cache_append";
+  if (int rc = cache_checks(what, dtype, cache_e4m3, slots, slot_bytes, tokens, kv_heads, dim, num_slots, k_cache, v_cache,
+                            k_scale, v_scale))
+    return rc;
+  DeviceState* st;
+  if (tokens == 0 || kv_heads == 0) return device_state(&st);
+  if (!K || !V) return set_error(BSK_ERR_INVALID_ARG, "%s: null pointer", what);
+  if (!rows_aligned(K, k_token_stride, k_head_stride, 2) || !rows_aligned(V, v_token_stride, v_head_stride, 2))
+    return set_error(BSK_ERR_INVALID_ARG, "%s: rows of K and V must be 16-byte aligned", what);
+  if (int rc = device_state(&st)) return rc;
+  bsk::KvCacheArgs a{};
+  cache_args(a, *st, k_cache, v_cache, k_scale, v_scale, slots, slot_bytes, tokens, kv_heads, num_slots);
+  a.x[0] = K; a.x[1] = V;
+  a.token_stride[0] = k_token_stride; a.token_stride[1] = v_token_stride;
+  a.head_stride[0] = k_head_stride; a.head_stride[1] = v_head_stride;
+  const int64_t threads = (int64_t)tokens * kv_heads * (dim / 8);
+  const unsigned grid = (unsigned)((threads + bsk::kCacheThreads - 1) / bsk::kCacheThreads);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  using namespace bsk;
+  BSK_BY_TYPE(kv_cache_append_kernel, dtype == 1, dim, cache_e4m3 != 0, <<<grid, kCacheThreads, 0, s>>>(a));
+  return launch_status("kv_cache_append launch");
+}
+
+int bsk_kv_cache_gather(int dtype, const void* k_cache, const void* v_cache, int cache_e4m3, const float* k_scale,
+                        const float* v_scale, const void* slots, int slot_bytes, void* K, void* V, int tokens, int kv_heads,
+                        int dim, int64_t num_slots, void* stream) {
+  const char* what = "kv_cache_gather";
+  if (int rc = cache_checks(what, dtype, cache_e4m3, slots, slot_bytes, tokens, kv_heads, dim, num_slots, k_cache, v_cache,
+                            k_scale, v_scale))
+    return rc;
+  DeviceState* st;
+  if (tokens == 0 || kv_heads == 0) return device_state(&st);
+  if (!K || !V) return set_error(BSK_ERR_INVALID_ARG, "%s: null pointer", what);
+  if (!aligned16(K) || !aligned16(V)) return set_error(BSK_ERR_INVALID_ARG, "%s: K and V must be 16-byte aligned", what);
+  if (int rc = device_state(&st)) return rc;
+  bsk::KvCacheArgs a{};
+  cache_args(a, *st, k_cache, v_cache, k_scale, v_scale, slots, slot_bytes, tokens, kv_heads, num_slots);
+  a.y[0] = K; a.y[1] = V;
+  const int64_t threads = (int64_t)tokens * kv_heads * (dim / 8);
+  const unsigned grid = (unsigned)((threads + bsk::kCacheThreads - 1) / bsk::kCacheThreads);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  using namespace bsk;
+  BSK_BY_TYPE(kv_cache_gather_kernel, dtype == 1, dim, cache_e4m3 != 0, <<<grid, kCacheThreads, 0, s>>>(a));
+  return launch_status("kv_cache_gather launch");
+}
+
+}  // extern "C"
+
+// ------------------------------------------------------------------------------------------------ packed and paged attention
+namespace {
+
+int heads_checks(const char* what, int dtype, int tokens, int batch, int heads, int kv_heads, int dim, float scale) {
+  if (dtype != 0 && dtype != 1) return set_error(BSK_ERR_INVALID_ARG, "%s: dtype must be 0 (bf16) or 1 (f16)", what);
+  if (dim != 64 && dim != 128) return set_error(BSK_ERR_UNSUPPORTED, "%s: head dim %d unsupported (64 or 128)", what, dim);
+  if (tokens < 0 || batch < 0) return set_error(BSK_ERR_INVALID_ARG, "%s: negative extent", what);
+  if (heads <= 0 || kv_heads <= 0 || heads % kv_heads)
+    return set_error(BSK_ERR_INVALID_ARG, "%s: heads (%d) must be a positive multiple of kv_heads (%d)", what, heads, kv_heads);
+  if (heads / kv_heads > 128)
+    return set_error(BSK_ERR_UNSUPPORTED, "%s: at most 128 heads per kv head, got %d", what, heads / kv_heads);
+  if (kv_heads > 65535) return set_error(BSK_ERR_UNSUPPORTED, "%s: at most 65535 kv heads", what);
+  if (!(scale > 0.0f) || !(scale < 1e30f)) return set_error(BSK_ERR_INVALID_ARG, "%s: scale must be positive and finite", what);
+  return BSK_OK;
+}
+
+template <bool kF16, int kD, bool kFp8>
+cudaError_t paged_decode_launch(const bsk::PagedArgs& a, unsigned tiles, int cluster, cudaStream_t s) {
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = cluster;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.gridDim = dim3(tiles * cluster, a.kv_heads, 1);
+  cfg.blockDim = dim3(bsk::kPagedThreads, 1, 1);
+  cfg.dynamicSmemBytes = bsk::PagedShape<kF16, kD, kFp8>::kSmemBytes;
+  cfg.stream = s;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, bsk::paged_decode_kernel<kF16, kD, kFp8>, a);
+}
+
+}  // namespace
+
+extern "C" {
+
+int bsk_attention_paged(int dtype, const void* Q, int64_t q_token_stride, int64_t q_head_stride, const void* k_cache,
+                        const void* v_cache, int cache_e4m3, const float* k_scale, const float* v_scale,
+                        const int32_t* block_table, int64_t table_stride, int table_width, const int32_t* kv_lens,
+                        const int32_t* cu_seqlens, void* O, int tokens, int batch, int heads, int kv_heads, int dim,
+                        int num_pages, int page_size, float scale, void* stream) {
+  const char* what = "attention_paged";
+  if (int rc = heads_checks(what, dtype, tokens, batch, heads, kv_heads, dim, scale)) return rc;
+  if (page_size < 8 || page_size > 1024 || (page_size & (page_size - 1)))
+    return set_error(BSK_ERR_UNSUPPORTED, "%s: page size %d unsupported (a power of two from 8 to 1024)", what, page_size);
+  if (num_pages < 0 || table_width < 0 || table_stride < 0) return set_error(BSK_ERR_INVALID_ARG, "%s: negative extent", what);
+  if ((int64_t)num_pages * page_size >= (int64_t)1 << 31 || (int64_t)table_width * page_size >= (int64_t)1 << 31)
+    return set_error(BSK_ERR_UNSUPPORTED, "%s: pages x page size must stay below 2^31 slots", what);
+  DeviceState* st;
+  if (tokens == 0) return device_state(&st);
+  if (!Q || !O || !cu_seqlens || (batch > 0 && !kv_lens) || (batch > 0 && table_width > 0 && !block_table) ||
+      (num_pages > 0 && (!k_cache || !v_cache || (cache_e4m3 && (!k_scale || !v_scale)))))
+    return set_error(BSK_ERR_INVALID_ARG, "%s: null pointer", what);
+  if (!rows_aligned(Q, q_token_stride, q_head_stride, 2) || !aligned16(O) || !aligned16(k_cache) || !aligned16(v_cache))
+    return set_error(BSK_ERR_INVALID_ARG, "%s: rows of Q, O and the caches must be 16-byte aligned", what);
+  if (int rc = device_state(&st)) return rc;
+  bsk::PagedArgs a{};
+  a.Q = Q;
+  a.q_token_stride = q_token_stride;
+  a.q_head_stride = q_head_stride;
+  a.O = O;
+  a.k_cache = k_cache;
+  a.v_cache = v_cache;
+  a.k_scale = k_scale;
+  a.v_scale = v_scale;
+  a.block_table = block_table;
+  a.table_stride = table_stride;
+  a.table_width = table_width;
+  a.kv_lens = kv_lens;
+  a.cu_seqlens = cu_seqlens;
+  a.tokens = tokens;
+  a.batch = batch;
+  a.heads = heads;
+  a.kv_heads = kv_heads;
+  a.group = heads / kv_heads;
+  a.num_pages = num_pages;
+  while ((1 << a.page_shift) < page_size) ++a.page_shift;
+  a.scale_log2 = scale * 1.4426950408889634f;
+  a.err = st->err_word;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const int64_t tiles = (int64_t)tokens * a.group / bsk::kPagedRows + batch + 1;
+  // CTAs per tile: doubled while the GPU's slots (2 CTAs per SM) are filled fewer than four times and each CTA keeps at
+  // least 128 keys of the longest sequence that the table can hold.
+  int cluster = 1;
+  const int64_t most_keys = (int64_t)table_width * page_size;
+  while (cluster < st->paged_max_cluster && tiles * kv_heads * cluster < (int64_t)8 * st->sm_count &&
+         most_keys >= (int64_t)cluster * 256)
+    cluster *= 2;
+  if (tiles * cluster >= (int64_t)1 << 31) return set_error(BSK_ERR_UNSUPPORTED, "%s: too many rows", what);
+  cudaError_t e = cudaSuccess;
+  BSK_BY_TYPE(e = paged_decode_launch, dtype == 1, dim, cache_e4m3 != 0, (a, (unsigned)tiles, cluster, s));
+  if (e != cudaSuccess) return cuda_fail(e, "attention_paged launch");
+  return launch_status("attention_paged launch");
+}
+
+int64_t bsk_attention_varlen_workspace_bytes(int tokens, int batch, int heads, int kv_heads, int dim, int backward) {
+  if (int rc = heads_checks("attention_varlen_workspace_bytes", 0, tokens, batch, heads, kv_heads, dim, 1.0f)) return rc;
+  (void)backward;
+  return 0;
+}
+
+int bsk_attention_varlen_fwd(int dtype, const void* Q, int64_t q_token_stride, int64_t q_head_stride, const void* K,
+                             int64_t k_token_stride, int64_t k_head_stride, const void* V, int64_t v_token_stride,
+                             int64_t v_head_stride, const int32_t* cu_seqlens, void* O, float* lse, int tokens, int batch,
+                             int heads, int kv_heads, int dim, float scale, int causal, void* workspace,
+                             int64_t workspace_bytes, void* stream) {
+  const char* what = "attention_varlen_fwd";
+  if (int rc = heads_checks(what, dtype, tokens, batch, heads, kv_heads, dim, scale)) return rc;
+  DeviceState* st;
+  if (tokens == 0) return device_state(&st);
+  const int64_t need = bsk_attention_varlen_workspace_bytes(tokens, batch, heads, kv_heads, dim, 0);
+  if (workspace_bytes < need || (need > 0 && !workspace))
+    return set_error(BSK_ERR_INVALID_ARG, "%s: workspace of %lld bytes needed", what, (long long)need);
+  if (!Q || !K || !V || !O || !cu_seqlens) return set_error(BSK_ERR_INVALID_ARG, "%s: null pointer", what);
+  if (!rows_aligned(Q, q_token_stride, q_head_stride, 2) || !rows_aligned(K, k_token_stride, k_head_stride, 2) ||
+      !rows_aligned(V, v_token_stride, v_head_stride, 2) || !aligned16(O) || !aligned16(workspace))
+    return set_error(BSK_ERR_INVALID_ARG, "%s: rows of Q, K, V and O must be 16-byte aligned", what);
+  if (int rc = device_state(&st)) return rc;
+  bsk::VarlenArgs a{};
+  a.Q = Q; a.K = K; a.V = V; a.O = O; a.lse = lse; a.cu = cu_seqlens;
+  a.q_ts = q_token_stride; a.q_hs = q_head_stride;
+  a.k_ts = k_token_stride; a.k_hs = k_head_stride;
+  a.v_ts = v_token_stride; a.v_hs = v_head_stride;
+  a.tokens = tokens; a.batch = batch; a.heads = heads; a.kv_heads = kv_heads; a.group = heads / kv_heads;
+  a.causal = causal;
+  a.scale = scale;
+  a.err = st->err_word;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const unsigned grid = (unsigned)(((int64_t)tokens * heads + 3) / 4);
+  if (dtype == 1 && dim == 128) bsk::varlen_simple_kernel<true, 128, 0><<<grid, 128, 0, s>>>(a);
+  else if (dtype == 1) bsk::varlen_simple_kernel<true, 64, 0><<<grid, 128, 0, s>>>(a);
+  else if (dim == 128) bsk::varlen_simple_kernel<false, 128, 0><<<grid, 128, 0, s>>>(a);
+  else bsk::varlen_simple_kernel<false, 64, 0><<<grid, 128, 0, s>>>(a);
+  return launch_status("attention_varlen_fwd launch");
+}
+
+int bsk_attention_varlen_bwd(int dtype, const void* dO, int64_t do_token_stride, int64_t do_head_stride, const void* Q,
+                             int64_t q_token_stride, int64_t q_head_stride, const void* K, int64_t k_token_stride,
+                             int64_t k_head_stride, const void* V, int64_t v_token_stride, int64_t v_head_stride,
+                             const void* O, const float* lse, const int32_t* cu_seqlens, void* dQ, void* dK, void* dV,
+                             int tokens, int batch, int heads, int kv_heads, int dim, float scale, int causal,
+                             void* workspace, int64_t workspace_bytes, void* stream) {
+  const char* what = "attention_varlen_bwd";
+  if (int rc = heads_checks(what, dtype, tokens, batch, heads, kv_heads, dim, scale)) return rc;
+  DeviceState* st;
+  if (tokens == 0) return device_state(&st);
+  const int64_t need = bsk_attention_varlen_workspace_bytes(tokens, batch, heads, kv_heads, dim, 1);
+  if (workspace_bytes < need || (need > 0 && !workspace))
+    return set_error(BSK_ERR_INVALID_ARG, "%s: workspace of %lld bytes needed", what, (long long)need);
+  if (!dO || !Q || !K || !V || !O || !lse || !cu_seqlens || !dQ || !dK || !dV)
+    return set_error(BSK_ERR_INVALID_ARG, "%s: null pointer", what);
+  if (!rows_aligned(Q, q_token_stride, q_head_stride, 2) || !rows_aligned(K, k_token_stride, k_head_stride, 2) ||
+      !rows_aligned(V, v_token_stride, v_head_stride, 2) || !rows_aligned(dO, do_token_stride, do_head_stride, 2) ||
+      !aligned16(O) || !aligned16(dQ) || !aligned16(dK) || !aligned16(dV) || !aligned16(workspace))
+    return set_error(BSK_ERR_INVALID_ARG, "%s: rows of the tensors must be 16-byte aligned", what);
+  if (int rc = device_state(&st)) return rc;
+  bsk::VarlenArgs a{};
+  a.Q = Q; a.K = K; a.V = V; a.dO = dO; a.O_in = O; a.lse = const_cast<float*>(lse); a.cu = cu_seqlens;
+  a.dQ = dQ; a.dK = dK; a.dV = dV;
+  a.q_ts = q_token_stride; a.q_hs = q_head_stride;
+  a.k_ts = k_token_stride; a.k_hs = k_head_stride;
+  a.v_ts = v_token_stride; a.v_hs = v_head_stride;
+  a.do_ts = do_token_stride; a.do_hs = do_head_stride;
+  a.tokens = tokens; a.batch = batch; a.heads = heads; a.kv_heads = kv_heads; a.group = heads / kv_heads;
+  a.causal = causal;
+  a.scale = scale;
+  a.err = st->err_word;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const unsigned gq = (unsigned)(((int64_t)tokens * heads + 3) / 4), gk = (unsigned)(((int64_t)tokens * kv_heads + 3) / 4);
+#define BSK_VARLEN_BWD(F16, DD)                                          \
+  do {                                                                   \
+    bsk::varlen_simple_kernel<F16, DD, 1><<<gq, 128, 0, s>>>(a);         \
+    bsk::varlen_simple_kernel<F16, DD, 2><<<gk, 128, 0, s>>>(a);         \
+  } while (0)
+  if (dtype == 1 && dim == 128) BSK_VARLEN_BWD(true, 128);
+  else if (dtype == 1) BSK_VARLEN_BWD(true, 64);
+  else if (dim == 128) BSK_VARLEN_BWD(false, 128);
+  else BSK_VARLEN_BWD(false, 64);
+#undef BSK_VARLEN_BWD
+  return launch_status("attention_varlen_bwd launch");
 }
 
 }  // extern "C"

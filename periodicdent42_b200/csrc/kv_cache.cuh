@@ -1,0 +1,156 @@
+// Paged key/value cache for sm_100a: rows written (copied, or quantised to e4m3) and read back.
+//
+// A cache is [pages, page size, kv heads, D] with D = 64 or 128, addressed by flat slots (page * page size + offset);
+// an e4m3 cache has one fp32 scale for each slot and head. Writing a row x of D elements:
+//     scale = max |x| / 448,   code_d = e4m3(x_d / scale)      (448: the largest e4m3 value)
+// with IEEE divisions, so a code is off by at most half an e4m3 step and never saturates; a row of zeros has scale 0 and
+// codes 0, a row that holds a NaN has scale NaN. Reading back gives code * scale, rounded once.
+//
+// Bound: HBM, each row is read and written once. One thread holds 8 elements of a K row and the same 8 of the V row
+// (two independent 16-byte loads in flight); D / 8 neighbouring lanes share a row and take its maximum by shuffles.
+// Slots outside [0, num_slots) are not touched: negative ones mark padding, others set the device error word.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+
+#include "ptx_sm100.cuh"
+
+namespace bsk {
+
+constexpr int kCacheThreads = 256;
+constexpr uint32_t kKidKvCache = 9;
+
+struct KvCacheArgs {
+  const void* x[2];                          // K, V rows to write (append)
+  int64_t token_stride[2], head_stride[2];   // of x, in elements
+  void* y[2];                                // contiguous [tokens, heads, D] to read into (gather)
+  void* cache[2];                            // k_cache, v_cache
+  float* scale[2];                           // k_scale, v_scale (e4m3 caches)
+  const void* slots;                         // int32 or int64 [tokens]
+  int slots64;
+  int tokens, heads;
+  int64_t num_slots;
+  uint32_t* err;
+};
+
+__device__ __forceinline__ int64_t cache_slot(const KvCacheArgs& a, int t) {
+  const int64_t s = a.slots64 ? static_cast<const int64_t*>(a.slots)[t] : static_cast<const int*>(a.slots)[t];
+  if (s >= a.num_slots) {
+    atomicCAS(a.err, 0u, kErrBounds | (kKidKvCache << 8) | (1u << 16));
+    return -1;
+  }
+  return s;
+}
+
+template <bool kF16>
+__device__ __forceinline__ float2 unpack2(uint32_t w) {
+  return kF16 ? __half22float2(*reinterpret_cast<__half2*>(&w)) : __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&w));
+}
+template <bool kF16>
+__device__ __forceinline__ uint32_t round2(float lo, float hi) {
+  if (kF16) {
+    __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<uint32_t*>(&h);
+  }
+  __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<uint32_t*>(&h);
+}
+
+template <bool kF16, int kD, bool kFp8>
+__global__ void __launch_bounds__(kCacheThreads) kv_cache_append_kernel(const KvCacheArgs a) {
+  constexpr int kTpr = kD / 8;  // lanes per row: 8 or 16
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * kCacheThreads + threadIdx.x;
+  // token * heads + head, below 2^31 (checked by the caller); a row's lanes are never split over two warps
+  const uint32_t row = static_cast<uint32_t>(i / kTpr);
+  const bool live = row < static_cast<uint32_t>(a.tokens) * a.heads;
+  const int t = live ? row / static_cast<uint32_t>(a.heads) : 0, h = live ? row % static_cast<uint32_t>(a.heads) : 0;
+  const int c = static_cast<int>(i % kTpr);
+  const int64_t slot = live ? cache_slot(a, t) : -1;
+  uint4 v[2];
+#pragma unroll
+  for (int w = 0; w < 2; ++w) {
+    v[w] = make_uint4(0, 0, 0, 0);
+    if (slot >= 0)
+      v[w] = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.x[w]) + t * a.token_stride[w] +
+                                                  h * a.head_stride[w]) + c);
+  }
+  const int64_t at = (slot * a.heads + h) * kTpr + c;
+#pragma unroll
+  for (int w = 0; w < 2; ++w) {
+    if (!kFp8) {
+      if (slot >= 0) static_cast<uint4*>(a.cache[w])[at] = v[w];
+      continue;
+    }
+    const uint32_t words[4] = {v[w].x, v[w].y, v[w].z, v[w].w};
+    float f[8];
+    uint32_t top = 0;  // largest |x| as bits: ordered like the values, a NaN above all of them
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float2 p = unpack2<kF16>(words[k]);
+      f[2 * k] = p.x;
+      f[2 * k + 1] = p.y;
+      top = max(top, max(__float_as_uint(p.x) & 0x7fffffffu, __float_as_uint(p.y) & 0x7fffffffu));
+    }
+#pragma unroll
+    for (int o = kTpr / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const float scale = __fdiv_rn(__uint_as_float(top), 448.0f);
+    uint2 codes = make_uint2(0, 0);
+    if (scale > 0.0f) {
+      uint32_t q[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        q[k] = __nv_cvt_float2_to_fp8x2(make_float2(__fdiv_rn(f[2 * k], scale), __fdiv_rn(f[2 * k + 1], scale)),
+                                        __NV_SATFINITE, __NV_E4M3);
+      codes = make_uint2(q[0] | (q[1] << 16), q[2] | (q[3] << 16));
+    }
+    if (slot >= 0) {
+      static_cast<uint2*>(a.cache[w])[at] = codes;
+      if (c == 0) a.scale[w][slot * a.heads + h] = scale;
+    }
+  }
+}
+
+template <bool kF16, int kD, bool kFp8>
+__global__ void __launch_bounds__(kCacheThreads) kv_cache_gather_kernel(const KvCacheArgs a) {
+  constexpr int kTpr = kD / 8;
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * kCacheThreads + threadIdx.x;
+  const uint32_t row = static_cast<uint32_t>(i / kTpr);  // below 2^31, as above
+  if (row >= static_cast<uint32_t>(a.tokens) * a.heads) return;
+  const int t = row / static_cast<uint32_t>(a.heads), h = row % static_cast<uint32_t>(a.heads);
+  const int c = static_cast<int>(i % kTpr);
+  const int64_t slot = cache_slot(a, t);
+  const int64_t at = (slot * a.heads + h) * kTpr + c;
+  uint4 out[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+  if (slot >= 0) {
+    if (!kFp8) {
+#pragma unroll
+      for (int w = 0; w < 2; ++w) out[w] = __ldg(static_cast<const uint4*>(a.cache[w]) + at);
+    } else {
+      uint2 q[2];
+      float s[2];
+#pragma unroll
+      for (int w = 0; w < 2; ++w) {
+        q[w] = __ldg(static_cast<const uint2*>(a.cache[w]) + at);
+        s[w] = __ldg(a.scale[w] + slot * a.heads + h);
+      }
+#pragma unroll
+      for (int w = 0; w < 2; ++w) {
+        uint32_t r[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const uint32_t two = ((k < 2 ? q[w].x : q[w].y) >> (16 * (k & 1))) & 0xffffu;
+          const __half2_raw hr = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(two), __NV_E4M3);
+          const float2 p = __half22float2(__half2(hr));  // exact: every e4m3 value is an fp16 value
+          r[k] = round2<kF16>(p.x * s[w], p.y * s[w]);
+        }
+        out[w] = make_uint4(r[0], r[1], r[2], r[3]);
+      }
+    }
+  }
+#pragma unroll
+  for (int w = 0; w < 2; ++w) static_cast<uint4*>(a.y[w])[static_cast<int64_t>(row) * kTpr + c] = out[w];
+}
+
+}  // namespace bsk

@@ -8,6 +8,7 @@ libbsk_sm100.so. There is no CPU fallback: CPU tensors raise ``ValueError`` (as 
 """
 from __future__ import annotations
 
+import math
 from typing import Optional, Tuple
 
 import torch
@@ -381,6 +382,169 @@ def block_mask_to_bsr(block_mask, B: int, H: int, nqb: int, causal: bool, device
     else:
         raise ValueError("block_mask must be 2-D or 4-D")
     return row_ptr.to(device=device, dtype=torch.int32), col_idx.to(device=device, dtype=torch.int32)
+
+
+# ----------------------------------------------------------------------------------------- rotary positions
+def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: Optional[str] = None, factor: float = 1.0,
+                       original_length: int = 4096, beta_fast: float = 32.0, beta_slow: float = 1.0, device=None):
+    """(inv_freq, scale) for :func:`rotary_embedding`: inv_freq[i] = base^(-2i / rotary_dim) as float32
+    [rotary_dim / 2] on ``device``, computed in 64 bits, and the factor on the rotated elements.
+
+    ``scaling`` stretches a model trained on ``original_length`` positions by ``factor``:
+      None      as trained, scale 1
+      "linear"  every frequency divided by factor, scale 1
+      "ntk"     base multiplied by factor^(rotary_dim / (rotary_dim - 2)) (the slowest frequency is divided by factor,
+                the fastest kept), scale 1
+      "yarn"    frequencies that turn more than beta_fast times in original_length kept, those that turn less than
+                beta_slow times divided by factor, a linear ramp over i between; scale 0.1 ln(factor) + 1"""
+    if rotary_dim < 2 or rotary_dim % 2:
+        raise ValueError(f"rotary_dim must be even and at least 2, got {rotary_dim}")
+    if not (base > 0 and math.isfinite(base)):
+        raise ValueError("base must be positive and finite")
+    if scaling not in (None, "linear", "ntk", "yarn"):
+        raise ValueError(f"unknown scaling {scaling!r}: None, 'linear', 'ntk' or 'yarn'")
+    if scaling is not None and not (factor >= 1 and math.isfinite(factor)):
+        raise ValueError("factor must be at least 1 and finite")
+    i = torch.arange(0, rotary_dim, 2, dtype=torch.float64) / rotary_dim
+    scale = 1.0
+    if scaling == "ntk":
+        if rotary_dim < 4:
+            raise ValueError("'ntk' scaling needs rotary_dim of at least 4")
+        base = base * factor ** (rotary_dim / (rotary_dim - 2))
+    inv_freq = base ** -i
+    if scaling == "linear":
+        inv_freq = inv_freq / factor
+    elif scaling == "yarn":
+        if original_length < 1 or not beta_fast > beta_slow > 0:
+            raise ValueError("'yarn' scaling needs original_length >= 1 and beta_fast > beta_slow > 0")
+        if base <= 1:
+            raise ValueError("'yarn' scaling needs a base above 1")
+
+        def index_of(turns):  # the (fractional) pair that turns this often in original_length positions
+            return rotary_dim * math.log(original_length / (turns * 2 * math.pi)) / (2 * math.log(base))
+
+        lo = max(math.floor(index_of(beta_fast)), 0)
+        hi = min(math.ceil(index_of(beta_slow)), rotary_dim - 1)
+        ramp = ((torch.arange(rotary_dim // 2, dtype=torch.float64) - lo) / max(hi - lo, 1e-3)).clamp(0, 1)
+        inv_freq = inv_freq * (1 - ramp) + inv_freq / factor * ramp
+        scale = 0.1 * math.log(factor) + 1.0
+    return inv_freq.to(torch.float32).to(device if device is not None else "cpu"), scale
+
+
+def rotary_embedding(Q: torch.Tensor, K: Optional[torch.Tensor], positions: torch.Tensor, inv_freq: torch.Tensor,
+                     interleaved: bool = False, scale: float = 1.0):
+    """Rotary positions of Q [tokens, heads, dim] and K [tokens, kv_heads, dim] (K may be None) in one launch; returns
+    new contiguous (Q', K'). fp16, bf16 or fp32; any strides with a unit inner stride are read in place.
+
+    Pair i of a head -- elements (i, i + r/2), or (2i, 2i+1) with ``interleaved`` -- turns by positions[t] * inv_freq[i]
+    and is multiplied by ``scale``; r = 2 * len(inv_freq), elements from r on are copied unchanged (and unscaled).
+    positions: int32 or int64 [tokens], any value (angles are reduced in 64 bits); inv_freq: float32 (see
+    :func:`rotary_frequencies`). Differentiable in Q and K."""
+    if torch.is_grad_enabled():
+        if inv_freq.requires_grad:
+            raise ValueError("rotary_embedding has no gradient for inv_freq")
+        if Q.requires_grad or (K is not None and K.requires_grad):
+            return _Rotary.apply(Q, K, positions, inv_freq, bool(interleaved), float(scale))
+    return _C().rotary(Q, K, positions, inv_freq, interleaved, scale, False)
+
+
+class _Rotary(torch.autograd.Function):
+    """Autograd for rotary positions: the gradient of a turn is the turn back."""
+
+    @staticmethod
+    def forward(ctx, Q, K, positions, inv_freq, interleaved, scale):
+        ctx.save_for_backward(positions, inv_freq)
+        ctx.interleaved, ctx.scale = interleaved, scale
+        ctx.set_materialize_grads(False)
+        return _C().rotary(Q, K, positions, inv_freq, interleaved, scale, False)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dQ, dK):
+        positions, inv_freq = ctx.saved_tensors
+        need_q = ctx.needs_input_grad[0] and dQ is not None
+        need_k = ctx.needs_input_grad[1] and dK is not None
+        if not need_q and not need_k:
+            return None, None, None, None, None, None
+        first, second = (dQ, dK if need_k else None) if need_q else (dK, None)
+        a, b = _C().rotary(first, second, positions, inv_freq, ctx.interleaved, ctx.scale, True)
+        return (a, b, None, None, None, None) if need_q else (None, a, None, None, None, None)
+
+
+# ----------------------------------------------------------------------------------------- paged key/value cache
+def kv_cache_append(K: torch.Tensor, V: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, slots: torch.Tensor,
+                    k_scale: Optional[torch.Tensor] = None, v_scale: Optional[torch.Tensor] = None) -> None:
+    """Write rows K, V [tokens, kv_heads, dim] (fp16 / bf16, dim 64 or 128) to the slots of a paged cache, in place.
+
+    k_cache, v_cache: contiguous [pages, page size, kv_heads, dim] of K's dtype, or float8_e4m3fn with k_scale, v_scale
+    float32 [pages, page size, kv_heads]: then each row is quantised as it is written (scale = max|x| / 448, code =
+    e4m3(x / scale); :func:`quantize_e4m3` per row). slots: int32 or int64 [tokens], page * page_size + offset, no slot
+    twice in a call; a negative slot marks padding and is skipped. A slot behind the cache is skipped and reported by
+    :func:`synchronize_and_check`. No gradient flows into a cache."""
+    _C().kv_cache_append(K, V, k_cache, v_cache, slots, k_scale, v_scale)
+
+
+def kv_cache_gather(k_cache: torch.Tensor, v_cache: torch.Tensor, slots: torch.Tensor,
+                    dtype: torch.dtype = torch.bfloat16, k_scale: Optional[torch.Tensor] = None,
+                    v_scale: Optional[torch.Tensor] = None):
+    """Read rows back from a paged cache (layout and slots as in :func:`kv_cache_append`; a slot may occur more than
+    once): (K, V) contiguous [tokens, kv_heads, dim] in ``dtype`` (float16 or bfloat16; the caches' own unless they hold
+    e4m3 codes, which are multiplied by their scales and rounded once). Negative slots read as zeros."""
+    if dtype not in (torch.float16, torch.bfloat16):
+        raise ValueError("kv_cache_gather: dtype must be torch.float16 or torch.bfloat16")
+    return _C().kv_cache_gather(k_cache, v_cache, slots, dtype == torch.float16, k_scale, v_scale)
+
+
+# ----------------------------------------------------------------------------------------- packed and paged attention
+def attention_paged(Q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
+                    kv_lens: torch.Tensor, cu_seqlens: torch.Tensor, scale: Optional[float] = None,
+                    k_scale: Optional[torch.Tensor] = None, v_scale: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Causal attention of each sequence's new tokens (one or many) over its cached tokens; returns O like Q.
+
+    Q: [tokens, heads, dim] (fp16 / bf16, dim 64 or 128), the new tokens of all sequences packed: sequence i owns rows
+    cu_seqlens[i] .. cu_seqlens[i+1]. Its keys are its first kv_lens[i] cached tokens, the new tokens' own among them
+    (:func:`kv_cache_append` first); new token t sees positions <= kv_lens[i] - n_i + t. heads is a multiple of the
+    caches' kv_heads: query head h reads kv head h // (heads / kv_heads).
+    block_table [batch, width]: page numbers, position p in page block_table[i, p // page_size]; caches and scales as in
+    :func:`kv_cache_append`, page size a power of two from 8 to 1024. Index tensors are int32 (int64 is narrowed).
+    A row that sees no key is zero, and so are rows behind the last sequence. Inference only (no gradient)."""
+    if scale is None:
+        scale = Q.shape[-1] ** -0.5 if Q.dim() and Q.shape[-1] else 1.0
+    return _C().attention_paged(Q, k_cache, v_cache, block_table, kv_lens, cu_seqlens, scale, k_scale, v_scale)
+
+
+def attention_varlen(Q: torch.Tensor, K: torch.Tensor, V: torch.Tensor, cu_seqlens: torch.Tensor,
+                     scale: Optional[float] = None, causal: bool = True) -> torch.Tensor:
+    """Attention over packed sequences of different lengths (each within itself, causal by default); returns O like Q.
+
+    Q [tokens, heads, dim], K and V [tokens, kv_heads, dim] (fp16 / bf16, dim 64 or 128, heads a multiple of kv_heads:
+    query head h reads kv head h // (heads / kv_heads)); sequence i owns rows cu_seqlens[i] .. cu_seqlens[i+1]
+    (int32 [batch + 1], starting at 0; any lengths, zero included). Rows behind the last sequence are zero.
+    Differentiable in Q, K and V (deterministic, no atomics)."""
+    if scale is None:
+        scale = Q.shape[-1] ** -0.5 if Q.dim() and Q.shape[-1] else 1.0
+    if torch.is_grad_enabled() and (Q.requires_grad or K.requires_grad or V.requires_grad):
+        return _VarlenAttention.apply(Q, K, V, cu_seqlens, float(scale), bool(causal))
+    return _C().attention_varlen_fwd(Q, K, V, cu_seqlens, scale, causal, False)[0]
+
+
+class _VarlenAttention(torch.autograd.Function):
+    """Autograd for packed attention: the forward keeps the row log-sum-exp, the backward recomputes the scores."""
+
+    @staticmethod
+    def forward(ctx, Q, K, V, cu_seqlens, scale, causal):
+        O, lse = _C().attention_varlen_fwd(Q, K, V, cu_seqlens, scale, causal, True)
+        ctx.save_for_backward(Q, K, V, O, lse, cu_seqlens)
+        ctx.scale, ctx.causal = scale, causal
+        return O
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dO):
+        Q, K, V, O, lse, cu_seqlens = ctx.saved_tensors
+        dQ, dK, dV = _C().attention_varlen_bwd(dO.to(Q.dtype), Q, K, V, O, lse, cu_seqlens, ctx.scale, ctx.causal)
+        need = ctx.needs_input_grad
+        return dQ if need[0] else None, dK if need[1] else None, dV if need[2] else None, None, None, None
 
 
 def synchronize_and_check() -> None:

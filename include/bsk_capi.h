@@ -394,13 +394,17 @@ int bsk_kv_cache_gather(int dtype, const void* k_cache, const void* v_cache, int
  *   cu_seqlens int32 [batch + 1], cu_seqlens[0] = 0, non-decreasing, at most `tokens`; kv_lens int32 [batch],
  *   at most table_width * page_size; entries outside their range are clamped, a page outside [0, num_pages) reads as
  *   zeros, and either sets the device error word.
+ *   workspace: device memory of bsk_attention_paged_workspace_bytes(...) bytes (may be 0), 16-byte aligned, not shared
+ *   by calls that may run at the same time.
  * No reference counterpart.
  */
 int bsk_attention_paged(int dtype, const void* Q, int64_t q_token_stride, int64_t q_head_stride, const void* k_cache,
                         const void* v_cache, int cache_e4m3, const float* k_scale, const float* v_scale,
                         const int32_t* block_table, int64_t table_stride, int table_width, const int32_t* kv_lens,
                         const int32_t* cu_seqlens, void* O, int tokens, int batch, int heads, int kv_heads, int dim,
-                        int num_pages, int page_size, float scale, void* stream);
+                        int num_pages, int page_size, float scale, void* workspace, int64_t workspace_bytes, void* stream);
+int64_t bsk_attention_paged_workspace_bytes(int tokens, int batch, int heads, int kv_heads, int dim, int cache_e4m3,
+                                            int num_pages);
 
 /*
  * Attention over packed sequences of different lengths, heads grouped over kv heads (types, dims and cu_seqlens as in

@@ -353,13 +353,19 @@ torch::Tensor attention_paged(torch::Tensor Q, torch::Tensor k_cache, torch::Ten
                     ": block_table [batch, width], kv_lens [batch] and cu_seqlens [batch + 1] differ in the batch");
   const Rows q = as_rows(Q);
   auto O = torch::empty({Q.size(0), Q.size(1), Q.size(2)}, Q.options());
+  const int64_t need = bsk_attention_paged_workspace_bytes(
+      narrow(Q.size(0), op, "tokens"), narrow(lens.size(0), op, "batch"), static_cast<int>(Q.size(1)),
+      static_cast<int>(k_cache.size(2)), static_cast<int>(Q.size(2)), e4m3, narrow(k_cache.size(0), op, "pages"));
+  TORCH_CHECK(need >= 0, "bsk_attention_paged_workspace_bytes failed: ", bsk_last_error());
+  torch::Tensor ws;
+  if (need > 0) ws = torch::empty({need}, Q.options().dtype(torch::kUInt8));
   check_rc(bsk_attention_paged(code, q.p(), q.ts, q.hs, k_cache.data_ptr(), v_cache.data_ptr(), e4m3, scale_ptr(k_scale),
                                scale_ptr(v_scale), table.data_ptr<int32_t>(), table.size(1),
                                narrow(table.size(1), op, "table width"), lens.data_ptr<int32_t>(), cu.data_ptr<int32_t>(),
                                O.data_ptr(), narrow(Q.size(0), op, "tokens"), narrow(lens.size(0), op, "batch"),
                                static_cast<int>(Q.size(1)), static_cast<int>(k_cache.size(2)), static_cast<int>(Q.size(2)),
                                narrow(k_cache.size(0), op, "pages"), static_cast<int>(page), static_cast<float>(scale),
-                               stream_of(Q)),
+                               need > 0 ? ws.data_ptr() : nullptr, need, stream_of(Q)),
            "bsk_attention_paged");
   return O;
 }

@@ -24,6 +24,7 @@
 #include "kv_cache.cuh"
 #include "paged_decode_sm100.cuh"
 #include "varlen_simple.cuh"
+#include "varattn_sm100.cuh"
 
 namespace {
 
@@ -175,6 +176,14 @@ void init_device(DeviceState& st, int dev) {
       allow_paged<false, 128, false>(), allow_paged<false, 128, true>(), allow_paged<false, 64, false>(),
       allow_paged<false, 64, true>(),   allow_paged<true, 128, false>(), allow_paged<true, 128, true>(),
       allow_paged<true, 64, false>(),   allow_paged<true, 64, true>(),
+      allow_smem(varattn_fwd_kernel<false, 128, false>, AttnShape<false, 128>::kSmemBytes),
+      allow_smem(varattn_fwd_kernel<false, 64, false>, AttnShape<false, 64>::kSmemBytes),
+      allow_smem(varattn_fwd_kernel<true, 128, false>, AttnShape<true, 128>::kSmemBytes),
+      allow_smem(varattn_fwd_kernel<true, 64, false>, AttnShape<true, 64>::kSmemBytes),
+      allow_smem(varattn_fwd_kernel<false, 128, true>, AttnShape<false, 128>::kSmemBytes),
+      allow_smem(varattn_fwd_kernel<false, 64, true>, AttnShape<false, 64>::kSmemBytes),
+      allow_smem(varattn_fwd_kernel<true, 128, true>, AttnShape<true, 128>::kSmemBytes),
+      allow_smem(varattn_fwd_kernel<true, 64, true>, AttnShape<true, 64>::kSmemBytes),
   };
   for (cudaError_t x : errs) {
     if (x != cudaSuccess) {
@@ -276,6 +285,42 @@ int make_map(CUtensorMap* m, CUtensorMapDataType dt, int elem_bytes, const void*
   cuuint32_t estr[2] = {1, 1};
   CUresult r = enc(m, dt, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                    CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return set_error(BSK_ERR_INVALID_ARG, "%s: cuTensorMapEncodeTiled failed (%d)", what, (int)r);
+  return BSK_OK;
+}
+
+// Tensor map of rows at two strides, [outer][mid][inner] 16-bit elements, boxes of 64 x box_mid x box_outer with 128-B
+// swizzle (a box's rows land one after another, mid fastest).
+int make_map3(CUtensorMap* m, bool f16, const void* base, uint64_t inner, uint64_t mid, uint64_t outer,
+              uint64_t mid_stride_bytes, uint64_t outer_stride_bytes, uint32_t box_mid, uint32_t box_outer,
+              const char* what) {
+  PFN_cuTensorMapEncodeTiled_v12000 enc;
+  if (int rc = encoder(&enc)) return rc;
+  cuuint64_t dims[3] = {inner, mid, outer};
+  cuuint64_t strides[2] = {mid_stride_bytes, outer_stride_bytes};
+  cuuint32_t box[3] = {64, box_mid, box_outer};
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = enc(m, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base),
+                   dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return set_error(BSK_ERR_INVALID_ARG, "%s: cuTensorMapEncodeTiled failed (%d)", what, (int)r);
+  return BSK_OK;
+}
+
+// Tensor map of one operand of a paged cache [rows = pages x page size][kv_heads][dim] (16-bit): boxes of box_rows rows of
+// one head as [8-row groups][64-column chunks][8 rows][64 columns], 128-B swizzle. Row coordinates in groups of 8.
+int make_map_paged(CUtensorMap* m, bool f16, const void* base, uint64_t dim, uint64_t kv_heads, uint64_t rows,
+                   uint32_t box_rows, const char* what) {
+  PFN_cuTensorMapEncodeTiled_v12000 enc;
+  if (int rc = encoder(&enc)) return rc;
+  const uint64_t row_bytes = kv_heads * dim * 2;
+  cuuint64_t dims[5] = {64, 8, dim / 64, rows / 8, kv_heads};
+  cuuint64_t strides[4] = {row_bytes, 128, 8 * row_bytes, dim * 2};
+  cuuint32_t box[5] = {64, 8, (cuuint32_t)(dim / 64), box_rows / 8, 1};
+  cuuint32_t estr[5] = {1, 1, 1, 1, 1};
+  CUresult r = enc(m, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5, const_cast<void*>(base),
+                   dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return set_error(BSK_ERR_INVALID_ARG, "%s: cuTensorMapEncodeTiled failed (%d)", what, (int)r);
   return BSK_OK;
 }
@@ -2057,6 +2102,29 @@ int heads_checks(const char* what, int dtype, int tokens, int batch, int heads, 
   return BSK_OK;
 }
 
+// Workspace of a work list: the entry count (16 bytes), then its entries.
+int64_t plan_bytes(int64_t tokens, int64_t batch, int64_t tt) {
+  return 16 + bsk::plan_slots(tokens, batch, tt) * (int64_t)sizeof(bsk::VarItem);
+}
+
+bool plan_fits(int64_t tokens, int64_t batch, int64_t tt, int64_t kv_heads) {
+  return bsk::plan_slots(tokens, batch, tt) * kv_heads < (int64_t)1 << 31;
+}
+
+void plan_launch(bsk::PlanArgs a, void* ws, const DeviceState& st, cudaStream_t s) {
+  a.count = static_cast<int*>(ws);
+  a.items = reinterpret_cast<bsk::VarItem*>(static_cast<char*>(ws) + 16);
+  a.err = st.err_word;
+  bsk::varattn_plan_kernel<<<1, bsk::kPlanThreads, 0, s>>>(a);
+}
+
+template <bool kF16, int kD, bool kPaged>
+void varattn_fwd_launch(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const bsk::VarFwdArgs& a,
+                        unsigned grid, cudaStream_t s) {
+  bsk::varattn_fwd_kernel<kF16, kD, kPaged>
+      <<<grid, bsk::kAttnThreads, bsk::AttnShape<kF16, kD>::kSmemBytes, s>>>(tq, tk, tv, a);
+}
+
 template <bool kF16, int kD, bool kFp8>
 cudaError_t paged_decode_launch(const bsk::PagedArgs& a, unsigned tiles, int cluster, cudaStream_t s) {
   cudaLaunchConfig_t cfg = {};
@@ -2075,13 +2143,31 @@ cudaError_t paged_decode_launch(const bsk::PagedArgs& a, unsigned tiles, int clu
 
 }  // namespace
 
+namespace {
+
+// Which kernel takes a paged call: the 128-row tcgen05 tiles when the sequences bring 64 rows (new tokens x heads of a
+// group) or more on average, the 16-row mma.sync tiles below that and for e4m3 caches.
+bool paged_in_tiles(int64_t tokens, int64_t batch, int64_t group, bool e4m3, int64_t num_pages) {
+  return !e4m3 && num_pages > 0 && batch > 0 && tokens * group >= 64 * batch;
+}
+
+}  // namespace
+
 extern "C" {
+
+int64_t bsk_attention_paged_workspace_bytes(int tokens, int batch, int heads, int kv_heads, int dim, int cache_e4m3,
+                                            int num_pages) {
+  if (int rc = heads_checks("attention_paged_workspace_bytes", 0, tokens, batch, heads, kv_heads, dim, 1.0f)) return rc;
+  const int group = heads / kv_heads;
+  if (!paged_in_tiles(tokens, batch, group, cache_e4m3 != 0, num_pages)) return 0;
+  return plan_bytes(tokens, batch, bsk::kVarBlk / group);
+}
 
 int bsk_attention_paged(int dtype, const void* Q, int64_t q_token_stride, int64_t q_head_stride, const void* k_cache,
                         const void* v_cache, int cache_e4m3, const float* k_scale, const float* v_scale,
                         const int32_t* block_table, int64_t table_stride, int table_width, const int32_t* kv_lens,
                         const int32_t* cu_seqlens, void* O, int tokens, int batch, int heads, int kv_heads, int dim,
-                        int num_pages, int page_size, float scale, void* stream) {
+                        int num_pages, int page_size, float scale, void* workspace, int64_t workspace_bytes, void* stream) {
   const char* what = "attention_paged";
   if (int rc = heads_checks(what, dtype, tokens, batch, heads, kv_heads, dim, scale)) return rc;
   if (page_size < 8 || page_size > 1024 || (page_size & (page_size - 1)))
@@ -2121,6 +2207,51 @@ int bsk_attention_paged(int dtype, const void* Q, int64_t q_token_stride, int64_
   a.scale_log2 = scale * 1.4426950408889634f;
   a.err = st->err_word;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (paged_in_tiles(tokens, batch, a.group, cache_e4m3 != 0, num_pages)) {
+    const int tt = bsk::kVarBlk / a.group;
+    const int64_t need = plan_bytes(tokens, batch, tt);
+    if (workspace_bytes < need || !workspace || !aligned16(workspace))
+      return set_error(BSK_ERR_INVALID_ARG, "%s: 16-byte aligned workspace of %lld bytes needed", what, (long long)need);
+    if (!plan_fits(tokens, batch, tt, kv_heads)) return set_error(BSK_ERR_UNSUPPORTED, "%s: too many rows", what);
+    const bool f16 = dtype == 1;
+    const uint64_t rows = (uint64_t)num_pages * page_size;
+    const uint32_t box = page_size < bsk::kVarBlk ? page_size : bsk::kVarBlk;
+    CUtensorMap tq, tk, tv;
+    if (int rc = make_map3(&tq, f16, Q, dim, heads, tokens, q_head_stride * 2, q_token_stride * 2, a.group, tt, "Q")) return rc;
+    if (int rc = make_map_paged(&tk, f16, k_cache, dim, kv_heads, rows, box, "k_cache")) return rc;
+    if (int rc = make_map_paged(&tv, f16, v_cache, dim, kv_heads, rows, box, "v_cache")) return rc;
+    bsk::PlanArgs p{};
+    p.cu = cu_seqlens;
+    p.kv_lens = kv_lens;
+    p.kv_room = (int64_t)table_width * page_size;
+    p.tokens = tokens;
+    p.batch = batch;
+    p.tt = tt;
+    p.causal = 1;
+    plan_launch(p, workspace, *st, s);
+    bsk::VarFwdArgs f{};
+    f.O = O;
+    f.count = static_cast<const int*>(workspace);
+    f.items = reinterpret_cast<const bsk::VarItem*>(static_cast<const char*>(workspace) + 16);
+    f.table = block_table;
+    f.table_stride = table_stride;
+    f.page_shift = a.page_shift;
+    f.num_pages = num_pages;
+    f.heads = heads;
+    f.kv_heads = kv_heads;
+    f.group = a.group;
+    f.causal = 1;
+    f.scale_log2 = a.scale_log2;
+    f.err = st->err_word;
+    f.timeout_ns = t_timeout_ns;
+    const int64_t most = bsk::plan_slots(tokens, batch, tt) * kv_heads;
+    const unsigned grid = (unsigned)(most < st->sm_count ? most : st->sm_count);
+    if (f16 && dim == 128) varattn_fwd_launch<true, 128, true>(tq, tk, tv, f, grid, s);
+    else if (f16) varattn_fwd_launch<true, 64, true>(tq, tk, tv, f, grid, s);
+    else if (dim == 128) varattn_fwd_launch<false, 128, true>(tq, tk, tv, f, grid, s);
+    else varattn_fwd_launch<false, 64, true>(tq, tk, tv, f, grid, s);
+    return launch_status("attention_paged launch");
+  }
   const int64_t tiles = (int64_t)tokens * a.group / bsk::kPagedRows + batch + 1;
   // CTAs per tile: doubled while the GPU's slots (2 CTAs per SM) are filled fewer than four times and each CTA keeps at
   // least 128 keys of the longest sequence that the table can hold.
@@ -2139,7 +2270,7 @@ int bsk_attention_paged(int dtype, const void* Q, int64_t q_token_stride, int64_
 int64_t bsk_attention_varlen_workspace_bytes(int tokens, int batch, int heads, int kv_heads, int dim, int backward) {
   if (int rc = heads_checks("attention_varlen_workspace_bytes", 0, tokens, batch, heads, kv_heads, dim, 1.0f)) return rc;
   (void)backward;
-  return 0;
+  return plan_bytes(tokens, batch, bsk::kVarBlk / (heads / kv_heads));
 }
 
 int bsk_attention_varlen_fwd(int dtype, const void* Q, int64_t q_token_stride, int64_t q_head_stride, const void* K,
@@ -2159,21 +2290,39 @@ int bsk_attention_varlen_fwd(int dtype, const void* Q, int64_t q_token_stride, i
       !rows_aligned(V, v_token_stride, v_head_stride, 2) || !aligned16(O) || !aligned16(workspace))
     return set_error(BSK_ERR_INVALID_ARG, "%s: rows of Q, K, V and O must be 16-byte aligned", what);
   if (int rc = device_state(&st)) return rc;
-  bsk::VarlenArgs a{};
-  a.Q = Q; a.K = K; a.V = V; a.O = O; a.lse = lse; a.cu = cu_seqlens;
-  a.q_ts = q_token_stride; a.q_hs = q_head_stride;
-  a.k_ts = k_token_stride; a.k_hs = k_head_stride;
-  a.v_ts = v_token_stride; a.v_hs = v_head_stride;
-  a.tokens = tokens; a.batch = batch; a.heads = heads; a.kv_heads = kv_heads; a.group = heads / kv_heads;
-  a.causal = causal;
-  a.scale = scale;
-  a.err = st->err_word;
+  const int group = heads / kv_heads, tt = bsk::kVarBlk / group;
+  if (!plan_fits(tokens, batch, tt, kv_heads)) return set_error(BSK_ERR_UNSUPPORTED, "%s: too many rows", what);
+  const bool f16 = dtype == 1;
+  CUtensorMap tq, tk, tv;
+  if (int rc = make_map3(&tq, f16, Q, dim, heads, tokens, q_head_stride * 2, q_token_stride * 2, group, tt, "Q")) return rc;
+  if (int rc = make_map3(&tk, f16, K, dim, kv_heads, tokens, k_head_stride * 2, k_token_stride * 2, 1, bsk::kVarBlk, "K")) return rc;
+  if (int rc = make_map3(&tv, f16, V, dim, kv_heads, tokens, v_head_stride * 2, v_token_stride * 2, 1, bsk::kVarBlk, "V")) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const unsigned grid = (unsigned)(((int64_t)tokens * heads + 3) / 4);
-  if (dtype == 1 && dim == 128) bsk::varlen_simple_kernel<true, 128, 0><<<grid, 128, 0, s>>>(a);
-  else if (dtype == 1) bsk::varlen_simple_kernel<true, 64, 0><<<grid, 128, 0, s>>>(a);
-  else if (dim == 128) bsk::varlen_simple_kernel<false, 128, 0><<<grid, 128, 0, s>>>(a);
-  else bsk::varlen_simple_kernel<false, 64, 0><<<grid, 128, 0, s>>>(a);
+  bsk::PlanArgs p{};
+  p.cu = cu_seqlens;
+  p.tokens = tokens;
+  p.batch = batch;
+  p.tt = tt;
+  p.causal = causal != 0;
+  plan_launch(p, workspace, *st, s);
+  bsk::VarFwdArgs f{};
+  f.O = O;
+  f.lse = lse;
+  f.count = static_cast<const int*>(workspace);
+  f.items = reinterpret_cast<const bsk::VarItem*>(static_cast<const char*>(workspace) + 16);
+  f.heads = heads;
+  f.kv_heads = kv_heads;
+  f.group = group;
+  f.causal = causal != 0;
+  f.scale_log2 = scale * 1.4426950408889634f;
+  f.err = st->err_word;
+  f.timeout_ns = t_timeout_ns;
+  const int64_t most = bsk::plan_slots(tokens, batch, tt) * kv_heads;
+  const unsigned grid = (unsigned)(most < st->sm_count ? most : st->sm_count);
+  if (f16 && dim == 128) varattn_fwd_launch<true, 128, false>(tq, tk, tv, f, grid, s);
+  else if (f16) varattn_fwd_launch<true, 64, false>(tq, tk, tv, f, grid, s);
+  else if (dim == 128) varattn_fwd_launch<false, 128, false>(tq, tk, tv, f, grid, s);
+  else varattn_fwd_launch<false, 64, false>(tq, tk, tv, f, grid, s);
   return launch_status("attention_varlen_fwd launch");
 }
 

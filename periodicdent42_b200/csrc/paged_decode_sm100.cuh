@@ -523,7 +523,7 @@ __global__ void __launch_bounds__(kPagedThreads) paged_decode_kernel(const Paged
       a0 += remote(cta_s + 4 * i, r) * f;
       a1 += remote(cta_s + 4 * i + 4, r) * f;
     }
-    const float inv = l > 0.0f ? 1.0f / l : 0.0f;  // a row without keys is zero
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // a row without keys is zero
     const int64_t t = lo + (row0 + row) / a.group;
     const int h = hkv * a.group + static_cast<int>((row0 + row) % a.group);
     *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.O) + (t * a.heads + h) * kD + col) = pack2<kF16>(a0 * inv, a1 * inv);

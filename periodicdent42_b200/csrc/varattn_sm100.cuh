@@ -1,0 +1,567 @@
+// Attention over packed sequences, or of chunks of new tokens over a paged cache, for sm_100a (fp16 / bf16, head dim 64 or
+// 128, grouped heads): forward, tcgen05.
+//
+// Work item = a tile of query rows -- TT = 128 / group tokens x the group's heads, so that the 128 rows of the tensor core's
+// tile all use the same keys -- and its key blocks [b0, b1) of 128 keys (varattn_plan.cuh). For every key block
+//     S_j = Q K_j^T                 tcgen05.mma 128x128x16 x (D/16) into TMEM S buffer j % 2
+//     P_j = exp2(S_j * c - m)       online softmax, 16-bit P written back into the S buffer
+//     O  += P_j V_j                 tcgen05.mma with A = P from TMEM, V an MN-major shared-memory operand
+// and O / l (and the log-sum-exp) at the end. The CTA's shape and its softmax are those of the block-sparse forward
+// (bsattn_sm100.cuh, where they are explained and measured): warp 0 TMA producer, warps 1 and 2 issue S and PV, warps 4-11
+// softmax (two warps per row quarter, each half of the keys), warps 12-15 output. What differs:
+//   - Q tiles come as 3-D boxes (64 columns x group heads x TT tokens) from any token / head stride, K and V tiles as boxes
+//     of one head x 128 tokens, or, paged, as one 5-D box per page: a copy costs about 70 ns of the CTA's one copy engine
+//     whatever its size, and pages of 16 rows need 16 of them per key block (2048 new tokens over 16384, 32 / 8 heads,
+//     D 128: 744 us; with one copy per 64-column chunk of a page 1000; pages of 32 rows 625, of 64 and more 610).
+//   - Keys that a row may not see are masked by position; only blocks that reach behind the tile's first row's limit
+//     compare. A row without any key keeps its maximum at -inf and is written as zero.
+//   - The last block of a sequence may hold foreign rows (the next sequence's, or stale page contents, NaN among them). Their
+//     scores are replaced, but P = 0 does not stop a NaN in V: warp 3 sets those V rows to zero in shared memory between the
+//     copy's arrival and the PV product (only such blocks take this detour).
+//
+// Bound: the tensor pipe and the softmax share the time (4 D flops and one exponential per score; see the forward's trace
+// in bsattn_sm100.cuh). Packing the group's heads into the tile means a causal tile spans only TT tokens, so less of its
+// last block is masked, and one K / V tile feeds the whole group.
+#pragma once
+
+#include "varattn_plan.cuh"
+
+namespace bsk {
+
+// Maxima that pass a NaN on (a NaN score has to reach the row's result).
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// Rows of a [128 x D] tile that no copy fills (128 is no multiple of the group): zeroed once by the whole CTA.
+__device__ __forceinline__ void zero_tile_rows(uint8_t* tile, int chunks, int first) {
+  for (int i = threadIdx.x; i < (kVarBlk - first) * chunks * 8; i += blockDim.x) {
+    const int r = first + i / (chunks * 8), c = i % (chunks * 8);
+    *reinterpret_cast<uint4*>(tile + (c >> 3) * kAttnChunk + r * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+  }
+}
+
+struct VarFwdArgs {
+  void* O;              // contiguous [tokens, heads, D]
+  float* lse;           // optional [tokens, heads], natural log
+  const VarItem* items;
+  const int* count;     // entries of `items`
+  const int* table;     // paged: block table
+  int64_t table_stride;
+  int page_shift, num_pages;
+  int heads, kv_heads, group, causal;
+  float scale_log2;
+  uint32_t* err;
+  uint64_t timeout_ns;
+};
+
+template <bool kF16, int kD, bool kPaged>
+__global__ void __launch_bounds__(kAttnThreads, 1)
+    varattn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+                       const __grid_constant__ CUtensorMap tmV, const VarFwdArgs a) {
+  using Sh = AttnShape<kF16, kD>;
+  constexpr int kTile = Sh::kTile;
+  constexpr int kHalfD = kD / 2;
+  // K / V tiles in shared memory: atoms of 8 rows x 128 bytes. Packed: a 64-column chunk's 16 atoms, then the next chunk's
+  // (one copy per chunk). Paged: the chunks of 8 rows together, so that one copy brings a whole page.
+  constexpr int kGroupPitch = kPaged ? 1024 * Sh::kChunks : 1024;  // from 8 rows to the next 8
+  constexpr int kChunkPitch = kPaged ? 1024 : kAttnChunk;          // from 64 columns to the next 64
+  constexpr uint32_t IDESC_S = ptx::instr_desc(128, 128, Sh::kFmt, Sh::kFmt, 0, 0);
+  constexpr uint32_t IDESC_PV = ptx::instr_desc(128, kD, Sh::kFmt, Sh::kFmt, 0, 1);
+
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sQ = smem;                      // [2] Q of alternate items
+  uint8_t* sKV = sQ + 2 * kTile;           // [kAttnKVSlots]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sKV + kAttnKVSlots * kTile);
+  uint64_t* q_full = bars + 0;                       // [2]
+  uint64_t* q_empty = bars + 2;                      // [2]
+  uint64_t* kv_full = bars + 4;                      // [kAttnKVSlots]
+  uint64_t* kv_empty = kv_full + kAttnKVSlots;       // [kAttnKVSlots]
+  uint64_t* raw_full = kv_empty + kAttnKVSlots;      // [kAttnKVSlots] a V tile with foreign rows has arrived
+  uint64_t* s_full = raw_full + kAttnKVSlots;        // [2]
+  uint64_t* s_free = s_full + 2;                     // [2]
+  uint64_t* p_full = s_free + 2;                     // [2]
+  uint64_t* o_done = p_full + 2;                     // [2]
+  uint64_t* xbar = o_done + 2;                       // [8]
+  uint64_t* drain = xbar + 8;                        // [2]
+  uint64_t* l_ready = drain + 2;
+  uint64_t* o_free = l_ready + 1;                    // [2]
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(o_free + 2);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
+  static_assert(4 + 3 * kAttnKVSlots + 2 + 2 + 2 + 2 + 8 + 2 + 1 + 2 <= 63, "barrier area exceeds its 512 bytes");
+  float* l_part = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(bars) + 512);  // [2 halves][128 rows]
+  float* m_row = l_part + 256;                                                       // [128 rows]
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const int group = a.group, tt = kVarBlk / group;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < 2; ++s) {
+      ptx::mbar_init(ptx::smem_u32(&q_full[s]), 1);
+      ptx::mbar_init(ptx::smem_u32(&q_empty[s]), 1);
+      ptx::mbar_init(ptx::smem_u32(&s_full[s]), 1);
+      ptx::mbar_init(ptx::smem_u32(&s_free[s]), 1);
+      ptx::mbar_init(ptx::smem_u32(&p_full[s]), 8);
+      ptx::mbar_init(ptx::smem_u32(&drain[s]), 1);
+      ptx::mbar_init(ptx::smem_u32(&o_done[s]), 1);
+      ptx::mbar_init(ptx::smem_u32(&o_free[s]), 4);
+    }
+    for (int s = 0; s < kAttnKVSlots; ++s) {
+      ptx::mbar_init(ptx::smem_u32(&kv_full[s]), 1);
+      ptx::mbar_init(ptx::smem_u32(&kv_empty[s]), 1);
+      ptx::mbar_init(ptx::smem_u32(&raw_full[s]), 1);
+    }
+    ptx::mbar_init(ptx::smem_u32(l_ready), 8);
+    for (int s = 0; s < 8; ++s) ptx::mbar_init(ptx::smem_u32(&xbar[s]), 2);
+    *abort_flag = 0;
+    ptx::fence_mbar_init();
+  }
+  if (tt * group < kVarBlk) {
+    for (int s = 0; s < 2; ++s) zero_tile_rows(sQ + s * kTile, Sh::kChunks, tt * group);
+    ptx::fence_proxy_async_smem();
+  }
+  if (warp == 0 && lane == 0) {
+    ptx::prefetch_tmap(&tmQ);
+    ptx::prefetch_tmap(&tmK);
+    ptx::prefetch_tmap(&tmV);
+  }
+  if (warp == 1) {
+    ptx::tmem_alloc(ptx::smem_u32(tmem_holder), kAttnTmemCols);
+    ptx::tmem_relinquish();
+  }
+  ptx::tc_fence_before();
+  __syncthreads();
+  ptx::tc_fence_after();
+  const uint32_t tmem_base = *tmem_holder;
+  WaitCtl ctl{abort_flag, a.err, a.timeout_ns, kKidVarAttn};
+  const int n_items = *a.count * a.kv_heads;  // (entry, kv head), heads innermost
+  const int cta = blockIdx.x, grid = gridDim.x;
+  // Item k of this CTA; false behind the list's end.
+  auto item_at = [&](int k, VarItem& it, int& hkv) -> bool {
+    const int i = zigzag(k, cta, grid, n_items);
+    if (i < 0) return false;
+    const int e = i / a.kv_heads;
+    hkv = i - e * a.kv_heads;
+    const int4* p = reinterpret_cast<const int4*>(a.items + e);
+    const int4 x = __ldg(p), y = __ldg(p + 1);
+    it = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+    return true;
+  };
+  // Keys of the sequence in the item's last block: below 128 its V tile holds foreign rows.
+  auto tail_rows = [](const VarItem& it) { return it.kv_len - (it.b1 - 1) * kVarBlk; };
+
+  static_assert(kAttnThreads == 512, "register split assumes 16 warps");
+  if (warp < 4) ptx::setmaxnreg_dec<kAttnRegsLow>();
+  if (warp >= 12) ptx::setmaxnreg_dec<kAttnRegsOut>();
+
+  if (warp == 0) {
+    // ------------------------------------------------------------------ TMA producer
+    // Packed: one thread. Paged: lane i copies the block's box i (a page, or 128 rows of a larger one); its table entry is
+    // read a block ahead, so the lookups cost neither latency nor a thread's turn per box (16 unrolled boxes in one thread
+    // took 4.4 us a block).
+    uint32_t slot = 0, slot_phase = 0, q_issued = 0, kv_issued = 0;
+    bool ok = true;
+    const uint32_t kv0 = ptx::smem_u32(sKV);
+    if (kPaged || lane == 0) {
+      const int page_rows = kPaged ? 1 << a.page_shift : 0;
+      const int box_rows = kPaged ? min(page_rows, kVarBlk) : kVarBlk;
+      const int pages_per_blk = kVarBlk / box_rows;
+      auto wait = [&](uint64_t* bar, uint32_t parity, uint32_t site) -> bool {
+        return kPaged ? warp_wait_bounded<false, 512>(ptx::smem_u32(bar), parity, ctl, site)
+                      : wait_bounded<false, 512>(ptx::smem_u32(bar), parity, ctl, site);
+      };
+      // Paged: this lane's table entry of key block b (-1: no box), and the first cache row it stands for; rows behind the
+      // cache (a bad page) read as zeros, boxes wholly behind the sequence's end are not copied.
+      auto entry = [&](const VarItem& it, int b) -> int {
+        const int key = b * kVarBlk + lane * box_rows;
+        return lane < pages_per_blk && key < it.kv_len ? __ldg(a.table + it.src * a.table_stride + (key >> a.page_shift)) : 0;
+      };
+      auto row_of = [&](const VarItem& it, int b, int page) -> int {
+        const int key = b * kVarBlk + lane * box_rows;
+        if (lane >= pages_per_blk || key >= it.kv_len) return -1;
+        if (page < 0 || page >= a.num_pages) {
+          atomicCAS(a.err, 0u, kErrBounds | (kKidVarAttn << 8) | (3u << 16));
+          return a.num_pages << a.page_shift;
+        }
+        return (page << a.page_shift) + (key & (page_rows - 1));
+      };
+      auto push = [&](const CUtensorMap* m, const VarItem& it, int hkv, int b, bool is_v, int row) -> bool {
+        if (!wait(&kv_empty[slot], slot_phase ^ 1, 2)) return false;
+        const bool foreign = is_v && b == it.b1 - 1 && tail_rows(it) < kVarBlk;
+        const uint32_t fb = ptx::smem_u32(foreign ? &raw_full[slot] : &kv_full[slot]);
+        const uint32_t dst = kv0 + slot * kTile + (kPaged ? lane * (box_rows >> 3) * kGroupPitch : 0);
+        if (lane == 0) {
+          const int boxes = kPaged ? min(pages_per_blk, (it.kv_len - b * kVarBlk + box_rows - 1) / box_rows) : 1;
+          ptx::mbar_arrive_expect_tx(fb, boxes * box_rows * kD * 2);
+        }
+        if constexpr (kPaged) {
+          __syncwarp();
+          if (row >= 0) ptx::tma_load_5d(dst, m, fb, 0, 0, 0, row >> 3, hkv);
+        } else {
+#pragma unroll
+          for (int c = 0; c < Sh::kChunks; ++c) ptx::tma_load_3d(dst + c * kAttnChunk, m, fb, 64 * c, hkv, row);
+        }
+        ++kv_issued;
+        if (++slot == kAttnKVSlots) { slot = 0; slot_phase ^= 1; }
+        return true;
+      };
+      VarItem it;
+      int hkv;
+      for (int k = 0; ok && item_at(k, it, hkv); ++k) {
+        if (it.b1 <= it.b0) continue;
+        int ahead = 0;
+        if constexpr (kPaged) ahead = entry(it, it.b0);
+        const uint32_t qbuf = q_issued & 1;
+        ok = wait(&q_empty[qbuf], ((q_issued >> 1) & 1) ^ 1, 1);
+        if (!ok) break;
+        if (lane == 0) {
+          const uint32_t qf = ptx::smem_u32(&q_full[qbuf]);
+          ptx::mbar_arrive_expect_tx(qf, tt * group * kD * 2);
+#pragma unroll
+          for (int c = 0; c < Sh::kChunks; ++c)
+            ptx::tma_load_3d(ptx::smem_u32(sQ) + qbuf * kTile + c * kAttnChunk, &tmQ, qf, 64 * c, hkv * group, it.row0);
+        }
+        ++q_issued;
+        int row = 0, prev = 0;
+        for (int b = it.b0; b < it.b1 && ok; ++b) {
+          if constexpr (kPaged) {
+            row = row_of(it, b, ahead);
+            if (b + 1 < it.b1) ahead = entry(it, b + 1);
+          } else {
+            row = it.src + b * kVarBlk;
+          }
+          ok = push(&tmK, it, hkv, b, false, row);
+          if (ok && b > it.b0) ok = push(&tmV, it, hkv, b - 1, true, prev);
+          prev = row;
+        }
+        if (ok) ok = push(&tmV, it, hkv, it.b1 - 1, true, prev);
+      }
+    }
+    if (lane == 0) {  // drain loads still in flight
+      WaitCtl dctl = ctl;
+      volatile int never = 0;
+      dctl.abort = &never;
+      for (uint32_t i = q_issued > 2 ? q_issued - 2 : 0; i < q_issued; ++i)
+        wait_bounded(ptx::smem_u32(&q_full[i & 1]), (i >> 1) & 1, dctl, 8);
+      const uint32_t first = kv_issued > kAttnKVSlots ? kv_issued - kAttnKVSlots : 0;
+      for (uint32_t i = first; i < kv_issued; ++i)
+        wait_bounded(ptx::smem_u32(&kv_full[i % kAttnKVSlots]), (i / kAttnKVSlots) & 1, dctl, 8);
+    }
+    __syncwarp();
+  } else if (warp == 1 || warp == 2) {
+    // ------------------------------------------------------------------ MMA issuers (one thread each)
+    if (lane == 0) {
+      const bool s_role = warp == 1;
+      uint32_t g = 0, rows = 0, seq = 0;  // blocks, items and ring positions passed
+      bool ok = true;
+      const uint32_t kv0 = ptx::smem_u32(sKV);
+      const uint64_t qdesc0 = ptx::smem_desc(ptx::smem_u32(sQ), 16, 1024);
+      const uint64_t kdesc0 = ptx::smem_desc(kv0, 16, kGroupPitch);           // K: K-major
+      const uint64_t vdesc0 = ptx::smem_desc(kv0, kChunkPitch, kGroupPitch);  // V: MN-major
+      VarItem it;
+      int hkv;
+      for (int k = 0; ok && item_at(k, it, hkv); ++k) {
+        const int n = it.b1 - it.b0;
+        if (n <= 0) continue;
+        const uint32_t qbuf = rows & 1;
+        if (s_role) {
+          ok = wait_bounded(ptx::smem_u32(&q_full[qbuf]), (rows >> 1) & 1, ctl, 14);
+          if (!ok) break;
+        }
+        for (int j = 0; j < n && ok; ++j, ++g) {
+          const uint32_t b = g & 1;
+          if (s_role) {
+            if (g >= 2) {  // PV_{g-2} read P from this buffer
+              ok = wait_bounded(ptx::smem_u32(&s_free[b]), ((g - 2) >> 1) & 1, ctl, 11);
+              if (!ok) break;
+            }
+            const uint32_t pos = seq + attn_k_pos(j);
+            const uint32_t sl = pos % kAttnKVSlots;
+            ok = wait_bounded(ptx::smem_u32(&kv_full[sl]), (pos / kAttnKVSlots) & 1, ctl, 12);
+            if (!ok) break;
+            ptx::tc_fence_after();
+            const uint64_t qd = qdesc0 + ((qbuf * kTile) >> 4), kd = kdesc0 + ((sl * kTile) >> 4);
+#pragma unroll
+            for (int x = 0; x < kD / 16; ++x) {
+              const uint32_t qo = ((x >> 2) * kAttnChunk + (x & 3) * 32) >> 4, ko = ((x >> 2) * kChunkPitch + (x & 3) * 32) >> 4;
+              ptx::mma_f16_ss(tmem_base + 128 * b, qd + qo, kd + ko, IDESC_S, x != 0);
+            }
+            ptx::mma_commit(ptx::smem_u32(&kv_empty[sl]));
+            ptx::mma_commit(ptx::smem_u32(&s_full[b]));
+            if (j == n - 1) ptx::mma_commit(ptx::smem_u32(&q_empty[qbuf]));
+          } else {
+            if (j == 0 && rows > 1) {  // the first PV of an item overwrites O buffer rows % 2
+              ok = wait_bounded(ptx::smem_u32(&o_free[rows & 1]), ((rows >> 1) - 1) & 1, ctl, 17);
+              if (!ok) break;
+            }
+            ok = wait_bounded(ptx::smem_u32(&p_full[b]), (g >> 1) & 1, ctl, 13);
+            if (!ok) break;
+            const uint32_t pos = seq + attn_v_pos(j, n);
+            const uint32_t sl = pos % kAttnKVSlots;
+            ok = wait_bounded(ptx::smem_u32(&kv_full[sl]), (pos / kAttnKVSlots) & 1, ctl, 15);
+            if (!ok) break;
+            ptx::tc_fence_after();
+            const uint64_t vd = vdesc0 + ((sl * kTile) >> 4);
+            const uint32_t t_o = tmem_base + kAttnTmemO + 128 * (rows & 1), t_p = tmem_base + 128 * b;
+#pragma unroll
+            for (int x = 0; x < 8; ++x)  // K step x: keys [16x, 16x+16) in P columns 8x (+32 for the second half)
+              ptx::mma_f16_ts(t_o, t_p + 8 * x + (x >= 4 ? 32 : 0), vd + ((2 * x * kGroupPitch) >> 4), IDESC_PV,
+                              (j == 0 && x == 0) ? 0u : 1u);
+            ptx::mma_commit(ptx::smem_u32(&kv_empty[sl]));
+            ptx::mma_commit(ptx::smem_u32(&s_free[b]));
+            if (j == n - 1) ptx::mma_commit(ptx::smem_u32(&o_done[rows & 1]));
+          }
+        }
+        seq += 2 * n;
+        ++rows;
+      }
+      const uint32_t dr = ptx::smem_u32(&drain[s_role ? 0 : 1]);
+      ptx::mma_commit(dr);
+      WaitCtl dctl = ctl;
+      volatile int never = 0;
+      dctl.abort = &never;
+      wait_bounded(dr, 0, dctl, 16);
+    }
+    __syncwarp();
+  } else if (warp == 3) {
+    // ------------------------------------------------------------------ foreign V rows -> zero
+    uint32_t seq = 0, phases = 0;  // ring positions passed; bit s: parity of raw_full[s]'s next completion
+    bool ok = true;
+    VarItem it;
+    int hkv;
+    for (int k = 0; ok && item_at(k, it, hkv); ++k) {
+      const int n = it.b1 - it.b0;
+      if (n <= 0) continue;
+      const int live = tail_rows(it);
+      if (live < kVarBlk) {
+        const uint32_t sl = (seq + 2 * n - 1) % kAttnKVSlots;  // the item's last V tile
+        ok = warp_wait_bounded<false, 256>(ptx::smem_u32(&raw_full[sl]), (phases >> sl) & 1, ctl, 30);
+        if (!ok) break;
+        phases ^= 1u << sl;
+        uint8_t* tile = sKV + sl * kTile;
+        constexpr int kPer = Sh::kChunks * 8;  // 16-byte pieces per row (a row's swizzle stays within its 128 bytes)
+        for (int i = lane; i < (kVarBlk - live) * kPer; i += 32) {
+          const int r = live + i / kPer, c = i % kPer;
+          *reinterpret_cast<uint4*>(tile + (r >> 3) * kGroupPitch + (c >> 3) * kChunkPitch + (r & 7) * 128 + (c & 7) * 16) =
+              make_uint4(0, 0, 0, 0);
+        }
+        ptx::fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&kv_full[sl]));
+      }
+      seq += 2 * n;
+    }
+  } else if (warp < 12) {
+    // ------------------------------------------------------------------ softmax (warps 4..11)
+    ptx::setmaxnreg_inc<kAttnRegsHigh>();
+    const int h = (warp - 4) >> 2;  // key half: S columns [64 h, 64 h + 64)
+    const int q = warp & 3;         // TMEM lane quarter
+    const int r = 32 * q + lane;    // row of the tile == TMEM lane
+    const int tok = r / group, hd = r - tok * group;  // its token and head
+    const uint32_t lane_off = static_cast<uint32_t>(32 * q) << 16;
+    const uint32_t tO0 = tmem_base + kAttnTmemO + lane_off + h * kHalfD;
+    const float c = a.scale_log2;
+    uint32_t g = 0, rows = 0, x_cnt = 0;
+    bool ok = true;
+    // Exchange with the warp of the other key half through the last column of each half of the S buffer.
+    auto exchange = [&](uint32_t tSb, float v, float& other) -> bool {
+      const uint32_t slot = x_cnt & 1;
+      ptx::tmem_st_32x32b_x1(tSb + 64 * h + 63, __float_as_uint(v));
+      ptx::tmem_wait_st();
+      ptx::tc_fence_before();
+      __syncwarp();
+      const uint32_t xb = ptx::smem_u32(&xbar[q * 2 + slot]);
+      if (lane == 0) ptx::mbar_arrive(xb);
+      if (!warp_wait_bounded(xb, (x_cnt >> 1) & 1, ctl, 23)) return false;
+      ++x_cnt;
+      ptx::tc_fence_after();
+      other = __uint_as_float(ptx::tmem_ld_32x32b_x1(tSb + 64 * (h ^ 1) + 63));
+      ptx::tmem_wait_ld();
+      return true;
+    };
+    VarItem next;
+    int next_h = 0;
+    bool more = item_at(0, next, next_h);
+    for (int k = 0; more && ok; ++k) {
+      const VarItem it = next;
+      const int hkv = next_h;
+      more = item_at(k + 1, next, next_h);  // looked up one item ahead
+      const int n = it.b1 - it.b0;
+      if (n <= 0) {
+        if (tok < it.ntok) {
+          const int64_t grow = static_cast<int64_t>(it.row0 + tok) * a.heads + hkv * group + hd;
+          uint4* orow = reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.O) + grow * kD + h * kHalfD);
+          const uint4 z = make_uint4(0, 0, 0, 0);
+#pragma unroll
+          for (int cc = 0; cc < kHalfD / 8; ++cc) orow[cc] = z;
+          if (a.lse && h == 0) a.lse[grow] = -INFINITY;
+        }
+        continue;
+      }
+      // keys at or behind `limit` are masked for this row; `clear`: key blocks below it are seen by every row of the tile
+      const int limit = a.causal ? it.pos0 + tok + 1 : it.kv_len;
+      const int clear = (a.causal ? it.pos0 + 1 : it.kv_len) >> 7;
+      float m_run = -INFINITY, l_run = 0.0f;
+      const uint32_t tO = tO0 + 128 * (rows & 1);
+      for (int j = 0; j < n; ++j, ++g) {
+        const int kb = it.b0 + j;
+        const uint32_t b = g & 1;
+        const uint32_t tS = tmem_base + 128 * b + lane_off;
+        ok = warp_wait_bounded(ptx::smem_u32(&s_full[b]), (g >> 1) & 1, ctl, 20);
+        if (!ok) break;
+        ptx::tc_fence_after();
+        uint32_t sv[64];
+        ptx::tmem_ld_32x32b_x32(tS + 64 * h, *reinterpret_cast<uint32_t(*)[32]>(&sv[0]));
+        ptx::tmem_ld_32x32b_x32(tS + 64 * h + 32, *reinterpret_cast<uint32_t(*)[32]>(&sv[32]));
+        ptx::tmem_wait_ld();
+        float* v = reinterpret_cast<float*>(sv);
+        if (kb >= clear) {
+          const int lim = limit - (kb * kVarBlk + 64 * h);
+#pragma unroll
+          for (int i = 0; i < 64; ++i)
+            if (i >= lim) v[i] = -INFINITY;
+        }
+        float pm[8];
+#pragma unroll
+        for (int x = 0; x < 8; ++x) pm[x] = v[x];
+#pragma unroll
+        for (int i = 8; i < 64; i += 16)
+#pragma unroll
+          for (int x = 0; x < 8; ++x)
+            pm[x] = i + 8 < 64 ? max3_nan(pm[x], v[i + x], v[(i + 8 + x) & 63]) : max_nan(pm[x], v[i + x]);
+        const float mh = max3_nan(max3_nan(pm[0], pm[1], pm[2]), max3_nan(pm[3], pm[4], pm[5]), max_nan(pm[6], pm[7]));
+        float mo;
+        ok = exchange(tS, mh, mo);
+        if (!ok) break;
+        const float mbs = max_nan(mh, mo) * c;
+        const bool move = !(mbs <= m_run + 8.0f);  // the reference maximum lags by at most 8: P <= 2^8; a NaN moves it
+        float alpha = 1.0f;
+        if (move) alpha = (m_run == -INFINITY) ? 0.0f : ex2_approx(m_run - mbs);
+        if (move) m_run = mbs;
+        const bool need_rescale = __any_sync(0xffffffffu, move && j > 0);
+        const float m_sub = (m_run == -INFINITY) ? 0.0f : m_run;
+        const uint64_t c2 = f2_pack(c, c), nm2 = f2_pack(-m_sub, -m_sub);
+        uint64_t acc[4] = {0ull, 0ull, 0ull, 0ull};
+#pragma unroll
+        for (int i = 0; i < 64; i += 2) {
+          float t0, t1, e0, e1;
+          f2_unpack(f2_fma(f2_pack(v[i], v[i + 1]), c2, nm2), t0, t1);
+          if (((i >> 1) & 7) >= 8 - kAttnPolyEighths) {
+            ex2_poly2(t0, t1, e0, e1);
+          } else {
+            e0 = ex2_approx(t0);
+            e1 = ex2_approx(t1);
+          }
+          acc[(i >> 1) & 3] = f2_add(acc[(i >> 1) & 3], f2_pack(e0, e1));
+          sv[i >> 1] = pack2<kF16>(e0, e1);
+        }
+        float rs;
+        {
+          const uint64_t a01 = f2_add(acc[0], acc[1]), a23 = f2_add(acc[2], acc[3]);
+          float lo, hi;
+          f2_unpack(f2_add(a01, a23), lo, hi);
+          rs = lo + hi;
+        }
+        l_run = l_run * alpha + rs;
+        if (need_rescale) {
+          ok = warp_wait_bounded(ptx::smem_u32(&s_free[(g - 1) & 1]), ((g - 1) >> 1) & 1, ctl, 21);
+          if (!ok) break;
+          ptx::tc_fence_after();
+          const float al = move ? alpha : 1.0f;
+#pragma unroll 1
+          for (int cc = 0; cc < kHalfD / 32; ++cc) {
+            uint32_t u[32];
+            ptx::tmem_ld_32x32b_x32(tO + cc * 32, u);
+            ptx::tmem_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) u[i] = __float_as_uint(__uint_as_float(u[i]) * al);
+            ptx::tmem_st_32x32b_x32(tO + cc * 32, u);
+          }
+        }
+        ptx::tmem_st_32x32b_x32(tS + 64 * h, *reinterpret_cast<uint32_t(*)[32]>(&sv[0]));
+        ptx::tmem_wait_st();
+        ptx::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&p_full[b]));
+      }
+      if (!ok) break;
+      if (rows > 0) {  // the output warps have read the previous item's sums
+        ok = warp_wait_bounded(ptx::smem_u32(&o_free[(rows - 1) & 1]), ((rows - 1) >> 1) & 1, ctl, 24);
+        if (!ok) break;
+      }
+      l_part[h * 128 + r] = l_run;
+      if (h == 0) m_row[r] = m_run;
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(l_ready));
+      ++rows;
+    }
+  } else {
+    // ------------------------------------------------------------------ output (warps 12..15)
+    const int q = warp & 3;
+    const int r = 32 * q + lane;
+    const int tok = r / group, hd = r - tok * group;
+    const uint32_t tO0 = tmem_base + kAttnTmemO + (static_cast<uint32_t>(32 * q) << 16);
+    const bool o_v8 = (reinterpret_cast<uintptr_t>(a.O) & 31) == 0;
+    uint32_t rows = 0;
+    bool ok = true;
+    VarItem it;
+    int hkv;
+    for (int k = 0; ok && item_at(k, it, hkv); ++k) {
+      if (it.b1 <= it.b0) continue;  // written by the softmax warps
+      ok = warp_wait_bounded<false, 256>(ptx::smem_u32(l_ready), rows & 1, ctl, 25);
+      if (ok) ok = warp_wait_bounded<false, 256>(ptx::smem_u32(&o_done[rows & 1]), (rows >> 1) & 1, ctl, 22);
+      if (!ok) break;
+      const uint32_t ob = rows & 1, tO = tO0 + 128 * ob;
+      ++rows;
+      ptx::tc_fence_after();
+      const float m_run = m_row[r];
+      const float l_tot = l_part[r] + l_part[128 + r];
+      const bool live = tok < it.ntok;
+      const int64_t grow = static_cast<int64_t>(it.row0 + tok) * a.heads + hkv * group + hd;
+      // A row without keys has its maximum at -inf (its sum may hold the exponentials' floor of 2^-125): zero. A maximum
+      // of +inf (scores beyond fp32) gives NaN, as the definition does.
+      const bool none = m_run == -INFINITY;
+      const float inv_l = m_run == INFINITY ? NAN : 1.0f / l_tot;
+      if (live && a.lse) a.lse[grow] = none ? -INFINITY : (m_run + log2f(l_tot)) * 0.6931471805599453f;
+      uint16_t* orow = static_cast<uint16_t*>(a.O) + grow * kD;
+#pragma unroll 1
+      for (int cc = 0; cc < kD / 32; ++cc) {
+        uint32_t u[32];
+        ptx::tmem_ld_32x32b_x32(tO + cc * 32, u);
+        ptx::tmem_wait_ld();
+        uint32_t pk[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          pk[i] = none ? 0u : pack2<kF16>(__uint_as_float(u[2 * i]) * inv_l, __uint_as_float(u[2 * i + 1]) * inv_l);
+        if (live && o_v8) {
+          st_global_v8(orow + cc * 32, pk);
+          st_global_v8(orow + cc * 32 + 16, pk + 8);
+        } else if (live) {
+          uint4* dst = reinterpret_cast<uint4*>(orow + cc * 32);
+#pragma unroll
+          for (int gg = 0; gg < 4; ++gg) dst[gg] = make_uint4(pk[4 * gg], pk[4 * gg + 1], pk[4 * gg + 2], pk[4 * gg + 3]);
+        }
+        __syncwarp();
+      }
+      ptx::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&o_free[ob]));
+    }
+  }
+
+  ptx::tc_fence_before();
+  __syncthreads();
+  ptx::tc_fence_after();
+  if (warp == 1) ptx::tmem_dealloc(tmem_base, kAttnTmemCols);
+}
+
+}  // namespace bsk

@@ -59,7 +59,7 @@ def test_cache_arguments():
 
 def _paged(**kw):
     a = dict(dtype=0, Q=P, q_ts=64, q_hs=64, kc=P, vc=P, e4m3=0, ks=None, vs=None, table=P, ts=2, width=2, lens=P, cu=P, O=P, tokens=1,
-             batch=1, heads=2, kv_heads=1, dim=64, pages=2, page=16, scale=0.1, stream=None)
+             batch=1, heads=2, kv_heads=1, dim=64, pages=2, page=16, scale=0.1, ws=P, ws_bytes=1 << 40, stream=None)
     a.update(kw)
     return _rc("bsk_attention_paged", *a.values())[0]
 

@@ -23,8 +23,8 @@
 #include "rotary.cuh"
 #include "kv_cache.cuh"
 #include "paged_decode_sm100.cuh"
-#include "varlen_simple.cuh"
 #include "varattn_sm100.cuh"
+#include "varattn_bwd_sm100.cuh"
 
 namespace {
 
@@ -176,6 +176,14 @@ void init_device(DeviceState& st, int dev) {
       allow_paged<false, 128, false>(), allow_paged<false, 128, true>(), allow_paged<false, 64, false>(),
       allow_paged<false, 64, true>(),   allow_paged<true, 128, false>(), allow_paged<true, 128, true>(),
       allow_paged<true, 64, false>(),   allow_paged<true, 64, true>(),
+      allow_smem(varattn_bwd_dq_kernel<false, 128>, BwdDqShape<false, 128>::kSmemBytes),
+      allow_smem(varattn_bwd_dq_kernel<false, 64>, BwdDqShape<false, 64>::kSmemBytes),
+      allow_smem(varattn_bwd_dq_kernel<true, 128>, BwdDqShape<true, 128>::kSmemBytes),
+      allow_smem(varattn_bwd_dq_kernel<true, 64>, BwdDqShape<true, 64>::kSmemBytes),
+      allow_smem(varattn_bwd_dkdv_kernel<false, 128>, BwdDkdvShape<false, 128>::kSmemBytes),
+      allow_smem(varattn_bwd_dkdv_kernel<false, 64>, BwdDkdvShape<false, 64>::kSmemBytes),
+      allow_smem(varattn_bwd_dkdv_kernel<true, 128>, BwdDkdvShape<true, 128>::kSmemBytes),
+      allow_smem(varattn_bwd_dkdv_kernel<true, 64>, BwdDkdvShape<true, 64>::kSmemBytes),
       allow_smem(varattn_fwd_kernel<false, 128, false>, AttnShape<false, 128>::kSmemBytes),
       allow_smem(varattn_fwd_kernel<false, 64, false>, AttnShape<false, 64>::kSmemBytes),
       allow_smem(varattn_fwd_kernel<true, 128, false>, AttnShape<true, 128>::kSmemBytes),
@@ -262,6 +270,15 @@ int encoder(PFN_cuTensorMapEncodeTiled_v12000* fn) {
       g_encode = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(f);
   });
   if (!g_encode) return set_error(BSK_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable from the driver");
+  // The encoder is a driver call and needs a current context, which a thread whose first CUDA work this is (torch's
+  // backward thread) has only chosen, not made current.
+  thread_local int t_ready_device = -1;
+  int dev = -1;
+  if (cudaGetDevice(&dev) == cudaSuccess && dev != t_ready_device) {
+    const cudaError_t e = cudaSetDevice(dev);
+    if (e != cudaSuccess) return cuda_fail(e, "cudaSetDevice");
+    t_ready_device = dev;
+  }
   *fn = g_encode;
   return BSK_OK;
 }
@@ -2269,8 +2286,11 @@ int bsk_attention_paged(int dtype, const void* Q, int64_t q_token_stride, int64_
 
 int64_t bsk_attention_varlen_workspace_bytes(int tokens, int batch, int heads, int kv_heads, int dim, int backward) {
   if (int rc = heads_checks("attention_varlen_workspace_bytes", 0, tokens, batch, heads, kv_heads, dim, 1.0f)) return rc;
-  (void)backward;
-  return plan_bytes(tokens, batch, bsk::kVarBlk / (heads / kv_heads));
+  const int tt = bsk::kVarBlk / (heads / kv_heads);
+  const int64_t plan = plan_bytes(tokens, batch, tt);
+  if (!backward) return plan;
+  // the two lists, then the tiles' row statistics
+  return plan + plan_bytes(tokens, batch, bsk::kVarBlk) + bsk::plan_slots(tokens, batch, tt) * kv_heads * 1024;
 }
 
 int bsk_attention_varlen_fwd(int dtype, const void* Q, int64_t q_token_stride, int64_t q_head_stride, const void* K,
@@ -2346,26 +2366,70 @@ int bsk_attention_varlen_bwd(int dtype, const void* dO, int64_t do_token_stride,
       !aligned16(O) || !aligned16(dQ) || !aligned16(dK) || !aligned16(dV) || !aligned16(workspace))
     return set_error(BSK_ERR_INVALID_ARG, "%s: rows of the tensors must be 16-byte aligned", what);
   if (int rc = device_state(&st)) return rc;
-  bsk::VarlenArgs a{};
-  a.Q = Q; a.K = K; a.V = V; a.dO = dO; a.O_in = O; a.lse = const_cast<float*>(lse); a.cu = cu_seqlens;
-  a.dQ = dQ; a.dK = dK; a.dV = dV;
-  a.q_ts = q_token_stride; a.q_hs = q_head_stride;
-  a.k_ts = k_token_stride; a.k_hs = k_head_stride;
-  a.v_ts = v_token_stride; a.v_hs = v_head_stride;
-  a.do_ts = do_token_stride; a.do_hs = do_head_stride;
-  a.tokens = tokens; a.batch = batch; a.heads = heads; a.kv_heads = kv_heads; a.group = heads / kv_heads;
-  a.causal = causal;
-  a.scale = scale;
-  a.err = st->err_word;
+  const int group = heads / kv_heads, tt = bsk::kVarBlk / group;
+  const int64_t slots = bsk::plan_slots(tokens, batch, tt), key_slots = bsk::plan_slots(tokens, batch, bsk::kVarBlk);
+  if (!plan_fits(tokens, batch, tt, kv_heads)) return set_error(BSK_ERR_UNSUPPORTED, "%s: too many rows", what);
+  const bool f16 = dtype == 1;
+  CUtensorMap tq, tk, tv, tdo;
+  if (int rc = make_map3(&tq, f16, Q, dim, heads, tokens, q_head_stride * 2, q_token_stride * 2, group, tt, "Q")) return rc;
+  if (int rc = make_map3(&tk, f16, K, dim, kv_heads, tokens, k_head_stride * 2, k_token_stride * 2, 1, bsk::kVarBlk, "K")) return rc;
+  if (int rc = make_map3(&tv, f16, V, dim, kv_heads, tokens, v_head_stride * 2, v_token_stride * 2, 1, bsk::kVarBlk, "V")) return rc;
+  if (int rc = make_map3(&tdo, f16, dO, dim, heads, tokens, do_head_stride * 2, do_token_stride * 2, group, tt, "dO")) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const unsigned gq = (unsigned)(((int64_t)tokens * heads + 3) / 4), gk = (unsigned)(((int64_t)tokens * kv_heads + 3) / 4);
-#define BSK_VARLEN_BWD(F16, DD)                                          \
-  do {                                                                   \
-    bsk::varlen_simple_kernel<F16, DD, 1><<<gq, 128, 0, s>>>(a);         \
-    bsk::varlen_simple_kernel<F16, DD, 2><<<gk, 128, 0, s>>>(a);         \
+  char* ws = static_cast<char*>(workspace);
+  char* ws_keys = ws + plan_bytes(tokens, batch, tt);
+  bsk::VarPrepArgs p{};
+  for (int i = 0; i < 2; ++i) {
+    bsk::PlanArgs& a = p.plan[i];
+    a.cu = cu_seqlens;
+    a.tokens = tokens;
+    a.batch = batch;
+    a.tt = tt;
+    a.causal = causal != 0;
+    a.keys = i;
+    a.count = reinterpret_cast<int*>(i ? ws_keys : ws);
+    a.items = reinterpret_cast<bsk::VarItem*>((i ? ws_keys : ws) + 16);
+    a.err = st->err_word;
+  }
+  p.dO = dO;
+  p.do_token_stride = do_token_stride;
+  p.do_head_stride = do_head_stride;
+  p.O = O;
+  p.lse = lse;
+  p.stats = reinterpret_cast<float*>(ws_keys + plan_bytes(tokens, batch, bsk::kVarBlk));
+  p.heads = heads;
+  p.kv_heads = kv_heads;
+  p.group = group;
+  bsk::VarBwdArgs a{};
+  a.stats = p.stats;
+  a.dQ = dQ;
+  a.dK = dK;
+  a.dV = dV;
+  a.q_items = p.plan[0].items;
+  a.k_items = p.plan[1].items;
+  a.q_count = p.plan[0].count;
+  a.k_count = p.plan[1].count;
+  a.heads = heads;
+  a.kv_heads = kv_heads;
+  a.group = group;
+  a.causal = causal != 0;
+  a.scale = scale;
+  a.scale_log2 = scale * 1.4426950408889634f;
+  a.err = st->err_word;
+  a.timeout_ns = t_timeout_ns;
+  const unsigned prep = (unsigned)(2 + slots * kv_heads);
+  const unsigned gq = (unsigned)(slots * kv_heads < st->sm_count ? slots * kv_heads : st->sm_count);
+  const unsigned gk = (unsigned)(key_slots * kv_heads < st->sm_count ? key_slots * kv_heads : st->sm_count);
+#define BSK_VARLEN_BWD(F16, DD)                                                                                        \
+  do {                                                                                                                 \
+    bsk::varattn_bwd_prep_kernel<F16, DD><<<prep, bsk::kPlanThreads, 0, s>>>(p);                                       \
+    bsk::varattn_bwd_dkdv_kernel<F16, DD><<<gk, bsk::kBwdThreads, bsk::BwdDkdvShape<F16, DD>::kSmemBytes, s>>>(tq, tk, \
+                                                                                                              tv, tdo, a); \
+    bsk::varattn_bwd_dq_kernel<F16, DD><<<gq, bsk::kBwdThreads, bsk::BwdDqShape<F16, DD>::kSmemBytes, s>>>(tq, tk, tv,  \
+                                                                                                          tdo, a);     \
   } while (0)
-  if (dtype == 1 && dim == 128) BSK_VARLEN_BWD(true, 128);
-  else if (dtype == 1) BSK_VARLEN_BWD(true, 64);
+  if (f16 && dim == 128) BSK_VARLEN_BWD(true, 128);
+  else if (f16) BSK_VARLEN_BWD(true, 64);
   else if (dim == 128) BSK_VARLEN_BWD(false, 128);
   else BSK_VARLEN_BWD(false, 64);
 #undef BSK_VARLEN_BWD

@@ -85,7 +85,8 @@ __device__ __forceinline__ bool plan_item(const PlanArgs& a, int slot, VarItem& 
   return true;
 }
 
-__global__ void __launch_bounds__(kPlanThreads) varattn_plan_kernel(const PlanArgs a) {
+// The whole list, by one CTA of kPlanThreads threads.
+__device__ __forceinline__ void build_plan(const PlanArgs& a) {
   __shared__ int hist[kPlanBuckets];
   __shared__ int warp_sum[kPlanThreads / 32];
   static_assert(kPlanBuckets == kPlanThreads, "one bucket per thread in the scan");
@@ -124,6 +125,8 @@ __global__ void __launch_bounds__(kPlanThreads) varattn_plan_kernel(const PlanAr
     if (plan_item(a, s, it)) a.items[atomicAdd(&hist[bucket(it)], 1)] = it;
   }
 }
+
+__global__ void __launch_bounds__(kPlanThreads) varattn_plan_kernel(const PlanArgs a) { build_plan(a); }
 
 // The k-th entry of CTA `cta` of `grid`: zigzag over the list of n entries. Returns -1 behind its end.
 __device__ __forceinline__ int zigzag(int k, int cta, int grid, int n) {

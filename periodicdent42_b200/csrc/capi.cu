@@ -57,7 +57,6 @@ struct DeviceState {
   int sm_count = 0;
   int pair_clusters = 0;       // co-resident 2-CTA clusters of the pair GEMM kernels (all share one footprint)
   int bsr_pair_clusters = 0;   // co-resident 2-CTA clusters of the pair BSR SpMM kernel (0: not used)
-  int paged_max_cluster = 8;   // CTAs per cluster of the paged decode kernel (16 where the device can place them)
   uint32_t* err_word = nullptr;
 };
 DeviceState g_devices[kMaxDevices];
@@ -70,12 +69,23 @@ cudaError_t allow_smem(K kernel, int bytes) {
   return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
 }
 
-// Shared memory and the 16-CTA clusters of one instantiation of the paged decode kernel.
-template <bool kF16, int kD, bool kFp8>
+// Shared memory of the paged decode kernels of 8 * kNQ rows.
+template <bool kF16, int kD, bool kFp8, int kNQ>
+cudaError_t allow_paged_one() {
+  const auto k = bsk::paged_decode_kernel<kF16, kD, kFp8, kNQ>;
+  using Sh = bsk::PagedShape<kD, kFp8, kNQ>;
+  static_assert(Sh::smem_bytes(Sh::kMaxWarps) <= 232448, "shared memory above the 227 KB per-CTA limit");
+  return allow_smem(k, Sh::smem_bytes(Sh::kMaxWarps));
+}
+template <int kNQ>
 cudaError_t allow_paged() {
-  const auto k = bsk::paged_decode_kernel<kF16, kD, kFp8>;
-  const cudaError_t e = allow_smem(k, bsk::PagedShape<kF16, kD, kFp8>::kSmemBytes);
-  return e != cudaSuccess ? e : cudaFuncSetAttribute(k, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  const cudaError_t e[] = {allow_paged_one<false, 128, false, kNQ>(), allow_paged_one<false, 128, true, kNQ>(),
+                           allow_paged_one<false, 64, false, kNQ>(),  allow_paged_one<false, 64, true, kNQ>(),
+                           allow_paged_one<true, 128, false, kNQ>(),  allow_paged_one<true, 128, true, kNQ>(),
+                           allow_paged_one<true, 64, false, kNQ>(),   allow_paged_one<true, 64, true, kNQ>()};
+  for (cudaError_t x : e)
+    if (x != cudaSuccess) return x;
+  return cudaSuccess;
 }
 
 // How many 2-CTA clusters of `kernel` can be resident at once (persistent grids are sized to this).
@@ -173,9 +183,7 @@ void init_device(DeviceState& st, int dev) {
       allow_smem(gemm_pair_sm100_kernel<2, Epi::F32PeerRows, 2>, kPairWideSmemBytes),
       allow_smem(gemm_pair_sm100_kernel<1, Epi::BF16Scaled, 2>, kPairWideSmemBytes),
       allow_smem(spmm_bsr_pair_sm100_kernel, kBsrPairSmemBytes),
-      allow_paged<false, 128, false>(), allow_paged<false, 128, true>(), allow_paged<false, 64, false>(),
-      allow_paged<false, 64, true>(),   allow_paged<true, 128, false>(), allow_paged<true, 128, true>(),
-      allow_paged<true, 64, false>(),   allow_paged<true, 64, true>(),
+      allow_paged<1>(), allow_paged<2>(), allow_paged<4>(),
       allow_smem(varattn_bwd_dq_kernel<false, 128>, BwdDqShape<false, 128>::kSmemBytes),
       allow_smem(varattn_bwd_dq_kernel<false, 64>, BwdDqShape<false, 64>::kSmemBytes),
       allow_smem(varattn_bwd_dq_kernel<true, 128>, BwdDqShape<true, 128>::kSmemBytes),
@@ -209,23 +217,6 @@ void init_device(DeviceState& st, int dev) {
     for (int i = 1; i < 4; ++i) st.pair_clusters = c[i] < st.pair_clusters ? c[i] : st.pair_clusters;
   }
   st.bsr_pair_clusters = max_clusters(spmm_bsr_pair_sm100_kernel, kPairThreads, kBsrPairSmemBytes);
-  {
-    cudaLaunchConfig_t cfg = {};
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = 16;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cfg.gridDim = dim3(16, 1, 1);
-    cfg.blockDim = dim3(kPagedThreads, 1, 1);
-    cfg.dynamicSmemBytes = PagedShape<false, 64, true>::kSmemBytes;  // the largest of the instantiations
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    int n = 0;
-    const cudaError_t x =
-        cudaOccupancyMaxActiveClusters(&n, reinterpret_cast<const void*>(paged_decode_kernel<false, 64, true>), &cfg);
-    if (x == cudaSuccess && n > 0) st.paged_max_cluster = 16;
-    else cudaGetLastError();
-  }
   if (st.pair_clusters <= 0) {
     st.status = BSK_ERR_CUDA;
     st.init_error = "cudaOccupancyMaxActiveClusters reports no co-resident CTA pair";
@@ -2142,20 +2133,29 @@ void varattn_fwd_launch(const CUtensorMap& tq, const CUtensorMap& tk, const CUte
       <<<grid, bsk::kAttnThreads, bsk::AttnShape<kF16, kD>::kSmemBytes, s>>>(tq, tk, tv, a);
 }
 
-template <bool kF16, int kD, bool kFp8>
-cudaError_t paged_decode_launch(const bsk::PagedArgs& a, unsigned tiles, int cluster, cudaStream_t s) {
+template <bool kF16, int kD, bool kFp8, int kNQ>
+cudaError_t paged_decode_launch_rows(const bsk::PagedArgs& a, unsigned tiles, int cluster, bool alone, cudaStream_t s) {
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = cluster;
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.gridDim = dim3(tiles * cluster, a.kv_heads, 1);
-  cfg.blockDim = dim3(bsk::kPagedThreads, 1, 1);
-  cfg.dynamicSmemBytes = bsk::PagedShape<kF16, kD, kFp8>::kSmemBytes;
+  using Sh = bsk::PagedShape<kD, kFp8, kNQ>;
+  const int warps = alone ? Sh::kMaxWarps : 4;
+  cfg.blockDim = dim3(32 * warps, 1, 1);
+  cfg.dynamicSmemBytes = Sh::smem_bytes(warps);
   cfg.stream = s;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, bsk::paged_decode_kernel<kF16, kD, kFp8>, a);
+  return cudaLaunchKernelEx(&cfg, bsk::paged_decode_kernel<kF16, kD, kFp8, kNQ>, a);
+}
+
+template <bool kF16, int kD, bool kFp8>
+cudaError_t paged_decode_launch(const bsk::PagedArgs& a, int nq, unsigned tiles, int cluster, bool alone, cudaStream_t s) {
+  if (nq == 1) return paged_decode_launch_rows<kF16, kD, kFp8, 1>(a, tiles, cluster, alone, s);
+  if (nq == 2) return paged_decode_launch_rows<kF16, kD, kFp8, 2>(a, tiles, cluster, alone, s);
+  return paged_decode_launch_rows<kF16, kD, kFp8, 4>(a, tiles, cluster, alone, s);
 }
 
 }  // namespace
@@ -2269,17 +2269,25 @@ int bsk_attention_paged(int dtype, const void* Q, int64_t q_token_stride, int64_
     else varattn_fwd_launch<false, 64, true>(tq, tk, tv, f, grid, s);
     return launch_status("attention_paged launch");
   }
-  const int64_t tiles = (int64_t)tokens * a.group / bsk::kPagedRows + batch + 1;
-  // CTAs per tile: doubled while the GPU's slots (2 CTAs per SM) are filled fewer than four times and each CTA keeps at
-  // least 128 keys of the longest sequence that the table can hold.
-  int cluster = 1;
+  // Rows per tile by what a sequence brings on average; then how many CTAs share a tile's keys and how many warps a CTA
+  // has. Measured (us, 32 / 8 heads, D 128, bf16 unless said otherwise; CTAs per tile x warps):
+  //   up to two CTAs per SM while each keeps 128 keys: 8 sequences of 4000: 1x4 57, 2x12 29, 4x4 29, 8x4 37;
+  //   above that, two CTAs per tile even out lengths until there are four per SM: 64 sequences of 97..8192, e4m3:
+  //   1x4 131, 2x4 121, 4x4 125 (all of 4096: 123, 122, 126); many short ones, 200 of 500: 1x4 74, 2x4 91;
+  //   warps: a CTA that has its SM to itself takes all that fit (registers): one of 100000: 8x4 161, 8x12 78; else four,
+  //   and more CTAs per SM, which hide each other's start and end (two of six warps: 64 sequences as above 2x6 136).
+  const int64_t avg = batch > 0 ? ((int64_t)tokens * a.group + batch - 1) / batch : 1;
+  const int nq = avg <= 8 ? 1 : avg <= 16 ? 2 : 4;
+  const int64_t tiles = (int64_t)tokens * a.group / (8 * nq) + batch + 1;
+  const int64_t items = (avg + 8 * nq - 1) / (8 * nq) * batch * kv_heads;  // tiles that have work, about
   const int64_t most_keys = (int64_t)table_width * page_size;
-  while (cluster < st->paged_max_cluster && tiles * kv_heads * cluster < (int64_t)8 * st->sm_count &&
-         most_keys >= (int64_t)cluster * 256)
-    cluster *= 2;
+  int cluster = 1;
+  while (cluster < 8 && items * cluster * 2 <= (int64_t)2 * st->sm_count && most_keys >= (int64_t)cluster * 256) cluster *= 2;
+  if (cluster == 1 && items <= (int64_t)4 * st->sm_count && most_keys >= 2048) cluster = 2;
+  const bool alone = items * cluster <= st->sm_count;
   if (tiles * cluster >= (int64_t)1 << 31) return set_error(BSK_ERR_UNSUPPORTED, "%s: too many rows", what);
   cudaError_t e = cudaSuccess;
-  BSK_BY_TYPE(e = paged_decode_launch, dtype == 1, dim, cache_e4m3 != 0, (a, (unsigned)tiles, cluster, s));
+  BSK_BY_TYPE(e = paged_decode_launch, dtype == 1, dim, cache_e4m3 != 0, (a, nq, (unsigned)tiles, cluster, alone, s));
   if (e != cudaSuccess) return cuda_fail(e, "attention_paged launch");
   return launch_status("attention_paged launch");
 }

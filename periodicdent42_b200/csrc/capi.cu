@@ -2126,6 +2126,35 @@ void plan_launch(bsk::PlanArgs a, void* ws, const DeviceState& st, cudaStream_t 
   bsk::varattn_plan_kernel<<<1, bsk::kPlanThreads, 0, s>>>(a);
 }
 
+// Workspace of a paged call in tiles: the list (with room for the pieces of split entries), the split entries, the pieces'
+// log2 sums and rows. Entries are split only where whole ones would leave the GPU less than twice its CTAs.
+struct PagedTilePlan {
+  int tt;
+  int split_ctas;  // 0: nothing is split
+  int pieces;
+  int64_t items_at, splits_at, lse_at, rows_at, total;
+};
+PagedTilePlan paged_tile_plan(int64_t tokens, int64_t batch, int heads, int kv_heads, int dim, int sm_count) {
+  PagedTilePlan p{};
+  const int group = heads / kv_heads;
+  p.tt = bsk::kVarBlk / group;
+  const int64_t slots = bsk::plan_slots(tokens, batch, p.tt);
+  p.split_ctas = ((tokens + p.tt - 1) / p.tt) * kv_heads < 2 * (int64_t)sm_count ? sm_count : 0;
+  p.pieces = p.split_ctas ? bsk::plan_pieces(p.split_ctas, kv_heads) : 0;
+  p.items_at = 16;
+  p.splits_at = p.items_at + (slots + p.pieces) * (int64_t)sizeof(bsk::VarItem);
+  p.lse_at = p.splits_at + p.pieces * (int64_t)sizeof(bsk::VarSplit);
+  p.rows_at = (p.lse_at + (int64_t)p.pieces * kv_heads * bsk::kVarBlk * 4 + 31) / 32 * 32;
+  p.total = p.rows_at + (int64_t)p.pieces * kv_heads * bsk::kVarBlk * dim * 4 + 32;  // (+ 32: rows start 32-byte aligned)
+  return p;
+}
+
+template <bool kF16, int kD>
+void varattn_combine_launch(const bsk::VarCombineArgs& a, int most, cudaStream_t s) {
+  bsk::varattn_combine_kernel<kF16, kD>
+      <<<dim3(most, a.kv_heads, bsk::kVarBlk / bsk::kCombineRows), bsk::kCombineRows * kD / 4, 0, s>>>(a);
+}
+
 template <bool kF16, int kD, bool kPaged>
 void varattn_fwd_launch(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const bsk::VarFwdArgs& a,
                         unsigned grid, cudaStream_t s) {
@@ -2175,9 +2204,10 @@ extern "C" {
 int64_t bsk_attention_paged_workspace_bytes(int tokens, int batch, int heads, int kv_heads, int dim, int cache_e4m3,
                                             int num_pages) {
   if (int rc = heads_checks("attention_paged_workspace_bytes", 0, tokens, batch, heads, kv_heads, dim, 1.0f)) return rc;
-  const int group = heads / kv_heads;
-  if (!paged_in_tiles(tokens, batch, group, cache_e4m3 != 0, num_pages)) return 0;
-  return plan_bytes(tokens, batch, bsk::kVarBlk / group);
+  if (!paged_in_tiles(tokens, batch, heads / kv_heads, cache_e4m3 != 0, num_pages)) return 0;
+  DeviceState* st;
+  if (int rc = device_state(&st)) return rc;
+  return paged_tile_plan(tokens, batch, heads, kv_heads, dim, st->sm_count).total;
 }
 
 int bsk_attention_paged(int dtype, const void* Q, int64_t q_token_stride, int64_t q_head_stride, const void* k_cache,
@@ -2225,11 +2255,15 @@ int bsk_attention_paged(int dtype, const void* Q, int64_t q_token_stride, int64_
   a.err = st->err_word;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (paged_in_tiles(tokens, batch, a.group, cache_e4m3 != 0, num_pages)) {
-    const int tt = bsk::kVarBlk / a.group;
-    const int64_t need = plan_bytes(tokens, batch, tt);
+    const PagedTilePlan w = paged_tile_plan(tokens, batch, heads, kv_heads, dim, st->sm_count);
+    const int tt = w.tt;
+    const int64_t need = w.total;
     if (workspace_bytes < need || !workspace || !aligned16(workspace))
       return set_error(BSK_ERR_INVALID_ARG, "%s: 16-byte aligned workspace of %lld bytes needed", what, (long long)need);
-    if (!plan_fits(tokens, batch, tt, kv_heads)) return set_error(BSK_ERR_UNSUPPORTED, "%s: too many rows", what);
+    const int64_t most = (bsk::plan_slots(tokens, batch, tt) + w.pieces) * kv_heads;
+    if (most >= (int64_t)1 << 31) return set_error(BSK_ERR_UNSUPPORTED, "%s: too many rows", what);
+    char* ws = static_cast<char*>(workspace);
+    char* rows_base = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(ws + w.rows_at) + 31) & ~uintptr_t(31));
     const bool f16 = dtype == 1;
     const uint64_t rows = (uint64_t)num_pages * page_size;
     const uint32_t box = page_size < bsk::kVarBlk ? page_size : bsk::kVarBlk;
@@ -2245,11 +2279,16 @@ int bsk_attention_paged(int dtype, const void* Q, int64_t q_token_stride, int64_
     p.batch = batch;
     p.tt = tt;
     p.causal = 1;
+    p.split_ctas = w.split_ctas;
+    p.kv_heads = kv_heads;
+    p.splits = reinterpret_cast<bsk::VarSplit*>(ws + w.splits_at);
     plan_launch(p, workspace, *st, s);
     bsk::VarFwdArgs f{};
     f.O = O;
-    f.count = static_cast<const int*>(workspace);
-    f.items = reinterpret_cast<const bsk::VarItem*>(static_cast<const char*>(workspace) + 16);
+    f.count = reinterpret_cast<const int*>(ws);
+    f.items = reinterpret_cast<const bsk::VarItem*>(ws + w.items_at);
+    f.part_lse = reinterpret_cast<float*>(ws + w.lse_at);
+    f.part_o = reinterpret_cast<float*>(rows_base);
     f.table = block_table;
     f.table_stride = table_stride;
     f.page_shift = a.page_shift;
@@ -2261,12 +2300,18 @@ int bsk_attention_paged(int dtype, const void* Q, int64_t q_token_stride, int64_
     f.scale_log2 = a.scale_log2;
     f.err = st->err_word;
     f.timeout_ns = t_timeout_ns;
-    const int64_t most = bsk::plan_slots(tokens, batch, tt) * kv_heads;
     const unsigned grid = (unsigned)(most < st->sm_count ? most : st->sm_count);
     if (f16 && dim == 128) varattn_fwd_launch<true, 128, true>(tq, tk, tv, f, grid, s);
     else if (f16) varattn_fwd_launch<true, 64, true>(tq, tk, tv, f, grid, s);
     else if (dim == 128) varattn_fwd_launch<false, 128, true>(tq, tk, tv, f, grid, s);
     else varattn_fwd_launch<false, 64, true>(tq, tk, tv, f, grid, s);
+    if (w.split_ctas) {
+      bsk::VarCombineArgs c{O, f.part_o, f.part_lse, p.splits, f.count, heads, kv_heads, a.group};
+      if (f16 && dim == 128) varattn_combine_launch<true, 128>(c, w.pieces / 2 + 1, s);
+      else if (f16) varattn_combine_launch<true, 64>(c, w.pieces / 2 + 1, s);
+      else if (dim == 128) varattn_combine_launch<false, 128>(c, w.pieces / 2 + 1, s);
+      else varattn_combine_launch<false, 64>(c, w.pieces / 2 + 1, s);
+    }
     return launch_status("attention_paged launch");
   }
   // Rows per tile by what a sequence brings on average; then how many CTAs share a tile's keys and how many warps a CTA
@@ -2395,6 +2440,7 @@ int bsk_attention_varlen_bwd(int dtype, const void* dO, int64_t do_token_stride,
     a.tt = tt;
     a.causal = causal != 0;
     a.keys = i;
+    a.tile_slots = 1;
     a.count = reinterpret_cast<int*>(i ? ws_keys : ws);
     a.items = reinterpret_cast<bsk::VarItem*>((i ? ws_keys : ws) + 16);
     a.err = st->err_word;

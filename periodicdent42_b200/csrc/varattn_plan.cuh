@@ -6,10 +6,15 @@
 // out in a fixed zigzag over the CTAs, so long and short ones even out without a counter in memory. The order inside a
 // length is arbitrary and changes no result, since an entry's arithmetic depends on the entry alone.
 //
+// Where there are few entries for the GPU (a small chunk over a long cache), long ones are split along their keys; the
+// pieces' results meet in a second kernel (varattn_combine_kernel).
+//
 // Tiles are numbered without a scan: tile j of sequence i is slot cu[i] / TT + i + j (sequences never overlap in it: the
 // next one's first slot is at least ceil(n_i / TT) further). Slots from cu[batch] / TT + batch on cover the rows behind the
 // last sequence, whose outputs are zero.
 #pragma once
+
+#include <climits>
 
 #include "paged_decode_sm100.cuh"
 
@@ -27,7 +32,12 @@ struct __align__(16) VarItem {
   int kv_len;  // keys of the sequence
   int pos0;    // position of the tile's first token (first key of the block, for dK / dV)
   int b0, b1;  // key blocks [b0, b1) (query tiles, for dK / dV)
-  int part;    // slot of the tile
+  int part;    // index of a split entry's piece, -1 for a whole entry (in the backward's lists: slot of the tile)
+};
+
+// An entry that was split along its keys: pieces [first, first + n) hold its partial results.
+struct __align__(16) VarSplit {
+  int row0, ntok, first, n;
 };
 
 struct PlanArgs {
@@ -36,10 +46,19 @@ struct PlanArgs {
   int64_t kv_room;     // keys that a block table row has room for
   int tokens, batch, tt, causal;
   int keys;            // 1: entries are key blocks
+  int tile_slots;      // 1: entries carry their slot in `part` (nothing is split)
+  int split_ctas;      // > 0: entries may be split along their keys to give this many CTAs work (kv_heads items an entry)
+  int kv_heads;
   VarItem* items;
-  int* count;
+  VarSplit* splits;
+  int* count;          // [0] entries, [1] split entries
   uint32_t* err;
 };
+
+// Pieces that split entries can have altogether. Entries longer than a CTA's share L = work * kv_heads / CTAs become
+// ceil(n / L) < 2 n / L pieces.
+__host__ __device__ inline int plan_pieces(int split_ctas, int kv_heads) { return 2 * split_ctas / kv_heads + 1; }
+constexpr int kPlanMinPiece = 4;  // key blocks: shorter pieces cost more in partial results than they save
 
 // Slots that a launch reserves for `tokens` rows of `batch` sequences in tiles of tt.
 __host__ __device__ inline int64_t plan_slots(int64_t tokens, int64_t batch, int64_t tt) { return tokens / tt + batch + 1; }
@@ -89,9 +108,18 @@ __device__ __forceinline__ bool plan_item(const PlanArgs& a, int slot, VarItem& 
 __device__ __forceinline__ void build_plan(const PlanArgs& a) {
   __shared__ int hist[kPlanBuckets];
   __shared__ int warp_sum[kPlanThreads / 32];
+  __shared__ unsigned long long work;             // key blocks of all entries
+  __shared__ int n_live, n_split, n_part, piece;  // entries with work; ...; key blocks that an entry may have unsplit
+  constexpr int kFew = 256;
+  __shared__ int few[kFew];                       // lengths of the first entries with work
   static_assert(kPlanBuckets == kPlanThreads, "one bucket per thread in the scan");
   const int slots = static_cast<int>(plan_slots(a.tokens, a.batch, a.keys ? kVarBlk : a.tt));
   hist[threadIdx.x] = 0;
+  if (threadIdx.x == 0) {
+    work = 0;
+    n_live = n_split = n_part = 0;
+    piece = INT_MAX;
+  }
   for (int i = threadIdx.x; i < a.batch; i += kPlanThreads) {
     int lo, hi;
     bool bad;
@@ -99,11 +127,42 @@ __device__ __forceinline__ void build_plan(const PlanArgs& a) {
     if (bad) atomicCAS(a.err, 0u, kErrBounds | (kKidVarAttn << 8) | (1u << 16));
   }
   __syncthreads();
-  // bucket 0: the longest entries
-  auto bucket = [](const VarItem& it) { return kPlanBuckets - 1 - min(it.b1 - it.b0, kPlanBuckets - 1); };
+  if (a.split_ctas > 0) {
+    for (int s = threadIdx.x; s < slots; s += kPlanThreads) {
+      VarItem it;
+      if (!plan_item(a, s, it) || it.b1 <= it.b0) continue;
+      atomicAdd(&work, static_cast<unsigned long long>(it.b1 - it.b0));
+      const int i = atomicAdd(&n_live, 1);
+      if (i < kFew) few[i] = it.b1 - it.b0;
+    }
+    __syncthreads();
+    if (threadIdx.x < 32) {
+      // A CTA's even share of the work; with fewer items than CTAs, the shortest pieces that leave one per CTA (else some
+      // CTAs would get two pieces, and the rest wait).
+      long long l = max((static_cast<long long>(work) * a.kv_heads + a.split_ctas - 1) / a.split_ctas,
+                        static_cast<long long>(kPlanMinPiece));
+      const int n = n_live;
+      if (n <= kFew && static_cast<int64_t>(n) * a.kv_heads < a.split_ctas)
+        while (true) {
+          int total = 0;
+          for (int i = threadIdx.x; i < n; i += 32) total += static_cast<int>((few[i] + l - 1) / l);
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+          if (static_cast<int64_t>(total) * a.kv_heads <= a.split_ctas) break;  // at the longest entry's length at the latest
+          l += max(1ll, l >> 5);
+        }
+      if (threadIdx.x == 0) piece = static_cast<int>(min(l, static_cast<long long>(INT_MAX)));
+    }
+    __syncthreads();
+  }
+  auto pieces_of = [&](const VarItem& it) { return max((it.b1 - it.b0 - 1) / piece + 1, 1); };
+  // bucket 0: the longest entries (or pieces)
+  auto bucket = [](int n) { return kPlanBuckets - 1 - min(n, kPlanBuckets - 1); };
   for (int s = threadIdx.x; s < slots; s += kPlanThreads) {
     VarItem it;
-    if (plan_item(a, s, it)) atomicAdd(&hist[bucket(it)], 1);
+    if (!plan_item(a, s, it)) continue;
+    const int p = pieces_of(it);
+    atomicAdd(&hist[bucket((it.b1 - it.b0) / p)], p);
   }
   __syncthreads();
   const int mine = hist[threadIdx.x];
@@ -118,11 +177,30 @@ __device__ __forceinline__ void build_plan(const PlanArgs& a) {
   int before = 0;
   for (int w = 0; w < static_cast<int>(threadIdx.x >> 5); ++w) before += warp_sum[w];
   hist[threadIdx.x] = before + incl - mine;
-  if (threadIdx.x == kPlanThreads - 1) *a.count = before + incl;
+  if (threadIdx.x == kPlanThreads - 1) a.count[0] = before + incl;
   __syncthreads();
   for (int s = threadIdx.x; s < slots; s += kPlanThreads) {
     VarItem it;
-    if (plan_item(a, s, it)) a.items[atomicAdd(&hist[bucket(it)], 1)] = it;
+    if (!plan_item(a, s, it)) continue;
+    const int n = it.b1 - it.b0, p = pieces_of(it);
+    const int at = atomicAdd(&hist[bucket(n / p)], p);
+    if (!a.tile_slots) it.part = -1;
+    if (p == 1) {
+      a.items[at] = it;
+      continue;
+    }
+    const int first = atomicAdd(&n_part, p), b0 = it.b0;
+    a.splits[atomicAdd(&n_split, 1)] = {it.row0, it.ntok, first, p};
+    for (int j = 0; j < p; ++j) {
+      it.b0 = b0 + static_cast<int>(static_cast<int64_t>(n) * j / p);
+      it.b1 = b0 + static_cast<int>(static_cast<int64_t>(n) * (j + 1) / p);
+      it.part = first + j;
+      a.items[at + j] = it;
+    }
+  }
+  if (a.split_ctas > 0) {
+    __syncthreads();
+    if (threadIdx.x == 0) a.count[1] = n_split;
   }
 }
 

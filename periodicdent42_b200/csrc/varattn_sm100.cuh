@@ -53,6 +53,8 @@ struct VarFwdArgs {
   float* lse;           // optional [tokens, heads], natural log
   const VarItem* items;
   const int* count;     // entries of `items`
+  float* part_o;        // split entries: [pieces][kv heads][128 rows][D], each piece's rows divided by its own sums
+  float* part_lse;      // [pieces][kv heads][128], log2 of the piece's sum of 2^score (-inf: no key)
   const int* table;     // paged: block table
   int64_t table_stride;
   int page_shift, num_pages;
@@ -531,6 +533,26 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       // of +inf (scores beyond fp32) gives NaN, as the definition does.
       const bool none = m_run == -INFINITY;
       const float inv_l = m_run == INFINITY ? NAN : 1.0f / l_tot;
+      if constexpr (kPaged) {
+        if (it.part >= 0) {  // one of several pieces: fp32 rows and their log2 sums, for the combining kernel
+          const int64_t prow = (static_cast<int64_t>(it.part) * a.kv_heads + hkv) * kVarBlk + r;
+          a.part_lse[prow] = none ? -INFINITY : m_run + log2f(l_tot);
+#pragma unroll 1
+          for (int cc = 0; cc < kD / 32; ++cc) {
+            uint32_t u[32];
+            ptx::tmem_ld_32x32b_x32(tO + cc * 32, u);
+            ptx::tmem_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) u[i] = none ? 0u : __float_as_uint(__uint_as_float(u[i]) * inv_l);
+#pragma unroll
+            for (int i = 0; i < 32; i += 8) st_global_v8(a.part_o + prow * kD + cc * 32 + i, u + i);
+          }
+          ptx::tc_fence_before();
+          __syncwarp();
+          if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&o_free[ob]));
+          continue;
+        }
+      }
       if (live && a.lse) a.lse[grow] = none ? -INFINITY : (m_run + log2f(l_tot)) * 0.6931471805599453f;
       uint16_t* orow = static_cast<uint16_t*>(a.O) + grow * kD;
 #pragma unroll 1
@@ -562,6 +584,48 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
   __syncthreads();
   ptx::tc_fence_after();
   if (warp == 1) ptx::tmem_dealloc(tmem_base, kAttnTmemCols);
+}
+
+// Pieces of split entries -> rows: with piece i's log2 sum L_i and its rows O_i,  O = sum_i 2^(L_i - max L) O_i / sum_i
+// 2^(L_i - max L). Block (split entry, kv head, 16 rows), D / 4 threads per row. Reads each partial result once, from L2.
+struct VarCombineArgs {
+  void* O;
+  const float* part_o;
+  const float* part_lse;
+  const VarSplit* splits;
+  const int* count;  // [1]: split entries
+  int heads, kv_heads, group;
+};
+constexpr int kCombineRows = 16;
+
+template <bool kF16, int kD>
+__global__ void __launch_bounds__(kCombineRows * kD / 4) varattn_combine_kernel(const VarCombineArgs a) {
+  if (static_cast<int>(blockIdx.x) >= a.count[1]) return;
+  const VarSplit sp = a.splits[blockIdx.x];
+  const int hkv = blockIdx.y, r = blockIdx.z * kCombineRows + threadIdx.x / (kD / 4), c = threadIdx.x % (kD / 4);
+  const int tok = r / a.group, hd = r - tok * a.group;
+  if (tok >= sp.ntok) return;
+  const int64_t row = (static_cast<int64_t>(sp.first) * a.kv_heads + hkv) * kVarBlk + r, step = static_cast<int64_t>(a.kv_heads) * kVarBlk;
+  float top = -INFINITY;
+#pragma unroll 4
+  for (int i = 0; i < sp.n; ++i) top = max_nan(top, __ldg(a.part_lse + row + i * step));
+  const float sub = top == -INFINITY ? 0.0f : top;
+  float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  float sum = 0.0f;
+#pragma unroll 4
+  for (int i = 0; i < sp.n; ++i) {
+    const float w = ex2_approx(__ldg(a.part_lse + row + i * step) - sub);
+    const float4 v = __ldg(reinterpret_cast<const float4*>(a.part_o + (row + i * step) * kD) + c);
+    sum += w;
+    acc.x += v.x * w;
+    acc.y += v.y * w;
+    acc.z += v.z * w;
+    acc.w += v.w * w;
+  }
+  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;  // no piece has a key: zero
+  const int64_t grow = static_cast<int64_t>(sp.row0 + tok) * a.heads + hkv * a.group + hd;
+  reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.O) + grow * kD)[c] =
+      make_uint2(pack2<kF16>(acc.x * inv, acc.y * inv), pack2<kF16>(acc.z * inv, acc.w * inv));
 }
 
 }  // namespace bsk

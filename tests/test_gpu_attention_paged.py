@@ -67,6 +67,21 @@ def test_against_definition(no_device_error, cuda_dev, new, kv, H, G, page, D, d
     assert torch.equal(out, bsk.attention_paged(q, block_table=table.long(), kv_lens=lens.long(), cu_seqlens=cu.long(), **c))
 
 
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("new,kv,H,G,D,page", [
+    ([2500], [2600], 32, 8, 64, 64),           # more tiles than CTAs twice over: nothing is split
+    ([70], [9000], 4, 2, 128, 32),             # few tiles, long keys: split many ways
+    ([33, 300, 1, 90], [5000, 310, 4096, 90], 8, 1, 64, 16),  # split and whole entries side by side
+    ([200, 40], [0, 3000], 4, 4, 128, 16),     # entries without keys beside split ones
+])
+def test_split_and_whole_entries(no_device_error, cuda_dev, new, kv, H, G, D, page, e4m3):
+    q, c, table, lens, cu = make(new, kv, H, G, D, page, torch.bfloat16, cuda_dev, e4m3)
+    out = bsk.attention_paged(q, block_table=table, kv_lens=lens, cu_seqlens=cu, **c)
+    check(out, q, c, table, kv, new)
+    for _ in range(2):  # the list's order may differ between calls, the results do not
+        assert torch.equal(out, bsk.attention_paged(q, block_table=table, kv_lens=lens, cu_seqlens=cu, **c))
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 def test_large_scores_and_scale(no_device_error, cuda_dev, dtype):
     q, c, table, lens, cu = make([3, 150], [900, 700], 8, 2, 128, 16, dtype, cuda_dev)

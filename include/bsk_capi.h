@@ -403,8 +403,7 @@ int bsk_attention_paged(int dtype, const void* Q, int64_t q_token_stride, int64_
                         const int32_t* block_table, int64_t table_stride, int table_width, const int32_t* kv_lens,
                         const int32_t* cu_seqlens, void* O, int tokens, int batch, int heads, int kv_heads, int dim,
                         int num_pages, int page_size, float scale, void* workspace, int64_t workspace_bytes, void* stream);
-int64_t bsk_attention_paged_workspace_bytes(int tokens, int batch, int heads, int kv_heads, int dim, int cache_e4m3,
-                                            int num_pages);
+int64_t bsk_attention_paged_workspace_bytes(int tokens, int batch, int heads, int kv_heads, int dim, int num_pages);
 
 /*
  * Attention over packed sequences of different lengths, heads grouped over kv heads (types, dims and cu_seqlens as in

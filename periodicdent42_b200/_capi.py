@@ -85,7 +85,7 @@ SIGNATURES = {
     "bsk_kv_cache_gather": (_i32, [_i32, _vp, _vp, _i32, _vp, _vp, _vp, _i32, _vp, _vp, _i32, _i32, _i32, _i64, _vp]),
     "bsk_attention_paged": (_i32, [_i32, _vp, _i64, _i64, _vp, _vp, _i32, _vp, _vp, _vp, _i64, _i32, _vp, _vp, _vp, _i32,
                                    _i32, _i32, _i32, _i32, _i32, _i32, _f32, _vp, _i64, _vp]),
-    "bsk_attention_paged_workspace_bytes": (_i64, [_i32, _i32, _i32, _i32, _i32, _i32, _i32]),
+    "bsk_attention_paged_workspace_bytes": (_i64, [_i32, _i32, _i32, _i32, _i32, _i32]),
     "bsk_attention_varlen_workspace_bytes": (_i64, [_i32, _i32, _i32, _i32, _i32, _i32]),
     "bsk_attention_varlen_fwd": (_i32, [_i32, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _i32, _i32,
                                         _i32, _i32, _i32, _f32, _i32, _vp, _i64, _vp]),

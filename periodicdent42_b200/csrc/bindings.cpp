@@ -355,7 +355,7 @@ torch::Tensor attention_paged(torch::Tensor Q, torch::Tensor k_cache, torch::Ten
   auto O = torch::empty({Q.size(0), Q.size(1), Q.size(2)}, Q.options());
   const int64_t need = bsk_attention_paged_workspace_bytes(
       narrow(Q.size(0), op, "tokens"), narrow(lens.size(0), op, "batch"), static_cast<int>(Q.size(1)),
-      static_cast<int>(k_cache.size(2)), static_cast<int>(Q.size(2)), e4m3, narrow(k_cache.size(0), op, "pages"));
+      static_cast<int>(k_cache.size(2)), static_cast<int>(Q.size(2)), narrow(k_cache.size(0), op, "pages"));
   TORCH_CHECK(need >= 0, "bsk_attention_paged_workspace_bytes failed: ", bsk_last_error());
   torch::Tensor ws;
   if (need > 0) ws = torch::empty({need}, Q.options().dtype(torch::kUInt8));

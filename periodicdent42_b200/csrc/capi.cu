@@ -88,6 +88,19 @@ cudaError_t allow_paged() {
   return cudaSuccess;
 }
 
+// The packed / paged attention forward, all types and head dims of one kind of K / V.
+template <int kKind>
+cudaError_t allow_varattn() {
+  using namespace bsk;
+  const cudaError_t e[] = {allow_smem(varattn_fwd_kernel<false, 128, kKind>, VarShape<false, 128, kKind>::kSmemBytes),
+                           allow_smem(varattn_fwd_kernel<false, 64, kKind>, VarShape<false, 64, kKind>::kSmemBytes),
+                           allow_smem(varattn_fwd_kernel<true, 128, kKind>, VarShape<true, 128, kKind>::kSmemBytes),
+                           allow_smem(varattn_fwd_kernel<true, 64, kKind>, VarShape<true, 64, kKind>::kSmemBytes)};
+  for (cudaError_t x : e)
+    if (x != cudaSuccess) return x;
+  return cudaSuccess;
+}
+
 // How many 2-CTA clusters of `kernel` can be resident at once (persistent grids are sized to this).
 template <class K>
 int max_clusters(K kernel, int threads, int smem) {
@@ -192,14 +205,7 @@ void init_device(DeviceState& st, int dev) {
       allow_smem(varattn_bwd_dkdv_kernel<false, 64>, BwdDkdvShape<false, 64>::kSmemBytes),
       allow_smem(varattn_bwd_dkdv_kernel<true, 128>, BwdDkdvShape<true, 128>::kSmemBytes),
       allow_smem(varattn_bwd_dkdv_kernel<true, 64>, BwdDkdvShape<true, 64>::kSmemBytes),
-      allow_smem(varattn_fwd_kernel<false, 128, false>, AttnShape<false, 128>::kSmemBytes),
-      allow_smem(varattn_fwd_kernel<false, 64, false>, AttnShape<false, 64>::kSmemBytes),
-      allow_smem(varattn_fwd_kernel<true, 128, false>, AttnShape<true, 128>::kSmemBytes),
-      allow_smem(varattn_fwd_kernel<true, 64, false>, AttnShape<true, 64>::kSmemBytes),
-      allow_smem(varattn_fwd_kernel<false, 128, true>, AttnShape<false, 128>::kSmemBytes),
-      allow_smem(varattn_fwd_kernel<false, 64, true>, AttnShape<false, 64>::kSmemBytes),
-      allow_smem(varattn_fwd_kernel<true, 128, true>, AttnShape<true, 128>::kSmemBytes),
-      allow_smem(varattn_fwd_kernel<true, 64, true>, AttnShape<true, 64>::kSmemBytes),
+      allow_varattn<bsk::kPacked>(), allow_varattn<bsk::kCache16>(), allow_varattn<bsk::kCacheE4m3>(),
   };
   for (cudaError_t x : errs) {
     if (x != cudaSuccess) {
@@ -316,11 +322,23 @@ int make_map3(CUtensorMap* m, bool f16, const void* base, uint64_t inner, uint64
 }
 
 // Tensor map of one operand of a paged cache [rows = pages x page size][kv_heads][dim] (16-bit): boxes of box_rows rows of
-// one head as [8-row groups][64-column chunks][8 rows][64 columns], 128-B swizzle. Row coordinates in groups of 8.
-int make_map_paged(CUtensorMap* m, bool f16, const void* base, uint64_t dim, uint64_t kv_heads, uint64_t rows,
+// one head as [8-row groups][64-column chunks][8 rows][64 columns], 128-B swizzle, row coordinates in groups of 8. e4m3:
+// boxes of whole rows of one head (dim bytes, swizzled within themselves), coordinates (column, head, row).
+int make_map_paged(CUtensorMap* m, bool f16, bool e4m3, const void* base, uint64_t dim, uint64_t kv_heads, uint64_t rows,
                    uint32_t box_rows, const char* what) {
   PFN_cuTensorMapEncodeTiled_v12000 enc;
   if (int rc = encoder(&enc)) return rc;
+  if (e4m3) {
+    cuuint64_t dims[3] = {dim, kv_heads, rows};
+    cuuint64_t strides[2] = {dim, kv_heads * dim};
+    cuuint32_t box[3] = {(cuuint32_t)dim, 1, box_rows};
+    cuuint32_t estr[3] = {1, 1, 1};
+    CUresult r = enc(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims, strides, box, estr,
+                     CU_TENSOR_MAP_INTERLEAVE_NONE, dim == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                     CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return set_error(BSK_ERR_INVALID_ARG, "%s: cuTensorMapEncodeTiled failed (%d)", what, (int)r);
+    return BSK_OK;
+  }
   const uint64_t row_bytes = kv_heads * dim * 2;
   cuuint64_t dims[5] = {64, 8, dim / 64, rows / 8, kv_heads};
   cuuint64_t strides[4] = {row_bytes, 128, 8 * row_bytes, dim * 2};
@@ -2155,11 +2173,18 @@ void varattn_combine_launch(const bsk::VarCombineArgs& a, int most, cudaStream_t
       <<<dim3(most, a.kv_heads, bsk::kVarBlk / bsk::kCombineRows), bsk::kCombineRows * kD / 4, 0, s>>>(a);
 }
 
-template <bool kF16, int kD, bool kPaged>
-void varattn_fwd_launch(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const bsk::VarFwdArgs& a,
-                        unsigned grid, cudaStream_t s) {
-  bsk::varattn_fwd_kernel<kF16, kD, kPaged>
-      <<<grid, bsk::kAttnThreads, bsk::AttnShape<kF16, kD>::kSmemBytes, s>>>(tq, tk, tv, a);
+template <int kKind>
+void varattn_fwd_launch(bool f16, int dim, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
+                        const bsk::VarFwdArgs& a, unsigned grid, cudaStream_t s) {
+  using namespace bsk;
+  if (f16 && dim == 128)
+    varattn_fwd_kernel<true, 128, kKind><<<grid, kAttnThreads, VarShape<true, 128, kKind>::kSmemBytes, s>>>(tq, tk, tv, a);
+  else if (f16)
+    varattn_fwd_kernel<true, 64, kKind><<<grid, kAttnThreads, VarShape<true, 64, kKind>::kSmemBytes, s>>>(tq, tk, tv, a);
+  else if (dim == 128)
+    varattn_fwd_kernel<false, 128, kKind><<<grid, kAttnThreads, VarShape<false, 128, kKind>::kSmemBytes, s>>>(tq, tk, tv, a);
+  else
+    varattn_fwd_kernel<false, 64, kKind><<<grid, kAttnThreads, VarShape<false, 64, kKind>::kSmemBytes, s>>>(tq, tk, tv, a);
 }
 
 template <bool kF16, int kD, bool kFp8, int kNQ>
@@ -2192,19 +2217,18 @@ cudaError_t paged_decode_launch(const bsk::PagedArgs& a, int nq, unsigned tiles,
 namespace {
 
 // Which kernel takes a paged call: the 128-row tcgen05 tiles when the sequences bring 64 rows (new tokens x heads of a
-// group) or more on average, the 16-row mma.sync tiles below that and for e4m3 caches.
-bool paged_in_tiles(int64_t tokens, int64_t batch, int64_t group, bool e4m3, int64_t num_pages) {
-  return !e4m3 && num_pages > 0 && batch > 0 && tokens * group >= 64 * batch;
+// group) or more on average, the mma.sync tiles of up to 32 rows below that.
+bool paged_in_tiles(int64_t tokens, int64_t batch, int64_t group, int64_t num_pages) {
+  return num_pages > 0 && batch > 0 && tokens * group >= 64 * batch;
 }
 
 }  // namespace
 
 extern "C" {
 
-int64_t bsk_attention_paged_workspace_bytes(int tokens, int batch, int heads, int kv_heads, int dim, int cache_e4m3,
-                                            int num_pages) {
+int64_t bsk_attention_paged_workspace_bytes(int tokens, int batch, int heads, int kv_heads, int dim, int num_pages) {
   if (int rc = heads_checks("attention_paged_workspace_bytes", 0, tokens, batch, heads, kv_heads, dim, 1.0f)) return rc;
-  if (!paged_in_tiles(tokens, batch, heads / kv_heads, cache_e4m3 != 0, num_pages)) return 0;
+  if (!paged_in_tiles(tokens, batch, heads / kv_heads, num_pages)) return 0;
   DeviceState* st;
   if (int rc = device_state(&st)) return rc;
   return paged_tile_plan(tokens, batch, heads, kv_heads, dim, st->sm_count).total;
@@ -2254,7 +2278,7 @@ int bsk_attention_paged(int dtype, const void* Q, int64_t q_token_stride, int64_
   a.scale_log2 = scale * 1.4426950408889634f;
   a.err = st->err_word;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (paged_in_tiles(tokens, batch, a.group, cache_e4m3 != 0, num_pages)) {
+  if (paged_in_tiles(tokens, batch, a.group, num_pages)) {
     const PagedTilePlan w = paged_tile_plan(tokens, batch, heads, kv_heads, dim, st->sm_count);
     const int tt = w.tt;
     const int64_t need = w.total;
@@ -2269,8 +2293,8 @@ int bsk_attention_paged(int dtype, const void* Q, int64_t q_token_stride, int64_
     const uint32_t box = page_size < bsk::kVarBlk ? page_size : bsk::kVarBlk;
     CUtensorMap tq, tk, tv;
     if (int rc = make_map3(&tq, f16, Q, dim, heads, tokens, q_head_stride * 2, q_token_stride * 2, a.group, tt, "Q")) return rc;
-    if (int rc = make_map_paged(&tk, f16, k_cache, dim, kv_heads, rows, box, "k_cache")) return rc;
-    if (int rc = make_map_paged(&tv, f16, v_cache, dim, kv_heads, rows, box, "v_cache")) return rc;
+    if (int rc = make_map_paged(&tk, f16, cache_e4m3 != 0, k_cache, dim, kv_heads, rows, box, "k_cache")) return rc;
+    if (int rc = make_map_paged(&tv, f16, cache_e4m3 != 0, v_cache, dim, kv_heads, rows, box, "v_cache")) return rc;
     bsk::PlanArgs p{};
     p.cu = cu_seqlens;
     p.kv_lens = kv_lens;
@@ -2293,6 +2317,8 @@ int bsk_attention_paged(int dtype, const void* Q, int64_t q_token_stride, int64_
     f.table_stride = table_stride;
     f.page_shift = a.page_shift;
     f.num_pages = num_pages;
+    f.k_scale = k_scale;
+    f.v_scale = v_scale;
     f.heads = heads;
     f.kv_heads = kv_heads;
     f.group = a.group;
@@ -2301,10 +2327,8 @@ int bsk_attention_paged(int dtype, const void* Q, int64_t q_token_stride, int64_
     f.err = st->err_word;
     f.timeout_ns = t_timeout_ns;
     const unsigned grid = (unsigned)(most < st->sm_count ? most : st->sm_count);
-    if (f16 && dim == 128) varattn_fwd_launch<true, 128, true>(tq, tk, tv, f, grid, s);
-    else if (f16) varattn_fwd_launch<true, 64, true>(tq, tk, tv, f, grid, s);
-    else if (dim == 128) varattn_fwd_launch<false, 128, true>(tq, tk, tv, f, grid, s);
-    else varattn_fwd_launch<false, 64, true>(tq, tk, tv, f, grid, s);
+    if (cache_e4m3) varattn_fwd_launch<bsk::kCacheE4m3>(f16, dim, tq, tk, tv, f, grid, s);
+    else varattn_fwd_launch<bsk::kCache16>(f16, dim, tq, tk, tv, f, grid, s);
     if (w.split_ctas) {
       bsk::VarCombineArgs c{O, f.part_o, f.part_lse, p.splits, f.count, heads, kv_heads, a.group};
       if (f16 && dim == 128) varattn_combine_launch<true, 128>(c, w.pieces / 2 + 1, s);
@@ -2392,10 +2416,7 @@ int bsk_attention_varlen_fwd(int dtype, const void* Q, int64_t q_token_stride, i
   f.timeout_ns = t_timeout_ns;
   const int64_t most = bsk::plan_slots(tokens, batch, tt) * kv_heads;
   const unsigned grid = (unsigned)(most < st->sm_count ? most : st->sm_count);
-  if (f16 && dim == 128) varattn_fwd_launch<true, 128, false>(tq, tk, tv, f, grid, s);
-  else if (f16) varattn_fwd_launch<true, 64, false>(tq, tk, tv, f, grid, s);
-  else if (dim == 128) varattn_fwd_launch<false, 128, false>(tq, tk, tv, f, grid, s);
-  else varattn_fwd_launch<false, 64, false>(tq, tk, tv, f, grid, s);
+  varattn_fwd_launch<bsk::kPacked>(f16, dim, tq, tk, tv, f, grid, s);
   return launch_status("attention_varlen_fwd launch");
 }
 

@@ -19,11 +19,24 @@
 //     scores are replaced, but P = 0 does not stop a NaN in V: warp 3 sets those V rows to zero in shared memory between the
 //     copy's arrival and the PV product (only such blocks take this detour).
 //
+// e4m3 caches (kKind 2): both products are fp16 products. Warps 12-15, which otherwise only write results, convert: codes
+// arrive by the same copies in a staging ring, a thread takes a key's row and writes it as fp16 (one instruction for two
+// codes, exact) to the K / V ring, rows behind the sequence as zeros. Warp 3 brings the blocks' scales. The keys' scales
+// multiply the scores. The values' scales multiply P, brought near 1 by a power of two R that follows the largest scale
+// seen (O is rescaled when R grows), so that P * scale stays within fp16's range: values' scales down to 2^-20 of the
+// largest keep P's full precision. bf16 queries are turned into fp16 in place, each row by its own power of two (exact but
+// for elements 2^-39 below the row's largest).
+// Bound here: the conversion's one warp per sub-partition beside the softmax's two (8100 warp instructions a block where
+// 16-bit caches take 4100). Its loops are not unrolled further than they are: the roles share the instruction cache, and
+// with more code they wait for instructions (1024 new tokens over 30000, 32 / 8 heads, D 128: 1500 us unrolled, 1120 so;
+// with the values' scales multiplied in the conversion 1480; 16-bit cache 555).
+//
 // Bound: the tensor pipe and the softmax share the time (4 D flops and one exponential per score; see the forward's trace
 // in bsattn_sm100.cuh). Packing the group's heads into the tile means a causal tile spans only TT tokens, so less of its
 // last block is masked, and one K / V tile feeds the whole group.
 #pragma once
 
+#include "bsattn_bwd_sm100.cuh"
 #include "varattn_plan.cuh"
 
 namespace bsk {
@@ -48,6 +61,24 @@ __device__ __forceinline__ void zero_tile_rows(uint8_t* tile, int chunks, int fi
   }
 }
 
+// Where the K / V rows come from.
+enum : int { kPacked = 0, kCache16 = 1, kCacheE4m3 = 2 };
+
+template <bool kF16, int kD, int kKind>
+struct VarShape {
+  static constexpr bool kE4m3 = kKind == kCacheE4m3;
+  static constexpr int kTile = kVarBlk * kD * 2;
+  static constexpr int kChunks = kD / 64;
+  static constexpr int kSlots = kE4m3 && kD == 128 ? 3 : 5;  // K / V ring
+  static constexpr int kStages = kE4m3 ? 3 : 0;              // staging ring of code tiles
+  static constexpr int kStageBytes = kVarBlk * kD;
+  // barriers 512 B, sums and maxima, and for e4m3: [2 buffers] keys' and values' scales, [2] rows' scales, [2] 2^-R steps
+  static constexpr int kSmallBytes = 512 + 3 * 128 * 4 + (kE4m3 ? (2 * 256 + 2 * 128 + 4) * 4 : 0);
+  static constexpr int kSmemBytes = 1024 + kTile * (2 + kSlots) + kStages * kStageBytes + kSmallBytes;
+  static constexpr uint32_t kFmt = kF16 || kE4m3 ? 0u : 1u;  // tcgen05 kind::f16 operands: 0 f16, 1 bf16
+  static_assert(kSmemBytes <= 232448, "shared memory above the 227 KB per-CTA limit");
+};
+
 struct VarFwdArgs {
   void* O;              // contiguous [tokens, heads, D]
   float* lse;           // optional [tokens, heads], natural log
@@ -58,37 +89,47 @@ struct VarFwdArgs {
   const int* table;     // paged: block table
   int64_t table_stride;
   int page_shift, num_pages;
+  const float* k_scale; // e4m3 caches: [pages, page size, kv heads]
+  const float* v_scale;
   int heads, kv_heads, group, causal;
   float scale_log2;
   uint32_t* err;
   uint64_t timeout_ns;
 };
 
-template <bool kF16, int kD, bool kPaged>
+template <bool kF16, int kD, int kKind>
 __global__ void __launch_bounds__(kAttnThreads, 1)
     varattn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                        const __grid_constant__ CUtensorMap tmV, const VarFwdArgs a) {
-  using Sh = AttnShape<kF16, kD>;
-  constexpr int kTile = Sh::kTile;
+  using Sh = VarShape<kF16, kD, kKind>;
+  constexpr bool kPaged = kKind != kPacked, kE4m3 = kKind == kCacheE4m3;
+  constexpr bool kOpF16 = kF16 || kE4m3;  // type of the products' operands
+  constexpr int kTile = Sh::kTile, kSlots = Sh::kSlots, kStages = Sh::kStages;
   constexpr int kHalfD = kD / 2;
   // K / V tiles in shared memory: atoms of 8 rows x 128 bytes. Packed: a 64-column chunk's 16 atoms, then the next chunk's
   // (one copy per chunk). Paged: the chunks of 8 rows together, so that one copy brings a whole page.
-  constexpr int kGroupPitch = kPaged ? 1024 * Sh::kChunks : 1024;  // from 8 rows to the next 8
-  constexpr int kChunkPitch = kPaged ? 1024 : kAttnChunk;          // from 64 columns to the next 64
+  constexpr int kGroupPitch = kKind == kCache16 ? 1024 * Sh::kChunks : 1024;  // from 8 rows to the next 8
+  constexpr int kChunkPitch = kKind == kCache16 ? 1024 : kAttnChunk;          // from 64 columns to the next 64
   constexpr uint32_t IDESC_S = ptx::instr_desc(128, 128, Sh::kFmt, Sh::kFmt, 0, 0);
   constexpr uint32_t IDESC_PV = ptx::instr_desc(128, kD, Sh::kFmt, Sh::kFmt, 0, 1);
 
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sQ = smem;                      // [2] Q of alternate items
-  uint8_t* sKV = sQ + 2 * kTile;           // [kAttnKVSlots]
-  uint64_t* bars = reinterpret_cast<uint64_t*>(sKV + kAttnKVSlots * kTile);
+  uint8_t* sKV = sQ + 2 * kTile;           // [kSlots]
+  uint8_t* sRaw = sKV + kSlots * kTile;    // [kStages] code tiles
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sRaw + kStages * Sh::kStageBytes);
   uint64_t* q_full = bars + 0;                       // [2]
   uint64_t* q_empty = bars + 2;                      // [2]
-  uint64_t* kv_full = bars + 4;                      // [kAttnKVSlots]
-  uint64_t* kv_empty = kv_full + kAttnKVSlots;       // [kAttnKVSlots]
-  uint64_t* raw_full = kv_empty + kAttnKVSlots;      // [kAttnKVSlots] a V tile with foreign rows has arrived
-  uint64_t* s_full = raw_full + kAttnKVSlots;        // [2]
+  uint64_t* kv_full = bars + 4;                      // [kSlots]
+  uint64_t* kv_empty = kv_full + kSlots;             // [kSlots]
+  uint64_t* raw_full = kv_empty + kSlots;            // [kSlots] a V tile with foreign rows has arrived (16-bit)
+  uint64_t* stg_full = raw_full;                     // [kStages] a code tile has arrived (e4m3)
+  uint64_t* stg_empty = stg_full + kStages;          // [kStages] it has been converted (4 warps)
+  uint64_t* q_raw = stg_empty + kStages;             // [2] Q as it was copied (e4m3)
+  uint64_t* sc_full = q_raw + 2;                     // [2] a block's scales are in shared memory (4 warps; e4m3)
+  constexpr int kMore = kE4m3 ? 2 * kStages + 4 : kSlots;
+  uint64_t* s_full = raw_full + kMore;               // [2]
   uint64_t* s_free = s_full + 2;                     // [2]
   uint64_t* p_full = s_free + 2;                     // [2]
   uint64_t* o_done = p_full + 2;                     // [2]
@@ -98,9 +139,13 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
   uint64_t* o_free = l_ready + 1;                    // [2]
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(o_free + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
-  static_assert(4 + 3 * kAttnKVSlots + 2 + 2 + 2 + 2 + 8 + 2 + 1 + 2 <= 63, "barrier area exceeds its 512 bytes");
+  static_assert(4 + 2 * kSlots + kMore + 2 + 2 + 2 + 2 + 8 + 2 + 1 + 2 <= 63, "barrier area exceeds its 512 bytes");
   float* l_part = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(bars) + 512);  // [2 halves][128 rows]
   float* m_row = l_part + 256;                                                       // [128 rows]
+  float* k_sc = m_row + 128;  // e4m3: [2][128] keys' scales
+  float* v_sc = k_sc + 256;   // [2][128] values' scales / 2^R
+  float* q_sc = v_sc + 256;   // [2][128] what the query rows were divided by
+  float* r_step = q_sc + 256; // [2] 2^(R before - R) of the block; [2] what an item's O is multiplied by at its end
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -108,8 +153,12 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < 2; ++s) {
-      ptx::mbar_init(ptx::smem_u32(&q_full[s]), 1);
+      ptx::mbar_init(ptx::smem_u32(&q_full[s]), kE4m3 ? 4 : 1);
       ptx::mbar_init(ptx::smem_u32(&q_empty[s]), 1);
+      if (kE4m3) {
+        ptx::mbar_init(ptx::smem_u32(&q_raw[s]), 1);
+        ptx::mbar_init(ptx::smem_u32(&sc_full[s]), 1);
+      }
       ptx::mbar_init(ptx::smem_u32(&s_full[s]), 1);
       ptx::mbar_init(ptx::smem_u32(&s_free[s]), 1);
       ptx::mbar_init(ptx::smem_u32(&p_full[s]), 8);
@@ -117,10 +166,14 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       ptx::mbar_init(ptx::smem_u32(&o_done[s]), 1);
       ptx::mbar_init(ptx::smem_u32(&o_free[s]), 4);
     }
-    for (int s = 0; s < kAttnKVSlots; ++s) {
-      ptx::mbar_init(ptx::smem_u32(&kv_full[s]), 1);
+    for (int s = 0; s < kSlots; ++s) {
+      ptx::mbar_init(ptx::smem_u32(&kv_full[s]), kE4m3 ? 4 : 1);
       ptx::mbar_init(ptx::smem_u32(&kv_empty[s]), 1);
-      ptx::mbar_init(ptx::smem_u32(&raw_full[s]), 1);
+      if (!kE4m3) ptx::mbar_init(ptx::smem_u32(&raw_full[s]), 1);
+    }
+    for (int s = 0; s < kStages; ++s) {
+      ptx::mbar_init(ptx::smem_u32(&stg_full[s]), 1);
+      ptx::mbar_init(ptx::smem_u32(&stg_empty[s]), 4);
     }
     ptx::mbar_init(ptx::smem_u32(l_ready), 8);
     for (int s = 0; s < 8; ++s) ptx::mbar_init(ptx::smem_u32(&xbar[s]), 2);
@@ -172,7 +225,10 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     // took 4.4 us a block).
     uint32_t slot = 0, slot_phase = 0, q_issued = 0, kv_issued = 0;
     bool ok = true;
-    const uint32_t kv0 = ptx::smem_u32(sKV);
+    constexpr int kRing = kE4m3 ? kStages : kSlots;  // the ring that copies go to
+    uint64_t* ring_full = kE4m3 ? stg_full : kv_full;
+    uint64_t* ring_empty = kE4m3 ? stg_empty : kv_empty;
+    const uint32_t kv0 = ptx::smem_u32(kE4m3 ? sRaw : sKV);
     if (kPaged || lane == 0) {
       const int page_rows = kPaged ? 1 << a.page_shift : 0;
       const int box_rows = kPaged ? min(page_rows, kVarBlk) : kVarBlk;
@@ -197,15 +253,19 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         return (page << a.page_shift) + (key & (page_rows - 1));
       };
       auto push = [&](const CUtensorMap* m, const VarItem& it, int hkv, int b, bool is_v, int row) -> bool {
-        if (!wait(&kv_empty[slot], slot_phase ^ 1, 2)) return false;
-        const bool foreign = is_v && b == it.b1 - 1 && tail_rows(it) < kVarBlk;
-        const uint32_t fb = ptx::smem_u32(foreign ? &raw_full[slot] : &kv_full[slot]);
-        const uint32_t dst = kv0 + slot * kTile + (kPaged ? lane * (box_rows >> 3) * kGroupPitch : 0);
+        if (!wait(&ring_empty[slot], slot_phase ^ 1, 2)) return false;
+        const bool foreign = !kE4m3 && is_v && b == it.b1 - 1 && tail_rows(it) < kVarBlk;
+        const uint32_t fb = ptx::smem_u32(foreign ? &raw_full[slot] : &ring_full[slot]);
+        uint32_t dst = kv0 + slot * (kE4m3 ? Sh::kStageBytes : kTile);
+        if (kPaged) dst += lane * (kE4m3 ? box_rows * kD : (box_rows >> 3) * kGroupPitch);
         if (lane == 0) {
           const int boxes = kPaged ? min(pages_per_blk, (it.kv_len - b * kVarBlk + box_rows - 1) / box_rows) : 1;
-          ptx::mbar_arrive_expect_tx(fb, boxes * box_rows * kD * 2);
+          ptx::mbar_arrive_expect_tx(fb, boxes * box_rows * kD * (kE4m3 ? 1 : 2));
         }
-        if constexpr (kPaged) {
+        if constexpr (kE4m3) {
+          __syncwarp();
+          if (row >= 0) ptx::tma_load_3d(dst, m, fb, 0, hkv, row);
+        } else if constexpr (kPaged) {
           __syncwarp();
           if (row >= 0) ptx::tma_load_5d(dst, m, fb, 0, 0, 0, row >> 3, hkv);
         } else {
@@ -213,7 +273,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
           for (int c = 0; c < Sh::kChunks; ++c) ptx::tma_load_3d(dst + c * kAttnChunk, m, fb, 64 * c, hkv, row);
         }
         ++kv_issued;
-        if (++slot == kAttnKVSlots) { slot = 0; slot_phase ^= 1; }
+        if (++slot == kRing) { slot = 0; slot_phase ^= 1; }
         return true;
       };
       VarItem it;
@@ -226,7 +286,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         ok = wait(&q_empty[qbuf], ((q_issued >> 1) & 1) ^ 1, 1);
         if (!ok) break;
         if (lane == 0) {
-          const uint32_t qf = ptx::smem_u32(&q_full[qbuf]);
+          const uint32_t qf = ptx::smem_u32(kE4m3 ? &q_raw[qbuf] : &q_full[qbuf]);
           ptx::mbar_arrive_expect_tx(qf, tt * group * kD * 2);
 #pragma unroll
           for (int c = 0; c < Sh::kChunks; ++c)
@@ -253,10 +313,10 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       volatile int never = 0;
       dctl.abort = &never;
       for (uint32_t i = q_issued > 2 ? q_issued - 2 : 0; i < q_issued; ++i)
-        wait_bounded(ptx::smem_u32(&q_full[i & 1]), (i >> 1) & 1, dctl, 8);
-      const uint32_t first = kv_issued > kAttnKVSlots ? kv_issued - kAttnKVSlots : 0;
+        wait_bounded(ptx::smem_u32(kE4m3 ? &q_raw[i & 1] : &q_full[i & 1]), (i >> 1) & 1, dctl, 8);
+      const uint32_t first = kv_issued > kRing ? kv_issued - kRing : 0;
       for (uint32_t i = first; i < kv_issued; ++i)
-        wait_bounded(ptx::smem_u32(&kv_full[i % kAttnKVSlots]), (i / kAttnKVSlots) & 1, dctl, 8);
+        wait_bounded(ptx::smem_u32(&ring_full[i % kRing]), (i / kRing) & 1, dctl, 8);
     }
     __syncwarp();
   } else if (warp == 1 || warp == 2) {
@@ -287,8 +347,8 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
               if (!ok) break;
             }
             const uint32_t pos = seq + attn_k_pos(j);
-            const uint32_t sl = pos % kAttnKVSlots;
-            ok = wait_bounded(ptx::smem_u32(&kv_full[sl]), (pos / kAttnKVSlots) & 1, ctl, 12);
+            const uint32_t sl = pos % kSlots;
+            ok = wait_bounded(ptx::smem_u32(&kv_full[sl]), (pos / kSlots) & 1, ctl, 12);
             if (!ok) break;
             ptx::tc_fence_after();
             const uint64_t qd = qdesc0 + ((qbuf * kTile) >> 4), kd = kdesc0 + ((sl * kTile) >> 4);
@@ -308,8 +368,8 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
             ok = wait_bounded(ptx::smem_u32(&p_full[b]), (g >> 1) & 1, ctl, 13);
             if (!ok) break;
             const uint32_t pos = seq + attn_v_pos(j, n);
-            const uint32_t sl = pos % kAttnKVSlots;
-            ok = wait_bounded(ptx::smem_u32(&kv_full[sl]), (pos / kAttnKVSlots) & 1, ctl, 15);
+            const uint32_t sl = pos % kSlots;
+            ok = wait_bounded(ptx::smem_u32(&kv_full[sl]), (pos / kSlots) & 1, ctl, 15);
             if (!ok) break;
             ptx::tc_fence_after();
             const uint64_t vd = vdesc0 + ((sl * kTile) >> 4);
@@ -335,17 +395,75 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     }
     __syncwarp();
   } else if (warp == 3) {
-    // ------------------------------------------------------------------ foreign V rows -> zero
+    // ------------------------------------------------------------------ foreign V rows -> zero; e4m3: scales
     uint32_t seq = 0, phases = 0;  // ring positions passed; bit s: parity of raw_full[s]'s next completion
     bool ok = true;
     VarItem it;
     int hkv;
-    for (int k = 0; ok && item_at(k, it, hkv); ++k) {
+    if constexpr (kE4m3) {
+      // Lane l has keys l, l + 32, l + 64, l + 96 of a block. Pages are looked up two blocks ahead of their scales' use and
+      // scales one, so neither load is waited for; behind the sequence, and on a bad page, a scale is 0.
+      uint32_t g = 0, rows = 0;
+      for (int k = 0; ok && item_at(k, it, hkv); ++k) {
+        if (it.b1 <= it.b0) continue;
+        int page[4] = {-1, -1, -1, -1};
+        float ks[4] = {}, vs[4] = {};
+        auto look_pages = [&](int b) {
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            const int key = b * kVarBlk + 32 * x + lane;
+            page[x] = b < it.b1 && key < it.kv_len ? __ldg(a.table + it.src * a.table_stride + (key >> a.page_shift)) : -1;
+          }
+        };
+        auto look_scales = [&](int b) {
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            const int key = b * kVarBlk + 32 * x + lane;
+            const bool held = page[x] >= 0 && page[x] < a.num_pages;
+            const int64_t at =
+                static_cast<int64_t>(held ? (page[x] << a.page_shift) + (key & ((1 << a.page_shift) - 1)) : 0) * a.kv_heads + hkv;
+            ks[x] = held ? __ldg(a.k_scale + at) : 0.0f;
+            vs[x] = held ? __ldg(a.v_scale + at) : 0.0f;
+          }
+        };
+        int r_exp = 0;  // exponent field of the largest value scale so far (R): P * scale * 2^(6 - R) stays below 2^15
+        for (int b = it.b0 - 2; b < it.b1; ++b) {  // (two rounds of lookups before the first block)
+          if (b >= it.b0) {
+            const uint32_t buf = g & 1;
+            if (g >= 2) {  // the softmax of block g - 2 has read this buffer
+              ok = warp_wait_bounded_hint<kBwdSuspendNs>(ptx::smem_u32(&p_full[buf]), ((g - 2) >> 1) & 1, ctl, 34);
+              if (!ok) break;
+            }
+            ++g;
+            const float most = fmaxf(fmaxf(vs[0], vs[1]), fmaxf(vs[2], vs[3]));
+            const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(most) & 0x7fffffffu);
+            const int want = min(max(static_cast<int>(top >> 23), 20), 240), before = r_exp;
+            if (b == it.b0 || want > r_exp) r_exp = want;
+            const float down = __int_as_float((260 - r_exp) << 23);  // 2^7 / 2^(R + 1)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              k_sc[128 * buf + 32 * x + lane] = ks[x];
+              v_sc[128 * buf + 32 * x + lane] = vs[x] * down;
+            }
+            if (lane == 0) {
+              r_step[buf] = b == it.b0 ? 1.0f : __int_as_float(max(127 + before - r_exp, 0) << 23);
+              if (b == it.b1 - 1) r_step[2 + (rows & 1)] = __int_as_float((r_exp - 6) << 23);
+            }
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&sc_full[buf]));
+          }
+          if (b + 1 >= it.b0) look_scales(b + 1);
+          look_pages(b + 2);
+        }
+        ++rows;
+      }
+    }
+    for (int k = 0; !kE4m3 && ok && item_at(k, it, hkv); ++k) {
       const int n = it.b1 - it.b0;
       if (n <= 0) continue;
       const int live = tail_rows(it);
       if (live < kVarBlk) {
-        const uint32_t sl = (seq + 2 * n - 1) % kAttnKVSlots;  // the item's last V tile
+        const uint32_t sl = (seq + 2 * n - 1) % kSlots;  // the item's last V tile
         ok = warp_wait_bounded<false, 256>(ptx::smem_u32(&raw_full[sl]), (phases >> sl) & 1, ctl, 30);
         if (!ok) break;
         phases ^= 1u << sl;
@@ -371,7 +489,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     const int tok = r / group, hd = r - tok * group;  // its token and head
     const uint32_t lane_off = static_cast<uint32_t>(32 * q) << 16;
     const uint32_t tO0 = tmem_base + kAttnTmemO + lane_off + h * kHalfD;
-    const float c = a.scale_log2;
+    float c = a.scale_log2;
     uint32_t g = 0, rows = 0, x_cnt = 0;
     bool ok = true;
     // Exchange with the warp of the other key half through the last column of each half of the S buffer.
@@ -418,6 +536,15 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         const int kb = it.b0 + j;
         const uint32_t b = g & 1;
         const uint32_t tS = tmem_base + 128 * b + lane_off;
+        if constexpr (kE4m3) {
+          ok = warp_wait_bounded(ptx::smem_u32(&sc_full[b]), (g >> 1) & 1, ctl, 19);
+          if (!ok) break;
+          if (j == 0) {  // the rows' scales come with the converted queries
+            ok = warp_wait_bounded(ptx::smem_u32(&q_full[rows & 1]), (rows >> 1) & 1, ctl, 18);
+            if (!ok) break;
+            c = a.scale_log2 * q_sc[(rows & 1) * 128 + r];
+          }
+        }
         ok = warp_wait_bounded(ptx::smem_u32(&s_full[b]), (g >> 1) & 1, ctl, 20);
         if (!ok) break;
         ptx::tc_fence_after();
@@ -426,6 +553,15 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         ptx::tmem_ld_32x32b_x32(tS + 64 * h + 32, *reinterpret_cast<uint32_t(*)[32]>(&sv[32]));
         ptx::tmem_wait_ld();
         float* v = reinterpret_cast<float*>(sv);
+        if constexpr (kE4m3) {
+          const float4* ks = reinterpret_cast<const float4*>(k_sc + 128 * b + 64 * h);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float4 x = ks[i];
+            f2_unpack(f2_mul(f2_pack(v[4 * i], v[4 * i + 1]), f2_pack(x.x, x.y)), v[4 * i], v[4 * i + 1]);
+            f2_unpack(f2_mul(f2_pack(v[4 * i + 2], v[4 * i + 3]), f2_pack(x.z, x.w)), v[4 * i + 2], v[4 * i + 3]);
+          }
+        }
         if (kb >= clear) {
           const int lim = limit - (kb * kVarBlk + 64 * h);
 #pragma unroll
@@ -449,7 +585,9 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         float alpha = 1.0f;
         if (move) alpha = (m_run == -INFINITY) ? 0.0f : ex2_approx(m_run - mbs);
         if (move) m_run = mbs;
-        const bool need_rescale = __any_sync(0xffffffffu, move && j > 0);
+        float step = 1.0f;  // O follows the values' scale reference
+        if constexpr (kE4m3) step = r_step[b];
+        const bool need_rescale = __any_sync(0xffffffffu, (move || step != 1.0f) && j > 0);
         const float m_sub = (m_run == -INFINITY) ? 0.0f : m_run;
         const uint64_t c2 = f2_pack(c, c), nm2 = f2_pack(-m_sub, -m_sub);
         uint64_t acc[4] = {0ull, 0ull, 0ull, 0ull};
@@ -464,7 +602,11 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
             e1 = ex2_approx(t1);
           }
           acc[(i >> 1) & 3] = f2_add(acc[(i >> 1) & 3], f2_pack(e0, e1));
-          sv[i >> 1] = pack2<kF16>(e0, e1);
+          if constexpr (kE4m3) {
+            const float2 x = *reinterpret_cast<const float2*>(v_sc + 128 * b + 64 * h + i);
+            f2_unpack(f2_mul(f2_pack(e0, e1), f2_pack(x.x, x.y)), e0, e1);
+          }
+          sv[i >> 1] = pack2<kOpF16>(e0, e1);
         }
         float rs;
         {
@@ -478,7 +620,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
           ok = warp_wait_bounded(ptx::smem_u32(&s_free[(g - 1) & 1]), ((g - 1) >> 1) & 1, ctl, 21);
           if (!ok) break;
           ptx::tc_fence_after();
-          const float al = move ? alpha : 1.0f;
+          const float al = (move ? alpha : 1.0f) * step;
 #pragma unroll 1
           for (int cc = 0; cc < kHalfD / 32; ++cc) {
             uint32_t u[32];
@@ -507,7 +649,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       ++rows;
     }
   } else {
-    // ------------------------------------------------------------------ output (warps 12..15)
+    // ------------------------------------------------------------------ output, conversion (warps 12..15)
     const int q = warp & 3;
     const int r = 32 * q + lane;
     const int tok = r / group, hd = r - tok * group;
@@ -515,10 +657,85 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     const bool o_v8 = (reinterpret_cast<uintptr_t>(a.O) & 31) == 0;
     uint32_t rows = 0;
     bool ok = true;
+    // e4m3: this thread converts row r of every tile. Ring positions passed (codes and fp16 tiles alike):
+    uint32_t pos = 0;
     VarItem it;
     int hkv;
     for (int k = 0; ok && item_at(k, it, hkv); ++k) {
       if (it.b1 <= it.b0) continue;  // written by the softmax warps
+      if constexpr (kE4m3) {
+        // queries: row r in place, bf16 -> fp16 with its largest element brought to [2^10, 2^11)
+        const uint32_t qbuf = rows & 1;
+        ok = warp_wait_bounded_hint<kBwdSuspendNs>(ptx::smem_u32(&q_raw[qbuf]), (rows >> 1) & 1, ctl, 31);
+        if (!ok) break;
+        float up = 1.0f;
+        if constexpr (!kF16) {
+          uint8_t* row = sQ + qbuf * kTile + r * 128;
+          uint32_t top = 0;
+          // (loops, not unrolled: the CTA's roles share the instruction cache, which the unrolled kernel overran -- a third of
+          // its time)
+#pragma unroll 1
+          for (int x = 0; x < kD / 8; ++x) {
+            const uint4 w = *reinterpret_cast<const uint4*>(row + (x >> 3) * kAttnChunk + (x & 7) * 16);
+            top = __vmaxu2(__vmaxu2(top, __vmaxu2(w.x & 0x7fff7fffu, w.y & 0x7fff7fffu)),
+                           __vmaxu2(w.z & 0x7fff7fffu, w.w & 0x7fff7fffu));
+          }
+          top = max(top >> 16, top & 0xffffu);
+          const int e = max(static_cast<int>(top >> 7), 40) - 137;
+          const float down = __int_as_float((127 - e) << 23);
+          up = __int_as_float((127 + e) << 23);
+          auto turn = [&](uint32_t u) {
+            const float2 f = unpack2<false>(u);
+            return pack_f16(f.x * down, f.y * down);
+          };
+#pragma unroll 1
+          for (int x = 0; x < kD / 8; ++x) {
+            uint4* at = reinterpret_cast<uint4*>(row + (x >> 3) * kAttnChunk + (x & 7) * 16);
+            const uint4 w = *at;
+            *at = make_uint4(turn(w.x), turn(w.y), turn(w.z), turn(w.w));
+          }
+          ptx::fence_proxy_async_smem();
+        }
+        q_sc[qbuf * 128 + r] = up;
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&q_full[qbuf]));
+        // One code tile -> fp16 tile: row r, 16 codes (16 bytes) at a time; both sides' 16-byte chunks are swizzled. Rows
+        // behind the sequence are zero.
+        const int tiles = 2 * (it.b1 - it.b0);
+        for (int x = 0; x < tiles; ++x, ++pos) {  // K_0, K_1, V_0, K_2, V_1, .., V_last
+          const int b = it.b0 + (x == 0 ? 0 : x == tiles - 1 ? tiles / 2 - 1 : (x & 1) ? (x + 1) / 2 : x / 2 - 1);
+          const uint32_t st = pos % kStages, sl = pos % kSlots;
+          ok = warp_wait_bounded_hint<kBwdSuspendNs>(ptx::smem_u32(&stg_full[st]), (pos / kStages) & 1, ctl, 32);
+          if (ok) ok = warp_wait_bounded_hint<kBwdSuspendNs>(ptx::smem_u32(&kv_empty[sl]), ((pos / kSlots) & 1) ^ 1, ctl, 33);
+          if (!ok) break;
+          const uint32_t live = b * kVarBlk + r < it.kv_len ? 0xffffffffu : 0u;
+          const uint8_t* src = sRaw + st * Sh::kStageBytes + r * kD;
+          uint8_t* dst = sKV + sl * kTile + r * 128;
+          const int sx = kD == 128 ? r & 7 : (r >> 1) & 3;
+#pragma unroll
+          for (int y = 0; y < kD / 16; y += 4) {  // a 64-column chunk: loads, then conversions
+            uint4 w[4];
+#pragma unroll
+            for (int z = 0; z < 4; ++z) w[z] = *reinterpret_cast<const uint4*>(src + (((y + z) ^ sx) << 4));
+#pragma unroll
+            for (int z = 0; z < 4; ++z) {
+              const uint32_t u[4] = {w[z].x & live, w[z].y & live, w[z].z & live, w[z].w & live};
+              uint8_t* d = dst + (y >> 2) * kAttnChunk;
+              *reinterpret_cast<uint4*>(d + (((2 * z) ^ (r & 7)) << 4)) =
+                  make_uint4(e4m3x2_lo(u[0]), e4m3x2_hi(u[0]), e4m3x2_lo(u[1]), e4m3x2_hi(u[1]));
+              *reinterpret_cast<uint4*>(d + (((2 * z + 1) ^ (r & 7)) << 4)) =
+                  make_uint4(e4m3x2_lo(u[2]), e4m3x2_hi(u[2]), e4m3x2_lo(u[3]), e4m3x2_hi(u[3]));
+            }
+          }
+          ptx::fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            ptx::mbar_arrive(ptx::smem_u32(&stg_empty[st]));
+            ptx::mbar_arrive(ptx::smem_u32(&kv_full[sl]));
+          }
+        }
+        if (!ok) break;
+      }
       ok = warp_wait_bounded<false, 256>(ptx::smem_u32(l_ready), rows & 1, ctl, 25);
       if (ok) ok = warp_wait_bounded<false, 256>(ptx::smem_u32(&o_done[rows & 1]), (rows >> 1) & 1, ctl, 22);
       if (!ok) break;
@@ -532,7 +749,8 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       // A row without keys has its maximum at -inf (its sum may hold the exponentials' floor of 2^-125): zero. A maximum
       // of +inf (scores beyond fp32) gives NaN, as the definition does.
       const bool none = m_run == -INFINITY;
-      const float inv_l = m_run == INFINITY ? NAN : 1.0f / l_tot;
+      float inv_l = m_run == INFINITY ? NAN : 1.0f / l_tot;
+      if constexpr (kE4m3) inv_l *= r_step[2 + ob];
       if constexpr (kPaged) {
         if (it.part >= 0) {  // one of several pieces: fp32 rows and their log2 sums, for the combining kernel
           const int64_t prow = (static_cast<int64_t>(it.part) * a.kv_heads + hkv) * kVarBlk + r;

@@ -4,6 +4,7 @@
 // and calls the C ABI (include/bsk_capi.h) on the current CUDA stream under a device guard.
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
 
 #include "bsk_capi.h"
@@ -445,6 +446,94 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> attention_varlen_bwd(tor
   return {dQ, dK, dV};
 }
 
+// ------------------------------------------------------------------ autograd (no Python between the engine and the kernels)
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+// Gradients that cannot be differentiated again: an error in the place of a silently wrong second derivative.
+variable_list once(variable_list grads, const char* what) {
+  if (!at::GradMode::is_enabled()) return grads;
+  for (auto& g : grads)  // (the error hangs on inputs that require a gradient only)
+    if (g.defined()) g = g.detach().set_requires_grad(true);
+  return (*std::make_shared<torch::autograd::DelayedError>(std::string(what) + " is not twice differentiable", grads.size()))(
+      std::move(grads));
+}
+
+// Packed attention: the forward keeps the rows' log-sum-exp, the backward recomputes the scores.
+struct VarlenAttention : public torch::autograd::Function<VarlenAttention> {
+  static torch::Tensor forward(AutogradContext* ctx, torch::Tensor Q, torch::Tensor K, torch::Tensor V,
+                               torch::Tensor cu_seqlens, double scale, bool causal) {
+    at::AutoDispatchBelowADInplaceOrView guard;
+    auto [O, lse] = attention_varlen_fwd(Q, K, V, cu_seqlens, scale, causal, true);
+    ctx->save_for_backward({Q, K, V, O, lse, cu_seqlens});
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["causal"] = causal;
+    return O;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto s = ctx->get_saved_variables();
+    variable_list out(6);
+    {
+      at::AutoGradMode no_grad(false);
+      auto [dQ, dK, dV] = attention_varlen_bwd(grads[0].to(s[0].scalar_type()), s[0], s[1], s[2], s[3], s[4], s[5],
+                                               ctx->saved_data["scale"].toDouble(), ctx->saved_data["causal"].toBool());
+      if (ctx->needs_input_grad(0)) out[0] = dQ;
+      if (ctx->needs_input_grad(1)) out[1] = dK;
+      if (ctx->needs_input_grad(2)) out[2] = dV;
+    }
+    return once(std::move(out), "attention_varlen");
+  }
+};
+
+torch::Tensor attention_varlen(torch::Tensor Q, torch::Tensor K, torch::Tensor V, torch::Tensor cu_seqlens, double scale,
+                               bool causal) {
+  if (at::GradMode::is_enabled() && (Q.requires_grad() || K.requires_grad() || V.requires_grad()))
+    return VarlenAttention::apply(Q, K, V, cu_seqlens, scale, causal);
+  return std::get<0>(attention_varlen_fwd(Q, K, V, cu_seqlens, scale, causal, false));
+}
+
+// Rotary positions: the gradient of a turn is the turn back.
+struct Rotary : public torch::autograd::Function<Rotary> {
+  static variable_list forward(AutogradContext* ctx, torch::Tensor Q, OptTensor K, torch::Tensor positions,
+                               torch::Tensor inv_freq, bool interleaved, double scale) {
+    at::AutoDispatchBelowADInplaceOrView guard;
+    auto [q, k] = rotary(Q, K, positions, inv_freq, interleaved, scale, false);
+    ctx->save_for_backward({positions, inv_freq});
+    ctx->saved_data["interleaved"] = interleaved;
+    ctx->saved_data["scale"] = scale;
+    ctx->set_materialize_grads(false);
+    variable_list out{q};
+    if (k) out.push_back(*k);
+    return out;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto s = ctx->get_saved_variables();
+    const bool need_q = ctx->needs_input_grad(0) && grads[0].defined();
+    const bool need_k = grads.size() > 1 && ctx->needs_input_grad(1) && grads[1].defined();
+    variable_list out(6);
+    if (need_q || need_k) {
+      at::AutoGradMode no_grad(false);
+      auto [a, b] = rotary(need_q ? grads[0] : grads[1], need_q && need_k ? OptTensor(grads[1]) : std::nullopt, s[0], s[1],
+                           ctx->saved_data["interleaved"].toBool(), ctx->saved_data["scale"].toDouble(), true);
+      if (need_q) out[0] = a;
+      if (need_k) out[1] = need_q ? *b : a;
+    }
+    return once(std::move(out), "rotary_embedding");
+  }
+};
+
+std::tuple<torch::Tensor, OptTensor> rotary_embedding(torch::Tensor Q, OptTensor K, torch::Tensor positions,
+                                                      torch::Tensor inv_freq, bool interleaved, double scale) {
+  if (at::GradMode::is_enabled()) {
+    TORCH_CHECK_VALUE(!inv_freq.requires_grad(), "rotary_embedding has no gradient for inv_freq");
+    if (Q.requires_grad() || (K && K->requires_grad())) {
+      auto out = Rotary::apply(Q, K, positions, inv_freq, interleaved, scale);
+      return {out[0], K ? OptTensor(out[1]) : std::nullopt};
+    }
+  }
+  return rotary(Q, K, positions, inv_freq, interleaved, scale, false);
+}
+
 int64_t device_error() {
   uint32_t w = 0;
   check_rc(bsk_device_error(&w), "bsk_device_error");
@@ -465,8 +554,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("Bqt"), py::arg("scale_a"), py::arg("scale_b"));
   m.def("bsattn_fwd", &bsattn_fwd, "block-sparse attention forward (sm_100a)", py::arg("Q"), py::arg("K"),
         py::arg("V"), py::arg("row_ptr"), py::arg("col_idx"), py::arg("scale"), py::arg("causal_diag") = true);
-  m.def("rotary", &rotary, "rotary positions of Q and K (sm_100a)", py::arg("Q"), py::arg("K"), py::arg("positions"),
-        py::arg("inv_freq"), py::arg("interleaved") = false, py::arg("scale") = 1.0, py::arg("backward") = false);
+  m.def("rotary_embedding", &rotary_embedding, "rotary positions of Q and K, with gradients (sm_100a)", py::arg("Q"),
+        py::arg("K"), py::arg("positions"), py::arg("inv_freq"), py::arg("interleaved") = false, py::arg("scale") = 1.0);
   m.def("kv_cache_append", &kv_cache_append, "write rows to a paged key/value cache (sm_100a)", py::arg("K"), py::arg("V"),
         py::arg("k_cache"), py::arg("v_cache"), py::arg("slots"), py::arg("k_scale") = py::none(),
         py::arg("v_scale") = py::none());
@@ -476,10 +565,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("attention_paged", &attention_paged, "attention of new tokens over a paged cache (sm_100a)", py::arg("Q"),
         py::arg("k_cache"), py::arg("v_cache"), py::arg("block_table"), py::arg("kv_lens"), py::arg("cu_seqlens"),
         py::arg("scale"), py::arg("k_scale") = py::none(), py::arg("v_scale") = py::none());
-  m.def("attention_varlen_fwd", &attention_varlen_fwd, "attention over packed sequences (sm_100a)", py::arg("Q"),
-        py::arg("K"), py::arg("V"), py::arg("cu_seqlens"), py::arg("scale"), py::arg("causal") = true,
-        py::arg("want_lse") = false);
-  m.def("attention_varlen_bwd", &attention_varlen_bwd, "its gradients (sm_100a)", py::arg("dO"), py::arg("Q"), py::arg("K"),
-        py::arg("V"), py::arg("O"), py::arg("lse"), py::arg("cu_seqlens"), py::arg("scale"), py::arg("causal") = true);
+  m.def("attention_varlen", &attention_varlen, "attention over packed sequences, with gradients (sm_100a)", py::arg("Q"),
+        py::arg("K"), py::arg("V"), py::arg("cu_seqlens"), py::arg("scale"), py::arg("causal") = true);
   m.def("device_error", &device_error, "read and clear the device error word");
 }

@@ -5,6 +5,7 @@
 #include <cuda_runtime.h>
 #include <cudaTypedefs.h>
 
+#include <atomic>
 #include <cstdarg>
 #include <cstdio>
 #include <cstdlib>
@@ -51,6 +52,7 @@ int cuda_fail(cudaError_t e, const char* what) {
 constexpr int kMaxDevices = 64;
 
 struct DeviceState {
+  std::atomic<bool> counted{false};
   std::once_flag once;
   int status = BSK_OK;
   std::string init_error;
@@ -247,11 +249,14 @@ int device_state(DeviceState** out) {
   int dev = -1;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return set_error(BSK_ERR_NO_DEVICE, "no CUDA device: %s", cudaGetErrorString(e));
-  int count = 0;
-  e = cudaGetDeviceCount(&count);
-  if (e != cudaSuccess || count == 0) return set_error(BSK_ERR_NO_DEVICE, "no CUDA device available");
   if (dev < 0 || dev >= kMaxDevices) return set_error(BSK_ERR_NO_DEVICE, "device ordinal %d out of range", dev);
   DeviceState& st = g_devices[dev];
+  if (!st.counted.load(std::memory_order_relaxed)) {  // (the count is not asked for again on every call)
+    int count = 0;
+    e = cudaGetDeviceCount(&count);
+    if (e != cudaSuccess || count == 0) return set_error(BSK_ERR_NO_DEVICE, "no CUDA device available");
+    st.counted.store(true, std::memory_order_relaxed);
+  }
   std::call_once(st.once, [&] { init_device(st, dev); });
   if (st.status != BSK_OK) return set_error(st.status, "%s", st.init_error.c_str());
   *out = &st;

@@ -439,36 +439,8 @@ def rotary_embedding(Q: torch.Tensor, K: Optional[torch.Tensor], positions: torc
     Pair i of a head -- elements (i, i + r/2), or (2i, 2i+1) with ``interleaved`` -- turns by positions[t] * inv_freq[i]
     and is multiplied by ``scale``; r = 2 * len(inv_freq), elements from r on are copied unchanged (and unscaled).
     positions: int32 or int64 [tokens], any value (angles are reduced in 64 bits); inv_freq: float32 (see
-    :func:`rotary_frequencies`). Differentiable in Q and K."""
-    if torch.is_grad_enabled():
-        if inv_freq.requires_grad:
-            raise ValueError("rotary_embedding has no gradient for inv_freq")
-        if Q.requires_grad or (K is not None and K.requires_grad):
-            return _Rotary.apply(Q, K, positions, inv_freq, bool(interleaved), float(scale))
-    return _C().rotary(Q, K, positions, inv_freq, interleaved, scale, False)
-
-
-class _Rotary(torch.autograd.Function):
-    """Autograd for rotary positions: the gradient of a turn is the turn back."""
-
-    @staticmethod
-    def forward(ctx, Q, K, positions, inv_freq, interleaved, scale):
-        ctx.save_for_backward(positions, inv_freq)
-        ctx.interleaved, ctx.scale = interleaved, scale
-        ctx.set_materialize_grads(False)
-        return _C().rotary(Q, K, positions, inv_freq, interleaved, scale, False)
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dQ, dK):
-        positions, inv_freq = ctx.saved_tensors
-        need_q = ctx.needs_input_grad[0] and dQ is not None
-        need_k = ctx.needs_input_grad[1] and dK is not None
-        if not need_q and not need_k:
-            return None, None, None, None, None, None
-        first, second = (dQ, dK if need_k else None) if need_q else (dK, None)
-        a, b = _C().rotary(first, second, positions, inv_freq, ctx.interleaved, ctx.scale, True)
-        return (a, b, None, None, None, None) if need_q else (None, a, None, None, None, None)
+    :func:`rotary_frequencies`). Differentiable (once) in Q and K."""
+    return _C().rotary_embedding(Q, K, positions, inv_freq, interleaved, scale)
 
 
 # ----------------------------------------------------------------------------------------- paged key/value cache
@@ -520,31 +492,10 @@ def attention_varlen(Q: torch.Tensor, K: torch.Tensor, V: torch.Tensor, cu_seqle
     Q [tokens, heads, dim], K and V [tokens, kv_heads, dim] (fp16 / bf16, dim 64 or 128, heads a multiple of kv_heads:
     query head h reads kv head h // (heads / kv_heads)); sequence i owns rows cu_seqlens[i] .. cu_seqlens[i+1]
     (int32 [batch + 1], starting at 0; any lengths, zero included). Rows behind the last sequence are zero.
-    Differentiable in Q, K and V (deterministic, no atomics)."""
+    Differentiable (once) in Q, K and V (deterministic, no atomics)."""
     if scale is None:
         scale = Q.shape[-1] ** -0.5 if Q.dim() and Q.shape[-1] else 1.0
-    if torch.is_grad_enabled() and (Q.requires_grad or K.requires_grad or V.requires_grad):
-        return _VarlenAttention.apply(Q, K, V, cu_seqlens, float(scale), bool(causal))
-    return _C().attention_varlen_fwd(Q, K, V, cu_seqlens, scale, causal, False)[0]
-
-
-class _VarlenAttention(torch.autograd.Function):
-    """Autograd for packed attention: the forward keeps the row log-sum-exp, the backward recomputes the scores."""
-
-    @staticmethod
-    def forward(ctx, Q, K, V, cu_seqlens, scale, causal):
-        O, lse = _C().attention_varlen_fwd(Q, K, V, cu_seqlens, scale, causal, True)
-        ctx.save_for_backward(Q, K, V, O, lse, cu_seqlens)
-        ctx.scale, ctx.causal = scale, causal
-        return O
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dO):
-        Q, K, V, O, lse, cu_seqlens = ctx.saved_tensors
-        dQ, dK, dV = _C().attention_varlen_bwd(dO.to(Q.dtype), Q, K, V, O, lse, cu_seqlens, ctx.scale, ctx.causal)
-        need = ctx.needs_input_grad
-        return dQ if need[0] else None, dK if need[1] else None, dV if need[2] else None, None, None, None
+    return _C().attention_varlen(Q, K, V, cu_seqlens, scale, causal)
 
 
 def synchronize_and_check() -> None:

@@ -157,6 +157,19 @@ def test_another_stream_and_captured_steps(no_device_error, cuda_dev):
             assert all(torch.equal(a, want[n]) for a, n in zip(out, ("O", "dQ", "dK", "dV")))
 
 
+def test_second_derivatives_are_refused(no_device_error, cuda_dev):
+    q, k, v, do, cu = make([20, 9], 2, 1, 64, torch.float16, cuda_dev)
+    q.requires_grad_(True)
+    (g,) = torch.autograd.grad(bsk.attention_varlen(q, k, v, cu), q, do, create_graph=True)
+    assert torch.equal(g.detach(), grads(q, k, v, do, cu)["dQ"])
+    with pytest.raises(RuntimeError, match="twice differentiable"):
+        g.float().sum().backward()
+    pos, f = torch.arange(29, device=cuda_dev), bsk.rotary_frequencies(64, device=cuda_dev)[0]
+    (g,) = torch.autograd.grad(bsk.rotary_embedding(q, None, pos, f)[0], q, do, create_graph=True)
+    with pytest.raises(RuntimeError, match="twice differentiable"):
+        g.float().sum().backward()
+
+
 def test_bad_lengths_are_reported_not_followed(cuda_dev):
     assert _capi.device_error() == 0
     q, k, v, do, cu = make([100, 60], 4, 2, 64, torch.bfloat16, cuda_dev)

@@ -1950,9 +1950,11 @@ bool rows_aligned(const void* p, int64_t token_stride, int64_t head_stride, int 
 
 template <class T, int kVec, bool kInter>
 int rotary_launch(const bsk::RotaryArgs& a, const DeviceState& st, cudaStream_t s) {
-  // Few tokens: one per block, so that the rows spread over the SMs. Many: up to 4, so that a block's threads all take
-  // part in the angles (rotary_dim / 2 of them per token).
-  const int tpb = a.tokens <= 8 * st.sm_count ? 1 : 4;
+  // Few tokens: one per block, so that the rows spread over the SMs. Many: as many as fill the threads' batches of rows
+  // once (at most 8: their angles are kept in shared memory).
+  const int groups = bsk::kRotaryThreads / (a.dim / (2 * kVec));
+  const int fill = groups * bsk::kRotaryBatch / (a.heads[0] + a.heads[1]);
+  const int tpb = a.tokens <= 4 * st.sm_count || fill < 1 ? 1 : fill > 8 ? 8 : fill;
   const int64_t grid = ((int64_t)a.tokens + tpb - 1) / tpb;
   const int smem = tpb * (a.rotary_dim / 2) * (int)sizeof(float2);
   bsk::rotary_kernel<T, kVec, kInter><<<(unsigned)grid, bsk::kRotaryThreads, smem, s>>>(a, tpb);
@@ -1960,13 +1962,18 @@ int rotary_launch(const bsk::RotaryArgs& a, const DeviceState& st, cudaStream_t 
 }
 
 template <class T>
-int rotary_pick(const bsk::RotaryArgs& a, bool inter, const DeviceState& st, cudaStream_t s) {
+int rotary_pick(bsk::RotaryArgs& a, bool inter, const DeviceState& st, cudaStream_t s) {
   constexpr int kVec = 16 / sizeof(T);
   bool wide = (a.dim - a.rotary_dim) % (2 * kVec) == 0 &&
               (inter ? a.rotary_dim % (2 * kVec) == 0 : (a.rotary_dim / 2) % kVec == 0);
   for (int w = 0; w < 2; ++w)
     if (a.heads[w])
       wide = wide && aligned16(a.y[w]) && rows_aligned(a.x[w], a.token_stride[w], a.head_stride[w], sizeof(T));
+  const auto by32 = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 32 == 0; };
+  a.aligned32 = a.dim * sizeof(T) % 32 == 0;
+  for (int w = 0; w < 2; ++w)
+    if (a.heads[w] && !(by32(a.x[w]) && by32(a.y[w]) && a.token_stride[w] * sizeof(T) % 32 == 0 && a.head_stride[w] * sizeof(T) % 32 == 0))
+      a.aligned32 = 0;
   if (wide) return inter ? rotary_launch<T, kVec, true>(a, st, s) : rotary_launch<T, kVec, false>(a, st, s);
   return inter ? rotary_launch<T, 1, true>(a, st, s) : rotary_launch<T, 1, false>(a, st, s);
 }
@@ -2045,8 +2052,15 @@ void cache_args(bsk::KvCacheArgs& a, const DeviceState& st, const void* k_cache,
   a.slots64 = slot_bytes == 8;
   a.tokens = tokens;
   a.heads = kv_heads;
+  a.heads_shift = (kv_heads & (kv_heads - 1)) ? -1 : __builtin_ctz(kv_heads);
   a.num_slots = num_slots;
   a.err = st.err_word;
+}
+
+template <bool kF16, int kD, bool kFp8>
+void cache_append_launch(const bsk::KvCacheArgs& a, int rows, unsigned grid, cudaStream_t s) {
+  if (rows == 1) bsk::kv_cache_append_kernel<kF16, kD, kFp8, 1><<<grid, bsk::kCacheThreads, 0, s>>>(a);
+  else bsk::kv_cache_append_kernel<kF16, kD, kFp8, 2><<<grid, bsk::kCacheThreads, 0, s>>>(a);
 }
 
 // Instantiation by element type, head dim and cache type.
@@ -2084,11 +2098,12 @@ int bsk_kv_cache_append(int dtype, const void* K, int64_t k_token_stride, int64_
   a.x[0] = K; a.x[1] = V;
   a.token_stride[0] = k_token_stride; a.token_stride[1] = v_token_stride;
   a.head_stride[0] = k_head_stride; a.head_stride[1] = v_head_stride;
+  // Two rows per thread once one per thread would fill the GPU's threads twice.
   const int64_t threads = (int64_t)tokens * kv_heads * (dim / 8);
-  const unsigned grid = (unsigned)((threads + bsk::kCacheThreads - 1) / bsk::kCacheThreads);
+  const int per = threads >= (int64_t)4096 * st->sm_count ? 2 : 1;
+  const unsigned grid = (unsigned)((threads + bsk::kCacheThreads * per - 1) / (bsk::kCacheThreads * per));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  using namespace bsk;
-  BSK_BY_TYPE(kv_cache_append_kernel, dtype == 1, dim, cache_e4m3 != 0, <<<grid, kCacheThreads, 0, s>>>(a));
+  BSK_BY_TYPE(cache_append_launch, dtype == 1, dim, cache_e4m3 != 0, (a, per, grid, s));
   return launch_status("kv_cache_append launch");
 }
 
@@ -2497,7 +2512,10 @@ int bsk_attention_varlen_bwd(int dtype, const void* dO, int64_t do_token_stride,
   a.scale_log2 = scale * 1.4426950408889634f;
   a.err = st->err_word;
   a.timeout_ns = t_timeout_ns;
-  const unsigned prep = (unsigned)(2 + slots * kv_heads);
+  // statistics: a block takes a tile slot for every groups-th kv head; few slots are spread over more blocks
+  const int64_t spread = 2 * (int64_t)st->sm_count / slots;
+  p.head_groups = (int)(spread < 1 ? 1 : spread > kv_heads ? kv_heads : spread);
+  const unsigned prep = (unsigned)(2 + slots * p.head_groups);
   const unsigned gq = (unsigned)(slots * kv_heads < st->sm_count ? slots * kv_heads : st->sm_count);
   const unsigned gk = (unsigned)(key_slots * kv_heads < st->sm_count ? key_slots * kv_heads : st->sm_count);
 #define BSK_VARLEN_BWD(F16, DD)                                                                                        \

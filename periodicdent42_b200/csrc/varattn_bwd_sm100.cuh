@@ -80,8 +80,9 @@ __device__ __forceinline__ void write_acc_half_if(uint32_t t_row, int x, uint16_
   }
 }
 
-// Blocks 0 and 1 build the two work lists (query tiles, key blocks); block 2 + s * kv_heads + h writes the statistics of tile
-// slot s for kv head h: D / 8 lanes per row, fp32 sums.
+// Blocks 0 and 1 build the two work lists (query tiles, key blocks); block 2 + s * groups + i writes the statistics of tile
+// slot s for kv heads i, i + groups, ..: D / 8 lanes per row, fp32 sums, the loads of all heads' rows independent of one
+// another.
 struct VarPrepArgs {
   PlanArgs plan[2];
   const void* dO;
@@ -89,7 +90,7 @@ struct VarPrepArgs {
   const void* O;        // contiguous
   const float* lse;     // [tokens, heads]
   float* stats;
-  int heads, kv_heads, group;
+  int heads, kv_heads, group, head_groups;
 };
 
 template <bool kF16, int kD>
@@ -98,34 +99,41 @@ __global__ void __launch_bounds__(kPlanThreads) varattn_bwd_prep_kernel(const __
     build_plan(a.plan[blockIdx.x]);
     return;
   }
-  constexpr int kTpr = kD / 8;
-  const int slot = (blockIdx.x - 2) / a.kv_heads, hkv = (blockIdx.x - 2) % a.kv_heads;
+  constexpr int kTpr = kD / 8, kRowsAtOnce = kPlanThreads / kTpr;  // 64 or 128 rows
+  const int slot = (blockIdx.x - 2) / a.head_groups, first = (blockIdx.x - 2) % a.head_groups;
   VarItem it;
   if (!plan_item(a.plan[0], slot, it) || it.b1 <= it.b0) return;
-  float* st = a.stats + (static_cast<int64_t>(slot) * a.kv_heads + hkv) * 256;
-  for (int i = threadIdx.x; i < kVarBlk * kTpr; i += kPlanThreads) {  // a row's lanes stay together: 1024 is a multiple of kTpr
-    const int r = i / kTpr, c = i % kTpr;
+  const int c = threadIdx.x % kTpr;
+#pragma unroll
+  for (int r0 = 0; r0 < kVarBlk; r0 += kRowsAtOnce) {
+    const int r = r0 + threadIdx.x / kTpr;
     const int tok = r / a.group, hd = r - tok * a.group;
     const bool live = tok < it.ntok;
-    const int64_t grow = static_cast<int64_t>(it.row0 + tok) * a.heads + hkv * a.group + hd;
-    float acc = 0.0f;
-    if (live) {
-      const uint4 x = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.dO) + (it.row0 + tok) * a.do_token_stride +
-                                                      (hkv * a.group + hd) * a.do_head_stride + 8 * c);
-      const uint4 y = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.O) + grow * kD + 8 * c);
+    const int64_t t = it.row0 + (live ? tok : 0);
+    const uint16_t* g_row = static_cast<const uint16_t*>(a.dO) + t * a.do_token_stride + hd * a.do_head_stride + 8 * c;
+    const uint16_t* o_row = static_cast<const uint16_t*>(a.O) + (t * a.heads + hd) * kD + 8 * c;
+#pragma unroll 4
+    for (int hkv = first; hkv < a.kv_heads; hkv += a.head_groups) {
+      uint4 x = make_uint4(0, 0, 0, 0), y = x;
+      if (live) {
+        x = __ldg(reinterpret_cast<const uint4*>(g_row + static_cast<int64_t>(hkv) * a.group * a.do_head_stride));
+        y = __ldg(reinterpret_cast<const uint4*>(o_row + static_cast<int64_t>(hkv) * a.group * kD));
+      }
       const uint32_t wx[4] = {x.x, x.y, x.z, x.w}, wy[4] = {y.x, y.y, y.z, y.w};
+      float acc = 0.0f;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const float2 fx = unpack2<kF16>(wx[k]), fy = unpack2<kF16>(wy[k]);
         acc = fmaf(fx.x, fy.x, acc);
         acc = fmaf(fx.y, fy.y, acc);
       }
-    }
 #pragma unroll
-    for (int o = kTpr / 2; o > 0; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
-    if (c == 0) {
-      st[r] = live ? -a.lse[grow] * 1.4426950408889634f : -INFINITY;
-      st[128 + r] = acc;
+      for (int o = kTpr / 2; o > 0; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
+      if (c == 0) {
+        float* st = a.stats + (static_cast<int64_t>(slot) * a.kv_heads + hkv) * 256 + r;
+        st[0] = live ? -__ldg(a.lse + t * a.heads + hkv * a.group + hd) * 1.4426950408889634f : -INFINITY;
+        st[128] = acc;
+      }
     }
   }
 }

@@ -71,6 +71,27 @@ def test_append_and_gather(no_device_error, cuda_dev, e4m3, dtype, T, heads, dim
     assert _same(bsk.kv_cache_gather(slots=twice, dtype=dtype, **got)[0], torch.cat([kr, kr.flip(0)]))
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_codes_next_to_rounding_middles(no_device_error, cuda_dev, dtype):
+    """Rows whose quotients lie on, just below and just above the middles between codes, in the normal and the subnormal
+    range: every code is that of the IEEE quotient."""
+    steps = torch.arange(16, dtype=torch.float64)
+    mids = torch.cat([(1 + (2 * steps[:8] + 1) / 16)[None] * 2.0 ** e for e in torch.arange(-6, 9)[:, None]])
+    subs = (2 * steps[:8] + 1) * 2.0 ** -10
+    q = torch.cat([mids.flatten(), subs, 2.0 ** -6 + subs[:1]]).clamp(max=447)
+    T = 4096
+    g = torch.Generator().manual_seed(1)
+    top = torch.rand(T, generator=g, dtype=torch.float64) * 4 + 0.01  # the rows' largest elements
+    pick = torch.randint(0, q.numel(), (T, 128), generator=g)
+    x = (q[pick] * top[:, None] / 448).to(dtype)
+    x[:, 0] = top.to(dtype)
+    x = (x * torch.where(torch.rand(T, 128, generator=g) < 0.5, -1, 1)).to(dtype)[:, None].contiguous().to(cuda_dev)
+    c = _cache(64, 64, 1, 128, None, cuda_dev, True)
+    want = _expected(c, x, x.flip(0), torch.arange(T, device=cuda_dev))
+    bsk.kv_cache_append(x, x.flip(0), slots=torch.arange(T, device=cuda_dev), **c)
+    assert all(_same(c[n], want[n]) for n in c)
+
+
 @pytest.mark.parametrize("other", [torch.bfloat16, torch.float16])
 def test_gather_of_codes_in_either_type(no_device_error, cuda_dev, other):
     c = _cache(3, 16, 2, 64, None, cuda_dev, True)

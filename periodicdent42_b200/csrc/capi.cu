@@ -2148,6 +2148,23 @@ int heads_checks(const char* what, int dtype, int tokens, int batch, int heads, 
   return BSK_OK;
 }
 
+// Launch that may start before the kernel ahead of it in the stream has ended (the kernel waits for it by itself, after
+// its own set-up).
+template <class... KArgs, class... Args>
+cudaError_t launch_overlapped(void (*kernel)(KArgs...), dim3 grid, int threads, int smem, cudaStream_t s, const Args&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads, 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 // Workspace of a work list: the entry count (16 bytes), then its entries.
 int64_t plan_bytes(int64_t tokens, int64_t batch, int64_t tt) {
   return 16 + bsk::plan_slots(tokens, batch, tt) * (int64_t)sizeof(bsk::VarItem);
@@ -2188,23 +2205,39 @@ PagedTilePlan paged_tile_plan(int64_t tokens, int64_t batch, int heads, int kv_h
 }
 
 template <bool kF16, int kD>
-void varattn_combine_launch(const bsk::VarCombineArgs& a, int most, cudaStream_t s) {
-  bsk::varattn_combine_kernel<kF16, kD>
-      <<<dim3(most, a.kv_heads, bsk::kVarBlk / bsk::kCombineRows), bsk::kCombineRows * kD / 4, 0, s>>>(a);
+cudaError_t varattn_combine_launch(const bsk::VarCombineArgs& a, int most, cudaStream_t s) {
+  return launch_overlapped(bsk::varattn_combine_kernel<kF16, kD>, dim3(most, a.kv_heads, bsk::kVarBlk / bsk::kCombineRows),
+                           bsk::kCombineRows * kD / 4, 0, s, a);
 }
 
 template <int kKind>
-void varattn_fwd_launch(bool f16, int dim, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
-                        const bsk::VarFwdArgs& a, unsigned grid, cudaStream_t s) {
+cudaError_t varattn_fwd_launch(bool f16, int dim, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
+                               const bsk::VarFwdArgs& a, unsigned grid, cudaStream_t s) {
   using namespace bsk;
   if (f16 && dim == 128)
-    varattn_fwd_kernel<true, 128, kKind><<<grid, kAttnThreads, VarShape<true, 128, kKind>::kSmemBytes, s>>>(tq, tk, tv, a);
-  else if (f16)
-    varattn_fwd_kernel<true, 64, kKind><<<grid, kAttnThreads, VarShape<true, 64, kKind>::kSmemBytes, s>>>(tq, tk, tv, a);
-  else if (dim == 128)
-    varattn_fwd_kernel<false, 128, kKind><<<grid, kAttnThreads, VarShape<false, 128, kKind>::kSmemBytes, s>>>(tq, tk, tv, a);
-  else
-    varattn_fwd_kernel<false, 64, kKind><<<grid, kAttnThreads, VarShape<false, 64, kKind>::kSmemBytes, s>>>(tq, tk, tv, a);
+    return launch_overlapped(varattn_fwd_kernel<true, 128, kKind>, grid, kAttnThreads, VarShape<true, 128, kKind>::kSmemBytes, s,
+                             tq, tk, tv, a);
+  if (f16)
+    return launch_overlapped(varattn_fwd_kernel<true, 64, kKind>, grid, kAttnThreads, VarShape<true, 64, kKind>::kSmemBytes, s,
+                             tq, tk, tv, a);
+  if (dim == 128)
+    return launch_overlapped(varattn_fwd_kernel<false, 128, kKind>, grid, kAttnThreads, VarShape<false, 128, kKind>::kSmemBytes,
+                             s, tq, tk, tv, a);
+  return launch_overlapped(varattn_fwd_kernel<false, 64, kKind>, grid, kAttnThreads, VarShape<false, 64, kKind>::kSmemBytes, s,
+                           tq, tk, tv, a);
+}
+
+template <bool kF16, int kD>
+cudaError_t varattn_bwd_launch(const bsk::VarPrepArgs& p, const bsk::VarBwdArgs& a, const CUtensorMap& tq, const CUtensorMap& tk,
+                               const CUtensorMap& tv, const CUtensorMap& tdo, unsigned prep, unsigned gk, unsigned gq,
+                               cudaStream_t s) {
+  using namespace bsk;
+  varattn_bwd_prep_kernel<kF16, kD><<<prep, kPlanThreads, 0, s>>>(p);
+  cudaError_t e = launch_overlapped(varattn_bwd_dkdv_kernel<kF16, kD>, gk, kBwdThreads, BwdDkdvShape<kF16, kD>::kSmemBytes, s, tq,
+                                    tk, tv, tdo, a);
+  if (e != cudaSuccess) return e;
+  return launch_overlapped(varattn_bwd_dq_kernel<kF16, kD>, gq, kBwdThreads, BwdDqShape<kF16, kD>::kSmemBytes, s, tq, tk, tv, tdo,
+                           a);
 }
 
 template <bool kF16, int kD, bool kFp8, int kNQ>
@@ -2236,10 +2269,13 @@ cudaError_t paged_decode_launch(const bsk::PagedArgs& a, int nq, unsigned tiles,
 
 namespace {
 
-// Which kernel takes a paged call: the 128-row tcgen05 tiles when the sequences bring 64 rows (new tokens x heads of a
-// group) or more on average, the mma.sync tiles of up to 32 rows below that.
+// Which kernel takes a paged call: the 128-row tcgen05 tiles when the sequences bring more than 32 rows (new tokens x heads
+// of a group) on average, the mma.sync tiles of up to 32 rows up to there (above, they read K and V more than once).
+// Measured (us, 32 / 8 heads, D 128, tiles / mma.sync; rows a sequence x sequences / cached tokens):
+//   16-bit: 64x1/30000 50 / 134, 48x32/4000 108 / 273, 32x32/4000 109 / 144, 32x8/4000 49 / 45, 32x8/300 23 / 17
+//   e4m3:   64x1/30000 69 / 138, 48x32/4000 187 / 298, 32x32/4000 187 / 163, 32x8/4000 68 / 51, 32x8/300 30 / 21
 bool paged_in_tiles(int64_t tokens, int64_t batch, int64_t group, int64_t num_pages) {
-  return num_pages > 0 && batch > 0 && tokens * group >= 64 * batch;
+  return num_pages > 0 && batch > 0 && tokens * group > 32 * batch;
 }
 
 }  // namespace
@@ -2347,15 +2383,15 @@ int bsk_attention_paged(int dtype, const void* Q, int64_t q_token_stride, int64_
     f.err = st->err_word;
     f.timeout_ns = t_timeout_ns;
     const unsigned grid = (unsigned)(most < st->sm_count ? most : st->sm_count);
-    if (cache_e4m3) varattn_fwd_launch<bsk::kCacheE4m3>(f16, dim, tq, tk, tv, f, grid, s);
-    else varattn_fwd_launch<bsk::kCache16>(f16, dim, tq, tk, tv, f, grid, s);
-    if (w.split_ctas) {
-      bsk::VarCombineArgs c{O, f.part_o, f.part_lse, p.splits, f.count, heads, kv_heads, a.group};
-      if (f16 && dim == 128) varattn_combine_launch<true, 128>(c, w.pieces / 2 + 1, s);
-      else if (f16) varattn_combine_launch<true, 64>(c, w.pieces / 2 + 1, s);
-      else if (dim == 128) varattn_combine_launch<false, 128>(c, w.pieces / 2 + 1, s);
-      else varattn_combine_launch<false, 64>(c, w.pieces / 2 + 1, s);
+    cudaError_t e = cache_e4m3 ? varattn_fwd_launch<bsk::kCacheE4m3>(f16, dim, tq, tk, tv, f, grid, s)
+                               : varattn_fwd_launch<bsk::kCache16>(f16, dim, tq, tk, tv, f, grid, s);
+    if (w.split_ctas && e == cudaSuccess) {
+      const bsk::VarCombineArgs c{O, f.part_o, f.part_lse, p.splits, f.count, heads, kv_heads, a.group};
+      const int most_split = w.pieces / 2 + 1;
+      if (f16) e = dim == 128 ? varattn_combine_launch<true, 128>(c, most_split, s) : varattn_combine_launch<true, 64>(c, most_split, s);
+      else e = dim == 128 ? varattn_combine_launch<false, 128>(c, most_split, s) : varattn_combine_launch<false, 64>(c, most_split, s);
     }
+    if (e != cudaSuccess) return cuda_fail(e, "attention_paged launch");
     return launch_status("attention_paged launch");
   }
   // Rows per tile by what a sequence brings on average; then how many CTAs share a tile's keys and how many warps a CTA
@@ -2436,7 +2472,8 @@ int bsk_attention_varlen_fwd(int dtype, const void* Q, int64_t q_token_stride, i
   f.timeout_ns = t_timeout_ns;
   const int64_t most = bsk::plan_slots(tokens, batch, tt) * kv_heads;
   const unsigned grid = (unsigned)(most < st->sm_count ? most : st->sm_count);
-  varattn_fwd_launch<bsk::kPacked>(f16, dim, tq, tk, tv, f, grid, s);
+  const cudaError_t e = varattn_fwd_launch<bsk::kPacked>(f16, dim, tq, tk, tv, f, grid, s);
+  if (e != cudaSuccess) return cuda_fail(e, "attention_varlen_fwd launch");
   return launch_status("attention_varlen_fwd launch");
 }
 
@@ -2518,19 +2555,12 @@ int bsk_attention_varlen_bwd(int dtype, const void* dO, int64_t do_token_stride,
   const unsigned prep = (unsigned)(2 + slots * p.head_groups);
   const unsigned gq = (unsigned)(slots * kv_heads < st->sm_count ? slots * kv_heads : st->sm_count);
   const unsigned gk = (unsigned)(key_slots * kv_heads < st->sm_count ? key_slots * kv_heads : st->sm_count);
-#define BSK_VARLEN_BWD(F16, DD)                                                                                        \
-  do {                                                                                                                 \
-    bsk::varattn_bwd_prep_kernel<F16, DD><<<prep, bsk::kPlanThreads, 0, s>>>(p);                                       \
-    bsk::varattn_bwd_dkdv_kernel<F16, DD><<<gk, bsk::kBwdThreads, bsk::BwdDkdvShape<F16, DD>::kSmemBytes, s>>>(tq, tk, \
-                                                                                                              tv, tdo, a); \
-    bsk::varattn_bwd_dq_kernel<F16, DD><<<gq, bsk::kBwdThreads, bsk::BwdDqShape<F16, DD>::kSmemBytes, s>>>(tq, tk, tv,  \
-                                                                                                          tdo, a);     \
-  } while (0)
-  if (f16 && dim == 128) BSK_VARLEN_BWD(true, 128);
-  else if (f16) BSK_VARLEN_BWD(true, 64);
-  else if (dim == 128) BSK_VARLEN_BWD(false, 128);
-  else BSK_VARLEN_BWD(false, 64);
-#undef BSK_VARLEN_BWD
+  cudaError_t e;
+  if (f16) e = dim == 128 ? varattn_bwd_launch<true, 128>(p, a, tq, tk, tv, tdo, prep, gk, gq, s)
+                          : varattn_bwd_launch<true, 64>(p, a, tq, tk, tv, tdo, prep, gk, gq, s);
+  else e = dim == 128 ? varattn_bwd_launch<false, 128>(p, a, tq, tk, tv, tdo, prep, gk, gq, s)
+                      : varattn_bwd_launch<false, 64>(p, a, tq, tk, tv, tdo, prep, gk, gq, s);
+  if (e != cudaSuccess) return cuda_fail(e, "attention_varlen_bwd launch");
   return launch_status("attention_varlen_bwd launch");
 }
 

@@ -95,6 +95,7 @@ struct VarPrepArgs {
 
 template <bool kF16, int kD>
 __global__ void __launch_bounds__(kPlanThreads) varattn_bwd_prep_kernel(const __grid_constant__ VarPrepArgs a) {
+  ptx::grid_launch_dependents();
   if (blockIdx.x < 2) {
     build_plan(a.plan[blockIdx.x]);
     return;
@@ -214,6 +215,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   WaitCtl ctl{abort_flag, a.err, a.timeout_ns, kKidVarAttnBwd};
   if (warp < 4) ptx::setmaxnreg_dec<kBwdRegsLow>();
 
+  ptx::grid_dependency_wait();
   const int n_items = *a.q_count * a.kv_heads;  // (entry, kv head), heads innermost
   const int cta = blockIdx.x, grid = gridDim.x, group = a.group, tt = kVarBlk / group;
   auto item_at = [&](int k, VarItem& it, int& hkv) -> bool {
@@ -546,6 +548,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   WaitCtl ctl{abort_flag, a.err, a.timeout_ns, kKidVarAttnBwd};
   if (warp < 4) ptx::setmaxnreg_dec<kBwdRegsLow>();
 
+  ptx::grid_launch_dependents();
+  ptx::grid_dependency_wait();
   const int n_items = *a.k_count * a.kv_heads;  // (entry, kv head), heads innermost
   const int cta = blockIdx.x, grid = gridDim.x, group = a.group, tt = kVarBlk / group;
   auto item_at = [&](int k, VarItem& it, int& hkv) -> bool {

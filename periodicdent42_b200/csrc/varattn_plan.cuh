@@ -204,7 +204,10 @@ __device__ __forceinline__ void build_plan(const PlanArgs& a) {
   }
 }
 
-__global__ void __launch_bounds__(kPlanThreads) varattn_plan_kernel(const PlanArgs a) { build_plan(a); }
+__global__ void __launch_bounds__(kPlanThreads) varattn_plan_kernel(const PlanArgs a) {
+  ptx::grid_launch_dependents();
+  build_plan(a);
+}
 
 // The k-th entry of CTA `cta` of `grid`: zigzag over the list of n entries. Returns -1 behind its end.
 __device__ __forceinline__ int zigzag(int k, int cta, int grid, int n) {

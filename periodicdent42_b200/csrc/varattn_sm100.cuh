@@ -198,6 +198,8 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
   ptx::tc_fence_after();
   const uint32_t tmem_base = *tmem_holder;
   WaitCtl ctl{abort_flag, a.err, a.timeout_ns, kKidVarAttn};
+  ptx::grid_launch_dependents();
+  ptx::grid_dependency_wait();  // the list; all of the above overlaps its construction
   const int n_items = *a.count * a.kv_heads;  // (entry, kv head), heads innermost
   const int cta = blockIdx.x, grid = gridDim.x;
   // Item k of this CTA; false behind the list's end.
@@ -818,6 +820,7 @@ constexpr int kCombineRows = 16;
 
 template <bool kF16, int kD>
 __global__ void __launch_bounds__(kCombineRows * kD / 4) varattn_combine_kernel(const VarCombineArgs a) {
+  ptx::grid_dependency_wait();
   if (static_cast<int>(blockIdx.x) >= a.count[1]) return;
   const VarSplit sp = a.splits[blockIdx.x];
   const int hkv = blockIdx.y, r = blockIdx.z * kCombineRows + threadIdx.x / (kD / 4), c = threadIdx.x % (kD / 4);

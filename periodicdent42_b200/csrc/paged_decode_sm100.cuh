@@ -137,14 +137,12 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4],
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// Two e4m3 codes (16 bits) -> two fp16 values, exactly.
-__device__ __forceinline__ uint32_t e4m3x2(uint16_t two) {
-  uint32_t h;
-  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(two));
-  return h;
+// Four e4m3 codes -> two pairs of fp16 values, exactly.
+__device__ __forceinline__ void e4m3x4(uint32_t four, uint32_t& lo, uint32_t& hi) {
+  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
+      : "=r"(lo), "=r"(hi)
+      : "r"(four));
 }
-__device__ __forceinline__ uint32_t e4m3x2_lo(uint32_t four) { return e4m3x2(static_cast<uint16_t>(four & 0xffffu)); }
-__device__ __forceinline__ uint32_t e4m3x2_hi(uint32_t four) { return e4m3x2(static_cast<uint16_t>(four >> 16)); }
 
 __device__ __forceinline__ float log2f_approx(float x) {
   float y;
@@ -443,7 +441,9 @@ __global__ void __launch_bounds__(32 * PagedShape<kD, kFp8, kNQ>::kMaxWarps) pag
           const uint32_t u[4] = {u4.x, u4.y, u4.z, u4.w}, v[4] = {v4.x, v4.y, v4.z, v4.w};
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            const uint32_t f[4] = {e4m3x2_lo(u[k]), e4m3x2_lo(v[k]), e4m3x2_hi(u[k]), e4m3x2_hi(v[k])};
+            uint32_t f[4];
+            e4m3x4(u[k], f[0], f[2]);
+            e4m3x4(v[k], f[1], f[3]);
 #pragma unroll
             for (int q = 0; q < kNQ; ++q)
               mma_16816<kMF16>(kChains == 2 && (k & 1) ? sc1[j][q] : sc[j][q], f, qf[q][4 * h + k][0], qf[q][4 * h + k][1]);
@@ -585,7 +585,9 @@ __global__ void __launch_bounds__(32 * PagedShape<kD, kFp8, kNQ>::kMaxWarps) pag
           for (int b = 0; b < 2; ++b) {  // columns 2 b and 2 b + 1 of word i
             const uint32_t u = __byte_perm(w[0][i], w[1][i], b ? 0x7362 : 0x5140);
             const uint32_t v = __byte_perm(w[2][i], w[3][i], b ? 0x7362 : 0x5140);
-            const uint32_t f[4] = {e4m3x2_lo(u), e4m3x2_hi(u), e4m3x2_lo(v), e4m3x2_hi(v)};
+            uint32_t f[4];
+            e4m3x4(u, f[0], f[1]);
+            e4m3x4(v, f[2], f[3]);
 #pragma unroll
             for (int q = 0; q < kNQ; ++q) mma_16816<kMF16>(o[2 * i + b][q], f, pf[q][0], pf[q][1]);
           }

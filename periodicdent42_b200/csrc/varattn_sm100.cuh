@@ -723,10 +723,11 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
             for (int z = 0; z < 4; ++z) {
               const uint32_t u[4] = {w[z].x & live, w[z].y & live, w[z].z & live, w[z].w & live};
               uint8_t* d = dst + (y >> 2) * kAttnChunk;
-              *reinterpret_cast<uint4*>(d + (((2 * z) ^ (r & 7)) << 4)) =
-                  make_uint4(e4m3x2_lo(u[0]), e4m3x2_hi(u[0]), e4m3x2_lo(u[1]), e4m3x2_hi(u[1]));
-              *reinterpret_cast<uint4*>(d + (((2 * z + 1) ^ (r & 7)) << 4)) =
-                  make_uint4(e4m3x2_lo(u[2]), e4m3x2_hi(u[2]), e4m3x2_lo(u[3]), e4m3x2_hi(u[3]));
+              uint32_t f[8];
+#pragma unroll
+              for (int i = 0; i < 4; ++i) e4m3x4(u[i], f[2 * i], f[2 * i + 1]);
+              *reinterpret_cast<uint4*>(d + (((2 * z) ^ (r & 7)) << 4)) = make_uint4(f[0], f[1], f[2], f[3]);
+              *reinterpret_cast<uint4*>(d + (((2 * z + 1) ^ (r & 7)) << 4)) = make_uint4(f[4], f[5], f[6], f[7]);
             }
           }
           ptx::fence_proxy_async_smem();

@@ -149,6 +149,67 @@ def test_another_stream_and_captured_graph(no_device_error, cuda_dev):
             assert torch.equal(out, want)
 
 
+@pytest.mark.parametrize("new,kv", [([3], [200]), ([150], [400])])  # either kernel
+def test_non_finite_keys_reach_the_rows_that_see_them_only(no_device_error, cuda_dev, new, kv):
+    for e4m3 in (False, True):
+        q, c, table, lens, cu = make(new, kv, 4, 2, 64, 16, torch.bfloat16, cuda_dev, e4m3)
+        want = bsk.attention_paged(q, block_table=table, kv_lens=lens, cu_seqlens=cu, **c)
+        p = kv[0] - 2  # seen by the last two new tokens
+        page, off = int(table[0, p // 16]), p % 16
+        # (a row of infinities gives sums of both signs, NaN; an infinite scale would give +inf or, rightly, -inf: weight 0)
+        for bad in (float("nan"),) if e4m3 else (float("nan"), float("inf")):
+            if e4m3:
+                c["k_scale"][page, off, 1] = bad
+            else:
+                c["k_cache"][page, off, 1] = bad
+            got = bsk.attention_paged(q, block_table=table, kv_lens=lens, cu_seqlens=cu, **c)
+            assert torch.equal(got[:-2], want[:-2]) and torch.equal(got[-2:, :2], want[-2:, :2])
+            assert torch.isnan(got[-2:, 2:]).all()
+
+
+def test_cache_behind_two_to_the_31_elements(no_device_error, cuda_dev):
+    """Slots whose elements lie more than 2^31 behind the cache's start, written, read back and attended to."""
+    G, D, page = 8, 128, 64
+    pages = (2 ** 31 // (G * D) + 4096) // page
+    c = {n: torch.zeros(pages, page, G, D, dtype=torch.bfloat16, device=cuda_dev) for n in ("k_cache", "v_cache")}
+    g = torch.Generator(device=cuda_dev).manual_seed(0)
+    L = 700
+    k, v = (torch.randn(L, G, D, generator=g, device=cuda_dev).bfloat16() for _ in range(2))
+    order = pages - 1 - torch.randperm(40, generator=g, device=cuda_dev)[: -(-L // page)]
+    at = torch.arange(L, device=cuda_dev)
+    slots = order[at // page] * page + at % page
+    assert int(slots.min()) * G * D > 2 ** 31
+    bsk.kv_cache_append(k, v, slots=slots, **c)
+    kr, vr = bsk.kv_cache_gather(slots=slots, **c)
+    assert torch.equal(kr, k) and torch.equal(vr, v)
+    table = order[None].int()
+    for n in (2, 100):
+        q = torch.randn(n, 16, D, generator=g, device=cuda_dev).bfloat16()
+        out = bsk.attention_paged(q, block_table=table, kv_lens=torch.tensor([L], device=cuda_dev),
+                                  cu_seqlens=torch.tensor([0, n], device=cuda_dev), **c)
+        allowed = torch.arange(L, device=cuda_dev) <= (L - n + torch.arange(n, device=cuda_dev))[:, None]
+        for h in (0, 7, 15):
+            want, bound = pa.attention64(q[:, h], k[:, h // 2], v[:, h // 2], allowed, D ** -0.5, q.dtype)[:2]
+            assert pa.worst(out[:, h], want, bound) <= 1.0
+
+
+def test_two_streams_at_once(no_device_error, cuda_dev):
+    """Calls that run side by side share nothing: each gives what it gives alone."""
+    jobs = [make(new, kv, 8, 2, 128, 16, torch.bfloat16, cuda_dev, e4m3, seed=i)
+            for i, (new, kv, e4m3) in enumerate([([40], [5000], False), ([40], [5000], True), ([1] * 9, [3000] * 9, True),
+                                                 ([300, 20], [900, 2000], False)])]
+    alone = [bsk.attention_paged(q, block_table=t, kv_lens=n, cu_seqlens=u, **c) for q, c, t, n, u in jobs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in jobs]
+    for _ in range(5):
+        outs = []
+        for s, (q, c, t, n, u) in zip(streams, jobs):
+            with torch.cuda.stream(s):
+                outs.append(bsk.attention_paged(q, block_table=t, kv_lens=n, cu_seqlens=u, **c))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs, alone))
+
+
 def test_bad_indices_are_reported_not_followed(cuda_dev):
     assert _capi.device_error() == 0
     for new, kv in (([1, 2], [40, 70]), ([150, 200], [400, 300])):

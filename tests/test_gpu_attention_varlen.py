@@ -72,6 +72,26 @@ def test_neighbours_do_not_reach_in(no_device_error, cuda_dev):
             assert torch.equal(got[n][77:280], want[n][77:280]), n
 
 
+def test_non_finite_values_reach_the_rows_that_see_them_only(no_device_error, cuda_dev):
+    """A NaN key is seen by itself and later rows; a NaN query row by itself, its dQ and (through dK, dV) all keys it sees."""
+    q, k, v, do, cu = make([300], 4, 2, 64, torch.bfloat16, cuda_dev)
+    want = grads(q, k, v, do, cu)
+    k2 = k.clone()
+    k2[200, 1, 3] = float("nan")
+    got = grads(q, k2, v, do, cu)
+    assert torch.equal(got["O"][:200], want["O"][:200]) and torch.equal(got["O"][200:, :2], want["O"][200:, :2])
+    assert torch.isnan(got["O"][200:, 2:]).all() and torch.isnan(got["dQ"][200:, 2:]).all()
+    q2 = q.clone()
+    q2[100, 0, 5] = float("inf")
+    got = grads(q2, k, v, do, cu)
+    rows = torch.ones(300, 4, dtype=torch.bool, device=cuda_dev)
+    rows[100, 0] = False
+    for n in ("O", "dQ"):
+        assert torch.equal(got[n][rows], want[n][rows]) and torch.isnan(got[n][100, 0]).all()
+    assert torch.equal(got["dK"][:, 1], want["dK"][:, 1]) and torch.isnan(got["dK"][:101, 0]).any(-1).all()
+    assert torch.equal(got["dK"][128:, 0], want["dK"][128:, 0])  # keys behind the row's last block
+
+
 def test_rows_behind_the_last_sequence_are_zero(no_device_error, cuda_dev):
     q, k, v, do, cu = make([100, 30, 171], 4, 2, 64, torch.float16, cuda_dev)
     want = grads(q[:130], k[:130], v[:130], do[:130], cu[:3])

@@ -394,8 +394,10 @@ int bsk_kv_cache_gather(int dtype, const void* k_cache, const void* v_cache, int
  *   cu_seqlens int32 [batch + 1], cu_seqlens[0] = 0, non-decreasing, at most `tokens`; kv_lens int32 [batch],
  *   at most table_width * page_size; entries outside their range are clamped, a page outside [0, num_pages) reads as
  *   zeros, and either sets the device error word.
+ *   A non-finite K reaches the rows that see it; a non-finite V also those of the same 128-key block that do not (their
+ *   weight is zero, and 0 x NaN is NaN). Cache contents behind a sequence's end reach nothing.
  *   workspace: device memory of bsk_attention_paged_workspace_bytes(...) bytes (may be 0), 16-byte aligned, not shared
- *   by calls that may run at the same time.
+ *   by calls that may run at the same time. The size depends on the current device.
  * No reference counterpart.
  */
 int bsk_attention_paged(int dtype, const void* Q, int64_t q_token_stride, int64_t q_head_stride, const void* k_cache,
@@ -413,6 +415,7 @@ int64_t bsk_attention_paged_workspace_bytes(int tokens, int batch, int heads, in
  * lse and writes contiguous dQ, dK, dV:
  *   dV = P^T dO,  dS = P * (dO V^T - rowsum(dO * O)),  dQ = scale * dS K,  dK = scale * dS^T Q
  * with dK, dV summed over the heads of a group, in a fixed order (no atomics). Rows behind the last sequence are zero.
+ * Sequences do not reach into one another, whatever their values; within one, non-finite values as in bsk_attention_paged.
  * workspace: device memory of bsk_attention_varlen_workspace_bytes(...) bytes, 16-byte aligned, not shared by calls
  * that may run at the same time. No reference counterpart.
  */

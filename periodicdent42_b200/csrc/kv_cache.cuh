@@ -9,7 +9,8 @@
 // The quotients are taken by Markstein's method (P. Markstein, "Computation of elementary functions on the IBM RISC System/6000
 // processor", 1990): with y the correctly rounded reciprocal of the scale, q = x y, r = q scale - x (exact in one fused
 // operation) and q - r y is the correctly rounded x / scale (in this form of the signs, also for x = -0). Three packed operations for two elements in place of a division
-// each (16 divisions a thread made the kernel issue-bound: 33 us for 16383 tokens of 8 heads, D 128, where the memory takes 16).
+// each. The quantising write stays bound by instruction issue: 16383 tokens of 8 heads, D 128, take 27 us (33 with the
+// divisions), where the memory would take 16; reading back takes the memory's time.
 //
 // Bound: HBM, each row is read and written once. One thread holds 8 elements of a K row and the same 8 of the V row
 // (independent 16-byte loads, of one row when there are few, else of two); D / 8 neighbouring lanes share a row and take its maximum by shuffles.

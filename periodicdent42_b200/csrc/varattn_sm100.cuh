@@ -73,7 +73,9 @@ struct VarShape {
   static constexpr int kStages = kE4m3 ? 3 : 0;              // staging ring of code tiles
   static constexpr int kStageBytes = kVarBlk * kD;
   // barriers 512 B, sums and maxima, and for e4m3: [2 buffers] keys' and values' scales, [2] rows' scales, [2] 2^-R steps
-  static constexpr int kSmallBytes = 512 + 3 * 128 * 4 + (kE4m3 ? (2 * 256 + 2 * 128 + 4) * 4 : 0);
+  // and [kEnds] items' closing factors
+  static constexpr int kEnds = 3;
+  static constexpr int kSmallBytes = 512 + 3 * 128 * 4 + (kE4m3 ? (2 * 256 + 2 * 128 + 2 + kEnds) * 4 : 0);
   static constexpr int kSmemBytes = 1024 + kTile * (2 + kSlots) + kStages * kStageBytes + kSmallBytes;
   static constexpr uint32_t kFmt = kF16 || kE4m3 ? 0u : 1u;  // tcgen05 kind::f16 operands: 0 f16, 1 bf16
   static_assert(kSmemBytes <= 232448, "shared memory above the 227 KB per-CTA limit");
@@ -145,7 +147,11 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
   float* k_sc = m_row + 128;  // e4m3: [2][128] keys' scales
   float* v_sc = k_sc + 256;   // [2][128] values' scales / 2^R
   float* q_sc = v_sc + 256;   // [2][128] what the query rows were divided by
-  float* r_step = q_sc + 256; // [2] 2^(R before - R) of the block; [2] what an item's O is multiplied by at its end
+  float* r_step = q_sc + 256; // [2] 2^(R before - R) of the block
+  // [kEnds] What an item's O is multiplied by at its end. Warp 3 writes an item's when the softmax of the block two before
+  // its last is over, which may be two items back: of item i it writes while the output warps may still have to read those
+  // of items i - 1 and i - 2. Item i - 3 is written: its output warps convert item i - 2's tiles only after that.
+  float* r_end = r_step + 2;
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -449,7 +455,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
             }
             if (lane == 0) {
               r_step[buf] = b == it.b0 ? 1.0f : __int_as_float(max(127 + before - r_exp, 0) << 23);
-              if (b == it.b1 - 1) r_step[2 + (rows & 1)] = __int_as_float((r_exp - 6) << 23);
+              if (b == it.b1 - 1) r_end[rows % Sh::kEnds] = __int_as_float((r_exp - 6) << 23);
             }
             __syncwarp();
             if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&sc_full[buf]));
@@ -743,6 +749,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       if (ok) ok = warp_wait_bounded<false, 256>(ptx::smem_u32(&o_done[rows & 1]), (rows >> 1) & 1, ctl, 22);
       if (!ok) break;
       const uint32_t ob = rows & 1, tO = tO0 + 128 * ob;
+      const float* end = r_end + rows % Sh::kEnds;
       ++rows;
       ptx::tc_fence_after();
       const float m_run = m_row[r];
@@ -753,7 +760,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       // of +inf (scores beyond fp32) gives NaN, as the definition does.
       const bool none = m_run == -INFINITY;
       float inv_l = m_run == INFINITY ? NAN : 1.0f / l_tot;
-      if constexpr (kE4m3) inv_l *= r_step[2 + ob];
+      if constexpr (kE4m3) inv_l *= *end;
       if constexpr (kPaged) {
         if (it.part >= 0) {  // one of several pieces: fp32 rows and their log2 sums, for the combining kernel
           const int64_t prow = (static_cast<int64_t>(it.part) * a.kv_heads + hkv) * kVarBlk + r;

@@ -1,0 +1,68 @@
+"""Attention over e4m3 caches where the values' scales differ: between sequences and heads, between keys, and rows of
+zeros -- against the 64-bit definition, elementwise within the roundings' bound."""
+import pytest
+import torch
+
+import periodicdent42_b200 as bsk
+from oracle import packed_attention as pa
+
+pytestmark = pytest.mark.gpu
+
+
+def make(new, kv, H, G, D, page, dtype, dev, seed, value_size):
+    """Inputs of one call over an e4m3 cache, pages in random order; value_size [sequences, longest, kv heads] multiplies
+    the value rows. Scales behind a sequence's end are NaN."""
+    g = torch.Generator(device=dev).manual_seed(seed)
+    need = [-(-n // page) for n in kv]
+    order = torch.randperm(sum(need), generator=g, device=dev)
+    table = torch.full((len(kv), max(need)), -1, dtype=torch.int32, device=dev)
+    k, v = (torch.randn(sum(need), page, G, D, generator=g, device=dev) for _ in range(2))
+    first = 0
+    held = torch.zeros(sum(need), page, dtype=torch.bool, device=dev)
+    for i, (n, p) in enumerate(zip(kv, need)):
+        at = order[first:first + p]
+        table[i, :p] = at
+        size = torch.ones(p * page, G, device=dev)
+        size[:n] = value_size[i, :n]
+        v[at] *= size.view(p, page, G, 1)
+        held[at] = (torch.arange(p * page, device=dev) < n).view(p, page)
+        first += p
+    c = {}
+    for n, x in (("k", k), ("v", v)):
+        c[n + "_cache"], c[n + "_scale"] = pa.quantise_rows(x)
+        c[n + "_scale"][~held] = float("nan")
+    q = torch.randn(sum(new), H, D, generator=g, device=dev).to(dtype)
+    at = dict(block_table=table, kv_lens=torch.tensor(kv, dtype=torch.int32, device=dev),
+              cu_seqlens=torch.tensor([0] + new, device=dev).cumsum(0).int())
+    return q, c, at
+
+
+def worst(out, q, c, at, kv, new):
+    want = pa.paged64(q, c["k_cache"], c["v_cache"], at["block_table"], kv, new, q.shape[2] ** -0.5, c["k_scale"], c["v_scale"])
+    return pa.worst(out, *want)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("D", [64, 128])
+def test_many_short_sequences(no_device_error, cuda_dev, D, dtype):
+    """More entries than CTAs several times over, each of a single key block, with values of another size for every
+    sequence and head: each entry's results carry its own scale."""
+    new = [20 + i % 60 for i in range(100)]
+    g = torch.Generator(device=cuda_dev).manual_seed(7)
+    size = torch.exp2(torch.randint(-8, 9, (100, 1, 8), generator=g, device=cuda_dev).float()).expand(-1, 80, -1)
+    q, c, at = make(new, new, 16, 8, D, 16, dtype, cuda_dev, D, size)
+    out = bsk.attention_paged(q, **at, **c)
+    assert worst(out, q, c, at, new, new) <= 1.0
+    for _ in range(3):
+        assert torch.equal(out, bsk.attention_paged(q, **at, **c))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_values_that_grow_along_the_sequence(no_device_error, cuda_dev, dtype):
+    """The scale reference moves from block to block (and the outputs so far with it), up and down."""
+    new, kv = [700, 60, 90], [900, 700, 90]
+    size = torch.exp2(torch.arange(900, device=cuda_dev) // 128 * 2.0 - 6)[None, :, None].repeat(3, 1, 2)
+    size[1] = size[1].flip(0)
+    q, c, at = make(new, kv, 4, 2, 128, 32, dtype, cuda_dev, 1, size)
+    out = bsk.attention_paged(q, **at, **c)
+    assert worst(out, q, c, at, kv, new) <= 1.0

@@ -691,7 +691,10 @@ __global__ void __launch_bounds__(32 * PagedShape<kD, kFp8, kNQ>::kMaxWarps) pag
       acc.z += v.z * f;
       acc.w += v.w * f;
     }
-    const float inv = l == 0.0f ? 0.0f : ex2_approx(wsub - ms) / l;  // a row without keys is zero
+    // A row without keys is zero; so is one whose values' scales are all zero, whatever its scores are (m_w = -inf: every
+    // weight was zero, and 2^-m may be infinite).
+    const float up = w == -INFINITY ? 1.0f : ex2_approx(wsub - ms);
+    const float inv = l == 0.0f ? 0.0f : up / l;
     const int64_t t = lo + (row0 + row) / a.group;
     const int h = hkv * a.group + static_cast<int>((row0 + row) % a.group);
     reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.O) + (t * a.heads + h) * kD)[c] =

@@ -592,7 +592,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         const bool move = !(mbs <= m_run + 8.0f);  // the reference maximum lags by at most 8: P <= 2^8; a NaN moves it
         float alpha = 1.0f;
         if (move) alpha = (m_run == -INFINITY) ? 0.0f : ex2_approx(m_run - mbs);
-        if (move) m_run = mbs;
+        if (move) m_run = max_nan(m_run, mbs);  // (a NaN stays, also through blocks that this row does not see)
         float step = 1.0f;  // O follows the values' scale reference
         if constexpr (kE4m3) step = r_step[b];
         const bool need_rescale = __any_sync(0xffffffffu, (move || step != 1.0f) && j > 0);

@@ -5,7 +5,8 @@ The bounds count roundings (u = eps / 2 of the type, u32 = 2^-24) and nothing el
   scores    fp32 sums of D exact products, scaled and exponentiated: a weight's relative error is at most
             e_w = 2 ((D + 8) u32 scale max_j sum_d |q_d k_jd| + 2.1e-4 + L 2^-24), twice since the sum of L weights has it
             too; 2.1e-4 covers the softmax's exponentials (each off by at most 1.05e-4).
-  O         sum_j P_j v_j with P rounded to 16 bits:  |dO| <= u |O| + (u_p + e_w) sum_j P_j |v_j| + tiny_p max_j|v_j| L
+  O         sum_j P_j v_j with P rounded to 16 bits:  |dO| <= u |O| + (u_p + e_w) sum_j P_j |v_j| + tiny_p sum_j |v_j|
+            (over an e4m3 cache the rounded weights are P_j times the values' scales, in fp16: see paged64)
   dV, dK, dQ: see gradients64."""
 from __future__ import annotations
 
@@ -47,8 +48,9 @@ def quantise_rows(x):
     return q.to(torch.float8_e4m3fn), scale
 
 
-def attention64(q, k, v, allowed, scale, dtype, p_dtype=None):
-    """One head: q [n, d], k, v [l, d] in any type, allowed [n, l]. Returns (O, bound, P, lse, e_w) in 64 bits."""
+def attention64(q, k, v, allowed, scale, dtype, p_dtype=None, p_tiny=None):
+    """One head: q [n, d], k, v [l, d] in any type, allowed [n, l]. P is rounded to p_dtype (default: dtype), with an absolute
+    error of p_tiny below its normal range. Returns (O, bound, P, lse, e_w) in 64 bits."""
     q, k, v = q.double(), k.double(), v.double()
     s = (q @ k.t() * scale).masked_fill(~allowed, -math.inf)
     lse = torch.logsumexp(s, -1) if k.shape[0] else torch.full((q.shape[0],), -math.inf, dtype=torch.float64, device=q.device)
@@ -60,7 +62,7 @@ def attention64(q, k, v, allowed, scale, dtype, p_dtype=None):
     top = mass.amax(-1, keepdim=True) if k.shape[0] else torch.zeros_like(some, dtype=torch.float64)
     e_w = 2 * ((q.shape[1] + 8) * U32 * top + EXP + max(1, k.shape[0]) * U32)
     reach = (allowed.double() @ v.abs())
-    bound = u * o.abs() + (half_step(pt) + e_w) * (p @ v.abs()) + tiny(pt) * reach + tiny(dtype)
+    bound = u * o.abs() + (half_step(pt) + e_w) * (p @ v.abs()) + (tiny(pt) if p_tiny is None else p_tiny) * reach + tiny(dtype)
     return o, bound, p, lse, e_w
 
 
@@ -116,7 +118,10 @@ def packed64(q, k, v, lens, causal, scale, do=None):
 
 def paged64(q, k_cache, v_cache, block_table, kv_lens, new, scale, k_scale=None, v_scale=None):
     """(O, bound) of attention over a paged cache; kv_lens and new are lists. Codes are multiplied by their scales in 64
-    bits; with e4m3 codes P is rounded to bf16 after its product with the values' scale (one more fp32 rounding)."""
+    bits. With e4m3 codes the weights P_j s_j (s_j: the value's scale; their product is one more fp32 rounding, which e_w's
+    factor of two has room for) are rounded to fp16 and meet the codes. They are brought near 1 first, so fp16's absolute
+    error of 2^-25 counts in units of the row's largest P_j s_j, or, where the reference is the largest scale alone, of 2^-6
+    of that (weights up to 2^7 are left room for): 2^-25 max(max_j P_j s_j, 2^-6 max_j s_j) sum_j |code_j|."""
     T, H, D = q.shape
     kv_heads, page = k_cache.shape[2], k_cache.shape[1]
     G = H // kv_heads
@@ -126,17 +131,29 @@ def paged64(q, k_cache, v_cache, block_table, kv_lens, new, scale, k_scale=None,
     for i, (n, L) in enumerate(zip(new, kv_lens)):
         pages = block_table[i, : -(-L // page)].long()
 
-        def rows(cache, sc):
-            x = torch.stack([cache[p].to(torch.float64) for p in pages.tolist()]).flatten(0, 1)[:L] if L else \
+        def rows(cache):
+            return torch.stack([cache[p].to(torch.float64) for p in pages.tolist()]).flatten(0, 1)[:L] if L else \
                 torch.zeros(0, kv_heads, D, dtype=torch.float64, device=q.device)
-            return x if sc is None else x * sc[pages].flatten(0, 1)[:L, :, None].double()
 
-        k, v = rows(k_cache, k_scale), rows(v_cache, v_scale)
+        def scales(sc):
+            return sc[pages].flatten(0, 1)[:L, :, None].double()
+
+        k, v = rows(k_cache), rows(v_cache)
+        if k_scale is not None:
+            codes, sv = v.abs(), scales(v_scale)
+            k, v = k * scales(k_scale), v * sv
         pos = L - n + torch.arange(n, device=q.device)
         allowed = torch.arange(L, device=q.device)[None, :] <= pos[:, None]
-        pt = q.dtype if k_scale is None else torch.bfloat16
         for h in range(H):
-            val, bound = attention64(q[a:a + n, h], k[:, h // G], v[:, h // G], allowed, scale, q.dtype, pt)[:2]
+            c = h // G
+            if k_scale is None:
+                val, bound = attention64(q[a:a + n, h], k[:, c], v[:, c], allowed, scale, q.dtype)[:2]
+            else:
+                val, bound, p = attention64(q[a:a + n, h], k[:, c], v[:, c], allowed, scale, q.dtype, torch.float16, 0.0)[:3]
+                if L:
+                    s = sv[:, c, 0]
+                    unit = torch.maximum((p * s).amax(-1), (allowed * s).amax(-1) * 2.0 ** -6)
+                    bound = bound + tiny(torch.float16) * unit[:, None] * (allowed.double() @ codes[:, c])
             o[a:a + n, h], b[a:a + n, h] = val, bound
         a += n
     return o, b

@@ -73,7 +73,7 @@ def test_rows_of_zeros_among_the_values(no_device_error, cuda_dev, dtype):
     """Value rows of zeros (scale 0) with scores far below zero: all of them zero, and one of three."""
     zero = torch.zeros(1, 300, 2, device=cuda_dev)
     some = (torch.arange(300, device=cuda_dev) % 3 > 0)[None, :, None].float().expand(-1, -1, 2)
-    for new, size in ((1, zero), (200, zero), (1, some)):  # either kernel
+    for new, size in ((1, zero), (200, zero), (200, some), (1, some)):  # either kernel
         q, c, at = make([new], [300], 4, 2, 128, 16, dtype, cuda_dev, 2, size)
         q.abs_().add_(2.0).mul_(8.0)
         c["k_cache"].view(torch.uint8).bitwise_or_(0x80)  # every key opposite to every query

@@ -22,14 +22,16 @@
 // e4m3 caches (kKind 2): both products are fp16 products. Warps 12-15, which otherwise only write results, convert: codes
 // arrive by the same copies in a staging ring, a thread takes a key's row and writes it as fp16 (one instruction for two
 // codes, exact) to the K / V ring, rows behind the sequence as zeros. Warp 3 brings the blocks' scales. The keys' scales
-// multiply the scores. The values' scales multiply P, brought near 1 by a power of two R that follows the largest scale
-// seen (O is rescaled when R grows), so that P * scale stays within fp16's range: values' scales down to 2^-20 of the
-// largest keep P's full precision. bf16 queries are turned into fp16 in place, each row by its own power of two (exact but
-// for elements 2^-39 below the row's largest).
+// multiply the scores. The values' scales multiply P, brought near 1 by a power of two R of each row that follows the
+// largest scale that the row has seen (O is rescaled when R grows), so that P * scale stays within fp16's range: values'
+// scales down to 2^-20 of that keep P's full precision. Warp 3 divides the scales by the tile's largest power of two; in the
+// last blocks, where a row may not see the key that it came from, the rest to the row's own goes into the exponent of P
+// (done in every block, this took a sixth more time). bf16 queries are turned into fp16 in place, each row by its own power
+// of two (exact but for elements 2^-39 below the row's largest).
 // Bound here: the conversion's one warp per sub-partition beside the softmax's two (8100 warp instructions a block where
-// 16-bit caches take 4100). Its loops are not unrolled further than they are: the roles share the instruction cache, and
-// with more code they wait for instructions (1024 new tokens over 30000, 32 / 8 heads, D 128: 1500 us unrolled, 1120 so;
-// with the values' scales multiplied in the conversion 1480; 16-bit cache 555).
+// 16-bit caches take 4100), and instructions: the roles share the instruction cache, and with more code in their loops they
+// wait for it. So the conversion's and the two issuers' loops are rolled (1024 new tokens over 30000, 32 / 8 heads, D 128:
+// 1039 us; conversion unrolled 1126, issuers unrolled 1189, both 1203; 16-bit cache 553).
 //
 // Bound: the tensor pipe and the softmax share the time (4 D flops and one exponential per score; see the forward's trace
 // in bsattn_sm100.cuh). Packing the group's heads into the tile means a causal tile spans only TT tokens, so less of its
@@ -61,6 +63,10 @@ __device__ __forceinline__ void zero_tile_rows(uint8_t* tile, int chunks, int fi
   }
 }
 
+// Exponent fields that value scales count as (e4m3 caches): 2^(133 - field) and 2^(field - 133) are normal numbers. A row's
+// reference is at most kScaleSpan below its tile's, so that 2^8 * 2^kScaleSpan, 64 times, is finite.
+constexpr int kScaleLow = 20, kScaleHigh = 240, kScaleSpan = 110;
+
 // Where the K / V rows come from.
 enum : int { kPacked = 0, kCache16 = 1, kCacheE4m3 = 2 };
 
@@ -72,10 +78,9 @@ struct VarShape {
   static constexpr int kSlots = kE4m3 && kD == 128 ? 3 : 5;  // K / V ring
   static constexpr int kStages = kE4m3 ? 3 : 0;              // staging ring of code tiles
   static constexpr int kStageBytes = kVarBlk * kD;
-  // barriers 512 B, sums and maxima, and for e4m3: [2 buffers] keys' and values' scales, [2] rows' scales, [2] 2^-R steps
-  // and [kEnds] items' closing factors
-  static constexpr int kEnds = 3;
-  static constexpr int kSmallBytes = 512 + 3 * 128 * 4 + (kE4m3 ? (2 * 256 + 2 * 128 + 2 + kEnds) * 4 : 0);
+  // barriers 512 B, sums and maxima, and for e4m3, two of each: keys' and values' scales, exponents of the largest value scale
+  // up to a key, rows' scales, rows' closing factors, the tile's exponent, the one before, its step
+  static constexpr int kSmallBytes = 512 + 3 * 128 * 4 + (kE4m3 ? (5 * 256 + 6) * 4 : 0);
   static constexpr int kSmemBytes = 1024 + kTile * (2 + kSlots) + kStages * kStageBytes + kSmallBytes;
   static constexpr uint32_t kFmt = kF16 || kE4m3 ? 0u : 1u;  // tcgen05 kind::f16 operands: 0 f16, 1 bf16
   static_assert(kSmemBytes <= 232448, "shared memory above the 227 KB per-CTA limit");
@@ -145,13 +150,13 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
   float* l_part = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(bars) + 512);  // [2 halves][128 rows]
   float* m_row = l_part + 256;                                                       // [128 rows]
   float* k_sc = m_row + 128;  // e4m3: [2][128] keys' scales
-  float* v_sc = k_sc + 256;   // [2][128] values' scales / 2^R
+  float* v_sc = k_sc + 256;   // [2][128] values' scales / 2^(exponent of the tile)
   float* q_sc = v_sc + 256;   // [2][128] what the query rows were divided by
-  float* r_step = q_sc + 256; // [2] 2^(R before - R) of the block
-  // [kEnds] What an item's O is multiplied by at its end. Warp 3 writes an item's when the softmax of the block two before
-  // its last is over, which may be two items back: of item i it writes while the output warps may still have to read those
-  // of items i - 1 and i - 2. Item i - 3 is written: its output warps convert item i - 2's tiles only after that.
-  float* r_end = r_step + 2;
+  int* v_top = reinterpret_cast<int*>(q_sc + 256);  // [2][128] exponent field of the largest value scale up to key i
+  float* r_end = reinterpret_cast<float*>(v_top + 256);  // [2][128] what the rows' O is multiplied by at the end of alternate items
+  int* r_tile = reinterpret_cast<int*>(r_end + 256);     // [2] exponent field of the tile's largest value scale so far
+  int* r_before = r_tile + 2;                            // [2] that before the block
+  float* r_step = reinterpret_cast<float*>(r_tile + 4);  // [2] 2^(r_before - r_tile)
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -360,7 +365,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
             if (!ok) break;
             ptx::tc_fence_after();
             const uint64_t qd = qdesc0 + ((qbuf * kTile) >> 4), kd = kdesc0 + ((sl * kTile) >> 4);
-#pragma unroll
+#pragma unroll(kE4m3 ? 1 : kD / 16)
             for (int x = 0; x < kD / 16; ++x) {
               const uint32_t qo = ((x >> 2) * kAttnChunk + (x & 3) * 32) >> 4, ko = ((x >> 2) * kChunkPitch + (x & 3) * 32) >> 4;
               ptx::mma_f16_ss(tmem_base + 128 * b, qd + qo, kd + ko, IDESC_S, x != 0);
@@ -382,7 +387,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
             ptx::tc_fence_after();
             const uint64_t vd = vdesc0 + ((sl * kTile) >> 4);
             const uint32_t t_o = tmem_base + kAttnTmemO + 128 * (rows & 1), t_p = tmem_base + 128 * b;
-#pragma unroll
+#pragma unroll(kE4m3 ? 1 : 8)
             for (int x = 0; x < 8; ++x)  // K step x: keys [16x, 16x+16) in P columns 8x (+32 for the second half)
               ptx::mma_f16_ts(t_o, t_p + 8 * x + (x >= 4 ? 32 : 0), vd + ((2 * x * kGroupPitch) >> 4), IDESC_PV,
                               (j == 0 && x == 0) ? 0u : 1u);
@@ -411,7 +416,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     if constexpr (kE4m3) {
       // Lane l has keys l, l + 32, l + 64, l + 96 of a block. Pages are looked up two blocks ahead of their scales' use and
       // scales one, so neither load is waited for; behind the sequence, and on a bad page, a scale is 0.
-      uint32_t g = 0, rows = 0;
+      uint32_t g = 0;
       for (int k = 0; ok && item_at(k, it, hkv); ++k) {
         if (it.b1 <= it.b0) continue;
         int page[4] = {-1, -1, -1, -1};
@@ -434,7 +439,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
             vs[x] = held ? __ldg(a.v_scale + at) : 0.0f;
           }
         };
-        int r_exp = 0;  // exponent field of the largest value scale so far (R): P * scale * 2^(6 - R) stays below 2^15
+        int r_exp = kScaleLow;  // the tile's largest value scale so far: a scale divided by 2^(r_exp - 133) is below 2^7
         for (int b = it.b0 - 2; b < it.b1; ++b) {  // (two rounds of lookups before the first block)
           if (b >= it.b0) {
             const uint32_t buf = g & 1;
@@ -443,19 +448,38 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
               if (!ok) break;
             }
             ++g;
-            const float most = fmaxf(fmaxf(vs[0], vs[1]), fmaxf(vs[2], vs[3]));
-            const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(most) & 0x7fffffffu);
-            const int want = min(max(static_cast<int>(top >> 23), 20), 240), before = r_exp;
-            if (b == it.b0 || want > r_exp) r_exp = want;
-            const float down = __int_as_float((260 - r_exp) << 23);  // 2^7 / 2^(R + 1)
+            int top[4], before = r_exp;  // exponents (a scale that is not finite counts as none)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              const int e = static_cast<int>(__float_as_uint(vs[x]) >> 23) & 255;
+              top[x] = e == 255 ? kScaleLow : min(max(e, kScaleLow), kScaleHigh);
+            }
+            int most[4];
+#pragma unroll
+            for (int x = 0; x < 4; ++x) most[x] = __reduce_max_sync(0xffffffffu, top[x]);
+            if (b >= min((it.pos0 + 1) >> 7, it.b1 - 1)) {  // some row may not see all of the block: the largest up to each key
+#pragma unroll 1
+              for (int o = 1; o < 32; o <<= 1)
+#pragma unroll
+                for (int x = 0; x < 4; ++x) top[x] = max(top[x], __shfl_up_sync(0xffffffffu, top[x], o));  // (lowest lanes: own)
+              int first = r_exp;
+#pragma unroll
+              for (int x = 0; x < 4; ++x) {
+                v_top[128 * buf + 32 * x + lane] = max(top[x], first);
+                first = max(first, most[x]);
+              }
+            }
+            r_exp = max(r_exp, max(max(most[0], most[1]), max(most[2], most[3])));
+            const float down = __int_as_float((260 - r_exp) << 23);  // 2^(133 - r_exp)
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
               k_sc[128 * buf + 32 * x + lane] = ks[x];
               v_sc[128 * buf + 32 * x + lane] = vs[x] * down;
             }
             if (lane == 0) {
-              r_step[buf] = b == it.b0 ? 1.0f : __int_as_float(max(127 + before - r_exp, 0) << 23);
-              if (b == it.b1 - 1) r_end[rows % Sh::kEnds] = __int_as_float((r_exp - 6) << 23);
+              r_tile[buf] = r_exp;
+              r_before[buf] = before;
+              r_step[buf] = __int_as_float(max(127 + before - r_exp, 0) << 23);
             }
             __syncwarp();
             if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&sc_full[buf]));
@@ -463,7 +487,6 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
           if (b + 1 >= it.b0) look_scales(b + 1);
           look_pages(b + 2);
         }
-        ++rows;
       }
     }
     for (int k = 0; !kE4m3 && ok && item_at(k, it, hkv); ++k) {
@@ -593,11 +616,29 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         float alpha = 1.0f;
         if (move) alpha = (m_run == -INFINITY) ? 0.0f : ex2_approx(m_run - mbs);
         if (move) m_run = max_nan(m_run, mbs);  // (a NaN stays, also through blocks that this row does not see)
-        float step = 1.0f;  // O follows the values' scale reference
-        if constexpr (kE4m3) step = r_step[b];
+        float step = 1.0f, lift = 0.0f;  // O follows the scale reference
+        // The row's scale reference where it is not the tile's: a row that sees part of the block has seen all before it. How far
+        // (log2) the tile's lies above the row's, and, with the row's last key in the block, the row's closing factor.
+        const bool edge = kE4m3 && kb >= min(clear, it.b1 - 1);
+        auto reference = [&]() -> int {
+          const int seen = limit - kb * kVarBlk;
+          return seen > 0 ? max(v_top[128 * b + min(seen, kVarBlk) - 1], r_tile[b] - kScaleSpan) : r_tile[b];
+        };
+        if constexpr (kE4m3) {
+          step = r_step[b];
+          if (edge) {
+            const int own = reference(), tile = r_tile[b];
+            lift = static_cast<float>(tile - own);
+            step = 1.0f;
+            if (limit > kb * kVarBlk) {  // (a row that sees none of the block keeps its O and its closing factor)
+              step = __int_as_float(max(127 + r_before[b] - own, 0) << 23);
+              if (h == 0) r_end[128 * (rows & 1) + r] = __int_as_float((own - 6) << 23);  // 2^(own - 133)
+            }
+          }
+        }
         const bool need_rescale = __any_sync(0xffffffffu, (move || step != 1.0f) && j > 0);
         const float m_sub = (m_run == -INFINITY) ? 0.0f : m_run;
-        const uint64_t c2 = f2_pack(c, c), nm2 = f2_pack(-m_sub, -m_sub);
+        const uint64_t c2 = f2_pack(c, c), nm2 = f2_pack(lift - m_sub, lift - m_sub);
         uint64_t acc[4] = {0ull, 0ull, 0ull, 0ull};
 #pragma unroll
         for (int i = 0; i < 64; i += 2) {
@@ -623,6 +664,8 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
           f2_unpack(f2_add(a01, a23), lo, hi);
           rs = lo + hi;
         }
+        if constexpr (kE4m3)
+          if (edge) rs *= __int_as_float((127 - (r_tile[b] - reference())) << 23);
         l_run = l_run * alpha + rs;
         if (need_rescale) {
           ok = warp_wait_bounded(ptx::smem_u32(&s_free[(g - 1) & 1]), ((g - 1) >> 1) & 1, ctl, 21);
@@ -720,7 +763,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
           const uint8_t* src = sRaw + st * Sh::kStageBytes + r * kD;
           uint8_t* dst = sKV + sl * kTile + r * 128;
           const int sx = kD == 128 ? r & 7 : (r >> 1) & 3;
-#pragma unroll
+#pragma unroll 1
           for (int y = 0; y < kD / 16; y += 4) {  // a 64-column chunk: loads, then conversions
             uint4 w[4];
 #pragma unroll
@@ -749,7 +792,6 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       if (ok) ok = warp_wait_bounded<false, 256>(ptx::smem_u32(&o_done[rows & 1]), (rows >> 1) & 1, ctl, 22);
       if (!ok) break;
       const uint32_t ob = rows & 1, tO = tO0 + 128 * ob;
-      const float* end = r_end + rows % Sh::kEnds;
       ++rows;
       ptx::tc_fence_after();
       const float m_run = m_row[r];
@@ -760,7 +802,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       // of +inf (scores beyond fp32) gives NaN, as the definition does.
       const bool none = m_run == -INFINITY;
       float inv_l = m_run == INFINITY ? NAN : 1.0f / l_tot;
-      if constexpr (kE4m3) inv_l *= *end;
+      if constexpr (kE4m3) inv_l *= r_end[128 * ob + r];
       if constexpr (kPaged) {
         if (it.part >= 0) {  // one of several pieces: fp32 rows and their log2 sums, for the combining kernel
           const int64_t prow = (static_cast<int64_t>(it.part) * a.kv_heads + hkv) * kVarBlk + r;

@@ -84,3 +84,30 @@ def test_rows_of_zeros_among_the_values(no_device_error, cuda_dev, dtype):
     c["k_scale"][at["block_table"][0, 0], 0] = float("nan")  # 0 x NaN is NaN, as by the definition
     c["v_scale"].zero_()
     assert torch.isnan(bsk.attention_paged(q, **at, **c)).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("new,kv,first", [(100, 100, 20), (70, 300, 260), (90, 5000, 4950), (130, 130, 128)])
+def test_values_that_a_row_does_not_see_leave_its_precision(no_device_error, cuda_dev, dtype, new, kv, first):
+    """Values from position `first` on are 2^34 times the ones before, whose rows keep their own precision."""
+    if dtype == torch.float16:  # (results within the type's normal range)
+        big, small = 2.0 ** 10, 2.0 ** -8
+    else:
+        big, small = 2.0 ** 20, 2.0 ** -14
+    size = torch.where(torch.arange(kv, device=cuda_dev) < first, small, big)[None, :, None].expand(-1, -1, 2)
+    q, c, at = make([new], [kv], 8, 2, 128, 16, dtype, cuda_dev, 3, size)
+    out = bsk.attention_paged(q, **at, **c)
+    assert worst(out, q, c, at, [kv], [new]) <= 1.0
+    dead = first - (kv - new)  # rows before it see small values only
+    assert (out[:dead].abs() < small * 8).all() and (out[dead:].abs().amax((1, 2)) > small * 8).all()
+
+
+def test_an_infinite_value_scale_leaves_other_rows(no_device_error, cuda_dev):
+    """Rows of tiles that end before the infinite value are untouched; rows that see it are not finite."""
+    size = torch.ones(1, 400, 2, device=cuda_dev)
+    q, c, at = make([400], [400], 4, 2, 64, 16, torch.bfloat16, cuda_dev, 4, size)
+    want = bsk.attention_paged(q, **at, **c)
+    for bad in (float("inf"), float("nan")):
+        c["v_scale"][at["block_table"][0, 300 // 16], 300 % 16] = bad
+        out = bsk.attention_paged(q, **at, **c)
+        assert torch.equal(out[:256], want[:256]) and not torch.isfinite(out[300:]).any()

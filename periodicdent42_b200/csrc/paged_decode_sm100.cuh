@@ -20,8 +20,9 @@
 // e4m3 caches: the contraction's order over D (for K) and the columns' order (for V) are permuted so that each thread
 // reads its codes as 16-byte words and converts them in registers, to fp16 (exact, one instruction for two codes; to bf16
 // it takes five, and the conversions then are half of the kernel's instructions). So both products are fp16 products:
-//   - bf16 queries are brought into fp16's range by a power of two per row (exact but for elements 2^-39 below the row's
-//     largest), which goes back into the scores together with the keys' scales;
+//   - bf16 queries are brought into fp16's range by a power of two per row, which goes back into the scores together with the
+//     keys' scales: the largest element to [2^15, 2^16) (in bf16 at most 65280, below fp16's 65504), so elements down to 2^-32
+//     of it stay exact and the error of the others is at most 2^-40 of it;
 //   - the values' scales enter the exponent: w_j = 2^(s_j + log2 scale_j - m_w) with a running maximum m_w of its own, so
 //     the rounded weights span (0, 1] whatever the scales are, and O = sum_j w_j code_j 2^(m_w) beside l = sum_j p_j 2^m.
 //
@@ -331,7 +332,7 @@ __global__ void __launch_bounds__(32 * PagedShape<kD, kFp8, kNQ>::kMaxWarps) pag
       qf[q][k][1] = live ? *reinterpret_cast<const uint32_t*>(p + d1) : 0u;
     }
     row_up[q] = 1.0f;
-    if constexpr (kFp8 && !kF16) {  // bf16 -> fp16, the row's largest element brought to [2^10, 2^11)
+    if constexpr (kFp8 && !kF16) {  // bf16 -> fp16, the row's largest element brought to [2^15, 2^16)
       uint32_t top = 0;
 #pragma unroll
       for (int k = 0; k < kKS; ++k)
@@ -342,7 +343,7 @@ __global__ void __launch_bounds__(32 * PagedShape<kD, kFp8, kNQ>::kMaxWarps) pag
         }
       top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      const int e = max(static_cast<int>(top >> 7), 40) - 137;  // exponent of the largest, less 10
+      const int e = max(static_cast<int>(top >> 7), 40) - 142;  // exponent of the largest, less 15
       const float down = __int_as_float((127 - e) << 23);
       row_up[q] = __int_as_float((127 + e) << 23);
 #pragma unroll

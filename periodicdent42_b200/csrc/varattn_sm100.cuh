@@ -27,7 +27,7 @@
 // scales down to 2^-20 of that keep P's full precision. Warp 3 divides the scales by the tile's largest power of two; in the
 // last blocks, where a row may not see the key that it came from, the rest to the row's own goes into the exponent of P
 // (done in every block, this took a sixth more time). bf16 queries are turned into fp16 in place, each row by its own power
-// of two (exact but for elements 2^-39 below the row's largest).
+// of two: exact for elements down to 2^-32 of the row's largest, the error of the others at most 2^-40 of it.
 // Bound here: the conversion's one warp per sub-partition beside the softmax's two (8100 warp instructions a block where
 // 16-bit caches take 4100), and instructions: the roles share the instruction cache, and with more code in their loops they
 // wait for it. So the conversion's and the two issuers' loops are rolled (1024 new tokens over 30000, 32 / 8 heads, D 128:
@@ -715,7 +715,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     for (int k = 0; ok && item_at(k, it, hkv); ++k) {
       if (it.b1 <= it.b0) continue;  // written by the softmax warps
       if constexpr (kE4m3) {
-        // queries: row r in place, bf16 -> fp16 with its largest element brought to [2^10, 2^11)
+        // queries: row r in place, bf16 -> fp16 with its largest element brought to [2^15, 2^16)
         const uint32_t qbuf = rows & 1;
         ok = warp_wait_bounded_hint<kBwdSuspendNs>(ptx::smem_u32(&q_raw[qbuf]), (rows >> 1) & 1, ctl, 31);
         if (!ok) break;
@@ -732,7 +732,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
                            __vmaxu2(w.z & 0x7fff7fffu, w.w & 0x7fff7fffu));
           }
           top = max(top >> 16, top & 0xffffu);
-          const int e = max(static_cast<int>(top >> 7), 40) - 137;
+          const int e = max(static_cast<int>(top >> 7), 40) - 142;
           const float down = __int_as_float((127 - e) << 23);
           up = __int_as_float((127 + e) << 23);
           auto turn = [&](uint32_t u) {

@@ -111,3 +111,16 @@ def test_an_infinite_value_scale_leaves_other_rows(no_device_error, cuda_dev):
         c["v_scale"][at["block_table"][0, 300 // 16], 300 % 16] = bad
         out = bsk.attention_paged(q, **at, **c)
         assert torch.equal(out[:256], want[:256]) and not torch.isfinite(out[300:]).any()
+
+
+@pytest.mark.parametrize("new", [1, 200])  # either kernel
+def test_queries_with_one_large_element(no_device_error, cuda_dev, new):
+    """A bf16 query whose scores come from elements 2^-31 of its largest (which meets zeros)."""
+    q, c, at = make([new], [300], 4, 2, 128, 16, torch.bfloat16, cuda_dev, 5, torch.ones(1, 300, 2, device=cuda_dev))
+    q.copy_((1 + q.abs().clamp(max=0.99)).mul(2.0 ** -11) * q.sign())
+    q[..., 3] = 2.0 ** 20
+    c["k_cache"].view(torch.uint8)[..., 3] = 0
+    c["k_scale"] *= 4096.0
+    assert worst(bsk.attention_paged(q, **at, **c), q, c, at, [300], [new]) <= 1.0
+    q[..., 3] = torch.finfo(torch.bfloat16).max  # the largest bf16 value turns into a finite fp16 value
+    assert torch.isfinite(bsk.attention_paged(q, **at, **c)).all()

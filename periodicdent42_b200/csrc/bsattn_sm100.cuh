@@ -473,7 +473,8 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
 #pragma unroll
         for (int i = 8; i < 64; i += 16)
 #pragma unroll
-          for (int k = 0; k < 8; ++k) pm[k] = max3f(pm[k], v[i + k], v[i + 8 + k]);
+          for (int k = 0; k < 8; ++k)  // (seven groups of 8 behind the first: the last one has no partner)
+            pm[k] = i + 8 < 64 ? max3f(pm[k], v[i + k], v[(i + 8 + k) & 63]) : fmaxf(pm[k], v[i + k]);
         const float mh = max3f(max3f(pm[0], pm[1], pm[2]), max3f(pm[3], pm[4], pm[5]), fmaxf(pm[6], pm[7]));
         float mo;
         ok = exchange(tS, mh, mo);

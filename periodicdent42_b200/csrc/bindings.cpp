@@ -7,6 +7,8 @@
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
 
+#include <limits>
+
 #include "bsk_capi.h"
 
 namespace {
@@ -200,12 +202,14 @@ Rows as_rows(const torch::Tensor& x, bool any_alignment = false) {
   return {t, T > 1 ? t.stride(0) : H * D, H > 1 ? t.stride(1) : D};
 }
 
-// 1-D (or 2-D) int32 index tensor on `like`'s device; int64 is narrowed.
+// 1-D (or 2-D) int32 index tensor on `like`'s device. int64 is narrowed to the nearest value: what does not fit stays out of
+// every range, so the kernels report it.
 torch::Tensor as_index(const torch::Tensor& t, const torch::Tensor& like, const char* op, const char* name, int64_t dim) {
   check_cuda(t, like, op, name);
   TORCH_CHECK_VALUE(t.dim() == dim, op, ": ", name, " must have ", dim, " dimension(s)");
   TORCH_CHECK_VALUE(t.scalar_type() == torch::kInt32 || t.scalar_type() == torch::kInt64, op, ": ", name, " must be int32 or int64");
-  return t.to(torch::kInt32).contiguous();
+  if (t.scalar_type() == torch::kInt32) return t.contiguous();
+  return t.clamp(-1, std::numeric_limits<int32_t>::max()).to(torch::kInt32).contiguous();
 }
 
 int narrow(int64_t v, const char* op, const char* name) {

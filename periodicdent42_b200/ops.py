@@ -478,7 +478,8 @@ def attention_paged(Q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     (:func:`kv_cache_append` first); new token t sees positions <= kv_lens[i] - n_i + t. heads is a multiple of the
     caches' kv_heads: query head h reads kv head h // (heads / kv_heads).
     block_table [batch, width]: page numbers, position p in page block_table[i, p // page_size]; caches and scales as in
-    :func:`kv_cache_append`, page size a power of two from 8 to 1024. Index tensors are int32 (int64 is narrowed).
+    :func:`kv_cache_append`, page size a power of two from 8 to 1024. Index tensors are int32 or int64 (narrowed first;
+    a value beyond 32 bits is out of range like any other).
     A row that sees no key is zero, and so are rows behind the last sequence. Stale contents of a page behind its
     sequence's end reach no row, NaN among them; a non-finite value inside a sequence may make rows of it NaN that see it
     with weight zero or, masked, share its block of keys. Inference only (no gradient)."""
@@ -493,7 +494,7 @@ def attention_varlen(Q: torch.Tensor, K: torch.Tensor, V: torch.Tensor, cu_seqle
 
     Q [tokens, heads, dim], K and V [tokens, kv_heads, dim] (fp16 / bf16, dim 64 or 128, heads a multiple of kv_heads:
     query head h reads kv head h // (heads / kv_heads)); sequence i owns rows cu_seqlens[i] .. cu_seqlens[i+1]
-    (int32 [batch + 1], starting at 0; any lengths, zero included). Rows behind the last sequence are zero.
+    (int32 or int64 [batch + 1], starting at 0; any lengths, zero included). Rows behind the last sequence are zero.
     Sequences do not reach one another, non-finite values included; inside one, a non-finite row of V may make rows NaN
     that it is masked for. Differentiable (once) in Q, K and V (deterministic, no atomics)."""
     if scale is None:

@@ -174,6 +174,20 @@ void check_cuda(const torch::Tensor& t, const torch::Tensor& like, const char* o
   TORCH_CHECK_VALUE(t.device() == like.device(), op, ": ", name, " is on another device");
 }
 
+// Derivatives that an operator does not have are errors, never left out silently: forward-mode tangents everywhere ...
+void no_tangent(const char* op, std::initializer_list<const torch::Tensor*> ts) {
+  for (const auto* t : ts)
+    if (t) TORCH_CHECK_NOT_IMPLEMENTED(!t->_fw_grad(0).defined(), op, " has no forward-mode derivative");
+}
+// ... and gradients of the operators for serving.
+void no_gradient(const char* op, std::initializer_list<const torch::Tensor*> ts) {
+  no_tangent(op, ts);
+  if (!at::GradMode::is_enabled()) return;
+  for (const auto* t : ts)
+    if (t) TORCH_CHECK_VALUE(!t->requires_grad(), op, " has no gradient: call it under torch.no_grad() or with detached tensors");
+}
+const torch::Tensor* some(const OptTensor& t) { return t ? &*t : nullptr; }
+
 int dtype_code(const torch::Tensor& t, const char* op, bool f32_ok = false) {
   const auto dt = t.scalar_type();
   if (dt == torch::kBFloat16) return 0;
@@ -294,6 +308,7 @@ void kv_cache_append(torch::Tensor K, torch::Tensor V, torch::Tensor k_cache, to
   const char* op = "kv_cache_append";
   check_cuda(K, K, op, "K");
   check_cuda(V, K, op, "V");
+  no_gradient(op, {&K, &V, &k_cache, &v_cache, some(k_scale), some(v_scale)});
   TORCH_CHECK_VALUE(K.dim() == 3 && V.sizes() == K.sizes(), op, ": K and V must be [tokens, kv_heads, dim] of one shape");
   const int code = dtype_code(K, op);
   TORCH_CHECK_VALUE(V.scalar_type() == K.scalar_type(), op, ": K and V must have one dtype");
@@ -319,6 +334,7 @@ std::tuple<torch::Tensor, torch::Tensor> kv_cache_gather(torch::Tensor k_cache, 
   const char* op = "kv_cache_gather";
   const auto dtype = f16 ? torch::kFloat16 : torch::kBFloat16;
   const bool e4m3 = check_caches(op, k_cache, k_cache, v_cache, k_scale, v_scale, dtype);
+  no_gradient(op, {&k_cache, &v_cache, some(k_scale), some(v_scale)});
   const at::cuda::CUDAGuard guard(k_cache.device());
   const auto at = check_slots(op, slots, k_cache);
   auto K = torch::empty({at.size(0), k_cache.size(2), k_cache.size(3)}, k_cache.options().dtype(dtype));
@@ -344,6 +360,7 @@ torch::Tensor attention_paged(torch::Tensor Q, torch::Tensor k_cache, torch::Ten
                               OptTensor v_scale) {
   const char* op = "attention_paged";
   check_cuda(Q, Q, op, "Q");
+  no_gradient(op, {&Q, &k_cache, &v_cache, some(k_scale), some(v_scale)});
   TORCH_CHECK_VALUE(Q.dim() == 3, op, ": Q must be [tokens, heads, dim]");
   const int code = dtype_code(Q, op);
   const bool e4m3 = check_caches(op, Q, k_cache, v_cache, k_scale, v_scale, Q.scalar_type());
@@ -491,6 +508,7 @@ struct VarlenAttention : public torch::autograd::Function<VarlenAttention> {
 
 torch::Tensor attention_varlen(torch::Tensor Q, torch::Tensor K, torch::Tensor V, torch::Tensor cu_seqlens, double scale,
                                bool causal) {
+  no_tangent("attention_varlen", {&Q, &K, &V});
   if (at::GradMode::is_enabled() && (Q.requires_grad() || K.requires_grad() || V.requires_grad()))
     return VarlenAttention::apply(Q, K, V, cu_seqlens, scale, causal);
   return std::get<0>(attention_varlen_fwd(Q, K, V, cu_seqlens, scale, causal, false));
@@ -528,6 +546,7 @@ struct Rotary : public torch::autograd::Function<Rotary> {
 
 std::tuple<torch::Tensor, OptTensor> rotary_embedding(torch::Tensor Q, OptTensor K, torch::Tensor positions,
                                                       torch::Tensor inv_freq, bool interleaved, double scale) {
+  no_tangent("rotary_embedding", {&Q, some(K), &inv_freq});
   if (at::GradMode::is_enabled()) {
     TORCH_CHECK_VALUE(!inv_freq.requires_grad(), "rotary_embedding has no gradient for inv_freq");
     if (Q.requires_grad() || (K && K->requires_grad())) {

@@ -439,7 +439,7 @@ def rotary_embedding(Q: torch.Tensor, K: Optional[torch.Tensor], positions: torc
     Pair i of a head -- elements (i, i + r/2), or (2i, 2i+1) with ``interleaved`` -- turns by positions[t] * inv_freq[i]
     and is multiplied by ``scale``; r = 2 * len(inv_freq), elements from r on are copied unchanged (and unscaled).
     positions: int32 or int64 [tokens], any value (angles are reduced in 64 bits); inv_freq: float32 (see
-    :func:`rotary_frequencies`). Differentiable (once) in Q and K."""
+    :func:`rotary_frequencies`). Differentiable (once, in reverse mode) in Q and K."""
     return _C().rotary_embedding(Q, K, positions, inv_freq, interleaved, scale)
 
 
@@ -452,7 +452,7 @@ def kv_cache_append(K: torch.Tensor, V: torch.Tensor, k_cache: torch.Tensor, v_c
     float32 [pages, page size, kv_heads]: then each row is quantised as it is written (scale = max|x| / 448, code =
     e4m3(x / scale); :func:`quantize_e4m3` per row). slots: int32 or int64 [tokens], page * page_size + offset, no slot
     twice in a call; a negative slot marks padding and is skipped. A slot behind the cache is skipped and reported by
-    :func:`synchronize_and_check`. No gradient flows into a cache."""
+    :func:`synchronize_and_check`. Has no gradient: tensors that require one are refused outside torch.no_grad()."""
     _C().kv_cache_append(K, V, k_cache, v_cache, slots, k_scale, v_scale)
 
 
@@ -461,7 +461,8 @@ def kv_cache_gather(k_cache: torch.Tensor, v_cache: torch.Tensor, slots: torch.T
                     v_scale: Optional[torch.Tensor] = None):
     """Read rows back from a paged cache (layout and slots as in :func:`kv_cache_append`; a slot may occur more than
     once): (K, V) contiguous [tokens, kv_heads, dim] in ``dtype`` (float16 or bfloat16; the caches' own unless they hold
-    e4m3 codes, which are multiplied by their scales and rounded once). Negative slots read as zeros."""
+    e4m3 codes, which are multiplied by their scales and rounded once). Negative slots read as zeros. Has no gradient, as
+    above."""
     if dtype not in (torch.float16, torch.bfloat16):
         raise ValueError("kv_cache_gather: dtype must be torch.float16 or torch.bfloat16")
     return _C().kv_cache_gather(k_cache, v_cache, slots, dtype == torch.float16, k_scale, v_scale)
@@ -482,7 +483,8 @@ def attention_paged(Q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     a value beyond 32 bits is out of range like any other).
     A row that sees no key is zero, and so are rows behind the last sequence. Stale contents of a page behind its
     sequence's end reach no row, NaN among them; a non-finite value inside a sequence may make rows of it NaN that see it
-    with weight zero or, masked, share its block of keys. Inference only (no gradient)."""
+    with weight zero or, masked, share its block of keys. For serving: has no gradient, and tensors that require one are
+    refused outside torch.no_grad()."""
     if scale is None:
         scale = Q.shape[-1] ** -0.5 if Q.dim() and Q.shape[-1] else 1.0
     return _C().attention_paged(Q, k_cache, v_cache, block_table, kv_lens, cu_seqlens, scale, k_scale, v_scale)
@@ -496,7 +498,7 @@ def attention_varlen(Q: torch.Tensor, K: torch.Tensor, V: torch.Tensor, cu_seqle
     query head h reads kv head h // (heads / kv_heads)); sequence i owns rows cu_seqlens[i] .. cu_seqlens[i+1]
     (int32 or int64 [batch + 1], starting at 0; any lengths, zero included). Rows behind the last sequence are zero.
     Sequences do not reach one another, non-finite values included; inside one, a non-finite row of V may make rows NaN
-    that it is masked for. Differentiable (once) in Q, K and V (deterministic, no atomics)."""
+    that it is masked for. Differentiable (once, in reverse mode) in Q, K and V (deterministic, no atomics)."""
     if scale is None:
         scale = Q.shape[-1] ** -0.5 if Q.dim() and Q.shape[-1] else 1.0
     return _C().attention_varlen(Q, K, V, cu_seqlens, scale, causal)

@@ -250,6 +250,7 @@ std::tuple<torch::Tensor, OptTensor> rotary(torch::Tensor Q, OptTensor K, torch:
   check_cuda(inv_freq, Q, op, "inv_freq");
   TORCH_CHECK_VALUE(inv_freq.dim() == 1 && inv_freq.scalar_type() == torch::kFloat32, op, ": inv_freq must be 1-D float32");
   TORCH_CHECK_VALUE(inv_freq.size(0) >= 1 && 2 * inv_freq.size(0) <= D, op, ": inv_freq must hold 1 to dim / 2 frequencies");
+  TORCH_CHECK_VALUE(scale > -1e30 && scale < 1e30, op, ": scale must be finite and below 1e30 in size");
   TORCH_CHECK_VALUE(D % 2 == 0 && D <= 512, op, ": the head dimension must be even and at most 512, got ", D);
   const at::cuda::CUDAGuard guard(Q.device());
   const auto pos = positions.contiguous(), freq = inv_freq.contiguous();
@@ -352,7 +353,7 @@ void check_heads(const char* op, const torch::Tensor& Q, int64_t kv_heads, doubl
   TORCH_CHECK_VALUE(kv_heads > 0 && Q.size(1) > 0 && Q.size(1) % kv_heads == 0, op, ": heads (", Q.size(1),
                     ") must be a positive multiple of kv_heads (", kv_heads, ")");
   TORCH_CHECK_VALUE(Q.size(1) / kv_heads <= 128, op, ": at most 128 heads per kv head");
-  TORCH_CHECK_VALUE(scale > 0.0 && scale < 1e30, op, ": scale must be positive and finite");
+  TORCH_CHECK_VALUE(static_cast<float>(scale) > 0.0f && scale < 1e30, op, ": scale must be positive and below 1e30 in float32");
 }
 
 torch::Tensor attention_paged(torch::Tensor Q, torch::Tensor k_cache, torch::Tensor v_cache, torch::Tensor block_table,

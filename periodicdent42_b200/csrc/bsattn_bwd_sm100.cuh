@@ -40,12 +40,13 @@ constexpr uint32_t kBwdSuspendNs = 2000;  // suspend hint of the compute and MMA
 constexpr int kBwdPolyEighths = BSK_BWD_POLY_EIGHTHS;
 
 // exp2 of a packed pair on the MUFU, or on the FMA pipe when `poly` (a compile-time choice after unrolling).
+template <int kFloor = -125>
 __device__ __forceinline__ uint64_t f2_ex2_split(uint64_t t, bool poly) {
   float a, b;
   f2_unpack(t, a, b);
   if (poly) {
     float ya, yb;
-    ex2_poly2(a, b, ya, yb);
+    ex2_poly2<kFloor>(a, b, ya, yb);
     return f2_pack(ya, yb);
   }
   return f2_pack(ex2_approx(a), ex2_approx(b));

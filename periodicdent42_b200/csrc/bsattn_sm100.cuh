@@ -152,11 +152,15 @@ __device__ __forceinline__ float max3f(float a, float b, float c) {
 // 2^x for a pair on the FMA pipe (Cody-Waite split, published FlashAttention-4 approach): x = n + f with
 // n = round(x) from the 1.5*2^23 magic addition, f in [-1/2, 1/2], 2^f by a cubic fitted here (constrained
 // minimax: 1 + 0.693282906 f + 0.242210542 f^2 + 0.055008705 f^3, max relative error 1.01e-4), and 2^n added
-// to the exponent field. Inputs below -125 are clamped (result ~2^-125; only masked elements get there).
+// to the exponent field. Inputs below the floor are clamped to it: -125 gives 2^-125, -127 gives zero (f = 0 there, so the
+// exponent field of 1 is taken to 0 and nothing is left; between -127 and -126, f >= 0 where n = -127, so the field never
+// goes below 0 and what is left is below 2^-126).
+template <int kFloor = -125>
 __device__ __forceinline__ void ex2_poly2(float x0, float x1, float& y0, float& y1) {
+  static_assert(kFloor >= -127, "the exponent field would wrap");
   const uint64_t kMagic = f2_pack(12582912.0f, 12582912.0f);
   const uint64_t kNegMagic = f2_pack(-12582912.0f, -12582912.0f);
-  const uint64_t xc = f2_pack(fmaxf(x0, -125.0f), fmaxf(x1, -125.0f));
+  const uint64_t xc = f2_pack(fmaxf(x0, static_cast<float>(kFloor)), fmaxf(x1, static_cast<float>(kFloor)));
   const uint64_t xr = f2_add(xc, kMagic);        // n in the low mantissa bits
   const uint64_t fl = f2_add(xr, kNegMagic);     // n as a float
   const uint64_t f = f2_fma(fl, f2_pack(-1.0f, -1.0f), xc);

@@ -427,7 +427,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
 #pragma unroll
         for (int i = 0; i < 64; i += 2) {
           float p0, p1;
-          f2_unpack(f2_ex2_split(f2_fma(f2_pack(__uint_as_float(pv[i]), __uint_as_float(pv[i + 1])), c2, off2),
+          f2_unpack(f2_ex2_split<kVarFloor>(f2_fma(f2_pack(__uint_as_float(pv[i]), __uint_as_float(pv[i + 1])), c2, off2),
                                  ((i >> 1) & 7) >= 8 - kBwdPolyEighths),
                     p0, p1);
           if (i >= lim) p0 = 0.0f;
@@ -775,11 +775,11 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
           for (int i = 0; i < 32; i += 4) {
             const float4 o = *reinterpret_cast<const float4*>(off_s + 32 * cc + i);
             float p0, p1, p2, p3;
-            f2_unpack(f2_ex2_split(f2_fma(f2_pack(__uint_as_float(sv[i]), __uint_as_float(sv[i + 1])), c2,
+            f2_unpack(f2_ex2_split<kVarFloor>(f2_fma(f2_pack(__uint_as_float(sv[i]), __uint_as_float(sv[i + 1])), c2,
                                           f2_pack(o.x, o.y)),
                                    ((i >> 1) & 7) >= 8 - kBwdPolyEighths),
                       p0, p1);
-            f2_unpack(f2_ex2_split(f2_fma(f2_pack(__uint_as_float(sv[i + 2]), __uint_as_float(sv[i + 3])), c2,
+            f2_unpack(f2_ex2_split<kVarFloor>(f2_fma(f2_pack(__uint_as_float(sv[i + 2]), __uint_as_float(sv[i + 3])), c2,
                                           f2_pack(o.z, o.w)),
                                    (((i >> 1) + 1) & 7) >= 8 - kBwdPolyEighths),
                       p2, p3);

@@ -67,6 +67,10 @@ __device__ __forceinline__ void zero_tile_rows(uint8_t* tile, int chunks, int fi
 // reference is at most kScaleSpan below its tile's, so that 2^8 * 2^kScaleSpan, 64 times, is finite.
 constexpr int kScaleLow = 20, kScaleHigh = 240, kScaleSpan = 110;
 
+// Floor of the exponentials on the FMA pipe: weights below 2^-126 are zero, so that no masked or far key, however large its
+// values are, adds to a row.
+constexpr int kVarFloor = -127;
+
 // Where the K / V rows come from.
 enum : int { kPacked = 0, kCache16 = 1, kCacheE4m3 = 2 };
 
@@ -645,7 +649,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
           float t0, t1, e0, e1;
           f2_unpack(f2_fma(f2_pack(v[i], v[i + 1]), c2, nm2), t0, t1);
           if (((i >> 1) & 7) >= 8 - kAttnPolyEighths) {
-            ex2_poly2(t0, t1, e0, e1);
+            ex2_poly2<kVarFloor>(t0, t1, e0, e1);
           } else {
             e0 = ex2_approx(t0);
             e1 = ex2_approx(t1);
@@ -798,7 +802,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       const float l_tot = l_part[r] + l_part[128 + r];
       const bool live = tok < it.ntok;
       const int64_t grow = static_cast<int64_t>(it.row0 + tok) * a.heads + hkv * group + hd;
-      // A row without keys has its maximum at -inf (its sum may hold the exponentials' floor of 2^-125): zero. A maximum
+      // A row without keys has its maximum at -inf: zero. A maximum
       // of +inf (scores beyond fp32) gives NaN, as the definition does.
       const bool none = m_run == -INFINITY;
       float inv_l = m_run == INFINITY ? NAN : 1.0f / l_tot;

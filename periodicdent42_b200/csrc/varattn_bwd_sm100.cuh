@@ -430,8 +430,6 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
           f2_unpack(f2_ex2_split<kVarFloor>(f2_fma(f2_pack(__uint_as_float(pv[i]), __uint_as_float(pv[i + 1])), c2, off2),
                                  ((i >> 1) & 7) >= 8 - kBwdPolyEighths),
                     p0, p1);
-          if (i >= lim) p0 = 0.0f;
-          if (i + 1 >= lim) p1 = 0.0f;
           pv[i] = __float_as_uint(p0);
           pv[i + 1] = __float_as_uint(p1);
         }
@@ -451,6 +449,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
             f2_unpack(f2_mul(f2_pack(__uint_as_float(pv[32 * cc + i]), __uint_as_float(pv[32 * cc + i + 1])),
                              f2_add(f2_pack(__uint_as_float(dv[i]), __uint_as_float(dv[i + 1])), ndlt2)),
                       g0, g1);
+            if (32 * cc + i >= lim) g0 = 0.0f;  // (the product, not P: dP of a masked key may be infinite)
+            if (32 * cc + i + 1 >= lim) g1 = 0.0f;
             pk[i >> 1] = pack2<kF16>(g0, g1);
           }
           ptx::tmem_st_32x32b_x16(tmem_base + lane_off + T_DS + 32 * x + 16 * cc, pk);
@@ -824,6 +824,13 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
                              f2_add(f2_pack(__uint_as_float(dv[i + 2]), __uint_as_float(dv[i + 3])),
                                     f2_pack(-d.z, -d.w))),
                       g2, g3);
+            if (diag) {  // (P is zero there, but dP of a masked row may be infinite)
+              const int col = 32 * cc + i;
+              if (col < lim) g0 = 0.0f;
+              if (col + 1 < lim) g1 = 0.0f;
+              if (col + 2 < lim) g2 = 0.0f;
+              if (col + 3 < lim) g3 = 0.0f;
+            }
             pk[i >> 1] = pack2<kF16>(g0, g1);
             pk[(i >> 1) + 1] = pack2<kF16>(g2, g3);
           }

@@ -35,3 +35,27 @@ def test_paged(no_device_error, cuda_dev, new):
     want = bsk.attention_paged(q, k, v, *at)
     v.view(400, 2, 64)[399] = LARGE
     assert torch.equal(bsk.attention_paged(q, k, v, *at)[:-1], want[:-1])
+
+
+@pytest.mark.parametrize("H,G,D", [(4, 2, 64), (3, 1, 128)])
+def test_gradients(no_device_error, cuda_dev, H, G, D):
+    """A value or an output's gradient so large that their product overflows does not reach rows that do not see it: dQ of the
+    rows before the value, dK of the keys behind the row."""
+    g = torch.Generator(device=cuda_dev).manual_seed(0)
+    q, do = (torch.randn(300, H, D, generator=g, device=cuda_dev).bfloat16() for _ in range(2))
+    k, v = (torch.randn(300, G, D, generator=g, device=cuda_dev).bfloat16() for _ in range(2))
+    cu = torch.tensor([0, 300], device=cuda_dev)
+
+    def grads(v, do):
+        x = [t.clone().requires_grad_(True) for t in (q, k, v)]
+        return torch.autograd.grad(bsk.attention_varlen(*x, cu), x, do)
+
+    want = grads(v, do)
+    for at in (33, 150, 299):
+        big = v.clone()
+        big[at] = LARGE
+        assert torch.equal(grads(big, do)[0][:at], want[0][:at])
+        big = do.clone()
+        big[at] = LARGE
+        got = grads(v, big)
+        assert torch.equal(got[1][at + 1:], want[1][at + 1:]) and torch.equal(got[2][at + 1:], want[2][at + 1:])

@@ -390,7 +390,8 @@ int bsk_kv_cache_gather(int dtype, const void* k_cache, const void* v_cache, int
  * token t sees the keys at positions <= kv_lens[i] - n_i + t. The key at position p is in page
  * block_table[i * table_stride + p / page_size] at offset p % page_size; the rest of the last page is never used.
  * O [tokens, heads, dim] is contiguous; a row that sees no key, and rows behind the last sequence, are zero.
- *   caches as in bsk_kv_cache_append; page_size a power of two, 8..1024; pages x page_size below 2^31
+ *   caches as in bsk_kv_cache_append; page_size a power of two, 8..1024; pages x page_size and
+ *   table_width x page_size at most 2^31 - 4096
  *   cu_seqlens int32 [batch + 1], cu_seqlens[0] = 0, non-decreasing, at most `tokens`; kv_lens int32 [batch],
  *   at most table_width * page_size; entries outside their range are clamped, a page outside [0, num_pages) reads as
  *   zeros, and either sets the device error word.

@@ -2300,8 +2300,10 @@ int bsk_attention_paged(int dtype, const void* Q, int64_t q_token_stride, int64_
   if (page_size < 8 || page_size > 1024 || (page_size & (page_size - 1)))
     return set_error(BSK_ERR_UNSUPPORTED, "%s: page size %d unsupported (a power of two from 8 to 1024)", what, page_size);
   if (num_pages < 0 || table_width < 0 || table_stride < 0) return set_error(BSK_ERR_INVALID_ARG, "%s: negative extent", what);
-  if ((int64_t)num_pages * page_size >= (int64_t)1 << 31 || (int64_t)table_width * page_size >= (int64_t)1 << 31)
-    return set_error(BSK_ERR_UNSUPPORTED, "%s: pages x page size must stay below 2^31 slots", what);
+  // (the kernels count positions in 32 bits, and round them up to their blocks)
+  constexpr int64_t kMostSlots = ((int64_t)1 << 31) - 4096;
+  if ((int64_t)num_pages * page_size > kMostSlots || (int64_t)table_width * page_size > kMostSlots)
+    return set_error(BSK_ERR_UNSUPPORTED, "%s: at most 2^31 - 4096 slots (pages x page size, table width x page size)", what);
   DeviceState* st;
   if (tokens == 0) return device_state(&st);
   if (!Q || !O || !cu_seqlens || (batch > 0 && !kv_lens) || (batch > 0 && table_width > 0 && !block_table) ||

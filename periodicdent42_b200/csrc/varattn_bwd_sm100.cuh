@@ -824,15 +824,17 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
                              f2_add(f2_pack(__uint_as_float(dv[i + 2]), __uint_as_float(dv[i + 3])),
                                     f2_pack(-d.z, -d.w))),
                       g2, g3);
-            if (diag) {  // (P is zero there, but dP of a masked row may be infinite)
-              const int col = 32 * cc + i;
-              if (col < lim) g0 = 0.0f;
-              if (col + 1 < lim) g1 = 0.0f;
-              if (col + 2 < lim) g2 = 0.0f;
-              if (col + 3 < lim) g3 = 0.0f;
-            }
             pk[i >> 1] = pack2<kF16>(g0, g1);
             pk[(i >> 1) + 1] = pack2<kF16>(g2, g3);
+          }
+          // P of a masked row is zero, but its dP may be infinite. (On the packed pairs, apart from the loop above: inside it, every
+          // block executed the selects, 18 % more instructions and 5 % more time.)
+          if (diag) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const int col = 32 * cc + 2 * i;
+              pk[i] &= (col < lim ? 0u : 0x0000ffffu) | (col + 1 < lim ? 0u : 0xffff0000u);
+            }
           }
           ptx::tmem_st_32x32b_x16(tp + 16 * cc, pk);
         }

@@ -355,7 +355,7 @@ void launch_attention_backward(const void* grad_out, const void* Q, const void* 
  * copied. `backward` turns by -t (the gradient with respect to the input, given the output's).
  *   Q, K      : rows of dim elements at token and head strides given in elements (either may have 0 heads);
  *               Q_out, K_out contiguous, not overlapping the inputs
- *   positions : int32 or int64 [tokens] (position_bytes 4 or 8); angles are reduced in 64 bits
+ *   positions : int32 or int64 [tokens] (position_bytes 4 or 8); angles are reduced in twice 64 bits
  *   dim       : even, at most 512; rotary_dim even, 2..dim; inv_freq fp32 [rotary_dim/2], device memory
  * No reference counterpart.
  */

@@ -7,8 +7,10 @@
 // `sign` = -1.
 //
 // Precision: a position of 10^6 leaves an fp32 angle 0.03 radians off, so the angle is taken in turns (t / 2 pi) in
-// 64 bits, its whole turns are dropped there, and only the remaining fraction of a turn goes to sincospif. The
-// rotation itself is fp32 and each result is rounded once.
+// 64 bits, its whole turns are dropped there, and only the remaining fraction of a turn goes to sincospif. A 64-bit product
+// would in turn be 2^-52 of its turns off (2^-14 radians at position 2^40), so what its roundings drop is kept as a second
+// 64-bit number: the fraction is exact to 2^-43 of a turn for every 64-bit position. The rotation itself is fp32 and each
+// result is rounded once.
 //
 // Bound: HBM, each row is read and written once. The angles cost one double product and one sincospif per (token,
 // pair): they are taken once per token by the block, kept in shared memory and used by all heads of Q and K. The rows of
@@ -59,6 +61,19 @@ template <>
 __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// position * frequency / 2 pi without its whole turns, in (-1, 1). Each number is a 64-bit one and what its rounding dropped.
+__device__ __forceinline__ double turn_fraction(int64_t position, float frequency) {
+  constexpr double kInv2Pi = 0.15915494309189535, kInv2PiLow = -9.839338337591243e-18;  // 1 / 2 pi to 107 bits
+  const double f = frequency;
+  const double g = f * kInv2Pi, g_low = fma(f, kInv2PiLow, fma(f, kInv2Pi, -g));  // turns per position
+  const double p = static_cast<double>(position);
+  // (positions above 2^53; the largest ones round to 2^63, which no int64 holds)
+  const double p_low = p < 0x1p63 ? static_cast<double>(position - static_cast<int64_t>(p))
+                                  : static_cast<double>(position - INT64_MAX) - 1.0;
+  const double t = p * g, t_low = fma(p_low, g, fma(p, g_low, fma(p, g, -t)));
+  return (t - rint(t)) + (t_low - rint(t_low));
+}
 
 template <class T, int N>
 struct alignas(sizeof(T) * N) Pack {
@@ -132,11 +147,10 @@ __global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const __grid_con
   load(g0);
   for (int i = threadIdx.x; i < nt * half; i += kRotaryThreads) {
     const int64_t t = t0 + i / half;
-    const double pos = a.positions64 ? static_cast<double>(static_cast<const int64_t*>(a.positions)[t])
-                                     : static_cast<double>(static_cast<const int*>(a.positions)[t]);
-    const double turns = pos * (static_cast<double>(a.inv_freq[i % half]) * 0.15915494309189533577);  // 1 / 2 pi
+    const int64_t at = a.positions64 ? static_cast<const int64_t*>(a.positions)[t] : static_cast<const int*>(a.positions)[t];
+    const double turn = turn_fraction(at, a.inv_freq[i % half]);
     float s, c;
-    sincospif(2.0f * static_cast<float>(turns - rint(turns)), &s, &c);
+    sincospif(2.0f * static_cast<float>(turn), &s, &c);
     rot[i] = make_float2(c * a.scale, a.sign * s * a.scale);
   }
   __syncthreads();

@@ -438,7 +438,7 @@ def rotary_embedding(Q: torch.Tensor, K: Optional[torch.Tensor], positions: torc
 
     Pair i of a head -- elements (i, i + r/2), or (2i, 2i+1) with ``interleaved`` -- turns by positions[t] * inv_freq[i]
     and is multiplied by ``scale``; r = 2 * len(inv_freq), elements from r on are copied unchanged (and unscaled).
-    positions: int32 or int64 [tokens], any value (angles are reduced in 64 bits); inv_freq: float32 (see
+    positions: int32 or int64 [tokens], any value (angles are exact to fp32 at every one of them); inv_freq: float32 (see
     :func:`rotary_frequencies`). Differentiable (once, in reverse mode) in Q and K."""
     return _C().rotary_embedding(Q, K, positions, inv_freq, interleaved, scale)
 

@@ -395,8 +395,9 @@ int bsk_kv_cache_gather(int dtype, const void* k_cache, const void* v_cache, int
  *   cu_seqlens int32 [batch + 1], cu_seqlens[0] = 0, non-decreasing, at most `tokens`; kv_lens int32 [batch],
  *   at most table_width * page_size; entries outside their range are clamped, a page outside [0, num_pages) reads as
  *   zeros, and either sets the device error word.
- *   A non-finite K reaches the rows that see it; a non-finite V also those of the same 128-key block that do not (their
+ *   A non-finite K reaches the rows that see it; a non-finite V may also reach rows fewer than 256 tokens before it (their
  *   weight is zero, and 0 x NaN is NaN). Cache contents behind a sequence's end reach nothing.
+ *   The weights are rounded to Q's type for their product with V; over e4m3 caches weight times value scale to fp16.
  *   workspace: device memory of bsk_attention_paged_workspace_bytes(...) bytes (may be 0), 16-byte aligned, not shared
  *   by calls that may run at the same time. The size depends on the current device.
  * No reference counterpart.
@@ -417,6 +418,7 @@ int64_t bsk_attention_paged_workspace_bytes(int tokens, int batch, int heads, in
  *   dV = P^T dO,  dS = P * (dO V^T - rowsum(dO * O)),  dQ = scale * dS K,  dK = scale * dS^T Q
  * with dK, dV summed over the heads of a group, in a fixed order (no atomics). Rows behind the last sequence are zero.
  * Sequences do not reach into one another, whatever their values; within one, non-finite values as in bsk_attention_paged.
+ * P and dS are rounded to the inputs' type for their products.
  * workspace: device memory of bsk_attention_varlen_workspace_bytes(...) bytes, 16-byte aligned, not shared by calls
  * that may run at the same time. No reference counterpart.
  */

@@ -7,13 +7,19 @@
 // codes 0, a row that holds a NaN has scale NaN. Reading back gives code * scale, rounded once.
 //
 // The quotients are taken by Markstein's method (P. Markstein, "Computation of elementary functions on the IBM RISC System/6000
-// processor", 1990): with y the correctly rounded reciprocal of the scale, q = x y, r = q scale - x (exact in one fused
-// operation) and q - r y is the correctly rounded x / scale (in this form of the signs, also for x = -0). Three packed operations for two elements in place of a division
-// each. The quantising write stays bound by instruction issue: 16383 tokens of 8 heads, D 128, take 27 us (33 with the
-// divisions), where the memory would take 16; reading back takes the memory's time.
+// processor", 1990): with y the correctly rounded reciprocal of the scale, q = x y, the residual r = q scale - x in one fused
+// operation, and q - r y in another, three packed operations for two elements in place of a division each. The residual is
+// exact but for 2 quotients in 1000, and the result is the correctly rounded x / scale for every pair of bf16 or fp16
+// mantissas (compared in exact arithmetic; in this form of the signs also for x = -0).
 //
-// Bound: HBM, each row is read and written once. One thread holds 8 elements of a K row and the same 8 of the V row
-// (independent 16-byte loads, of one row when there are few, else of two); D / 8 neighbouring lanes share a row and take its maximum by shuffles.
+// Bound: each row is read and written once, and few instructions are left beside that. Measured (16383 tokens of 8 heads,
+// D 128, inputs larger than L2, in a graph; the memory's time at the rate of a copy in parentheses):
+//   append as e4m3 26 us (16): instruction issue, 580 warp instructions for two K and two V rows of 8 elements a lane
+//     (33 us with divisions);  append of 16 bits 23 us (20);
+//   gather from e4m3 20 us (16), of 8191 tokens 10.8 (7.8), from 16 bits 12.5 (10.3): the loads' latency, slot -> codes, with
+//     one row of K and of V a thread.
+// One thread holds 8 elements of a K row and the same 8 of the V row (independent 16-byte loads; the append of one row when
+// there are few, else of two); D / 8 neighbouring lanes share a row and take its maximum by shuffles.
 // Slots outside [0, num_slots) are not touched: negative ones mark padding, others set the device error word.
 #pragma once
 

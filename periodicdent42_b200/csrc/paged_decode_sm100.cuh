@@ -26,8 +26,8 @@
 //   - the values' scales enter the exponent: w_j = 2^(s_j + log2 scale_j - m_w) with a running maximum m_w of its own, so
 //     the rounded weights span (0, 1] whatever the scales are, and O = sum_j w_j code_j 2^(m_w) beside l = sum_j p_j 2^m.
 //
-// P (or w) is rounded to 16 bits for the second product (relative error 2^-9 bf16, 2^-12 fp16 a weight, the outputs' own
-// rounding or finer); its sum is taken in fp32 before the rounding.
+// P (or w) is rounded to 16 bits for the second product (half a step: 2^-8 of a weight in bf16, 2^-11 in fp16, the
+// outputs' own rounding or finer); its sum is taken in fp32 before the rounding.
 #pragma once
 
 #include <cuda_bf16.h>

@@ -17,8 +17,8 @@
 // a block (its tokens' heads of Q, then of K) are dealt out to groups of threads, a thread keeping its place within the
 // head (its VEC pairs: 32 bytes of a 16-byte-aligned row); kRotaryBatch rows per thread are loaded before the angles
 // are taken and before any is stored, so that enough loads are in flight, and neighbouring pieces move as one 32-byte
-// access (16383 tokens of 32 + 8 heads, D 128, bf16, interleaved: 60 us a pass, 5.6 TB/s; in 16-byte accesses 108; one
-// row at a time 89).
+// access (16383 tokens of 32 + 8 heads, D 128, bf16, half of the head turned, interleaved: 60 us a pass, 5.6 TB/s; in
+// 16-byte accesses 108; one row at a time 89; all of the head turned, either layout: 70..73, 4.7 TB/s).
 #pragma once
 
 #include <cuda_bf16.h>

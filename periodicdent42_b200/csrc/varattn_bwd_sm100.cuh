@@ -11,7 +11,8 @@
 // The CTA's shape is that of the block-sparse backward (bsattn_bwd_sm100.cuh, where it is explained and measured): warp 0
 // TMA producer, warp 1 MMA issuer, warps 4-11 two warpgroups that each take 64 columns of the 128 x 128 score tiles, P kept
 // in fp32 registers between its use for dV and for dS; P^T and dS^T / dS are rounded to the inputs' type for the second
-// products (an error of 2^-9 bf16, 2^-12 fp16 a weight, that of the results' own rounding). What differs:
+// products (half a step: 2^-8 of a weight in bf16, 2^-11 in fp16, as the results' own rounding; gradients come out
+// 1.5 times as far from the 64-bit ones, normwise, as results rounded once). What differs:
 //   - masks go by position: keys behind a row (causal) or behind the sequence's end get P = 0;
 //   - rows of a tile that are not the sequence's own (behind its end, or the 128 mod group rows that no copy fills) would
 //     enter the sums as 0 x their value, so warp 2 sets them to zero in shared memory between the copy's arrival and the
@@ -827,8 +828,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
             pk[i >> 1] = pack2<kF16>(g0, g1);
             pk[(i >> 1) + 1] = pack2<kF16>(g2, g3);
           }
-          // P of a masked row is zero, but its dP may be infinite. (On the packed pairs, apart from the loop above: inside it, every
-          // block executed the selects, 18 % more instructions and 5 % more time.)
+          // P of a masked row is zero, but its dP may be infinite. (On the packed pairs, apart from the loop above: inside it,
+          // every block executed the selects, 18 % more instructions and 5 % more time.)
           if (diag) {
 #pragma unroll
             for (int i = 0; i < 16; ++i) {

@@ -483,8 +483,9 @@ def attention_paged(Q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     a value beyond 32 bits is out of range like any other).
     A row that sees no key is zero, and so are rows behind the last sequence. Stale contents of a page behind its
     sequence's end reach no row, NaN among them; a non-finite value inside a sequence may make rows of it NaN that see it
-    with weight zero or, masked, share its block of keys. For serving: has no gradient, and tensors that require one are
-    refused outside torch.no_grad()."""
+    with weight zero or are masked for it, fewer than 256 tokens before it. The softmax's weights are rounded to Q's type for
+    their product with V; over e4m3 caches they are weight times the value's scale, rounded to fp16. For serving: has no
+    gradient, and tensors that require one are refused outside torch.no_grad()."""
     if scale is None:
         scale = Q.shape[-1] ** -0.5 if Q.dim() and Q.shape[-1] else 1.0
     return _C().attention_paged(Q, k_cache, v_cache, block_table, kv_lens, cu_seqlens, scale, k_scale, v_scale)
@@ -498,7 +499,8 @@ def attention_varlen(Q: torch.Tensor, K: torch.Tensor, V: torch.Tensor, cu_seqle
     query head h reads kv head h // (heads / kv_heads)); sequence i owns rows cu_seqlens[i] .. cu_seqlens[i+1]
     (int32 or int64 [batch + 1], starting at 0; any lengths, zero included). Rows behind the last sequence are zero.
     Sequences do not reach one another, non-finite values included; inside one, a non-finite row of V may make rows NaN
-    that it is masked for. Differentiable (once, in reverse mode) in Q, K and V (deterministic, no atomics)."""
+    that are masked for it, fewer than 256 tokens before it. Differentiable (once, in reverse mode) in Q, K and V
+    (deterministic, no atomics). The softmax's weights and, for the gradients, dS are rounded to Q's type for their products."""
     if scale is None:
         scale = Q.shape[-1] ** -0.5 if Q.dim() and Q.shape[-1] else 1.0
     return _C().attention_varlen(Q, K, V, cu_seqlens, scale, causal)

@@ -234,6 +234,9 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
   };
   // Keys of the sequence in the item's last block: below 128 its V tile holds foreign rows.
   auto tail_rows = [](const VarItem& it) { return it.kv_len - (it.b1 - 1) * kVarBlk; };
+  // e4m3: the first block that may be the last one that some row sees keys of: that of the first token's own key, or the item's
+  // last. The blocks before it are seen whole by every row that sees any key.
+  auto first_edge = [](const VarItem& it) { return min(it.pos0 >> 7, it.b1 - 1); };
 
   static_assert(kAttnThreads == 512, "register split assumes 16 warps");
   if (warp < 4) ptx::setmaxnreg_dec<kAttnRegsLow>();
@@ -465,7 +468,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
             int most[4];
 #pragma unroll
             for (int x = 0; x < 4; ++x) most[x] = __reduce_max_sync(0xffffffffu, top[x]);
-            if (b >= min((it.pos0 + 1) >> 7, it.b1 - 1)) {  // some row may not see all of the block: the largest up to each key
+            if (b >= first_edge(it)) {  // some row may not see all of the block: the largest up to each key
 #pragma unroll 1
               for (int o = 1; o < 32; o <<= 1)
 #pragma unroll
@@ -627,7 +630,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         float step = 1.0f, lift = 0.0f;  // O follows the scale reference
         // The row's scale reference where it is not the tile's: a row that sees part of the block has seen all before it. How far
         // (log2) the tile's lies above the row's, and, with the row's last key in the block, the row's closing factor.
-        const bool edge = kE4m3 && kb >= min(clear, it.b1 - 1);
+        const bool edge = kE4m3 && kb >= first_edge(it);
         auto reference = [&]() -> int {
           const int seen = limit - kb * kVarBlk;
           return seen > 0 ? max(v_top[128 * b + min(seen, kVarBlk) - 1], r_tile[b] - kScaleSpan) : r_tile[b];

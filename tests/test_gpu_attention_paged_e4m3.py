@@ -124,3 +124,18 @@ def test_queries_with_one_large_element(no_device_error, cuda_dev, new):
     assert worst(bsk.attention_paged(q, **at, **c), q, c, at, [300], [new]) <= 1.0
     q[..., 3] = torch.finfo(torch.bfloat16).max  # the largest bf16 value turns into a finite fp16 value
     assert torch.isfinite(bsk.attention_paged(q, **at, **c)).all()
+
+
+@pytest.mark.parametrize("H,G,D", [(3, 1, 64), (16, 2, 128), (33, 1, 64)])
+def test_chunks_that_start_at_every_place_of_a_block(no_device_error, cuda_dev, H, G, D):
+    """Tiles that begin on either side of a key block's end, rows without keys in front of it, several entries per CTA."""
+    start = [-2, -1, 0, 1, 41, 126, 127, 128, 129, 254, 255, 256, 382, 383, 384, 511, 639]
+    new = [1 + (29 * i) % 90 for i in range(3 * len(start))]
+    kv = [max(n + start[i % len(start)], 0) for i, n in enumerate(new)]
+    g = torch.Generator(device=cuda_dev).manual_seed(1)
+    size = torch.exp2(torch.randint(-6, 7, (len(new), 1, G), generator=g, device=cuda_dev).float()).expand(-1, max(kv), -1)
+    q, c, at = make(new, kv, H, G, D, 16, torch.bfloat16, cuda_dev, 6, size)
+    out = bsk.attention_paged(q, **at, **c)
+    assert worst(out, q, c, at, kv, new) <= 1.0
+    for _ in range(3):
+        assert torch.equal(out, bsk.attention_paged(q, **at, **c))

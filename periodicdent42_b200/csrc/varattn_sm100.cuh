@@ -31,7 +31,7 @@
 // Bound here: the conversion's one warp per sub-partition beside the softmax's two (8100 warp instructions a block where
 // 16-bit caches take 4100), and instructions: the roles share the instruction cache, and with more code in their loops they
 // wait for it. So the conversion's and the two issuers' loops are rolled (1024 new tokens over 30000, 32 / 8 heads, D 128:
-// 1039 us; conversion unrolled 1126, issuers unrolled 1189, both 1203; 16-bit cache 553).
+// 1047 us; when it was 1033: conversion unrolled 1126, issuers unrolled 1189, both 1203; 16-bit cache 555).
 //
 // P is rounded to the operands' type (half a step: 2^-8 of a weight in bf16, 2^-11 in fp16), its sums are fp32 and taken before.
 //

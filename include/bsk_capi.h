@@ -436,6 +436,31 @@ int bsk_attention_varlen_bwd(int dtype, const void* dO, int64_t do_token_stride,
                              void* workspace, int64_t workspace_bytes, void* stream);
 
 /*
+ * The same attention with a sliding window (causal): a row at position p sees the keys at positions p - window + 1 .. p
+ * and the first `sinks` ones (0 .. sinks - 1, up to p). window >= 1, sinks >= 0; otherwise as the functions above, their
+ * workspaces included. The work is that of the keys that are seen: key blocks that no row of a tile sees are not read. Over a
+ * paged cache, pages wholly outside what a sequence's new tokens see are neither read nor looked up (their table entries may
+ * hold anything). A non-finite V may reach rows that have left it behind by fewer than 256 tokens, as it may those before it.
+ */
+int bsk_attention_paged_window(int dtype, const void* Q, int64_t q_token_stride, int64_t q_head_stride, const void* k_cache,
+                               const void* v_cache, int cache_e4m3, const float* k_scale, const float* v_scale,
+                               const int32_t* block_table, int64_t table_stride, int table_width, const int32_t* kv_lens,
+                               const int32_t* cu_seqlens, void* O, int tokens, int batch, int heads, int kv_heads, int dim,
+                               int num_pages, int page_size, float scale, int window, int sinks, void* workspace,
+                               int64_t workspace_bytes, void* stream);
+int bsk_attention_varlen_window_fwd(int dtype, const void* Q, int64_t q_token_stride, int64_t q_head_stride, const void* K,
+                                    int64_t k_token_stride, int64_t k_head_stride, const void* V, int64_t v_token_stride,
+                                    int64_t v_head_stride, const int32_t* cu_seqlens, void* O, float* lse, int tokens,
+                                    int batch, int heads, int kv_heads, int dim, float scale, int window, int sinks,
+                                    void* workspace, int64_t workspace_bytes, void* stream);
+int bsk_attention_varlen_window_bwd(int dtype, const void* dO, int64_t do_token_stride, int64_t do_head_stride, const void* Q,
+                                    int64_t q_token_stride, int64_t q_head_stride, const void* K, int64_t k_token_stride,
+                                    int64_t k_head_stride, const void* V, int64_t v_token_stride, int64_t v_head_stride,
+                                    const void* O, const float* lse, const int32_t* cu_seqlens, void* dQ, void* dK, void* dV,
+                                    int tokens, int batch, int heads, int kv_heads, int dim, float scale, int window,
+                                    int sinks, void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
  * Drop-in for the reference's launcher signature (BlackwellSparseK/src/kernel_launch.cu:33-61).
  * A is BSR with blocks of (M/A_M_blocks) x (K/A_K_blocks). A B with every block present is read as the dense
  * row-major [K, N] matrix the reference Python layer passes (BlackwellSparseK/python/ops.py:104-107); a B with

@@ -88,7 +88,16 @@ def gradients64(q, k, v, do, allowed, scale, dtype):
     return {"O": (o, bo), "dQ": (dq, bq), "dK": (dk, bk), "dV": (dv, bv)}
 
 
-def packed64(q, k, v, lens, causal, scale, do=None):
+def visible(place, keys, window=None, sinks=0):
+    """Which of `keys` positions rows at positions `place` see, causally: the last `window` up to their own and the first
+    `sinks`."""
+    key = torch.arange(keys, device=place.device)[None, :]
+    here = place[:, None]
+    seen = key <= here
+    return seen if window is None else seen & ((here - key < window) | (key < sinks))
+
+
+def packed64(q, k, v, lens, causal, scale, do=None, window=None, sinks=0):
     """Packed sequences with grouped heads: dict name -> (value, bound) of O (and the gradients when do is given). The sum
     over a group's heads is made before the one rounding of dK and dV; the heads' bounds add up."""
     T, H, D = q.shape
@@ -101,7 +110,7 @@ def packed64(q, k, v, lens, causal, scale, do=None):
     for n in lens:
         rows = slice(a, a + n)
         allowed = torch.ones(n, n, dtype=torch.bool, device=q.device)
-        allowed = allowed.tril() if causal else allowed
+        allowed = visible(torch.arange(n, device=q.device), n, window, sinks) if causal else allowed
         for h in range(H):
             c = h // G
             if do is None:
@@ -116,7 +125,7 @@ def packed64(q, k, v, lens, causal, scale, do=None):
     return out
 
 
-def paged64(q, k_cache, v_cache, block_table, kv_lens, new, scale, k_scale=None, v_scale=None):
+def paged64(q, k_cache, v_cache, block_table, kv_lens, new, scale, k_scale=None, v_scale=None, window=None, sinks=0):
     """(O, bound) of attention over a paged cache; kv_lens and new are lists. Codes are multiplied by their scales in 64
     bits. With e4m3 codes the weights P_j s_j (s_j: the value's scale; their product is one more fp32 rounding, which e_w's
     factor of two has room for) are rounded to fp16 and meet the codes. They are brought near 1 first, so fp16's absolute
@@ -143,7 +152,7 @@ def paged64(q, k_cache, v_cache, block_table, kv_lens, new, scale, k_scale=None,
             codes, sv = v.abs(), scales(v_scale)
             k, v = k * scales(k_scale), v * sv
         pos = L - n + torch.arange(n, device=q.device)
-        allowed = torch.arange(L, device=q.device)[None, :] <= pos[:, None]
+        allowed = visible(pos, L, window, sinks)
         for h in range(H):
             c = h // G
             if k_scale is None:

@@ -16,6 +16,8 @@ import os
 import subprocess
 import sys
 import sysconfig
+import tempfile
+from concurrent.futures import ThreadPoolExecutor
 
 PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 REPO_DIR = os.path.dirname(PKG_DIR)
@@ -25,9 +27,9 @@ CAPI_LIB = os.path.join(PKG_DIR, "libbsk_sm100.so")
 TORCH_EXT = os.path.join(PKG_DIR, "_C.so")
 
 NVCC_ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
-CAPI_SOURCES = [os.path.join(CSRC, "capi.cu")]
+CAPI_SOURCES = [os.path.join(CSRC, f) for f in ("capi.cu", "window.cu")]
 CAPI_DEPS = CAPI_SOURCES + sorted(
-    os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith(".cuh")
+    os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith((".cuh", ".h"))
 ) + [os.path.join(INCLUDE, "bsk_capi.h")]
 
 
@@ -55,9 +57,13 @@ def build_capi(force: bool = False, extra: list[str] | None = None) -> str:
     if not force and not _stale(CAPI_LIB, CAPI_DEPS):
         return CAPI_LIB
     tmp = CAPI_LIB + ".tmp"
-    cmd = [_nvcc(), *NVCC_ARCH, "-lineinfo", "-O3", "-std=c++17", "-I", INCLUDE, "-shared", "-Xcompiler", "-fPIC",
-           "-Xcompiler", "-fvisibility=default", *(extra or []), "-o", tmp, *CAPI_SOURCES]
-    _run(cmd)
+    flags = ["-lineinfo", "-O3", "-std=c++17", "-I", INCLUDE, "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=default",
+             *(extra or [])]
+    with tempfile.TemporaryDirectory() as d:  # the sources compile at the same time
+        objects = [os.path.join(d, os.path.basename(f) + ".o") for f in CAPI_SOURCES]
+        with ThreadPoolExecutor(len(objects)) as pool:
+            list(pool.map(lambda x: _run([_nvcc(), *NVCC_ARCH, *flags, "-c", "-o", x[1], x[0]]), zip(CAPI_SOURCES, objects)))
+        _run([_nvcc(), *NVCC_ARCH, "-shared", "-o", tmp, *objects])
     os.replace(tmp, CAPI_LIB)
     return CAPI_LIB
 

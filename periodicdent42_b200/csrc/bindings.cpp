@@ -356,11 +356,23 @@ void check_heads(const char* op, const torch::Tensor& Q, int64_t kv_heads, doubl
   TORCH_CHECK_VALUE(static_cast<float>(scale) > 0.0f && scale < 1e30, op, ": scale must be positive and below 1e30 in float32");
 }
 
+// window 0: none (the Python layer's None). Larger ones than any sequence are as good as that.
+void check_window(const char* op, int64_t& window, int64_t& sinks, bool causal) {
+  TORCH_CHECK_VALUE(window >= 0, op, ": window must be at least 1, got ", window);
+  TORCH_CHECK_VALUE(sinks >= 0, op, ": sinks must not be negative, got ", sinks);
+  TORCH_CHECK_VALUE(window > 0 || sinks == 0, op, ": sinks go with a window");
+  TORCH_CHECK_VALUE(window == 0 || causal, op, ": a window needs causal attention");
+  constexpr int64_t kMost = std::numeric_limits<int32_t>::max();
+  window = std::min(window, kMost);
+  sinks = std::min(sinks, kMost);
+}
+
 torch::Tensor attention_paged(torch::Tensor Q, torch::Tensor k_cache, torch::Tensor v_cache, torch::Tensor block_table,
                               torch::Tensor kv_lens, torch::Tensor cu_seqlens, double scale, OptTensor k_scale,
-                              OptTensor v_scale) {
+                              OptTensor v_scale, int64_t window, int64_t sinks) {
   const char* op = "attention_paged";
   check_cuda(Q, Q, op, "Q");
+  check_window(op, window, sinks, true);
   no_gradient(op, {&Q, &k_cache, &v_cache, some(k_scale), some(v_scale)});
   TORCH_CHECK_VALUE(Q.dim() == 3, op, ": Q must be [tokens, heads, dim]");
   const int code = dtype_code(Q, op);
@@ -382,14 +394,23 @@ torch::Tensor attention_paged(torch::Tensor Q, torch::Tensor k_cache, torch::Ten
   TORCH_CHECK(need >= 0, "bsk_attention_paged_workspace_bytes failed: ", bsk_last_error());
   torch::Tensor ws;
   if (need > 0) ws = torch::empty({need}, Q.options().dtype(torch::kUInt8));
-  check_rc(bsk_attention_paged(code, q.p(), q.ts, q.hs, k_cache.data_ptr(), v_cache.data_ptr(), e4m3, scale_ptr(k_scale),
-                               scale_ptr(v_scale), table.data_ptr<int32_t>(), table.size(1),
-                               narrow(table.size(1), op, "table width"), lens.data_ptr<int32_t>(), cu.data_ptr<int32_t>(),
-                               O.data_ptr(), narrow(Q.size(0), op, "tokens"), narrow(lens.size(0), op, "batch"),
-                               static_cast<int>(Q.size(1)), static_cast<int>(k_cache.size(2)), static_cast<int>(Q.size(2)),
-                               narrow(k_cache.size(0), op, "pages"), static_cast<int>(page), static_cast<float>(scale),
-                               need > 0 ? ws.data_ptr() : nullptr, need, stream_of(Q)),
-           "bsk_attention_paged");
+  const int tokens = narrow(Q.size(0), op, "tokens"), batch = narrow(lens.size(0), op, "batch"), heads = static_cast<int>(Q.size(1)),
+            kv_heads = static_cast<int>(k_cache.size(2)), dim = static_cast<int>(Q.size(2)),
+            pages = narrow(k_cache.size(0), op, "pages"), width = narrow(table.size(1), op, "table width");
+  void* const ws_ptr = need > 0 ? ws.data_ptr() : nullptr;
+  if (window > 0)
+    check_rc(bsk_attention_paged_window(code, q.p(), q.ts, q.hs, k_cache.data_ptr(), v_cache.data_ptr(), e4m3, scale_ptr(k_scale),
+                                        scale_ptr(v_scale), table.data_ptr<int32_t>(), table.size(1), width,
+                                        lens.data_ptr<int32_t>(), cu.data_ptr<int32_t>(), O.data_ptr(), tokens, batch, heads,
+                                        kv_heads, dim, pages, static_cast<int>(page), static_cast<float>(scale),
+                                        static_cast<int>(window), static_cast<int>(sinks), ws_ptr, need, stream_of(Q)),
+             "bsk_attention_paged_window");
+  else
+    check_rc(bsk_attention_paged(code, q.p(), q.ts, q.hs, k_cache.data_ptr(), v_cache.data_ptr(), e4m3, scale_ptr(k_scale),
+                                 scale_ptr(v_scale), table.data_ptr<int32_t>(), table.size(1), width, lens.data_ptr<int32_t>(),
+                                 cu.data_ptr<int32_t>(), O.data_ptr(), tokens, batch, heads, kv_heads, dim, pages,
+                                 static_cast<int>(page), static_cast<float>(scale), ws_ptr, need, stream_of(Q)),
+             "bsk_attention_paged");
   return O;
 }
 
@@ -415,7 +436,7 @@ void check_varlen(const char* op, const torch::Tensor& Q, const torch::Tensor& K
 // (O, LSE): the log-sum-exp [tokens, heads] only when asked for (else an empty tensor).
 std::tuple<torch::Tensor, torch::Tensor> attention_varlen_fwd(torch::Tensor Q, torch::Tensor K, torch::Tensor V,
                                                               torch::Tensor cu_seqlens, double scale, bool causal,
-                                                              bool want_lse) {
+                                                              int64_t window, int64_t sinks, bool want_lse) {
   const char* op = "attention_varlen";
   check_varlen(op, Q, K, V, scale);
   const int code = dtype_code(Q, op);
@@ -427,18 +448,27 @@ std::tuple<torch::Tensor, torch::Tensor> attention_varlen_fwd(torch::Tensor Q, t
   auto O = torch::empty({Q.size(0), Q.size(1), Q.size(2)}, Q.options());
   auto lse = torch::empty({want_lse ? Q.size(0) : 0, Q.size(1)}, Q.options().dtype(torch::kFloat32));
   auto ws = varlen_workspace(Q, batch, K.size(1), false);
-  check_rc(bsk_attention_varlen_fwd(code, q.p(), q.ts, q.hs, k.p(), k.ts, k.hs, v.p(), v.ts, v.hs, cu.data_ptr<int32_t>(),
-                                    O.data_ptr(), want_lse ? lse.data_ptr<float>() : nullptr, static_cast<int>(Q.size(0)),
-                                    narrow(batch, op, "batch"), static_cast<int>(Q.size(1)), static_cast<int>(K.size(1)),
-                                    static_cast<int>(Q.size(2)), static_cast<float>(scale), causal, ws.data_ptr(),
-                                    ws.numel(), stream_of(Q)),
-           "bsk_attention_varlen_fwd");
+  float* const lse_ptr = want_lse ? lse.data_ptr<float>() : nullptr;
+  const int tokens = static_cast<int>(Q.size(0)), n = narrow(batch, op, "batch"), heads = static_cast<int>(Q.size(1)),
+            kv_heads = static_cast<int>(K.size(1)), dim = static_cast<int>(Q.size(2));
+  if (window > 0)
+    check_rc(bsk_attention_varlen_window_fwd(code, q.p(), q.ts, q.hs, k.p(), k.ts, k.hs, v.p(), v.ts, v.hs, cu.data_ptr<int32_t>(),
+                                             O.data_ptr(), lse_ptr, tokens, n, heads, kv_heads, dim, static_cast<float>(scale),
+                                             static_cast<int>(window), static_cast<int>(sinks), ws.data_ptr(), ws.numel(),
+                                             stream_of(Q)),
+             "bsk_attention_varlen_window_fwd");
+  else
+    check_rc(bsk_attention_varlen_fwd(code, q.p(), q.ts, q.hs, k.p(), k.ts, k.hs, v.p(), v.ts, v.hs, cu.data_ptr<int32_t>(),
+                                      O.data_ptr(), lse_ptr, tokens, n, heads, kv_heads, dim, static_cast<float>(scale), causal,
+                                      ws.data_ptr(), ws.numel(), stream_of(Q)),
+             "bsk_attention_varlen_fwd");
   return {O, lse};
 }
 
 std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> attention_varlen_bwd(torch::Tensor dO, torch::Tensor Q, torch::Tensor K,
                                                                              torch::Tensor V, torch::Tensor O, torch::Tensor lse,
-                                                                             torch::Tensor cu_seqlens, double scale, bool causal) {
+                                                                             torch::Tensor cu_seqlens, double scale, bool causal,
+                                                                             int64_t window, int64_t sinks) {
   const char* op = "attention_varlen backward";
   check_varlen(op, Q, K, V, scale);
   const int code = dtype_code(Q, op);
@@ -459,12 +489,21 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> attention_varlen_bwd(tor
   auto dK = torch::empty({K.size(0), K.size(1), K.size(2)}, K.options());
   auto dV = torch::empty_like(dK);
   auto ws = varlen_workspace(Q, batch, K.size(1), true);
-  check_rc(bsk_attention_varlen_bwd(code, g.p(), g.ts, g.hs, q.p(), q.ts, q.hs, k.p(), k.ts, k.hs, v.p(), v.ts, v.hs,
-                                    O.data_ptr(), lse.data_ptr<float>(), cu.data_ptr<int32_t>(), dQ.data_ptr(),
-                                    dK.data_ptr(), dV.data_ptr(), static_cast<int>(Q.size(0)), narrow(batch, op, "batch"),
-                                    static_cast<int>(Q.size(1)), static_cast<int>(K.size(1)), static_cast<int>(Q.size(2)),
-                                    static_cast<float>(scale), causal, ws.data_ptr(), ws.numel(), stream_of(Q)),
-           "bsk_attention_varlen_bwd");
+  const int tokens = static_cast<int>(Q.size(0)), n = narrow(batch, op, "batch"), heads = static_cast<int>(Q.size(1)),
+            kv_heads = static_cast<int>(K.size(1)), dim = static_cast<int>(Q.size(2));
+  if (window > 0)
+    check_rc(bsk_attention_varlen_window_bwd(code, g.p(), g.ts, g.hs, q.p(), q.ts, q.hs, k.p(), k.ts, k.hs, v.p(), v.ts, v.hs,
+                                             O.data_ptr(), lse.data_ptr<float>(), cu.data_ptr<int32_t>(), dQ.data_ptr(),
+                                             dK.data_ptr(), dV.data_ptr(), tokens, n, heads, kv_heads, dim,
+                                             static_cast<float>(scale), static_cast<int>(window), static_cast<int>(sinks),
+                                             ws.data_ptr(), ws.numel(), stream_of(Q)),
+             "bsk_attention_varlen_window_bwd");
+  else
+    check_rc(bsk_attention_varlen_bwd(code, g.p(), g.ts, g.hs, q.p(), q.ts, q.hs, k.p(), k.ts, k.hs, v.p(), v.ts, v.hs,
+                                      O.data_ptr(), lse.data_ptr<float>(), cu.data_ptr<int32_t>(), dQ.data_ptr(), dK.data_ptr(),
+                                      dV.data_ptr(), tokens, n, heads, kv_heads, dim, static_cast<float>(scale), causal,
+                                      ws.data_ptr(), ws.numel(), stream_of(Q)),
+             "bsk_attention_varlen_bwd");
   return {dQ, dK, dV};
 }
 
@@ -484,21 +523,24 @@ variable_list once(variable_list grads, const char* what) {
 // Packed attention: the forward keeps the rows' log-sum-exp, the backward recomputes the scores.
 struct VarlenAttention : public torch::autograd::Function<VarlenAttention> {
   static torch::Tensor forward(AutogradContext* ctx, torch::Tensor Q, torch::Tensor K, torch::Tensor V,
-                               torch::Tensor cu_seqlens, double scale, bool causal) {
+                               torch::Tensor cu_seqlens, double scale, bool causal, int64_t window, int64_t sinks) {
     at::AutoDispatchBelowADInplaceOrView guard;
-    auto [O, lse] = attention_varlen_fwd(Q, K, V, cu_seqlens, scale, causal, true);
+    auto [O, lse] = attention_varlen_fwd(Q, K, V, cu_seqlens, scale, causal, window, sinks, true);
     ctx->save_for_backward({Q, K, V, O, lse, cu_seqlens});
     ctx->saved_data["scale"] = scale;
     ctx->saved_data["causal"] = causal;
+    ctx->saved_data["window"] = window;
+    ctx->saved_data["sinks"] = sinks;
     return O;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto s = ctx->get_saved_variables();
-    variable_list out(6);
+    variable_list out(8);
     {
       at::AutoGradMode no_grad(false);
       auto [dQ, dK, dV] = attention_varlen_bwd(grads[0].to(s[0].scalar_type()), s[0], s[1], s[2], s[3], s[4], s[5],
-                                               ctx->saved_data["scale"].toDouble(), ctx->saved_data["causal"].toBool());
+                                               ctx->saved_data["scale"].toDouble(), ctx->saved_data["causal"].toBool(),
+                                               ctx->saved_data["window"].toInt(), ctx->saved_data["sinks"].toInt());
       if (ctx->needs_input_grad(0)) out[0] = dQ;
       if (ctx->needs_input_grad(1)) out[1] = dK;
       if (ctx->needs_input_grad(2)) out[2] = dV;
@@ -508,11 +550,12 @@ struct VarlenAttention : public torch::autograd::Function<VarlenAttention> {
 };
 
 torch::Tensor attention_varlen(torch::Tensor Q, torch::Tensor K, torch::Tensor V, torch::Tensor cu_seqlens, double scale,
-                               bool causal) {
+                               bool causal, int64_t window, int64_t sinks) {
   no_tangent("attention_varlen", {&Q, &K, &V});
+  check_window("attention_varlen", window, sinks, causal);
   if (at::GradMode::is_enabled() && (Q.requires_grad() || K.requires_grad() || V.requires_grad()))
-    return VarlenAttention::apply(Q, K, V, cu_seqlens, scale, causal);
-  return std::get<0>(attention_varlen_fwd(Q, K, V, cu_seqlens, scale, causal, false));
+    return VarlenAttention::apply(Q, K, V, cu_seqlens, scale, causal, window, sinks);
+  return std::get<0>(attention_varlen_fwd(Q, K, V, cu_seqlens, scale, causal, window, sinks, false));
 }
 
 // Rotary positions: the gradient of a turn is the turn back.
@@ -588,8 +631,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("v_scale") = py::none());
   m.def("attention_paged", &attention_paged, "attention of new tokens over a paged cache (sm_100a)", py::arg("Q"),
         py::arg("k_cache"), py::arg("v_cache"), py::arg("block_table"), py::arg("kv_lens"), py::arg("cu_seqlens"),
-        py::arg("scale"), py::arg("k_scale") = py::none(), py::arg("v_scale") = py::none());
+        py::arg("scale"), py::arg("k_scale") = py::none(), py::arg("v_scale") = py::none(), py::arg("window") = 0,
+        py::arg("sinks") = 0);
   m.def("attention_varlen", &attention_varlen, "attention over packed sequences, with gradients (sm_100a)", py::arg("Q"),
-        py::arg("K"), py::arg("V"), py::arg("cu_seqlens"), py::arg("scale"), py::arg("causal") = true);
+        py::arg("K"), py::arg("V"), py::arg("cu_seqlens"), py::arg("scale"), py::arg("causal") = true, py::arg("window") = 0,
+        py::arg("sinks") = 0);
   m.def("device_error", &device_error, "read and clear the device error word");
 }

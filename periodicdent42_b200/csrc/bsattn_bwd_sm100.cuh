@@ -118,7 +118,7 @@ __global__ void __launch_bounds__(256) bsattn_bwd_delta_kernel(const uint16_t* _
 // Column lists of the block mask: for every (b,h) pair, the query blocks of each key block-column in ascending
 // order (a counting sort of the row lists, one thread per pair). col_ptr shares row_ptr's numbering: pair p's
 // entries occupy [row_ptr[p*nqb], row_ptr[(p+1)*nqb]) in both. Out-of-range key blocks are dropped and flagged.
-__global__ void bsattn_mask_transpose_kernel(const int* __restrict__ row_ptr, const int* __restrict__ col_idx,
+static __global__ void bsattn_mask_transpose_kernel(const int* __restrict__ row_ptr, const int* __restrict__ col_idx,
                                              int pairs, int nqb, int* __restrict__ col_ptr,
                                              int* __restrict__ row_idx, int* __restrict__ cursor,
                                              int* __restrict__ bad) {
@@ -156,7 +156,7 @@ __global__ void bsattn_mask_transpose_kernel(const int* __restrict__ row_ptr, co
 // col_ptr, and each column's thread writes its query blocks in ascending order. Same output as the kernel above.
 constexpr int kTransposeSmemMaxBlocks = 512;  // bit map of 512 x 512 bits = 32 KB
 
-__global__ void __launch_bounds__(256) bsattn_mask_transpose_smem_kernel(const int* __restrict__ row_ptr,
+static __global__ void __launch_bounds__(256) bsattn_mask_transpose_smem_kernel(const int* __restrict__ row_ptr,
                                                                          const int* __restrict__ col_idx, int pairs,
                                                                          int nqb, int* __restrict__ col_ptr,
                                                                          int* __restrict__ row_idx,
@@ -211,7 +211,7 @@ __global__ void __launch_bounds__(256) bsattn_mask_transpose_smem_kernel(const i
 
 // Block mask of dense (every key block) or causal// Block mask of dense (every key block) or causal (key blocks 0..i of query block i) attention for `pairs`
 // (b,h) pairs: one thread per block-row writes its row pointer and column list.
-__global__ void attn_full_mask_kernel(int pairs, int nqb, int causal, int* __restrict__ row_ptr,
+static __global__ void attn_full_mask_kernel(int pairs, int nqb, int causal, int* __restrict__ row_ptr,
                                       int* __restrict__ col_idx) {
   const int rows = pairs * nqb;
   const int64_t per_pair = causal ? static_cast<int64_t>(nqb) * (nqb + 1) / 2 : static_cast<int64_t>(nqb) * nqb;

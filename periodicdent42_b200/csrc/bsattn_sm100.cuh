@@ -610,7 +610,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
 
 // One warp waits on an mbarrier that nothing completes; the bounded wait runs out, records
 // kErrWaitTimeout in the error word and the kernel returns. Used by the failure-detection self-test.
-__global__ void wait_probe_kernel(uint32_t* err, uint64_t timeout_ns) {
+static __global__ void wait_probe_kernel(uint32_t* err, uint64_t timeout_ns) {
   __shared__ uint64_t bar;
   __shared__ int abort_flag;
   if (threadIdx.x == 0) {
@@ -626,7 +626,7 @@ __global__ void wait_probe_kernel(uint32_t* err, uint64_t timeout_ns) {
 // y[i] = 2^x[i] by the softmax's exponential routes, for the accuracy self-test: fma_pipe = 1 takes the
 // FMA-pipe polynomial (ex2_poly2, on the pairs (x[2j], x[2j+1]) exactly as the softmax feeds it), 0 the
 // MUFU instruction (ex2.approx.ftz). Grid-stride over pairs; an odd tail element is paired with itself.
-__global__ void exp2_probe_kernel(const float* __restrict__ x, float* __restrict__ y, int n, int fma_pipe) {
+static __global__ void exp2_probe_kernel(const float* __restrict__ x, float* __restrict__ y, int n, int fma_pipe) {
   const int pairs = (n + 1) / 2;
   for (int j = blockIdx.x * blockDim.x + threadIdx.x; j < pairs; j += gridDim.x * blockDim.x) {
     const int i0 = 2 * j, i1 = (2 * j + 1 < n) ? 2 * j + 1 : 2 * j;

@@ -1,6 +1,6 @@
 // Host side of the C ABI (include/bsk_capi.h): argument validation, per-device set-up, TMA tensor-map
-// encoding and kernel launches. One translation unit holds every kernel of the library so that the
-// device error word below is a single symbol.
+// encoding and kernel launches. Every kernel of the library is compiled here but those of window.cu; kernels get the device
+// error word below as an argument.
 #include <cuda.h>
 #include <cuda_runtime.h>
 #include <cudaTypedefs.h>
@@ -26,6 +26,8 @@
 #include "paged_decode_sm100.cuh"
 #include "varattn_sm100.cuh"
 #include "varattn_bwd_sm100.cuh"
+#include "attention_launch.cuh"
+#include "window.h"
 
 namespace {
 
@@ -58,6 +60,8 @@ struct DeviceState {
   std::string init_error;
   int sm_count = 0;
   int pair_clusters = 0;       // co-resident 2-CTA clusters of the pair GEMM kernels (all share one footprint)
+  std::once_flag window_once;  // the kernels of window.cu are set up on their first call
+  cudaError_t window_status = cudaSuccess;
   int bsr_pair_clusters = 0;   // co-resident 2-CTA clusters of the pair BSR SpMM kernel (0: not used)
   uint32_t* err_word = nullptr;
 };
@@ -65,43 +69,6 @@ DeviceState g_devices[kMaxDevices];
 
 std::once_flag g_encode_once;
 PFN_cuTensorMapEncodeTiled_v12000 g_encode = nullptr;
-
-template <class K>
-cudaError_t allow_smem(K kernel, int bytes) {
-  return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-}
-
-// Shared memory of the paged decode kernels of 8 * kNQ rows.
-template <bool kF16, int kD, bool kFp8, int kNQ>
-cudaError_t allow_paged_one() {
-  const auto k = bsk::paged_decode_kernel<kF16, kD, kFp8, kNQ>;
-  using Sh = bsk::PagedShape<kD, kFp8, kNQ>;
-  static_assert(Sh::smem_bytes(Sh::kMaxWarps) <= 232448, "shared memory above the 227 KB per-CTA limit");
-  return allow_smem(k, Sh::smem_bytes(Sh::kMaxWarps));
-}
-template <int kNQ>
-cudaError_t allow_paged() {
-  const cudaError_t e[] = {allow_paged_one<false, 128, false, kNQ>(), allow_paged_one<false, 128, true, kNQ>(),
-                           allow_paged_one<false, 64, false, kNQ>(),  allow_paged_one<false, 64, true, kNQ>(),
-                           allow_paged_one<true, 128, false, kNQ>(),  allow_paged_one<true, 128, true, kNQ>(),
-                           allow_paged_one<true, 64, false, kNQ>(),   allow_paged_one<true, 64, true, kNQ>()};
-  for (cudaError_t x : e)
-    if (x != cudaSuccess) return x;
-  return cudaSuccess;
-}
-
-// The packed / paged attention forward, all types and head dims of one kind of K / V.
-template <int kKind>
-cudaError_t allow_varattn() {
-  using namespace bsk;
-  const cudaError_t e[] = {allow_smem(varattn_fwd_kernel<false, 128, kKind>, VarShape<false, 128, kKind>::kSmemBytes),
-                           allow_smem(varattn_fwd_kernel<false, 64, kKind>, VarShape<false, 64, kKind>::kSmemBytes),
-                           allow_smem(varattn_fwd_kernel<true, 128, kKind>, VarShape<true, 128, kKind>::kSmemBytes),
-                           allow_smem(varattn_fwd_kernel<true, 64, kKind>, VarShape<true, 64, kKind>::kSmemBytes)};
-  for (cudaError_t x : e)
-    if (x != cudaSuccess) return x;
-  return cudaSuccess;
-}
 
 // How many 2-CTA clusters of `kernel` can be resident at once (persistent grids are sized to this).
 template <class K>
@@ -198,16 +165,7 @@ void init_device(DeviceState& st, int dev) {
       allow_smem(gemm_pair_sm100_kernel<2, Epi::F32PeerRows, 2>, kPairWideSmemBytes),
       allow_smem(gemm_pair_sm100_kernel<1, Epi::BF16Scaled, 2>, kPairWideSmemBytes),
       allow_smem(spmm_bsr_pair_sm100_kernel, kBsrPairSmemBytes),
-      allow_paged<1>(), allow_paged<2>(), allow_paged<4>(),
-      allow_smem(varattn_bwd_dq_kernel<false, 128>, BwdDqShape<false, 128>::kSmemBytes),
-      allow_smem(varattn_bwd_dq_kernel<false, 64>, BwdDqShape<false, 64>::kSmemBytes),
-      allow_smem(varattn_bwd_dq_kernel<true, 128>, BwdDqShape<true, 128>::kSmemBytes),
-      allow_smem(varattn_bwd_dq_kernel<true, 64>, BwdDqShape<true, 64>::kSmemBytes),
-      allow_smem(varattn_bwd_dkdv_kernel<false, 128>, BwdDkdvShape<false, 128>::kSmemBytes),
-      allow_smem(varattn_bwd_dkdv_kernel<false, 64>, BwdDkdvShape<false, 64>::kSmemBytes),
-      allow_smem(varattn_bwd_dkdv_kernel<true, 128>, BwdDkdvShape<true, 128>::kSmemBytes),
-      allow_smem(varattn_bwd_dkdv_kernel<true, 64>, BwdDkdvShape<true, 64>::kSmemBytes),
-      allow_varattn<bsk::kPacked>(), allow_varattn<bsk::kCache16>(), allow_varattn<bsk::kCacheE4m3>(),
+      allow_attention<false>(),
   };
   for (cudaError_t x : errs) {
     if (x != cudaSuccess) {
@@ -2063,18 +2021,6 @@ void cache_append_launch(const bsk::KvCacheArgs& a, int rows, unsigned grid, cud
   else bsk::kv_cache_append_kernel<kF16, kD, kFp8, 2><<<grid, bsk::kCacheThreads, 0, s>>>(a);
 }
 
-// Instantiation by element type, head dim and cache type.
-#define BSK_BY_TYPE(KERNEL, f16, dim, fp8, ...)                             \
-  do {                                                                      \
-    if (f16) {                                                              \
-      if (dim == 128) { if (fp8) KERNEL<true, 128, true> __VA_ARGS__; else KERNEL<true, 128, false> __VA_ARGS__; } \
-      else            { if (fp8) KERNEL<true, 64, true> __VA_ARGS__; else KERNEL<true, 64, false> __VA_ARGS__; }   \
-    } else {                                                                \
-      if (dim == 128) { if (fp8) KERNEL<false, 128, true> __VA_ARGS__; else KERNEL<false, 128, false> __VA_ARGS__; } \
-      else            { if (fp8) KERNEL<false, 64, true> __VA_ARGS__; else KERNEL<false, 64, false> __VA_ARGS__; }   \
-    }                                                                       \
-  } while (0)
-
 }  // namespace
 
 extern "C" {
@@ -2148,23 +2094,6 @@ int heads_checks(const char* what, int dtype, int tokens, int batch, int heads, 
   return BSK_OK;
 }
 
-// Launch that may start before the kernel ahead of it in the stream has ended (the kernel waits for it by itself, after
-// its own set-up).
-template <class... KArgs, class... Args>
-cudaError_t launch_overlapped(void (*kernel)(KArgs...), dim3 grid, int threads, int smem, cudaStream_t s, const Args&... args) {
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3(threads, 1, 1);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = s;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, args...);
-}
-
 // Workspace of a work list: the entry count (16 bytes), then its entries.
 int64_t plan_bytes(int64_t tokens, int64_t batch, int64_t tt) {
   return 16 + bsk::plan_slots(tokens, batch, tt) * (int64_t)sizeof(bsk::VarItem);
@@ -2206,68 +2135,9 @@ PagedTilePlan paged_tile_plan(int64_t tokens, int64_t batch, int heads, int kv_h
 
 template <bool kF16, int kD>
 cudaError_t varattn_combine_launch(const bsk::VarCombineArgs& a, int most, cudaStream_t s) {
-  return launch_overlapped(bsk::varattn_combine_kernel<kF16, kD>, dim3(most, a.kv_heads, bsk::kVarBlk / bsk::kCombineRows),
+  return bsk::launch_overlapped(bsk::varattn_combine_kernel<kF16, kD>, dim3(most, a.kv_heads, bsk::kVarBlk / bsk::kCombineRows),
                            bsk::kCombineRows * kD / 4, 0, s, a);
 }
-
-template <int kKind>
-cudaError_t varattn_fwd_launch(bool f16, int dim, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
-                               const bsk::VarFwdArgs& a, unsigned grid, cudaStream_t s) {
-  using namespace bsk;
-  if (f16 && dim == 128)
-    return launch_overlapped(varattn_fwd_kernel<true, 128, kKind>, grid, kAttnThreads, VarShape<true, 128, kKind>::kSmemBytes, s,
-                             tq, tk, tv, a);
-  if (f16)
-    return launch_overlapped(varattn_fwd_kernel<true, 64, kKind>, grid, kAttnThreads, VarShape<true, 64, kKind>::kSmemBytes, s,
-                             tq, tk, tv, a);
-  if (dim == 128)
-    return launch_overlapped(varattn_fwd_kernel<false, 128, kKind>, grid, kAttnThreads, VarShape<false, 128, kKind>::kSmemBytes,
-                             s, tq, tk, tv, a);
-  return launch_overlapped(varattn_fwd_kernel<false, 64, kKind>, grid, kAttnThreads, VarShape<false, 64, kKind>::kSmemBytes, s,
-                           tq, tk, tv, a);
-}
-
-template <bool kF16, int kD>
-cudaError_t varattn_bwd_launch(const bsk::VarPrepArgs& p, const bsk::VarBwdArgs& a, const CUtensorMap& tq, const CUtensorMap& tk,
-                               const CUtensorMap& tv, const CUtensorMap& tdo, unsigned prep, unsigned gk, unsigned gq,
-                               cudaStream_t s) {
-  using namespace bsk;
-  varattn_bwd_prep_kernel<kF16, kD><<<prep, kPlanThreads, 0, s>>>(p);
-  cudaError_t e = launch_overlapped(varattn_bwd_dkdv_kernel<kF16, kD>, gk, kBwdThreads, BwdDkdvShape<kF16, kD>::kSmemBytes, s, tq,
-                                    tk, tv, tdo, a);
-  if (e != cudaSuccess) return e;
-  return launch_overlapped(varattn_bwd_dq_kernel<kF16, kD>, gq, kBwdThreads, BwdDqShape<kF16, kD>::kSmemBytes, s, tq, tk, tv, tdo,
-                           a);
-}
-
-template <bool kF16, int kD, bool kFp8, int kNQ>
-cudaError_t paged_decode_launch_rows(const bsk::PagedArgs& a, unsigned tiles, int cluster, bool alone, cudaStream_t s) {
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = cluster;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cfg.gridDim = dim3(tiles * cluster, a.kv_heads, 1);
-  using Sh = bsk::PagedShape<kD, kFp8, kNQ>;
-  const int warps = alone ? Sh::kMaxWarps : 4;
-  cfg.blockDim = dim3(32 * warps, 1, 1);
-  cfg.dynamicSmemBytes = Sh::smem_bytes(warps);
-  cfg.stream = s;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, bsk::paged_decode_kernel<kF16, kD, kFp8, kNQ>, a);
-}
-
-template <bool kF16, int kD, bool kFp8>
-cudaError_t paged_decode_launch(const bsk::PagedArgs& a, int nq, unsigned tiles, int cluster, bool alone, cudaStream_t s) {
-  if (nq == 1) return paged_decode_launch_rows<kF16, kD, kFp8, 1>(a, tiles, cluster, alone, s);
-  if (nq == 2) return paged_decode_launch_rows<kF16, kD, kFp8, 2>(a, tiles, cluster, alone, s);
-  return paged_decode_launch_rows<kF16, kD, kFp8, 4>(a, tiles, cluster, alone, s);
-}
-
-}  // namespace
-
-namespace {
 
 // Which kernel takes a paged call: the 128-row tcgen05 tiles when the sequences bring more than 32 rows (new tokens x heads
 // of a group) on average, the mma.sync tiles of up to 32 rows up to there (above, they read K and V more than once).
@@ -2283,21 +2153,43 @@ bool paged_in_tiles(int64_t tokens, int64_t batch, int64_t group, int64_t num_pa
 
 }  // namespace
 
-extern "C" {
+namespace {
 
-int64_t bsk_attention_paged_workspace_bytes(int tokens, int batch, int heads, int kv_heads, int dim, int num_pages) {
-  if (int rc = heads_checks("attention_paged_workspace_bytes", 0, tokens, batch, heads, kv_heads, dim, 1.0f)) return rc;
-  if (!paged_in_tiles(tokens, batch, heads / kv_heads, num_pages)) return 0;
-  DeviceState* st;
-  if (int rc = device_state(&st)) return rc;
-  return paged_tile_plan(tokens, batch, heads, kv_heads, dim, st->sm_count).total;
+// A window of the last keys and a few first ones (causal attention): a row at position p sees keys (p - window, p] and
+// [0, sinks). window 0: every key up to its own.
+struct Window {
+  int window = 0, sinks = 0;
+};
+
+int window_checks(const char* what, int window, int sinks) {
+  if (window < 1) return set_error(BSK_ERR_INVALID_ARG, "%s: window must be at least 1, got %d", what, window);
+  if (sinks < 0) return set_error(BSK_ERR_INVALID_ARG, "%s: sinks must not be negative, got %d", what, sinks);
+  return BSK_OK;
 }
 
-int bsk_attention_paged(int dtype, const void* Q, int64_t q_token_stride, int64_t q_head_stride, const void* k_cache,
-                        const void* v_cache, int cache_e4m3, const float* k_scale, const float* v_scale,
-                        const int32_t* block_table, int64_t table_stride, int table_width, const int32_t* kv_lens,
-                        const int32_t* cu_seqlens, void* O, int tokens, int batch, int heads, int kv_heads, int dim,
-                        int num_pages, int page_size, float scale, void* workspace, int64_t workspace_bytes, void* stream) {
+// Nothing to leave out in sequences of at most `longest` keys: the kernels without a window take the call.
+Window window_within(Window w, int64_t longest) { return (int64_t)w.window + w.sinks >= longest ? Window{} : w; }
+
+int window_ready(DeviceState& st) {
+  std::call_once(st.window_once, [&] { st.window_status = bsk::window_allow(); });
+  if (st.window_status != cudaSuccess) return cuda_fail(st.window_status, "window: set up");
+  return BSK_OK;
+}
+
+int64_t varlen_workspace(int64_t tokens, int64_t batch, int heads, int kv_heads, int dim, bool backward) {
+  const int tt = bsk::kVarBlk / (heads / kv_heads);
+  const int64_t plan = plan_bytes(tokens, batch, tt);
+  if (!backward) return plan;
+  // the two lists, then the tiles' row statistics
+  return plan + plan_bytes(tokens, batch, bsk::kVarBlk) + bsk::plan_slots(tokens, batch, tt) * kv_heads * 1024;
+}
+
+int attention_paged(int dtype, const void* Q, int64_t q_token_stride, int64_t q_head_stride, const void* k_cache,
+                    const void* v_cache, int cache_e4m3, const float* k_scale, const float* v_scale,
+                    const int32_t* block_table, int64_t table_stride, int table_width, const int32_t* kv_lens,
+                    const int32_t* cu_seqlens, void* O, int tokens, int batch, int heads, int kv_heads, int dim,
+                    int num_pages, int page_size, float scale, Window win, void* workspace, int64_t workspace_bytes,
+                    void* stream) {
   const char* what = "attention_paged";
   if (int rc = heads_checks(what, dtype, tokens, batch, heads, kv_heads, dim, scale)) return rc;
   if (page_size < 8 || page_size > 1024 || (page_size & (page_size - 1)))
@@ -2315,7 +2207,12 @@ int bsk_attention_paged(int dtype, const void* Q, int64_t q_token_stride, int64_
   if (!rows_aligned(Q, q_token_stride, q_head_stride, 2) || !aligned16(O) || !aligned16(k_cache) || !aligned16(v_cache))
     return set_error(BSK_ERR_INVALID_ARG, "%s: rows of Q, O and the caches must be 16-byte aligned", what);
   if (int rc = device_state(&st)) return rc;
+  win = window_within(win, (int64_t)table_width * page_size);
+  if (win.window)
+    if (int rc = window_ready(*st)) return rc;
   bsk::PagedArgs a{};
+  a.window = win.window;
+  a.sinks = win.sinks;
   a.Q = Q;
   a.q_token_stride = q_token_stride;
   a.q_head_stride = q_head_stride;
@@ -2364,6 +2261,8 @@ int bsk_attention_paged(int dtype, const void* Q, int64_t q_token_stride, int64_
     p.batch = batch;
     p.tt = tt;
     p.causal = 1;
+    p.window = win.window;
+    p.sinks = win.sinks;
     p.split_ctas = w.split_ctas;
     p.kv_heads = kv_heads;
     p.splits = reinterpret_cast<bsk::VarSplit*>(ws + w.splits_at);
@@ -2384,12 +2283,15 @@ int bsk_attention_paged(int dtype, const void* Q, int64_t q_token_stride, int64_
     f.kv_heads = kv_heads;
     f.group = a.group;
     f.causal = 1;
+    f.window = win.window;
+    f.sinks = win.sinks;
     f.scale_log2 = a.scale_log2;
     f.err = st->err_word;
     f.timeout_ns = t_timeout_ns;
     const unsigned grid = (unsigned)(most < st->sm_count ? most : st->sm_count);
-    cudaError_t e = cache_e4m3 ? varattn_fwd_launch<bsk::kCacheE4m3>(f16, dim, tq, tk, tv, f, grid, s)
-                               : varattn_fwd_launch<bsk::kCache16>(f16, dim, tq, tk, tv, f, grid, s);
+    cudaError_t e = win.window   ? bsk::window_fwd(cache_e4m3 ? bsk::kCacheE4m3 : bsk::kCache16, f16, dim, tq, tk, tv, f, grid, s)
+                    : cache_e4m3 ? bsk::varattn_fwd_launch<bsk::kCacheE4m3, false>(f16, dim, tq, tk, tv, f, grid, s)
+                                 : bsk::varattn_fwd_launch<bsk::kCache16, false>(f16, dim, tq, tk, tv, f, grid, s);
     if (w.split_ctas && e == cudaSuccess) {
       const bsk::VarCombineArgs c{O, f.part_o, f.part_lse, p.splits, f.count, heads, kv_heads, a.group};
       const int most_split = w.pieces / 2 + 1;
@@ -2410,37 +2312,31 @@ int bsk_attention_paged(int dtype, const void* Q, int64_t q_token_stride, int64_
   const int nq = avg <= 8 ? 1 : avg <= 16 ? 2 : 4;
   const int64_t tiles = (int64_t)tokens * a.group / (8 * nq) + batch + 1;
   const int64_t items = (avg + 8 * nq - 1) / (8 * nq) * batch * kv_heads;  // tiles that have work, about
-  const int64_t most_keys = (int64_t)table_width * page_size;
+  // (a window leaves a tile its last keys, those of its other tokens, and the sinks)
+  const int64_t room = (int64_t)table_width * page_size, reach = (int64_t)win.window + win.sinks + 8 * nq;
+  const int64_t most_keys = win.window && reach < room ? reach : room;
   int cluster = 1;
   while (cluster < 8 && items * cluster * 2 <= (int64_t)2 * st->sm_count && most_keys >= (int64_t)cluster * 256) cluster *= 2;
   if (cluster == 1 && items <= (int64_t)4 * st->sm_count && most_keys >= 2048) cluster = 2;
   const bool alone = items * cluster <= st->sm_count;
   if (tiles * cluster >= (int64_t)1 << 31) return set_error(BSK_ERR_UNSUPPORTED, "%s: too many rows", what);
-  cudaError_t e = cudaSuccess;
-  BSK_BY_TYPE(e = paged_decode_launch, dtype == 1, dim, cache_e4m3 != 0, (a, nq, (unsigned)tiles, cluster, alone, s));
+  const bsk::PagedGrid g{nq, (unsigned)tiles, cluster, alone};
+  const cudaError_t e = win.window ? bsk::window_decode(dtype == 1, dim, cache_e4m3 != 0, a, g, s)
+                                   : bsk::paged_decode_launch<false>(dtype == 1, dim, cache_e4m3 != 0, a, g, s);
   if (e != cudaSuccess) return cuda_fail(e, "attention_paged launch");
   return launch_status("attention_paged launch");
 }
 
-int64_t bsk_attention_varlen_workspace_bytes(int tokens, int batch, int heads, int kv_heads, int dim, int backward) {
-  if (int rc = heads_checks("attention_varlen_workspace_bytes", 0, tokens, batch, heads, kv_heads, dim, 1.0f)) return rc;
-  const int tt = bsk::kVarBlk / (heads / kv_heads);
-  const int64_t plan = plan_bytes(tokens, batch, tt);
-  if (!backward) return plan;
-  // the two lists, then the tiles' row statistics
-  return plan + plan_bytes(tokens, batch, bsk::kVarBlk) + bsk::plan_slots(tokens, batch, tt) * kv_heads * 1024;
-}
-
-int bsk_attention_varlen_fwd(int dtype, const void* Q, int64_t q_token_stride, int64_t q_head_stride, const void* K,
-                             int64_t k_token_stride, int64_t k_head_stride, const void* V, int64_t v_token_stride,
-                             int64_t v_head_stride, const int32_t* cu_seqlens, void* O, float* lse, int tokens, int batch,
-                             int heads, int kv_heads, int dim, float scale, int causal, void* workspace,
-                             int64_t workspace_bytes, void* stream) {
+int attention_varlen_fwd(int dtype, const void* Q, int64_t q_token_stride, int64_t q_head_stride, const void* K,
+                         int64_t k_token_stride, int64_t k_head_stride, const void* V, int64_t v_token_stride,
+                         int64_t v_head_stride, const int32_t* cu_seqlens, void* O, float* lse, int tokens, int batch,
+                         int heads, int kv_heads, int dim, float scale, int causal, Window win, void* workspace,
+                         int64_t workspace_bytes, void* stream) {
   const char* what = "attention_varlen_fwd";
   if (int rc = heads_checks(what, dtype, tokens, batch, heads, kv_heads, dim, scale)) return rc;
   DeviceState* st;
   if (tokens == 0) return device_state(&st);
-  const int64_t need = bsk_attention_varlen_workspace_bytes(tokens, batch, heads, kv_heads, dim, 0);
+  const int64_t need = varlen_workspace(tokens, batch, heads, kv_heads, dim, false);
   if (workspace_bytes < need || (need > 0 && !workspace))
     return set_error(BSK_ERR_INVALID_ARG, "%s: workspace of %lld bytes needed", what, (long long)need);
   if (!Q || !K || !V || !O || !cu_seqlens) return set_error(BSK_ERR_INVALID_ARG, "%s: null pointer", what);
@@ -2448,6 +2344,9 @@ int bsk_attention_varlen_fwd(int dtype, const void* Q, int64_t q_token_stride, i
       !rows_aligned(V, v_token_stride, v_head_stride, 2) || !aligned16(O) || !aligned16(workspace))
     return set_error(BSK_ERR_INVALID_ARG, "%s: rows of Q, K, V and O must be 16-byte aligned", what);
   if (int rc = device_state(&st)) return rc;
+  win = window_within(win, tokens);
+  if (win.window)
+    if (int rc = window_ready(*st)) return rc;
   const int group = heads / kv_heads, tt = bsk::kVarBlk / group;
   if (!plan_fits(tokens, batch, tt, kv_heads)) return set_error(BSK_ERR_UNSUPPORTED, "%s: too many rows", what);
   const bool f16 = dtype == 1;
@@ -2462,6 +2361,8 @@ int bsk_attention_varlen_fwd(int dtype, const void* Q, int64_t q_token_stride, i
   p.batch = batch;
   p.tt = tt;
   p.causal = causal != 0;
+  p.window = win.window;
+  p.sinks = win.sinks;
   plan_launch(p, workspace, *st, s);
   bsk::VarFwdArgs f{};
   f.O = O;
@@ -2472,27 +2373,31 @@ int bsk_attention_varlen_fwd(int dtype, const void* Q, int64_t q_token_stride, i
   f.kv_heads = kv_heads;
   f.group = group;
   f.causal = causal != 0;
+  f.window = win.window;
+  f.sinks = win.sinks;
   f.scale_log2 = scale * 1.4426950408889634f;
   f.err = st->err_word;
   f.timeout_ns = t_timeout_ns;
   const int64_t most = bsk::plan_slots(tokens, batch, tt) * kv_heads;
   const unsigned grid = (unsigned)(most < st->sm_count ? most : st->sm_count);
-  const cudaError_t e = varattn_fwd_launch<bsk::kPacked>(f16, dim, tq, tk, tv, f, grid, s);
+  const cudaError_t e = win.window ? bsk::window_fwd(bsk::kPacked, f16, dim, tq, tk, tv, f, grid, s)
+                                   : bsk::varattn_fwd_launch<bsk::kPacked, false>(f16, dim, tq, tk, tv, f, grid, s);
   if (e != cudaSuccess) return cuda_fail(e, "attention_varlen_fwd launch");
   return launch_status("attention_varlen_fwd launch");
 }
 
-int bsk_attention_varlen_bwd(int dtype, const void* dO, int64_t do_token_stride, int64_t do_head_stride, const void* Q,
-                             int64_t q_token_stride, int64_t q_head_stride, const void* K, int64_t k_token_stride,
-                             int64_t k_head_stride, const void* V, int64_t v_token_stride, int64_t v_head_stride,
-                             const void* O, const float* lse, const int32_t* cu_seqlens, void* dQ, void* dK, void* dV,
-                             int tokens, int batch, int heads, int kv_heads, int dim, float scale, int causal,
-                             void* workspace, int64_t workspace_bytes, void* stream) {
+int attention_varlen_bwd(int dtype, const void* dO, int64_t do_token_stride, int64_t do_head_stride, const void* Q,
+                         int64_t q_token_stride, int64_t q_head_stride, const void* K, int64_t k_token_stride,
+                         int64_t k_head_stride, const void* V, int64_t v_token_stride, int64_t v_head_stride,
+                         const void* O, const float* lse, const int32_t* cu_seqlens, void* dQ, void* dK, void* dV,
+                         int tokens, int batch, int heads, int kv_heads, int dim, float scale, int causal, Window win,
+                         void* workspace,
+                         int64_t workspace_bytes, void* stream) {
   const char* what = "attention_varlen_bwd";
   if (int rc = heads_checks(what, dtype, tokens, batch, heads, kv_heads, dim, scale)) return rc;
   DeviceState* st;
   if (tokens == 0) return device_state(&st);
-  const int64_t need = bsk_attention_varlen_workspace_bytes(tokens, batch, heads, kv_heads, dim, 1);
+  const int64_t need = varlen_workspace(tokens, batch, heads, kv_heads, dim, true);
   if (workspace_bytes < need || (need > 0 && !workspace))
     return set_error(BSK_ERR_INVALID_ARG, "%s: workspace of %lld bytes needed", what, (long long)need);
   if (!dO || !Q || !K || !V || !O || !lse || !cu_seqlens || !dQ || !dK || !dV)
@@ -2502,6 +2407,9 @@ int bsk_attention_varlen_bwd(int dtype, const void* dO, int64_t do_token_stride,
       !aligned16(O) || !aligned16(dQ) || !aligned16(dK) || !aligned16(dV) || !aligned16(workspace))
     return set_error(BSK_ERR_INVALID_ARG, "%s: rows of the tensors must be 16-byte aligned", what);
   if (int rc = device_state(&st)) return rc;
+  win = window_within(win, tokens);
+  if (win.window)
+    if (int rc = window_ready(*st)) return rc;
   const int group = heads / kv_heads, tt = bsk::kVarBlk / group;
   const int64_t slots = bsk::plan_slots(tokens, batch, tt), key_slots = bsk::plan_slots(tokens, batch, bsk::kVarBlk);
   if (!plan_fits(tokens, batch, tt, kv_heads)) return set_error(BSK_ERR_UNSUPPORTED, "%s: too many rows", what);
@@ -2522,6 +2430,8 @@ int bsk_attention_varlen_bwd(int dtype, const void* dO, int64_t do_token_stride,
     a.batch = batch;
     a.tt = tt;
     a.causal = causal != 0;
+    a.window = win.window;
+    a.sinks = win.sinks;
     a.keys = i;
     a.tile_slots = 1;
     a.count = reinterpret_cast<int*>(i ? ws_keys : ws);
@@ -2550,6 +2460,8 @@ int bsk_attention_varlen_bwd(int dtype, const void* dO, int64_t do_token_stride,
   a.kv_heads = kv_heads;
   a.group = group;
   a.causal = causal != 0;
+  a.window = win.window;
+  a.sinks = win.sinks;
   a.scale = scale;
   a.scale_log2 = scale * 1.4426950408889634f;
   a.err = st->err_word;
@@ -2557,16 +2469,98 @@ int bsk_attention_varlen_bwd(int dtype, const void* dO, int64_t do_token_stride,
   // statistics: a block takes a tile slot for every groups-th kv head; few slots are spread over more blocks
   const int64_t spread = 2 * (int64_t)st->sm_count / slots;
   p.head_groups = (int)(spread < 1 ? 1 : spread > kv_heads ? kv_heads : spread);
-  const unsigned prep = (unsigned)(2 + slots * p.head_groups);
-  const unsigned gq = (unsigned)(slots * kv_heads < st->sm_count ? slots * kv_heads : st->sm_count);
-  const unsigned gk = (unsigned)(key_slots * kv_heads < st->sm_count ? key_slots * kv_heads : st->sm_count);
-  cudaError_t e;
-  if (f16) e = dim == 128 ? varattn_bwd_launch<true, 128>(p, a, tq, tk, tv, tdo, prep, gk, gq, s)
-                          : varattn_bwd_launch<true, 64>(p, a, tq, tk, tv, tdo, prep, gk, gq, s);
-  else e = dim == 128 ? varattn_bwd_launch<false, 128>(p, a, tq, tk, tv, tdo, prep, gk, gq, s)
-                      : varattn_bwd_launch<false, 64>(p, a, tq, tk, tv, tdo, prep, gk, gq, s);
+  const bsk::VarBwdGrids g{(unsigned)(2 + slots * p.head_groups),
+                           (unsigned)(key_slots * kv_heads < st->sm_count ? key_slots * kv_heads : st->sm_count),
+                           (unsigned)(slots * kv_heads < st->sm_count ? slots * kv_heads : st->sm_count)};
+  const cudaError_t e = win.window ? bsk::window_bwd(f16, dim, p, a, tq, tk, tv, tdo, g, s)
+                                   : bsk::varattn_bwd_launch<false>(f16, dim, p, a, tq, tk, tv, tdo, g, s);
   if (e != cudaSuccess) return cuda_fail(e, "attention_varlen_bwd launch");
   return launch_status("attention_varlen_bwd launch");
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t bsk_attention_paged_workspace_bytes(int tokens, int batch, int heads, int kv_heads, int dim, int num_pages) {
+  if (int rc = heads_checks("attention_paged_workspace_bytes", 0, tokens, batch, heads, kv_heads, dim, 1.0f)) return rc;
+  if (!paged_in_tiles(tokens, batch, heads / kv_heads, num_pages)) return 0;
+  DeviceState* st;
+  if (int rc = device_state(&st)) return rc;
+  return paged_tile_plan(tokens, batch, heads, kv_heads, dim, st->sm_count).total;
+}
+
+int bsk_attention_paged(int dtype, const void* Q, int64_t q_token_stride, int64_t q_head_stride, const void* k_cache,
+                        const void* v_cache, int cache_e4m3, const float* k_scale, const float* v_scale,
+                        const int32_t* block_table, int64_t table_stride, int table_width, const int32_t* kv_lens,
+                        const int32_t* cu_seqlens, void* O, int tokens, int batch, int heads, int kv_heads, int dim,
+                        int num_pages, int page_size, float scale, void* workspace, int64_t workspace_bytes, void* stream) {
+  return attention_paged(dtype, Q, q_token_stride, q_head_stride, k_cache, v_cache, cache_e4m3, k_scale, v_scale, block_table,
+                         table_stride, table_width, kv_lens, cu_seqlens, O, tokens, batch, heads, kv_heads, dim, num_pages,
+                         page_size, scale, Window{}, workspace, workspace_bytes, stream);
+}
+
+int bsk_attention_paged_window(int dtype, const void* Q, int64_t q_token_stride, int64_t q_head_stride, const void* k_cache,
+                               const void* v_cache, int cache_e4m3, const float* k_scale, const float* v_scale,
+                               const int32_t* block_table, int64_t table_stride, int table_width, const int32_t* kv_lens,
+                               const int32_t* cu_seqlens, void* O, int tokens, int batch, int heads, int kv_heads, int dim,
+                               int num_pages, int page_size, float scale, int window, int sinks, void* workspace,
+                               int64_t workspace_bytes, void* stream) {
+  if (int rc = window_checks("attention_paged", window, sinks)) return rc;
+  return attention_paged(dtype, Q, q_token_stride, q_head_stride, k_cache, v_cache, cache_e4m3, k_scale, v_scale, block_table,
+                         table_stride, table_width, kv_lens, cu_seqlens, O, tokens, batch, heads, kv_heads, dim, num_pages,
+                         page_size, scale, Window{window, sinks}, workspace, workspace_bytes, stream);
+}
+
+int64_t bsk_attention_varlen_workspace_bytes(int tokens, int batch, int heads, int kv_heads, int dim, int backward) {
+  if (int rc = heads_checks("attention_varlen_workspace_bytes", 0, tokens, batch, heads, kv_heads, dim, 1.0f)) return rc;
+  return varlen_workspace(tokens, batch, heads, kv_heads, dim, backward != 0);
+}
+
+int bsk_attention_varlen_fwd(int dtype, const void* Q, int64_t q_token_stride, int64_t q_head_stride, const void* K,
+                             int64_t k_token_stride, int64_t k_head_stride, const void* V, int64_t v_token_stride,
+                             int64_t v_head_stride, const int32_t* cu_seqlens, void* O, float* lse, int tokens, int batch,
+                             int heads, int kv_heads, int dim, float scale, int causal, void* workspace,
+                             int64_t workspace_bytes, void* stream) {
+  return attention_varlen_fwd(dtype, Q, q_token_stride, q_head_stride, K, k_token_stride, k_head_stride, V, v_token_stride,
+                              v_head_stride, cu_seqlens, O, lse, tokens, batch, heads, kv_heads, dim, scale, causal, Window{},
+                              workspace, workspace_bytes, stream);
+}
+
+int bsk_attention_varlen_window_fwd(int dtype, const void* Q, int64_t q_token_stride, int64_t q_head_stride, const void* K,
+                             int64_t k_token_stride, int64_t k_head_stride, const void* V, int64_t v_token_stride,
+                             int64_t v_head_stride, const int32_t* cu_seqlens, void* O, float* lse, int tokens, int batch,
+                             int heads, int kv_heads, int dim, float scale, int window, int sinks, void* workspace,
+                             int64_t workspace_bytes, void* stream) {
+  if (int rc = window_checks("attention_varlen_fwd", window, sinks)) return rc;
+  return attention_varlen_fwd(dtype, Q, q_token_stride, q_head_stride, K, k_token_stride, k_head_stride, V, v_token_stride,
+                              v_head_stride, cu_seqlens, O, lse, tokens, batch, heads, kv_heads, dim, scale, 1,
+                              Window{window, sinks}, workspace, workspace_bytes, stream);
+}
+
+int bsk_attention_varlen_bwd(int dtype, const void* dO, int64_t do_token_stride, int64_t do_head_stride, const void* Q,
+                             int64_t q_token_stride, int64_t q_head_stride, const void* K, int64_t k_token_stride,
+                             int64_t k_head_stride, const void* V, int64_t v_token_stride, int64_t v_head_stride,
+                             const void* O, const float* lse, const int32_t* cu_seqlens, void* dQ, void* dK, void* dV,
+                             int tokens, int batch, int heads, int kv_heads, int dim, float scale, int causal,
+                             void* workspace,
+                             int64_t workspace_bytes, void* stream) {
+  return attention_varlen_bwd(dtype, dO, do_token_stride, do_head_stride, Q, q_token_stride, q_head_stride, K, k_token_stride,
+                              k_head_stride, V, v_token_stride, v_head_stride, O, lse, cu_seqlens, dQ, dK, dV, tokens, batch,
+                              heads, kv_heads, dim, scale, causal, Window{}, workspace, workspace_bytes, stream);
+}
+
+int bsk_attention_varlen_window_bwd(int dtype, const void* dO, int64_t do_token_stride, int64_t do_head_stride, const void* Q,
+                             int64_t q_token_stride, int64_t q_head_stride, const void* K, int64_t k_token_stride,
+                             int64_t k_head_stride, const void* V, int64_t v_token_stride, int64_t v_head_stride,
+                             const void* O, const float* lse, const int32_t* cu_seqlens, void* dQ, void* dK, void* dV,
+                             int tokens, int batch, int heads, int kv_heads, int dim, float scale, int window, int sinks,
+                             void* workspace,
+                             int64_t workspace_bytes, void* stream) {
+  if (int rc = window_checks("attention_varlen_bwd", window, sinks)) return rc;
+  return attention_varlen_bwd(dtype, dO, do_token_stride, do_head_stride, Q, q_token_stride, q_head_stride, K, k_token_stride,
+                              k_head_stride, V, v_token_stride, v_head_stride, O, lse, cu_seqlens, dQ, dK, dV, tokens, batch,
+                              heads, kv_heads, dim, scale, 1, Window{window, sinks}, workspace, workspace_bytes, stream);
 }
 
 }  // extern "C"

@@ -58,6 +58,7 @@ struct PagedArgs {
   int tokens, batch, heads, kv_heads, group;  // group = heads / kv_heads
   int table_width, page_shift, num_pages;
   float scale_log2;           // softmax scale * log2(e)
+  int window, sinks;          // kWin: a row at position p sees keys (p - window, p] and [0, sinks)
   uint32_t* err;
 };
 
@@ -168,7 +169,7 @@ struct PagedShape {
   }
 };
 
-template <bool kF16, int kD, bool kFp8, int kNQ>
+template <bool kF16, int kD, bool kFp8, int kNQ, bool kWin = false>
 __global__ void __launch_bounds__(32 * PagedShape<kD, kFp8, kNQ>::kMaxWarps) paged_decode_kernel(const PagedArgs a) {
   using Sh = PagedShape<kD, kFp8, kNQ>;
   constexpr int kRows = Sh::kRows, kKeys = Sh::kKeys, kChunks = Sh::kChunks, kRowBytes = Sh::kRowBytes;
@@ -242,8 +243,16 @@ __global__ void __launch_bounds__(32 * PagedShape<kD, kFp8, kNQ>::kMaxWarps) pag
   const int keys_end = max(first_pos + last_row / a.group + 1, 0);                 // keys that the tile's last row sees
   const int clear = first_pos + static_cast<int>(row0 / a.group) + 1;              // keys that every row sees
 
+  // A window leaves out the keys between the sinks and `reach`, the first one that the tile's first row sees; all rows see the
+  // keys from `reach_all` on. Only pieces with keys that some row sees are walked: piece i of the list is the cache's piece i,
+  // or i + skip behind the sinks' pieces.
+  const int reach = kWin ? max(max(clear - 1, 0) - a.window + 1, 0) : 0;
+  const int reach_all = kWin ? keys_end - a.window : 0;
+  const int sink_pieces = kWin ? a.sinks / kKeys + (a.sinks % kKeys != 0) : 0;
+  const int skip = kWin ? max(reach / kKeys - sink_pieces, 0) : 0;
+
   // ---- keys in pieces of kKeys: a run of them for each CTA of the cluster, dealt out to its warps
-  const int pieces = (keys_end + kKeys - 1) / kKeys, per = (pieces + nrank - 1) / nrank;
+  const int pieces = (keys_end + kKeys - 1) / kKeys - skip, per = (pieces + nrank - 1) / nrank;
   const int first_piece = min(static_cast<int>(rank) * per, pieces) + warp;
   const int end_piece = min(static_cast<int>(rank + 1) * per, pieces);
   const int n_stages = first_piece < end_piece ? (end_piece - first_piece + n_warps - 1) / n_warps : 0;
@@ -251,7 +260,10 @@ __global__ void __launch_bounds__(32 * PagedShape<kD, kFp8, kNQ>::kMaxWarps) pag
   // ---- copies: stage s of this warp = keys [key0(s), key0(s) + kKeys)
   const uint32_t wbase = ptx::smem_u32(smem) + warp * Sh::kWarpBytes;
   const int* table = a.block_table + seq * a.table_stride;
-  auto key0 = [&](int s) { return (first_piece + s * n_warps) * kKeys; };
+  auto key0 = [&](int s) {
+    const int i = first_piece + s * n_warps;
+    return (kWin && i >= sink_pieces ? i + skip : i) * kKeys;
+  };
   constexpr int kSl = (kKeys + 31) / 32;
   int slot_of[kSl];  // lane l: slots of keys l (and l + 32) of the stage to be copied next, -1: none
   auto look_up = [&](int s) {
@@ -259,7 +271,7 @@ __global__ void __launch_bounds__(32 * PagedShape<kD, kFp8, kNQ>::kMaxWarps) pag
     for (int x = 0; x < kSl; ++x) {
       const int key = key0(s) + lane + 32 * x;
       slot_of[x] = -1;
-      if (s < n_stages && lane + 32 * x < kKeys && key < keys_end) {
+      if (s < n_stages && lane + 32 * x < kKeys && key < keys_end && (!kWin || key >= reach || key < a.sinks)) {
         const int page = __ldg(&table[key >> a.page_shift]);
         if (page < 0 || page >= a.num_pages)
           paged_flag(a.err, 3);
@@ -365,6 +377,7 @@ __global__ void __launch_bounds__(32 * PagedShape<kD, kFp8, kNQ>::kMaxWarps) pag
     for (int y = 0; y < 2; ++y) {
       const int64_t row = row0 + 8 * q + 2 * t4 + y;
       limit[q][y] = row < rows ? first_pos + static_cast<int>(row / a.group) + 1 : 0;
+      if (kWin) limit[q][y] = max(limit[q][y], 0);
       row_scale[q][y] = a.scale_log2;
       if constexpr (kFp8 && !kF16) row_scale[q][y] *= __shfl_sync(0xffffffffu, row_up[q], 4 * (2 * t4 + y));
     }
@@ -462,7 +475,7 @@ __global__ void __launch_bounds__(32 * PagedShape<kD, kFp8, kNQ>::kMaxWarps) pag
     // ---- scores in log2 units, mask, running maxima
     float lv[kFp8 ? kBlk : 1][2];  // log2 of the values' scales of this thread's keys
     const int kbase = key0(s);
-    const bool edge = kbase + kKeys > clear;  // some row does not see the whole stage
+    const bool edge = kbase + kKeys > clear || (kWin && kbase < reach_all && kbase + kKeys > a.sinks);  // some row does not see the whole stage
 #pragma unroll
     for (int j = 0; j < kBlk; ++j) {
       float ks[2] = {1.0f, 1.0f};
@@ -486,7 +499,7 @@ __global__ void __launch_bounds__(32 * PagedShape<kD, kFp8, kNQ>::kMaxWarps) pag
           const int key = kbase + 16 * j + r8 + 8 * (x >> 1);
 #pragma unroll
           for (int q = 0; q < kNQ; ++q)
-            if (key >= limit[q][x & 1]) sc[j][q][x] = -INFINITY;
+            if (key >= limit[q][x & 1] || (kWin && key < limit[q][x & 1] - a.window && key >= a.sinks)) sc[j][q][x] = -INFINITY;
           if constexpr (kFp8)  // a key that no row sees: its scale is not looked at
             if (key >= keys_end) lv[j][x >> 1] = -INFINITY;
         }

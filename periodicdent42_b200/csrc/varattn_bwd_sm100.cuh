@@ -40,6 +40,7 @@ struct VarBwdArgs {
   int heads, kv_heads, group, causal;
   float scale;           // softmax scale
   float scale_log2;      // scale * log2(e)
+  int window, sinks;     // kWin: a row at position p sees keys (p - window, p] and [0, sinks)
   uint32_t* err;
   uint64_t timeout_ns;
 };
@@ -157,7 +158,7 @@ __global__ void __launch_bounds__(kPlanThreads) varattn_bwd_prep_kernel(const __
 // accumulator [256, 256 + D), dS (packed pairs) [384, 448). Warpgroup x takes keys [64x, 64x + 64) of a block. Order per block
 // j: S(j), dP(j); once S(j) sits in registers the next block's S is issued; once dS(j) is in TMEM, dQ += dS(j) K_j and the next
 // block's dP.
-template <bool kF16, int kD>
+template <bool kF16, int kD, bool kWin = false>
 __global__ void __launch_bounds__(kBwdThreads, 1)
     varattn_bwd_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                          const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmdO,
@@ -234,6 +235,11 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   auto item_at = [&](int k, VarItem& it, int& hkv) -> bool {
     return var_item(a.q_items, n_items, a.kv_heads, zigzag(k, cta, grid, n_items), it, hkv);
   };
+  // Key block of entry b of the item's list (see win_skip).
+  const int sink_blocks = kWin ? win_sink_blocks(a.sinks) : 0;
+  auto block_of = [&](const VarItem& it, int b) -> int {
+    return kWin && b >= sink_blocks ? b + win_skip(it.pos0, a.window, a.sinks) : b;
+  };
 
   if (warp == 0) {
     // ------------------------------------------------------------------ TMA producer (one thread)
@@ -267,8 +273,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         }
         ++qd_issued;
         qd_phase ^= 1;
-        for (int b = it.b0; b < it.b1 && ok; ++b) {
-          const int row = it.src + b * kVarBlk;
+        for (int x = it.b0; x < it.b1 && ok; ++x) {
+          const int b = block_of(it, x), row = it.src + b * kVarBlk;
           const bool foreign = it.kv_len - b * kVarBlk < kVarBlk;
           ok = push(&tmK, hkv, row, foreign) && push(&tmV, hkv, row, foreign);
         }
@@ -373,7 +379,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     for (int k = 0; ok && item_at(k, it, hkv); ++k) {
       const int n = it.b1 - it.b0;
       if (n <= 0) continue;
-      const int live = it.kv_len - (it.b1 - 1) * kVarBlk;
+      const int live = it.kv_len - block_of(it, it.b1 - 1) * kVarBlk;
       if (live < kVarBlk)
         for (int w = 0; w < 2 && ok; ++w) {  // the item's last K tile and its last V tile
           const uint32_t sl = (seq + 2 * n - 2 + w) % kSlots;
@@ -411,7 +417,10 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       const uint64_t off2 = f2_pack(off, off), ndlt2 = f2_pack(ndlt, ndlt);
       const int limit = a.causal ? it.pos0 + tok + 1 : it.kv_len;        // keys at or behind it are masked for this row
       const int clear = (a.causal ? it.pos0 + 1 : it.kv_len) >> 7;       // key blocks below it are seen by every row
-      for (int kb = it.b0; kb < it.b1; ++kb) {
+      // a window also masks keys before `lo` (the sinks apart); key blocks that start before `lo_all` have such keys for some row
+      const int lo = it.pos0 + tok - a.window + 1, lo_all = it.pos0 + tt - a.window;
+      for (int j = it.b0; j < it.b1; ++j) {
+        const int kb = block_of(it, j);
         ok = warp_wait_bounded_hint<kBwdSuspendNs>(ptx::smem_u32(s_full), s_cnt & 1, ctl, 20);
         if (!ok) break;
         ++s_cnt;
@@ -425,6 +434,14 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         __syncwarp();
         if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(s_free));  // the next block's S may overwrite it
         const int lim = kb >= clear ? limit - (kb * kVarBlk + 64 * x) : 64;
+        uint32_t seen[2] = {~0u, ~0u};
+        if constexpr (kWin) {
+          if (kb >= clear || (kb * kVarBlk < lo_all && (kb + 1) * kVarBlk > a.sinks)) {
+            const int base = kb * kVarBlk + 64 * x;
+            seen[0] = seen_bits(base, limit, lo, a.sinks);
+            seen[1] = seen_bits(base + 32, limit, lo, a.sinks);
+          }
+        }
 #pragma unroll
         for (int i = 0; i < 64; i += 2) {
           float p0, p1;
@@ -450,8 +467,9 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
             f2_unpack(f2_mul(f2_pack(__uint_as_float(pv[32 * cc + i]), __uint_as_float(pv[32 * cc + i + 1])),
                              f2_add(f2_pack(__uint_as_float(dv[i]), __uint_as_float(dv[i + 1])), ndlt2)),
                       g0, g1);
-            if (32 * cc + i >= lim) g0 = 0.0f;  // (the product, not P: dP of a masked key may be infinite)
-            if (32 * cc + i + 1 >= lim) g1 = 0.0f;
+            // (the product, not P: dP of a masked key may be infinite)
+            if (kWin ? !(seen[cc] >> i & 1) : 32 * cc + i >= lim) g0 = 0.0f;
+            if (kWin ? !(seen[cc] >> (i + 1) & 1) : 32 * cc + i + 1 >= lim) g1 = 0.0f;
             pk[i >> 1] = pack2<kF16>(g0, g1);
           }
           ptx::tmem_st_32x32b_x16(tmem_base + lane_off + T_DS + 32 * x + 16 * cc, pk);
@@ -484,7 +502,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
 // P^T of warpgroup x's query rows [64x, 64x + 64) at [64x, 64x + 32); dP^T [128,256) -> packed dS^T likewise at [128 + 64x, ...);
 // dV accumulator [256, 256 + D), dK [256 + D, 256 + 2D). Order per tile t: S^T(t), dP^T(t); P^T written -> dV(t), S^T(t+1); dS^T
 // written -> dK(t), dP^T(t+1).
-template <bool kF16, int kD>
+template <bool kF16, int kD, bool kWin = false>
 __global__ void __launch_bounds__(kBwdThreads, 1)
     varattn_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                            const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmdO,
@@ -762,7 +780,17 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         const float* off_s = reinterpret_cast<const float*>(sQD + slot * kSlotBytes + 2 * kTile) + 64 * x;
         const float* dlt_s = off_s + 128;
         const uint32_t ts = tmem_base + lane_off + T_S + 64 * x, tp = tmem_base + lane_off + T_DP + 64 * x;
-        const bool diag = a.causal && t * tt < it.pos0 + kVarBlk - 1;
+        bool diag = a.causal && t * tt < it.pos0 + kVarBlk - 1;
+        // With a window, so are the columns from `far` on: tokens that are `window` or more behind this key (a sink has none).
+        int far = 64;
+        if constexpr (kWin) {
+          const int key = it.pos0 + r;
+          if (t * tt + tt > it.pos0 + a.window && it.pos0 + kVarBlk > a.sinks) {
+            diag = true;
+            if (key >= a.sinks)
+              far = static_cast<int>(min(max(static_cast<int64_t>(key) + a.window - t * tt, int64_t{0}), int64_t{kVarBlk})) * group - 64 * x;
+          }
+        }
         float pf[64];  // P^T (fp32) of this warp's 64 query positions, kept for dS^T
         // Two chunks of 32 positions; chunk cc's packed values (16 columns) land at ts + 16cc, inside the columns
         // [0, 32) this warp has already read, never over chunk 1's unread scores.
@@ -786,10 +814,10 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
                       p2, p3);
             if (diag) {
               const int col = 32 * cc + i;
-              if (col < lim) p0 = 0.0f;
-              if (col + 1 < lim) p1 = 0.0f;
-              if (col + 2 < lim) p2 = 0.0f;
-              if (col + 3 < lim) p3 = 0.0f;
+              if (col < lim || (kWin && col >= far)) p0 = 0.0f;
+              if (col + 1 < lim || (kWin && col + 1 >= far)) p1 = 0.0f;
+              if (col + 2 < lim || (kWin && col + 2 >= far)) p2 = 0.0f;
+              if (col + 3 < lim || (kWin && col + 3 >= far)) p3 = 0.0f;
             }
             pf[32 * cc + i] = p0;
             pf[32 * cc + i + 1] = p1;
@@ -834,7 +862,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
               const int col = 32 * cc + 2 * i;
-              pk[i] &= (col < lim ? 0u : 0x0000ffffu) | (col + 1 < lim ? 0u : 0xffff0000u);
+              pk[i] &= (col < lim || (kWin && col >= far) ? 0u : 0x0000ffffu) |
+                       (col + 1 < lim || (kWin && col + 1 >= far) ? 0u : 0xffff0000u);
             }
           }
           ptx::tmem_st_32x32b_x16(tp + 16 * cc, pk);

@@ -49,6 +49,7 @@ struct PlanArgs {
   int tile_slots;      // 1: entries carry their slot in `part` (nothing is split)
   int split_ctas;      // > 0: entries may be split along their keys to give this many CTAs work (kv_heads items an entry)
   int kv_heads;
+  int window, sinks;   // window > 0 (causal): a row at position p sees keys (p - window, p] and [0, sinks)
   VarItem* items;
   VarSplit* splits;
   int* count;          // [0] entries, [1] split entries
@@ -62,6 +63,14 @@ constexpr int kPlanMinPiece = 4;  // key blocks: shorter pieces cost more in par
 
 // Slots that a launch reserves for `tokens` rows of `batch` sequences in tiles of tt.
 __host__ __device__ inline int64_t plan_slots(int64_t tokens, int64_t batch, int64_t tt) { return tokens / tt + batch + 1; }
+
+// With a window, a query tile's list of key blocks has a gap: first the blocks of the sinks, [0, win_sink_blocks), then those
+// from the first row's window on. An entry's [b0, b1) counts the blocks of that list; entry j stands for key block j, or j +
+// win_skip behind the sinks' blocks. (Without a gap win_skip is 0.)
+__host__ __device__ __forceinline__ int win_sink_blocks(int sinks) { return sinks / kVarBlk + (sinks % kVarBlk != 0); }
+__device__ __forceinline__ int win_skip(int pos0, int window, int sinks) {
+  return max((max(max(pos0, 0) - window + 1, 0) / kVarBlk) - win_sink_blocks(sinks), 0);
+}
 
 // Entry of `slot`, or false where the slot is empty.
 __device__ __forceinline__ bool plan_item(const PlanArgs& a, int slot, VarItem& it) {
@@ -88,6 +97,8 @@ __device__ __forceinline__ bool plan_item(const PlanArgs& a, int slot, VarItem& 
   if (a.keys) {
     const int tiles = (n + a.tt - 1) / a.tt;
     it = {r0, n, r0 / a.tt + lo, n, t0, a.causal ? t0 / a.tt : 0, tiles, slot};
+    if (a.window > 0 && t0 >= a.sinks)  // the last token whose window reaches the block's last key
+      it.b1 = static_cast<int>(min(static_cast<int64_t>(tiles), (static_cast<int64_t>(t0) + kVarBlk - 2 + a.window) / a.tt + 1));
     return true;
   }
   int kv = n;
@@ -101,6 +112,7 @@ __device__ __forceinline__ bool plan_item(const PlanArgs& a, int slot, VarItem& 
   const int ntok = min(a.tt, n - t0), pos0 = kv - n + t0;
   const int end = a.causal ? max(pos0 + ntok, 0) : kv;
   it = {r0 + t0, ntok, a.kv_lens ? lo : r0, kv, pos0, 0, (end + kVarBlk - 1) / kVarBlk, slot};
+  if (a.window > 0) it.b1 -= win_skip(pos0, a.window, a.sinks);
   return true;
 }
 
@@ -204,7 +216,7 @@ __device__ __forceinline__ void build_plan(const PlanArgs& a) {
   }
 }
 
-__global__ void __launch_bounds__(kPlanThreads) varattn_plan_kernel(const PlanArgs a) {
+static __global__ void __launch_bounds__(kPlanThreads) varattn_plan_kernel(const PlanArgs a) {
   ptx::grid_launch_dependents();
   build_plan(a);
 }

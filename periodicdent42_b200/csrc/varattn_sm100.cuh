@@ -108,11 +108,37 @@ struct VarFwdArgs {
   const float* v_scale;
   int heads, kv_heads, group, causal;
   float scale_log2;
+  int window, sinks;    // kWin: a row at position p sees keys (p - window, p] and [0, sinks)
   uint32_t* err;
   uint64_t timeout_ns;
 };
 
-template <bool kF16, int kD, int kKind>
+// Bits [0, n) of a word.
+__device__ __forceinline__ uint32_t bits_below(int n) { return n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1u; }
+
+// Which of the 32 keys from `base` on a row sees that sees [0, limit) of [lo, ..) and [0, sinks).
+__device__ __forceinline__ uint32_t seen_bits(int base, int limit, int lo, int sinks) {
+  return bits_below(limit - base) & (~bits_below(lo - base) | bits_below(sinks - base));
+}
+
+// Largest value scale's exponent of keys [first, end) of a block (e4m3 caches with a window). top[i]: that of key i's segment of
+// 32 up to key i, from key i on, and of key i alone, a byte each; segs: the four segments' own, a byte each.
+__device__ __forceinline__ int range_top(const int* top, uint32_t segs, int first, int end) {
+  if (first >= end) return 0;
+  const int s0 = first >> 5, s1 = (end - 1) >> 5;
+  if (s0 == s1) {
+    if ((first & 31) == 0) return top[end - 1] & 255;
+    if ((end & 31) == 0) return (top[first] >> 8) & 255;
+    int m = 0;
+    for (int i = first; i < end; ++i) m = max(m, top[i] >> 16);
+    return m;
+  }
+  int m = max((top[first] >> 8) & 255, top[end - 1] & 255);
+  for (int s = s0 + 1; s < s1; ++s) m = max(m, static_cast<int>((segs >> (8 * s)) & 255));
+  return m;
+}
+
+template <bool kF16, int kD, int kKind, bool kWin = false>
 __global__ void __launch_bounds__(kAttnThreads, 1)
     varattn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                        const __grid_constant__ CUtensorMap tmV, const VarFwdArgs a) {
@@ -232,8 +258,16 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     it = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
     return true;
   };
+  // Key block of entry b of the item's list (see win_skip), and whether some row of the tile sees some key of [key, key + n).
+  const int sink_blocks = kWin ? win_sink_blocks(a.sinks) : 0;
+  auto block_of = [&](const VarItem& it, int b) -> int {
+    return kWin && b >= sink_blocks ? b + win_skip(it.pos0, a.window, a.sinks) : b;
+  };
+  auto in_reach = [&](const VarItem& it, int key, int n) -> bool {
+    return !kWin || key < a.sinks || key + n > max(it.pos0, 0) - a.window + 1;
+  };
   // Keys of the sequence in the item's last block: below 128 its V tile holds foreign rows.
-  auto tail_rows = [](const VarItem& it) { return it.kv_len - (it.b1 - 1) * kVarBlk; };
+  auto tail_rows = [&](const VarItem& it) { return it.kv_len - block_of(it, it.b1 - 1) * kVarBlk; };
   // e4m3: the first block that may be the last one that some row sees keys of: that of the first token's own key, or the item's
   // last. The blocks before it are seen whole by every row that sees any key.
   auto first_edge = [](const VarItem& it) { return min(it.pos0 >> 7, it.b1 - 1); };
@@ -265,11 +299,13 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       // cache (a bad page) read as zeros, boxes wholly behind the sequence's end are not copied.
       auto entry = [&](const VarItem& it, int b) -> int {
         const int key = b * kVarBlk + lane * box_rows;
-        return lane < pages_per_blk && key < it.kv_len ? __ldg(a.table + it.src * a.table_stride + (key >> a.page_shift)) : 0;
+        return lane < pages_per_blk && key < it.kv_len && in_reach(it, key, box_rows)
+                   ? __ldg(a.table + it.src * a.table_stride + (key >> a.page_shift)) : 0;
       };
       auto row_of = [&](const VarItem& it, int b, int page) -> int {
         const int key = b * kVarBlk + lane * box_rows;
         if (lane >= pages_per_blk || key >= it.kv_len) return -1;
+        if (!in_reach(it, key, box_rows)) return a.num_pages << a.page_shift;  // a page that may have been given back: zeros
         if (page < 0 || page >= a.num_pages) {
           atomicCAS(a.err, 0u, kErrBounds | (kKidVarAttn << 8) | (3u << 16));
           return a.num_pages << a.page_shift;
@@ -278,7 +314,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       };
       auto push = [&](const CUtensorMap* m, const VarItem& it, int hkv, int b, bool is_v, int row) -> bool {
         if (!wait(&ring_empty[slot], slot_phase ^ 1, 2)) return false;
-        const bool foreign = !kE4m3 && is_v && b == it.b1 - 1 && tail_rows(it) < kVarBlk;
+        const bool foreign = !kE4m3 && is_v && it.kv_len - b * kVarBlk < kVarBlk;
         const uint32_t fb = ptx::smem_u32(foreign ? &raw_full[slot] : &ring_full[slot]);
         uint32_t dst = kv0 + slot * (kE4m3 ? Sh::kStageBytes : kTile);
         if (kPaged) dst += lane * (kE4m3 ? box_rows * kD : (box_rows >> 3) * kGroupPitch);
@@ -305,7 +341,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       for (int k = 0; ok && item_at(k, it, hkv); ++k) {
         if (it.b1 <= it.b0) continue;
         int ahead = 0;
-        if constexpr (kPaged) ahead = entry(it, it.b0);
+        if constexpr (kPaged) ahead = entry(it, block_of(it, it.b0));
         const uint32_t qbuf = q_issued & 1;
         ok = wait(&q_empty[qbuf], ((q_issued >> 1) & 1) ^ 1, 1);
         if (!ok) break;
@@ -317,19 +353,21 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
             ptx::tma_load_3d(ptx::smem_u32(sQ) + qbuf * kTile + c * kAttnChunk, &tmQ, qf, 64 * c, hkv * group, it.row0);
         }
         ++q_issued;
-        int row = 0, prev = 0;
-        for (int b = it.b0; b < it.b1 && ok; ++b) {
+        int row = 0, prev = 0, before = 0;
+        for (int x = it.b0; x < it.b1 && ok; ++x) {
+          const int b = block_of(it, x);
           if constexpr (kPaged) {
             row = row_of(it, b, ahead);
-            if (b + 1 < it.b1) ahead = entry(it, b + 1);
+            if (x + 1 < it.b1) ahead = entry(it, block_of(it, x + 1));
           } else {
             row = it.src + b * kVarBlk;
           }
           ok = push(&tmK, it, hkv, b, false, row);
-          if (ok && b > it.b0) ok = push(&tmV, it, hkv, b - 1, true, prev);
+          if (ok && x > it.b0) ok = push(&tmV, it, hkv, before, true, prev);
           prev = row;
+          before = b;
         }
-        if (ok) ok = push(&tmV, it, hkv, it.b1 - 1, true, prev);
+        if (ok) ok = push(&tmV, it, hkv, before, true, prev);
       }
     }
     if (lane == 0) {  // drain loads still in flight
@@ -435,14 +473,15 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         auto look_pages = [&](int b) {
 #pragma unroll
           for (int x = 0; x < 4; ++x) {
-            const int key = b * kVarBlk + 32 * x + lane;
-            page[x] = b < it.b1 && key < it.kv_len ? __ldg(a.table + it.src * a.table_stride + (key >> a.page_shift)) : -1;
+            const int key = block_of(it, b) * kVarBlk + 32 * x + lane;
+            page[x] = b < it.b1 && key < it.kv_len && in_reach(it, key, 1)
+                          ? __ldg(a.table + it.src * a.table_stride + (key >> a.page_shift)) : -1;
           }
         };
         auto look_scales = [&](int b) {
 #pragma unroll
           for (int x = 0; x < 4; ++x) {
-            const int key = b * kVarBlk + 32 * x + lane;
+            const int key = block_of(it, b) * kVarBlk + 32 * x + lane;
             const bool held = page[x] >= 0 && page[x] < a.num_pages;
             const int64_t at =
                 static_cast<int64_t>(held ? (page[x] << a.page_shift) + (key & ((1 << a.page_shift) - 1)) : 0) * a.kv_heads + hkv;
@@ -468,7 +507,20 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
             int most[4];
 #pragma unroll
             for (int x = 0; x < 4; ++x) most[x] = __reduce_max_sync(0xffffffffu, top[x]);
-            if (b >= first_edge(it)) {  // some row may not see all of the block: the largest up to each key
+            if constexpr (kWin) {  // up to each key and from it on, within its segment of 32
+              int up[4], down[4];
+#pragma unroll
+              for (int x = 0; x < 4; ++x) up[x] = down[x] = top[x];
+#pragma unroll 1
+              for (int o = 1; o < 32; o <<= 1)
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                  up[x] = max(up[x], __shfl_up_sync(0xffffffffu, up[x], o));
+                  down[x] = max(down[x], __shfl_down_sync(0xffffffffu, down[x], o));
+                }
+#pragma unroll
+              for (int x = 0; x < 4; ++x) v_top[128 * buf + 32 * x + lane] = up[x] | down[x] << 8 | top[x] << 16;
+            } else if (b >= first_edge(it)) {  // some row may not see all of the block: the largest up to each key
 #pragma unroll 1
               for (int o = 1; o < 32; o <<= 1)
 #pragma unroll
@@ -489,7 +541,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
             }
             if (lane == 0) {
               r_tile[buf] = r_exp;
-              r_before[buf] = before;
+              r_before[buf] = kWin ? most[0] | most[1] << 8 | most[2] << 16 | most[3] << 24 : before;
               r_step[buf] = __int_as_float(max(127 + before - r_exp, 0) << 23);
             }
             __syncwarp();
@@ -572,10 +624,14 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       // keys at or behind `limit` are masked for this row; `clear`: key blocks below it are seen by every row of the tile
       const int limit = a.causal ? it.pos0 + tok + 1 : it.kv_len;
       const int clear = (a.causal ? it.pos0 + 1 : it.kv_len) >> 7;
+      // a window also masks keys before `lo` (the sinks apart); key blocks that start before `lo_all` have such keys for some row
+      const int lo = max(it.pos0 + tok, 0) - a.window + 1, lo_all = max(it.pos0 + tt, 0) - a.window;
       float m_run = -INFINITY, l_run = 0.0f;
+      int own = kScaleLow, ref = kScaleLow;  // e4m3 with a window: largest value scale that the row has seen, and its reference
       const uint32_t tO = tO0 + 128 * (rows & 1);
       for (int j = 0; j < n; ++j, ++g) {
-        const int kb = it.b0 + j;
+        const int kb = block_of(it, it.b0 + j);
+        const bool cut = kWin && (kb >= clear || (kb * kVarBlk < lo_all && (kb + 1) * kVarBlk > a.sinks));
         const uint32_t b = g & 1;
         const uint32_t tS = tmem_base + 128 * b + lane_off;
         if constexpr (kE4m3) {
@@ -604,7 +660,15 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
             f2_unpack(f2_mul(f2_pack(v[4 * i + 2], v[4 * i + 3]), f2_pack(x.z, x.w)), v[4 * i + 2], v[4 * i + 3]);
           }
         }
-        if (kb >= clear) {
+        if constexpr (kWin) {
+          if (cut) {
+            const int base = kb * kVarBlk + 64 * h;
+            const uint32_t seen[2] = {seen_bits(base, limit, lo, a.sinks), seen_bits(base + 32, limit, lo, a.sinks)};
+#pragma unroll
+            for (int i = 0; i < 64; ++i)
+              if (!(seen[i >> 5] >> (i & 31) & 1)) v[i] = -INFINITY;
+          }
+        } else if (kb >= clear) {
           const int lim = limit - (kb * kVarBlk + 64 * h);
 #pragma unroll
           for (int i = 0; i < 64; ++i)
@@ -630,12 +694,27 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         float step = 1.0f, lift = 0.0f;  // O follows the scale reference
         // The row's scale reference where it is not the tile's: a row that sees part of the block has seen all before it. How far
         // (log2) the tile's lies above the row's, and, with the row's last key in the block, the row's closing factor.
-        const bool edge = kE4m3 && kb >= first_edge(it);
+        const bool edge = kE4m3 && !kWin && kb >= first_edge(it);
         auto reference = [&]() -> int {
           const int seen = limit - kb * kVarBlk;
           return seen > 0 ? max(v_top[128 * b + min(seen, kVarBlk) - 1], r_tile[b] - kScaleSpan) : r_tile[b];
         };
-        if constexpr (kE4m3) {
+        if constexpr (kE4m3 && kWin) {
+          // Rows leave their first keys out one by one, so each row keeps the largest scale of its own keys throughout.
+          const uint32_t segs = r_before[b];
+          if (cut) {
+            const int base = kb * kVarBlk, end = min(limit - base, kVarBlk);
+            own = max(own, max(range_top(v_top + 128 * b, segs, max(lo - base, 0), end),
+                               range_top(v_top + 128 * b, segs, 0, min(a.sinks - base, end))));
+          } else {
+            const uint32_t two = __vmaxu2(segs & 0x00ff00ffu, (segs >> 8) & 0x00ff00ffu);
+            own = max(own, static_cast<int>(max(two & 0xffffu, two >> 16)));
+          }
+          const int now = max(own, r_tile[b] - kScaleSpan);
+          step = __int_as_float(max(127 + ref - now, 0) << 23);
+          lift = static_cast<float>(r_tile[b] - now);
+          ref = now;
+        } else if constexpr (kE4m3) {
           step = r_step[b];
           if (edge) {
             const int own = reference(), tile = r_tile[b];
@@ -675,7 +754,9 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
           f2_unpack(f2_add(a01, a23), lo, hi);
           rs = lo + hi;
         }
-        if constexpr (kE4m3)
+        if constexpr (kE4m3 && kWin)
+          rs *= __int_as_float((127 - (r_tile[b] - ref)) << 23);
+        else if constexpr (kE4m3)
           if (edge) rs *= __int_as_float((127 - (r_tile[b] - reference())) << 23);
         l_run = l_run * alpha + rs;
         if (need_rescale) {
@@ -706,6 +787,8 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       }
       l_part[h * 128 + r] = l_run;
       if (h == 0) m_row[r] = m_run;
+      if constexpr (kE4m3 && kWin)
+        if (h == 0) r_end[128 * (rows & 1) + r] = __int_as_float((ref - 6) << 23);  // 2^(ref - 133)
       __syncwarp();
       if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(l_ready));
       ++rows;
@@ -770,7 +853,8 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
           ok = warp_wait_bounded_hint<kBwdSuspendNs>(ptx::smem_u32(&stg_full[st]), (pos / kStages) & 1, ctl, 32);
           if (ok) ok = warp_wait_bounded_hint<kBwdSuspendNs>(ptx::smem_u32(&kv_empty[sl]), ((pos / kSlots) & 1) ^ 1, ctl, 33);
           if (!ok) break;
-          const uint32_t live = b * kVarBlk + r < it.kv_len ? 0xffffffffu : 0u;
+          const int key = block_of(it, b) * kVarBlk + r;
+          const uint32_t live = key < it.kv_len && in_reach(it, key, 1) ? 0xffffffffu : 0u;
           const uint8_t* src = sRaw + st * Sh::kStageBytes + r * kD;
           uint8_t* dst = sKV + sl * kTile + r * 128;
           const int sx = kD == 128 ? r & 7 : (r >> 1) & 3;

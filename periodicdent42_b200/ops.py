@@ -471,7 +471,8 @@ def kv_cache_gather(k_cache: torch.Tensor, v_cache: torch.Tensor, slots: torch.T
 # ----------------------------------------------------------------------------------------- packed and paged attention
 def attention_paged(Q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
                     kv_lens: torch.Tensor, cu_seqlens: torch.Tensor, scale: Optional[float] = None,
-                    k_scale: Optional[torch.Tensor] = None, v_scale: Optional[torch.Tensor] = None) -> torch.Tensor:
+                    k_scale: Optional[torch.Tensor] = None, v_scale: Optional[torch.Tensor] = None,
+                    window: Optional[int] = None, sinks: int = 0) -> torch.Tensor:
     """Causal attention of each sequence's new tokens (one or many) over its cached tokens; returns O like Q.
 
     Q: [tokens, heads, dim] (fp16 / bf16, dim 64 or 128), the new tokens of all sequences packed: sequence i owns rows
@@ -481,29 +482,45 @@ def attention_paged(Q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     block_table [batch, width]: page numbers, position p in page block_table[i, p // page_size]; caches and scales as in
     :func:`kv_cache_append`, page size a power of two from 8 to 1024. Index tensors are int32 or int64 (narrowed first;
     a value beyond 32 bits is out of range like any other).
+    window: a token at position p sees the last ``window`` positions up to its own, p - window + 1 .. p, and the first ``sinks``
+    ones. Pages wholly outside what a sequence's new tokens see are neither read nor looked up: they may be given back, and
+    their table entries hold anything.
     A row that sees no key is zero, and so are rows behind the last sequence. Stale contents of a page behind its
     sequence's end reach no row, NaN among them; a non-finite value inside a sequence may make rows of it NaN that see it
-    with weight zero or are masked for it, fewer than 256 tokens before it. The softmax's weights are rounded to Q's type for
-    their product with V; over e4m3 caches they are weight times the value's scale, rounded to fp16. For serving: has no
+    with weight zero or are masked for it, fewer than 256 tokens before it (or behind, where a window leaves it out). The softmax's
+    weights are rounded to Q's type for their product with V; over e4m3 caches they are weight times the value's scale, rounded to fp16. For serving: has no
     gradient, and tensors that require one are refused outside torch.no_grad()."""
     if scale is None:
         scale = Q.shape[-1] ** -0.5 if Q.dim() and Q.shape[-1] else 1.0
-    return _C().attention_paged(Q, k_cache, v_cache, block_table, kv_lens, cu_seqlens, scale, k_scale, v_scale)
+    return _C().attention_paged(Q, k_cache, v_cache, block_table, kv_lens, cu_seqlens, scale, k_scale, v_scale,
+                                _window("attention_paged", window), sinks)
+
+
+def _window(op: str, window: Optional[int]) -> int:
+    """The extension's form of a window: 0 for None."""
+    if window is None:
+        return 0
+    if window < 1:
+        raise ValueError(f"{op}: window must be at least 1, got {window}")
+    return window
 
 
 def attention_varlen(Q: torch.Tensor, K: torch.Tensor, V: torch.Tensor, cu_seqlens: torch.Tensor,
-                     scale: Optional[float] = None, causal: bool = True) -> torch.Tensor:
+                     scale: Optional[float] = None, causal: bool = True, window: Optional[int] = None,
+                     sinks: int = 0) -> torch.Tensor:
     """Attention over packed sequences of different lengths (each within itself, causal by default); returns O like Q.
 
     Q [tokens, heads, dim], K and V [tokens, kv_heads, dim] (fp16 / bf16, dim 64 or 128, heads a multiple of kv_heads:
     query head h reads kv head h // (heads / kv_heads)); sequence i owns rows cu_seqlens[i] .. cu_seqlens[i+1]
     (int32 or int64 [batch + 1], starting at 0; any lengths, zero included). Rows behind the last sequence are zero.
+    window (causal only): token t of a sequence sees its last ``window`` tokens up to itself, t - window + 1 .. t, and the
+    first ``sinks`` ones; the work is that of the tokens that are seen.
     Sequences do not reach one another, non-finite values included; inside one, a non-finite row of V may make rows NaN
-    that are masked for it, fewer than 256 tokens before it. Differentiable (once, in reverse mode) in Q, K and V
+    that are masked for it, fewer than 256 tokens before it (or behind, where a window leaves it out). Differentiable (once, in reverse mode) in Q, K and V
     (deterministic, no atomics). The softmax's weights and, for the gradients, dS are rounded to Q's type for their products."""
     if scale is None:
         scale = Q.shape[-1] ** -0.5 if Q.dim() and Q.shape[-1] else 1.0
-    return _C().attention_varlen(Q, K, V, cu_seqlens, scale, causal)
+    return _C().attention_varlen(Q, K, V, cu_seqlens, scale, causal, _window("attention_varlen", window), sinks)
 
 
 def synchronize_and_check() -> None:

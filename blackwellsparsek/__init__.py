@@ -12,8 +12,8 @@ only re-exports, so the two import names always run the same code.
 """
 from periodicdent42_b200 import __version__
 from periodicdent42_b200.ops import (attention_forward, attention_paged, attention_varlen, gemm, gemm_fp8,
-                                     kv_cache_append, kv_cache_gather, quantize_e4m3, rotary_embedding,
-                                     rotary_frequencies, sparse_mm, sparse_mm_benchmark)
+                                     kv_cache_append, kv_cache_gather, kv_cache_plan, qk_norm_rotary, quantize_e4m3,
+                                     rotary_axes, rotary_embedding, rotary_frequencies, sparse_mm, sparse_mm_benchmark)
 from periodicdent42_b200.utils import convert_to_bsr, estimate_speedup, get_optimal_block_size, validate_sparse_matrix
 
 from . import ops, utils  # noqa: E402  (the reference's submodules: bsk.ops, bsk.utils)

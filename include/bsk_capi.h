@@ -365,6 +365,41 @@ int bsk_rotary(int dtype, const void* Q, int64_t q_token_stride, int64_t q_head_
                int interleaved, float scale, int backward, void* stream);
 
 /*
+ * The same with several axes (time, height and width of patches, say): pair i turns by positions[axes[i] * tokens + t] *
+ * inv_freq[i]. positions [num_axes, tokens]; axes int32 [rotary_dim/2], device memory, each in [0, num_axes) (others count as
+ * the nearest and set the device error word).
+ */
+int bsk_rotary_axes(int dtype, const void* Q, int64_t q_token_stride, int64_t q_head_stride, void* Q_out, int heads,
+                    const void* K, int64_t k_token_stride, int64_t k_head_stride, void* K_out, int kv_heads,
+                    const void* positions, int position_bytes, const int32_t* axes, int num_axes, const float* inv_freq,
+                    int tokens, int dim, int rotary_dim, int interleaved, float scale, int backward, void* stream);
+
+/*
+ * RMS norm of each head of Q and K, then the rotation, in one pass: z = x / sqrt(mean(x^2) + eps) * weight over the head's
+ * dim elements, and z turned as by bsk_rotary (axes may be NULL: one axis). Rows, types and outputs as there; q_weight and
+ * k_weight [dim] of the rows' type, or fp32 with weight_f32. The backward takes the results' gradients dQ_out, dK_out
+ * (strides in elements) and the inputs, and writes contiguous dQ, dK and the weights' gradients dq_weight, dk_weight (of the
+ * weights' type; either may be NULL), the sums over rows in a fixed order (no atomics). Everything is fp32 inside, each result
+ * rounded once.
+ *   eps : at least 1e-30; workspace: bsk_qk_norm_rotary_workspace_bytes(...) bytes of device memory, 16-byte aligned, not
+ *   shared by calls that may run at the same time. The size depends on the current device.
+ * No reference counterpart.
+ */
+int bsk_qk_norm_rotary(int dtype, const void* Q, int64_t q_token_stride, int64_t q_head_stride, void* Q_out, int heads,
+                       const void* K, int64_t k_token_stride, int64_t k_head_stride, void* K_out, int kv_heads,
+                       const void* q_weight, const void* k_weight, int weight_f32, const void* positions, int position_bytes,
+                       const int32_t* axes, int num_axes, const float* inv_freq, int tokens, int dim, int rotary_dim,
+                       int interleaved, float scale, float eps, void* stream);
+int64_t bsk_qk_norm_rotary_workspace_bytes(int tokens, int heads, int kv_heads, int dim);
+int bsk_qk_norm_rotary_bwd(int dtype, const void* dQ_out, int64_t dq_token_stride, int64_t dq_head_stride, const void* Q,
+                           int64_t q_token_stride, int64_t q_head_stride, void* dQ, int heads, const void* dK_out,
+                           int64_t dk_token_stride, int64_t dk_head_stride, const void* K, int64_t k_token_stride,
+                           int64_t k_head_stride, void* dK, int kv_heads, const void* q_weight, const void* k_weight,
+                           int weight_f32, void* dq_weight, void* dk_weight, const void* positions, int position_bytes,
+                           const int32_t* axes, int num_axes, const float* inv_freq, int tokens, int dim, int rotary_dim,
+                           int interleaved, float scale, float eps, void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
  * Paged key/value cache: caches [pages, page size, kv_heads, dim] (dim 64 or 128) of the rows' type (dtype 0 = bf16,
  * 1 = f16) or, with cache_e4m3, of e4m3 codes with fp32 scales [pages, page size, kv_heads].
  * append writes row t of K and V [tokens, kv_heads, dim] (16-byte aligned rows, strides in elements) to flat slot
@@ -381,6 +416,24 @@ int bsk_kv_cache_append(int dtype, const void* K, int64_t k_token_stride, int64_
 int bsk_kv_cache_gather(int dtype, const void* k_cache, const void* v_cache, int cache_e4m3, const float* k_scale,
                         const float* v_scale, const void* slots, int slot_bytes, void* K, void* V, int tokens, int kv_heads,
                         int dim, int64_t num_slots, void* stream);
+
+/*
+ * A serving step's bookkeeping for a paged cache, on the device. Request i has kv_lens[i] cached tokens and new_lens[i] new
+ * ones, whose rows follow one another in the order of the requests; its pages are in row i of block_table (at table_stride).
+ * free_pages is a stack of page numbers of which the first *free_count are free: pages are taken from its end, in the order of
+ * the requests and, in one, of the positions. Written: cu_seqlens [batch + 1], kv_lens_out [batch] (kv_lens + new_lens),
+ * positions [tokens] and slots [tokens] of every new token (slot = page * page_size + position % page_size, as
+ * bsk_kv_cache_append takes them), the block table's entries of the pages taken, and free_count_out [1]. Rows behind the last
+ * request's (padding) get slot -1 and position 0. Nothing else is changed: the same call again gives the same again.
+ * Each of these sets the device error word: a negative length (counts as 0); new tokens beyond a row of the table (slot -1) or
+ * beyond `tokens` rows (left out); no page left, or a request's own entry negative (slot -1, and the entry of a page not found
+ * becomes -1); free_count outside [0, num_free] (counts as the nearest). Outputs may not overlap inputs.
+ * No reference counterpart.
+ */
+int bsk_kv_cache_plan(const int32_t* kv_lens, const int32_t* new_lens, int batch, int32_t* block_table, int64_t table_stride,
+                      int table_width, const int32_t* free_pages, int num_free, const int32_t* free_count, int page_size,
+                      int64_t* slots, int32_t* positions, int tokens, int32_t* cu_seqlens, int32_t* kv_lens_out,
+                      int32_t* free_count_out, void* stream);
 
 /*
  * Attention of new tokens over a paged cache, causal, heads grouped over kv heads (dtype 0 = bf16, 1 = f16; dim 64 or

@@ -27,10 +27,11 @@ def tiny(dtype: torch.dtype) -> float:
     return torch.finfo(dtype).tiny * torch.finfo(dtype).eps / 2 if dtype != torch.bfloat16 else 0.0
 
 
-def rotary64(x, positions, inv_freq, interleaved, scale, sign=1.0):
-    """The rotation pair by pair; x [tokens, heads, dim]."""
+def rotary64(x, positions, inv_freq, interleaved, scale, sign=1.0, axes=None):
+    """The rotation pair by pair; x [tokens, heads, dim]. With axes, positions are [axes, tokens] and pair i takes axes[i]."""
     r = 2 * inv_freq.numel()
-    angle = sign * positions.double()[:, None] * inv_freq.double()[None, :]
+    place = positions.double()[:, None] if axes is None else positions[axes.long()].double().t()
+    angle = sign * place * inv_freq.double()[None, :]
     c, s = (angle.cos() * scale)[:, None, :], (angle.sin() * scale)[:, None, :]
     y = x.double().clone()
     ia = torch.arange(0, r, 2) if interleaved else torch.arange(r // 2)
@@ -38,6 +39,66 @@ def rotary64(x, positions, inv_freq, interleaved, scale, sign=1.0):
     a, b = x.double()[..., ia], x.double()[..., ib]
     y[..., ia], y[..., ib] = a * c - b * s, a * s + b * c
     return y
+
+
+def _norm_error(D):
+    """Relative error of 1 / rms: the squares' sum (D roundings of half weight under the root), the mean's and eps' (three), and
+    rsqrt's 2 ulp."""
+    return ((D + 3) / 2 + 4) * U32
+
+
+# the rotation's fp32 error for a pair (a, b): 2^-20 (|a| + |b|) |scale|: sine and cosine (fraction of a turn in fp32, 2 pi 2^-25,
+# two roundings each) and the products'
+TURN = 2.0 ** -20
+
+
+def norm_rotary64(x, weight, positions, inv_freq, interleaved, scale, eps, axes=None, dy=None):
+    """Norm of each head and rotation: dict name -> (value, bound) of y, and with dy of dx and dw. fp32 inside, each result
+    rounded once to its type."""
+    f, w = x.double(), weight.double()
+    D, u = x.shape[-1], half_step(x.dtype)
+    inv = 1.0 / (f.square().mean(-1, keepdim=True) + eps).sqrt()
+    unit = f * inv
+    z = unit * w
+    e = _norm_error(D)
+    y = rotary64(z, positions, inv_freq, interleaved, scale, axes=axes)
+    big = 2 * max(1.0, abs(scale)) * z.abs().amax(-1, keepdim=True)
+    out = {"y": (y, u * y.abs() + (e + 3 * U32 + TURN) * big + tiny(x.dtype))}
+    if dy is None:
+        return out
+    dz = rotary64(dy, positions, inv_freq, interleaved, scale, -1.0, axes)
+    e_dz = TURN * 2 * max(1.0, abs(scale)) * dy.double().abs().amax(-1, keepdim=True)
+    g = dz * w
+    e_g = e_dz * w.abs() + U32 * g.abs()
+    dot = (g * unit).mean(-1, keepdim=True)
+    e_dot = (e_g * unit.abs() + (e + (D + 3) * U32) * (g * unit).abs()).mean(-1, keepdim=True)
+    dx = (g - unit * dot) * inv
+    e_dx = inv * (e_g + unit.abs() * (e_dot + (e + 3 * U32) * dot.abs()) + (e + 3 * U32) * (g - unit * dot).abs())
+    # rows near the types' largest values have gradients below 2^-126: 1 / rms is rounded to a multiple of 2^-149 in fp32 and dx
+    # to one of the type's smallest subnormal, half a step each
+    low = torch.finfo(x.dtype).smallest_normal * torch.finfo(x.dtype).eps / 2 + 2.0 ** -150 * (g - unit * dot).abs()
+    out["dx"] = (dx, u * dx.abs() + e_dx + low)
+    dw = (dz * unit).sum((0, 1))
+    n = x.shape[0] * x.shape[1]
+    e_dw = (e_dz * unit.abs() + (e + (n + 3) * U32) * (dz * unit).abs()).sum((0, 1))
+    out["dw"] = (dw, half_step(weight.dtype) * dw.abs() + e_dw + tiny(weight.dtype))
+    return out
+
+
+def plan_steps(kv_lens, new_lens, table, stack, page, tokens):
+    """A serving step request by request on lists: (slots, positions, cu_seqlens, kv_lens, stack, table) after it."""
+    table, stack = [row[:] for row in table], stack[:]
+    slots, places, cu, after = [], [], [0], []
+    for i, (k, n) in enumerate(zip(kv_lens, new_lens)):
+        for p in range(k, k + n):
+            if p % page == 0:
+                table[i][p // page] = stack.pop()
+            slots.append(table[i][p // page] * page + p % page)
+            places.append(p)
+        cu.append(cu[-1] + n)
+        after.append(k + n)
+    rest = tokens - len(slots)
+    return slots + [-1] * rest, places + [0] * rest, cu, after, stack, table
 
 
 def quantise_rows(x):

@@ -18,8 +18,8 @@ functions and signatures, backed by hand-written tcgen05/TMA kernels behind a C 
 __version__ = "0.9.0+sm100a"
 
 from .ops import (attention_forward, attention_paged, attention_varlen, gemm, gemm_fp8, gemm_from_host, has_cuda_ext,
-                  kv_cache_append, kv_cache_gather, quantize_e4m3, rotary_embedding, rotary_frequencies, sparse_mm,
-                  sparse_mm_benchmark, synchronize_and_check)
+                  kv_cache_append, kv_cache_gather, kv_cache_plan, qk_norm_rotary, quantize_e4m3, rotary_axes, rotary_embedding,
+                  rotary_frequencies, sparse_mm, sparse_mm_benchmark, synchronize_and_check)
 from .utils import convert_to_bsr, get_optimal_block_size, validate_sparse_matrix
 
 __all__ = [
@@ -37,6 +37,9 @@ __all__ = [
     "attention_varlen",
     "kv_cache_append",
     "kv_cache_gather",
+    "kv_cache_plan",
+    "qk_norm_rotary",
+    "rotary_axes",
     "rotary_embedding",
     "rotary_frequencies",
     "has_cuda_ext",

@@ -80,6 +80,15 @@ SIGNATURES = {
                               _i32, _i32, _f32, _i32, _vp, _vp]),
     "bsk_rotary": (_i32, [_i32, _vp, _i64, _i64, _vp, _i32, _vp, _i64, _i64, _vp, _i32, _vp, _i32, _vp, _i32, _i32,
                           _i32, _i32, _f32, _i32, _vp]),
+    "bsk_rotary_axes": (_i32, [_i32, _vp, _i64, _i64, _vp, _i32, _vp, _i64, _i64, _vp, _i32, _vp, _i32, _vp, _i32, _vp, _i32,
+                               _i32, _i32, _i32, _f32, _i32, _vp]),
+    "bsk_qk_norm_rotary": (_i32, [_i32, _vp, _i64, _i64, _vp, _i32, _vp, _i64, _i64, _vp, _i32, _vp, _vp, _i32, _vp, _i32, _vp,
+                                  _i32, _vp, _i32, _i32, _i32, _i32, _f32, _f32, _vp]),
+    "bsk_qk_norm_rotary_workspace_bytes": (_i64, [_i32, _i32, _i32, _i32]),
+    "bsk_qk_norm_rotary_bwd": (_i32, [_i32, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i32, _vp, _i64, _i64, _vp, _i64, _i64, _vp,
+                                      _i32, _vp, _vp, _i32, _vp, _vp, _vp, _i32, _vp, _i32, _vp, _i32, _i32, _i32, _i32, _f32,
+                                      _f32, _vp, _i64, _vp]),
+    "bsk_kv_cache_plan": (_i32, [_vp, _vp, _i32, _vp, _i64, _i32, _vp, _i32, _vp, _i32, _vp, _vp, _i32, _vp, _vp, _vp, _vp]),
     "bsk_kv_cache_append": (_i32, [_i32, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i32, _vp, _vp, _vp, _i32, _i32,
                                    _i32, _i32, _i64, _vp]),
     "bsk_kv_cache_gather": (_i32, [_i32, _vp, _vp, _i32, _vp, _vp, _vp, _i32, _vp, _vp, _i32, _i32, _i32, _i64, _vp]),

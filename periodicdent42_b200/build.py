@@ -27,7 +27,7 @@ CAPI_LIB = os.path.join(PKG_DIR, "libbsk_sm100.so")
 TORCH_EXT = os.path.join(PKG_DIR, "_C.so")
 
 NVCC_ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
-CAPI_SOURCES = [os.path.join(CSRC, f) for f in ("capi.cu", "window.cu")]
+CAPI_SOURCES = [os.path.join(CSRC, f) for f in ("capi.cu", "window.cu", "norm_rotary.cu")]
 CAPI_DEPS = CAPI_SOURCES + sorted(
     os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith((".cuh", ".h"))
 ) + [os.path.join(INCLUDE, "bsk_capi.h")]

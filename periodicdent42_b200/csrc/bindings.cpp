@@ -168,6 +168,8 @@ torch::Tensor bsattn_fwd(torch::Tensor Q, torch::Tensor K, torch::Tensor V, torc
 // ------------------------------------------------------------------ rotary, paged cache, packed and paged attention
 // Argument errors of these operators are ValueErrors (TORCH_CHECK_VALUE), as in the Python layer.
 using OptTensor = std::optional<torch::Tensor>;
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
 
 void check_cuda(const torch::Tensor& t, const torch::Tensor& like, const char* op, const char* name) {
   TORCH_CHECK_VALUE(t.is_cuda(), op, ": CUDA tensors required (CPU not supported), ", name, " is not one");
@@ -231,12 +233,17 @@ int narrow(int64_t v, const char* op, const char* name) {
   return static_cast<int>(v);
 }
 
-std::tuple<torch::Tensor, OptTensor> rotary(torch::Tensor Q, OptTensor K, torch::Tensor positions, torch::Tensor inv_freq,
-                                            bool interleaved, double scale, bool backward) {
-  const char* op = "rotary_embedding";
+// Checked positions ([tokens], or with axes [num_axes, tokens]), axes and frequencies of rows Q (and K) [tokens, heads, dim].
+struct Angles {
+  torch::Tensor pos, axes, freq;
+  int num_axes = 1;
+  const int32_t* axes_ptr() const { return axes.defined() ? axes.data_ptr<int32_t>() : nullptr; }
+};
+
+Angles check_rotary(const char* op, const torch::Tensor& Q, const OptTensor& K, const torch::Tensor& positions,
+                    const torch::Tensor& inv_freq, const OptTensor& axes, double scale) {
   check_cuda(Q, Q, op, "Q");
   TORCH_CHECK_VALUE(Q.dim() == 3, op, ": Q must be [tokens, heads, dim]");
-  const int code = dtype_code(Q, op, true);
   const int64_t T = Q.size(0), D = Q.size(2);
   if (K) {
     check_cuda(*K, Q, op, "K");
@@ -244,7 +251,12 @@ std::tuple<torch::Tensor, OptTensor> rotary(torch::Tensor Q, OptTensor K, torch:
     TORCH_CHECK_VALUE(K->scalar_type() == Q.scalar_type(), op, ": K and Q must have one dtype");
   }
   check_cuda(positions, Q, op, "positions");
-  TORCH_CHECK_VALUE(positions.dim() == 1 && positions.size(0) == T, op, ": positions must be [tokens]");
+  if (axes) {
+    TORCH_CHECK_VALUE(positions.dim() == 2 && positions.size(0) >= 1 && positions.size(1) == T, op,
+                      ": positions must be [number of axes, tokens]");
+  } else {
+    TORCH_CHECK_VALUE(positions.dim() == 1 && positions.size(0) == T, op, ": positions must be [tokens]");
+  }
   TORCH_CHECK_VALUE(positions.scalar_type() == torch::kInt32 || positions.scalar_type() == torch::kInt64, op,
                     ": positions must be int32 or int64");
   check_cuda(inv_freq, Q, op, "inv_freq");
@@ -253,7 +265,24 @@ std::tuple<torch::Tensor, OptTensor> rotary(torch::Tensor Q, OptTensor K, torch:
   TORCH_CHECK_VALUE(scale > -1e30 && scale < 1e30, op, ": scale must be finite and below 1e30 in size");
   TORCH_CHECK_VALUE(D % 2 == 0 && D <= 512, op, ": the head dimension must be even and at most 512, got ", D);
   const at::cuda::CUDAGuard guard(Q.device());
-  const auto pos = positions.contiguous(), freq = inv_freq.contiguous();
+  Angles a;
+  a.pos = positions.contiguous();
+  a.freq = inv_freq.contiguous();
+  if (axes) {
+    a.axes = as_index(*axes, Q, op, "axes", 1);
+    TORCH_CHECK_VALUE(a.axes.size(0) == inv_freq.size(0), op, ": axes must hold one axis for each frequency");
+    a.num_axes = narrow(positions.size(0), op, "number of axes");
+  }
+  return a;
+}
+
+std::tuple<torch::Tensor, OptTensor> rotary(torch::Tensor Q, OptTensor K, torch::Tensor positions, torch::Tensor inv_freq,
+                                            OptTensor axes, bool interleaved, double scale, bool backward) {
+  const char* op = "rotary_embedding";
+  const Angles g = check_rotary(op, Q, K, positions, inv_freq, axes, scale);
+  const int code = dtype_code(Q, op, true);
+  const int64_t T = Q.size(0), D = Q.size(2);
+  const at::cuda::CUDAGuard guard(Q.device());
   const Rows q = as_rows(Q, true);
   auto qo = torch::empty({T, Q.size(1), D}, Q.options());
   Rows k{};
@@ -262,13 +291,115 @@ std::tuple<torch::Tensor, OptTensor> rotary(torch::Tensor Q, OptTensor K, torch:
     k = as_rows(*K, true);
     ko = torch::empty({T, K->size(1), D}, K->options());
   }
-  check_rc(bsk_rotary(code, q.p(), q.ts, q.hs, qo.data_ptr(), narrow(Q.size(1), op, "heads"), K ? k.p() : nullptr, k.ts,
-                      k.hs, K ? ko->data_ptr() : nullptr, K ? narrow(K->size(1), op, "kv_heads") : 0, pos.data_ptr(),
-                      static_cast<int>(pos.element_size()), freq.data_ptr<float>(), narrow(T, op, "tokens"),
-                      static_cast<int>(D), static_cast<int>(2 * freq.size(0)), interleaved, static_cast<float>(scale),
-                      backward, stream_of(Q)),
-           "bsk_rotary");
+  const int heads = narrow(Q.size(1), op, "heads"), kv_heads = K ? narrow(K->size(1), op, "kv_heads") : 0,
+            tokens = narrow(T, op, "tokens"), dim = static_cast<int>(D), turned = static_cast<int>(2 * g.freq.size(0)),
+            bytes = static_cast<int>(g.pos.element_size());
+  const void* kp = K ? k.p() : nullptr;
+  void* kop = K ? ko->data_ptr() : nullptr;
+  if (axes)
+    check_rc(bsk_rotary_axes(code, q.p(), q.ts, q.hs, qo.data_ptr(), heads, kp, k.ts, k.hs, kop, kv_heads, g.pos.data_ptr(), bytes,
+                             g.axes_ptr(), g.num_axes, g.freq.data_ptr<float>(), tokens, dim, turned, interleaved,
+                             static_cast<float>(scale), backward, stream_of(Q)),
+             "bsk_rotary_axes");
+  else
+    check_rc(bsk_rotary(code, q.p(), q.ts, q.hs, qo.data_ptr(), heads, kp, k.ts, k.hs, kop, kv_heads, g.pos.data_ptr(), bytes,
+                        g.freq.data_ptr<float>(), tokens, dim, turned, interleaved, static_cast<float>(scale), backward,
+                        stream_of(Q)),
+             "bsk_rotary");
   return {qo, ko};
+}
+
+// A head's norm weight: [dim] of the rows' type or float32.
+void check_weight(const char* op, const char* name, const torch::Tensor& w, const torch::Tensor& x) {
+  check_cuda(w, x, op, name);
+  TORCH_CHECK_VALUE(w.dim() == 1 && w.size(0) == x.size(2), op, ": ", name, " must be [dim]");
+  TORCH_CHECK_VALUE(w.scalar_type() == x.scalar_type() || w.scalar_type() == torch::kFloat32, op, ": ", name,
+                    " must be of the rows' dtype or float32");
+}
+
+void check_norm(const char* op, const torch::Tensor& Q, const OptTensor& K, const torch::Tensor& q_weight, const OptTensor& k_weight,
+                double eps) {
+  check_weight(op, "q_weight", q_weight, Q);
+  TORCH_CHECK_VALUE(K.has_value() == k_weight.has_value(), op, ": K and k_weight go together");
+  if (K) {
+    check_weight(op, "k_weight", *k_weight, *K);
+    TORCH_CHECK_VALUE(k_weight->scalar_type() == q_weight.scalar_type(), op, ": the weights must have one dtype");
+  }
+  TORCH_CHECK_VALUE(eps >= 1e-30 && eps < 1e30, op, ": eps must be at least 1e-30 and finite");
+}
+
+std::tuple<torch::Tensor, OptTensor> norm_rotary_fwd(torch::Tensor Q, OptTensor K, torch::Tensor q_weight, OptTensor k_weight,
+                                                     torch::Tensor positions, torch::Tensor inv_freq, OptTensor axes,
+                                                     bool interleaved, double scale, double eps) {
+  const char* op = "qk_norm_rotary";
+  const Angles g = check_rotary(op, Q, K, positions, inv_freq, axes, scale);
+  const int code = dtype_code(Q, op, true);
+  check_norm(op, Q, K, q_weight, k_weight, eps);
+  const at::cuda::CUDAGuard guard(Q.device());
+  const int64_t T = Q.size(0), D = Q.size(2);
+  const auto qw = q_weight.contiguous(), kw = K ? k_weight->contiguous() : torch::Tensor();
+  const Rows q = as_rows(Q, true), k = K ? as_rows(*K, true) : Rows{};
+  auto qo = torch::empty({T, Q.size(1), D}, Q.options());
+  OptTensor ko;
+  if (K) ko = torch::empty({T, K->size(1), D}, K->options());
+  check_rc(bsk_qk_norm_rotary(code, q.p(), q.ts, q.hs, qo.data_ptr(), narrow(Q.size(1), op, "heads"), K ? k.p() : nullptr, k.ts, k.hs,
+                              K ? ko->data_ptr() : nullptr, K ? narrow(K->size(1), op, "kv_heads") : 0, qw.data_ptr(),
+                              K ? kw.data_ptr() : nullptr, qw.scalar_type() == torch::kFloat32, g.pos.data_ptr(),
+                              static_cast<int>(g.pos.element_size()), g.axes_ptr(), g.num_axes, g.freq.data_ptr<float>(),
+                              narrow(T, op, "tokens"), static_cast<int>(D), static_cast<int>(2 * g.freq.size(0)), interleaved,
+                              static_cast<float>(scale), static_cast<float>(eps), stream_of(Q)),
+           "bsk_qk_norm_rotary");
+  return {qo, ko};
+}
+
+// (dQ, dK, dq_weight, dk_weight); a result's gradient that is absent gives none for its input and weight.
+variable_list norm_rotary_bwd(OptTensor dQo, OptTensor dKo, torch::Tensor Q, OptTensor K, torch::Tensor q_weight, OptTensor k_weight,
+                              torch::Tensor positions, torch::Tensor inv_freq, OptTensor axes, bool interleaved, double scale,
+                              double eps) {
+  const char* op = "qk_norm_rotary backward";
+  const Angles g = check_rotary(op, Q, K, positions, inv_freq, axes, scale);
+  const int code = dtype_code(Q, op, true);
+  check_norm(op, Q, K, q_weight, k_weight, eps);
+  const at::cuda::CUDAGuard guard(Q.device());
+  const int64_t T = Q.size(0), D = Q.size(2);
+  const bool has_q = dQo.has_value(), has_k = K && dKo.has_value();
+  const auto rows_of = [&](const OptTensor& t, const torch::Tensor& like) {
+    check_cuda(*t, like, op, "a gradient");
+    TORCH_CHECK_VALUE(t->sizes() == like.sizes(), op, ": a gradient differs from its result in shape");
+    return as_rows(t->to(like.scalar_type()), true);
+  };
+  Rows dq{}, dk{}, q{}, k{};
+  torch::Tensor dQ, dK, dqw, dkw, qw, kw;
+  if (has_q) {
+    dq = rows_of(dQo, Q);
+    q = as_rows(Q, true);
+    dQ = torch::empty({T, Q.size(1), D}, Q.options());
+    qw = q_weight.contiguous();
+    dqw = torch::empty({D}, q_weight.options());
+  }
+  if (has_k) {
+    dk = rows_of(dKo, *K);
+    k = as_rows(*K, true);
+    dK = torch::empty({T, K->size(1), D}, K->options());
+    kw = k_weight->contiguous();
+    dkw = torch::empty({D}, k_weight->options());
+  }
+  const int tokens = narrow(T, op, "tokens"), heads = has_q ? narrow(Q.size(1), op, "heads") : 0,
+            kv_heads = has_k ? narrow(K->size(1), op, "kv_heads") : 0;
+  const int64_t need = bsk_qk_norm_rotary_workspace_bytes(tokens, heads, kv_heads, static_cast<int>(D));
+  TORCH_CHECK(need >= 0, "bsk_qk_norm_rotary_workspace_bytes failed: ", bsk_last_error());
+  auto ws = torch::empty({need}, Q.options().dtype(torch::kUInt8));
+  if (has_q && heads == 0) dqw.zero_();
+  if (has_k && kv_heads == 0) dkw.zero_();
+  const auto at = [](const torch::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; };
+  check_rc(bsk_qk_norm_rotary_bwd(code, at(dq.t), dq.ts, dq.hs, at(q.t), q.ts, q.hs, at(dQ), heads, at(dk.t), dk.ts, dk.hs, at(k.t),
+                                  k.ts, k.hs, at(dK), kv_heads, at(qw), at(kw), q_weight.scalar_type() == torch::kFloat32, at(dqw),
+                                  at(dkw), g.pos.data_ptr(), static_cast<int>(g.pos.element_size()), g.axes_ptr(), g.num_axes,
+                                  g.freq.data_ptr<float>(), tokens, static_cast<int>(D), static_cast<int>(2 * g.freq.size(0)),
+                                  interleaved, static_cast<float>(scale), static_cast<float>(eps), ws.data_ptr(), need,
+                                  stream_of(Q)),
+           "bsk_qk_norm_rotary_bwd");
+  return {dQ, dK, dqw, dkw};
 }
 
 // The caches' checks shared by append, gather and attention: returns whether they hold e4m3 codes.
@@ -346,6 +477,41 @@ std::tuple<torch::Tensor, torch::Tensor> kv_cache_gather(torch::Tensor k_cache, 
                                static_cast<int>(K.size(2)), k_cache.size(0) * k_cache.size(1), stream_of(K)),
            "bsk_kv_cache_gather");
   return {K, V};
+}
+
+// (slots, positions, cu_seqlens, kv_lens, free_count) after a step; entries of opened pages are written to block_table.
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor, torch::Tensor, torch::Tensor> kv_cache_plan(
+    torch::Tensor kv_lens, torch::Tensor new_lens, torch::Tensor block_table, torch::Tensor free_pages, torch::Tensor free_count,
+    int64_t page_size, int64_t tokens) {
+  const char* op = "kv_cache_plan";
+  check_cuda(block_table, block_table, op, "block_table");
+  TORCH_CHECK_VALUE(block_table.dim() == 2 && block_table.scalar_type() == torch::kInt32, op, ": block_table must be int32 [batch, width]");
+  const int64_t batch = block_table.size(0), width = block_table.size(1);
+  TORCH_CHECK_VALUE((width <= 1 || block_table.stride(1) == 1) && (batch <= 1 || block_table.stride(0) >= std::max<int64_t>(width, 1)),
+                    op, ": rows of block_table must be contiguous and apart");
+  const at::cuda::CUDAGuard guard(block_table.device());
+  const auto kv = as_index(kv_lens, block_table, op, "kv_lens", 1), n = as_index(new_lens, block_table, op, "new_lens", 1);
+  TORCH_CHECK_VALUE(kv.size(0) == batch && n.size(0) == batch, op, ": kv_lens, new_lens and block_table differ in the batch");
+  for (const auto& [t, name] : {std::pair<const torch::Tensor&, const char*>{free_pages, "free_pages"}, {free_count, "free_count"}}) {
+    check_cuda(t, block_table, op, name);
+    TORCH_CHECK_VALUE(t.dim() == 1 && t.scalar_type() == torch::kInt32, op, ": ", name, " must be 1-D int32");
+  }
+  TORCH_CHECK_VALUE(free_count.size(0) == 1, op, ": free_count must hold one number");
+  TORCH_CHECK_VALUE(page_size >= 1, op, ": page_size must be positive, got ", page_size);
+  const int rows = narrow(tokens, op, "tokens");
+  const auto pages = free_pages.contiguous();
+  const auto i32 = block_table.options();
+  auto slots = torch::empty({tokens}, i32.dtype(torch::kInt64));
+  auto positions = torch::empty({tokens}, i32), cu = torch::empty({batch + 1}, i32), lens = torch::empty({batch}, i32),
+       left = torch::empty({1}, i32);
+  check_rc(bsk_kv_cache_plan(kv.data_ptr<int32_t>(), n.data_ptr<int32_t>(), narrow(batch, op, "batch"), block_table.data_ptr<int32_t>(),
+                             batch > 1 ? block_table.stride(0) : width, narrow(width, op, "table width"), pages.data_ptr<int32_t>(),
+                             narrow(pages.size(0), op, "free pages"), free_count.data_ptr<int32_t>(), narrow(page_size, op, "page_size"),
+                             slots.data_ptr<int64_t>(), positions.data_ptr<int32_t>(), rows, cu.data_ptr<int32_t>(),
+                             lens.data_ptr<int32_t>(), left.data_ptr<int32_t>(), stream_of(block_table)),
+           "bsk_kv_cache_plan");
+  if (!block_table.is_inference()) block_table.unsafeGetTensorImpl()->bump_version();
+  return {slots, positions, cu, lens, left};
 }
 
 void check_heads(const char* op, const torch::Tensor& Q, int64_t kv_heads, double scale) {
@@ -508,9 +674,6 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> attention_varlen_bwd(tor
 }
 
 // ------------------------------------------------------------------ autograd (no Python between the engine and the kernels)
-using torch::autograd::AutogradContext;
-using torch::autograd::variable_list;
-
 // Gradients that cannot be differentiated again: an error in the place of a silently wrong second derivative.
 variable_list once(variable_list grads, const char* what) {
   if (!at::GradMode::is_enabled()) return grads;
@@ -561,10 +724,10 @@ torch::Tensor attention_varlen(torch::Tensor Q, torch::Tensor K, torch::Tensor V
 // Rotary positions: the gradient of a turn is the turn back.
 struct Rotary : public torch::autograd::Function<Rotary> {
   static variable_list forward(AutogradContext* ctx, torch::Tensor Q, OptTensor K, torch::Tensor positions,
-                               torch::Tensor inv_freq, bool interleaved, double scale) {
+                               torch::Tensor inv_freq, OptTensor axes, bool interleaved, double scale) {
     at::AutoDispatchBelowADInplaceOrView guard;
-    auto [q, k] = rotary(Q, K, positions, inv_freq, interleaved, scale, false);
-    ctx->save_for_backward({positions, inv_freq});
+    auto [q, k] = rotary(Q, K, positions, inv_freq, axes, interleaved, scale, false);
+    ctx->save_for_backward({positions, inv_freq, axes ? *axes : torch::Tensor()});
     ctx->saved_data["interleaved"] = interleaved;
     ctx->saved_data["scale"] = scale;
     ctx->set_materialize_grads(false);
@@ -576,11 +739,12 @@ struct Rotary : public torch::autograd::Function<Rotary> {
     const auto s = ctx->get_saved_variables();
     const bool need_q = ctx->needs_input_grad(0) && grads[0].defined();
     const bool need_k = grads.size() > 1 && ctx->needs_input_grad(1) && grads[1].defined();
-    variable_list out(6);
+    variable_list out(7);
     if (need_q || need_k) {
       at::AutoGradMode no_grad(false);
       auto [a, b] = rotary(need_q ? grads[0] : grads[1], need_q && need_k ? OptTensor(grads[1]) : std::nullopt, s[0], s[1],
-                           ctx->saved_data["interleaved"].toBool(), ctx->saved_data["scale"].toDouble(), true);
+                           s[2].defined() ? OptTensor(s[2]) : std::nullopt, ctx->saved_data["interleaved"].toBool(),
+                           ctx->saved_data["scale"].toDouble(), true);
       if (need_q) out[0] = a;
       if (need_k) out[1] = need_q ? *b : a;
     }
@@ -589,16 +753,67 @@ struct Rotary : public torch::autograd::Function<Rotary> {
 };
 
 std::tuple<torch::Tensor, OptTensor> rotary_embedding(torch::Tensor Q, OptTensor K, torch::Tensor positions,
-                                                      torch::Tensor inv_freq, bool interleaved, double scale) {
+                                                      torch::Tensor inv_freq, bool interleaved, double scale, OptTensor axes) {
   no_tangent("rotary_embedding", {&Q, some(K), &inv_freq});
   if (at::GradMode::is_enabled()) {
     TORCH_CHECK_VALUE(!inv_freq.requires_grad(), "rotary_embedding has no gradient for inv_freq");
     if (Q.requires_grad() || (K && K->requires_grad())) {
-      auto out = Rotary::apply(Q, K, positions, inv_freq, interleaved, scale);
+      auto out = Rotary::apply(Q, K, positions, inv_freq, axes, interleaved, scale);
       return {out[0], K ? OptTensor(out[1]) : std::nullopt};
     }
   }
-  return rotary(Q, K, positions, inv_freq, interleaved, scale, false);
+  return rotary(Q, K, positions, inv_freq, axes, interleaved, scale, false);
+}
+
+// Norm and rotation: the backward takes the inputs again and recomputes the rows' norms.
+struct NormRotary : public torch::autograd::Function<NormRotary> {
+  static variable_list forward(AutogradContext* ctx, torch::Tensor Q, OptTensor K, torch::Tensor q_weight, OptTensor k_weight,
+                               torch::Tensor positions, torch::Tensor inv_freq, OptTensor axes, bool interleaved, double scale,
+                               double eps) {
+    at::AutoDispatchBelowADInplaceOrView guard;
+    auto [q, k] = norm_rotary_fwd(Q, K, q_weight, k_weight, positions, inv_freq, axes, interleaved, scale, eps);
+    ctx->save_for_backward({Q, K ? *K : torch::Tensor(), q_weight, K ? *k_weight : torch::Tensor(), positions, inv_freq,
+                            axes ? *axes : torch::Tensor()});
+    ctx->saved_data["interleaved"] = interleaved;
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["eps"] = eps;
+    ctx->set_materialize_grads(false);
+    variable_list out{q};
+    if (k) out.push_back(*k);
+    return out;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto s = ctx->get_saved_variables();
+    const auto opt = [](const torch::Tensor& t) { return t.defined() ? OptTensor(t) : std::nullopt; };
+    // only the halves that something asks for
+    const bool need_q = (ctx->needs_input_grad(0) || ctx->needs_input_grad(2)) && grads[0].defined();
+    const bool need_k = grads.size() > 1 && (ctx->needs_input_grad(1) || ctx->needs_input_grad(3)) && grads[1].defined();
+    variable_list out(10);
+    if (need_q || need_k) {
+      at::AutoGradMode no_grad(false);
+      auto d = norm_rotary_bwd(need_q ? OptTensor(grads[0]) : std::nullopt, need_k ? OptTensor(grads[1]) : std::nullopt, s[0],
+                               opt(s[1]), s[2], opt(s[3]), s[4], s[5], opt(s[6]), ctx->saved_data["interleaved"].toBool(),
+                               ctx->saved_data["scale"].toDouble(), ctx->saved_data["eps"].toDouble());
+      for (int i = 0; i < 4; ++i)
+        if (ctx->needs_input_grad(i)) out[i] = d[i];
+    }
+    return once(std::move(out), "qk_norm_rotary");
+  }
+};
+
+std::tuple<torch::Tensor, OptTensor> qk_norm_rotary(torch::Tensor Q, OptTensor K, torch::Tensor q_weight, OptTensor k_weight,
+                                                    torch::Tensor positions, torch::Tensor inv_freq, bool interleaved, double scale,
+                                                    double eps, OptTensor axes) {
+  const char* op = "qk_norm_rotary";
+  no_tangent(op, {&Q, some(K), &q_weight, some(k_weight), &inv_freq});
+  if (at::GradMode::is_enabled()) {
+    TORCH_CHECK_VALUE(!inv_freq.requires_grad(), op, " has no gradient for inv_freq");
+    if (Q.requires_grad() || q_weight.requires_grad() || (K && K->requires_grad()) || (k_weight && k_weight->requires_grad())) {
+      auto out = NormRotary::apply(Q, K, q_weight, k_weight, positions, inv_freq, axes, interleaved, scale, eps);
+      return {out[0], K ? OptTensor(out[1]) : std::nullopt};
+    }
+  }
+  return norm_rotary_fwd(Q, K, q_weight, k_weight, positions, inv_freq, axes, interleaved, scale, eps);
 }
 
 int64_t device_error() {
@@ -622,7 +837,14 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("bsattn_fwd", &bsattn_fwd, "block-sparse attention forward (sm_100a)", py::arg("Q"), py::arg("K"),
         py::arg("V"), py::arg("row_ptr"), py::arg("col_idx"), py::arg("scale"), py::arg("causal_diag") = true);
   m.def("rotary_embedding", &rotary_embedding, "rotary positions of Q and K, with gradients (sm_100a)", py::arg("Q"),
-        py::arg("K"), py::arg("positions"), py::arg("inv_freq"), py::arg("interleaved") = false, py::arg("scale") = 1.0);
+        py::arg("K"), py::arg("positions"), py::arg("inv_freq"), py::arg("interleaved") = false, py::arg("scale") = 1.0,
+        py::arg("axes") = py::none());
+  m.def("qk_norm_rotary", &qk_norm_rotary, "norm of each head of Q and K, then rotary positions, with gradients (sm_100a)",
+        py::arg("Q"), py::arg("K"), py::arg("q_weight"), py::arg("k_weight"), py::arg("positions"), py::arg("inv_freq"),
+        py::arg("interleaved") = false, py::arg("scale") = 1.0, py::arg("eps") = 1e-6, py::arg("axes") = py::none());
+  m.def("kv_cache_plan", &kv_cache_plan, "block tables, slots and positions of a serving step (sm_100a)", py::arg("kv_lens"),
+        py::arg("new_lens"), py::arg("block_table"), py::arg("free_pages"), py::arg("free_count"), py::arg("page_size"),
+        py::arg("tokens"));
   m.def("kv_cache_append", &kv_cache_append, "write rows to a paged key/value cache (sm_100a)", py::arg("K"), py::arg("V"),
         py::arg("k_cache"), py::arg("v_cache"), py::arg("slots"), py::arg("k_scale") = py::none(),
         py::arg("v_scale") = py::none());

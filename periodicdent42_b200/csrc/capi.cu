@@ -23,6 +23,8 @@
 #include "bsattn_bwd_sm100.cuh"
 #include "rotary.cuh"
 #include "kv_cache.cuh"
+#include "kv_plan.cuh"
+#include "norm_rotary.h"
 #include "paged_decode_sm100.cuh"
 #include "varattn_sm100.cuh"
 #include "varattn_bwd_sm100.cuh"
@@ -1938,13 +1940,11 @@ int rotary_pick(bsk::RotaryArgs& a, bool inter, const DeviceState& st, cudaStrea
 
 }  // namespace
 
-extern "C" {
+namespace {
 
-int bsk_rotary(int dtype, const void* Q, int64_t q_token_stride, int64_t q_head_stride, void* Q_out, int heads,
-               const void* K, int64_t k_token_stride, int64_t k_head_stride, void* K_out, int kv_heads,
-               const void* positions, int position_bytes, const float* inv_freq, int tokens, int dim, int rotary_dim,
-               int interleaved, float scale, int backward, void* stream) {
-  const char* what = "rotary";
+// What rotary positions and the norm in front of them have in common.
+int rotary_checks(const char* what, int dtype, int tokens, int heads, int kv_heads, int dim, int rotary_dim, int position_bytes,
+                  const int32_t* axes, int num_axes, float scale) {
   if (dtype < 0 || dtype > 2) return set_error(BSK_ERR_INVALID_ARG, "%s: dtype must be 0 (bf16), 1 (f16) or 2 (f32)", what);
   if (tokens < 0 || heads < 0 || kv_heads < 0) return set_error(BSK_ERR_INVALID_ARG, "%s: negative extent", what);
   if (dim <= 0 || dim % 2 || dim > bsk::kRotaryMaxDim)
@@ -1953,7 +1953,17 @@ int bsk_rotary(int dtype, const void* Q, int64_t q_token_stride, int64_t q_head_
     return set_error(BSK_ERR_INVALID_ARG, "%s: rotary dim %d must be even and within [2, %d]", what, rotary_dim, dim);
   if (position_bytes != 4 && position_bytes != 8)
     return set_error(BSK_ERR_INVALID_ARG, "%s: positions must be 4- or 8-byte integers", what);
+  if (axes && num_axes < 1) return set_error(BSK_ERR_INVALID_ARG, "%s: axes need at least one row of positions", what);
   if (!(scale > -1e30f && scale < 1e30f)) return set_error(BSK_ERR_INVALID_ARG, "%s: scale must be finite", what);
+  return BSK_OK;
+}
+
+int rotary(int dtype, const void* Q, int64_t q_token_stride, int64_t q_head_stride, void* Q_out, int heads, const void* K,
+           int64_t k_token_stride, int64_t k_head_stride, void* K_out, int kv_heads, const void* positions, int position_bytes,
+           const int32_t* axes, int num_axes, const float* inv_freq, int tokens, int dim, int rotary_dim, int interleaved,
+           float scale, int backward, void* stream) {
+  const char* what = "rotary";
+  if (int rc = rotary_checks(what, dtype, tokens, heads, kv_heads, dim, rotary_dim, position_bytes, axes, num_axes, scale)) return rc;
   DeviceState* st;
   if (tokens == 0 || (heads == 0 && kv_heads == 0)) return device_state(&st);
   if (!positions || !inv_freq || (heads && (!Q || !Q_out)) || (kv_heads && (!K || !K_out)))
@@ -1967,6 +1977,9 @@ int bsk_rotary(int dtype, const void* Q, int64_t q_token_stride, int64_t q_head_
   a.heads[0] = heads; a.heads[1] = kv_heads;
   a.positions = positions;
   a.positions64 = position_bytes == 8;
+  a.axes = axes;
+  a.num_axes = num_axes;
+  a.err = st->err_word;
   a.inv_freq = inv_freq;
   a.tokens = tokens;
   a.dim = dim;
@@ -1977,6 +1990,121 @@ int bsk_rotary(int dtype, const void* Q, int64_t q_token_stride, int64_t q_head_
   if (dtype == 0) return rotary_pick<__nv_bfloat16>(a, interleaved != 0, *st, s);
   if (dtype == 1) return rotary_pick<__half>(a, interleaved != 0, *st, s);
   return rotary_pick<float>(a, interleaved != 0, *st, s);
+}
+
+// The arguments of the norm's two passes; `x` alone is checked against null here.
+int norm_rotary_args(const char* what, bsk::NormRotaryArgs& a, int dtype, const void* Q, int64_t q_token_stride,
+                     int64_t q_head_stride, void* Q_out, int heads, const void* K, int64_t k_token_stride, int64_t k_head_stride,
+                     void* K_out, int kv_heads, const void* q_weight, const void* k_weight, int weight_f32, const void* positions,
+                     int position_bytes, const int32_t* axes, int num_axes, const float* inv_freq, int tokens, int dim,
+                     int rotary_dim, float scale, float eps) {
+  if (int rc = rotary_checks(what, dtype, tokens, heads, kv_heads, dim, rotary_dim, position_bytes, axes, num_axes, scale)) return rc;
+  if (!(eps >= 1e-30f && eps < 1e30f)) return set_error(BSK_ERR_INVALID_ARG, "%s: eps must be at least 1e-30 and finite", what);
+  if (tokens == 0 || (heads == 0 && kv_heads == 0)) return BSK_OK;
+  if (!positions || !inv_freq || (heads && (!Q || !Q_out || !q_weight)) || (kv_heads && (!K || !K_out || !k_weight)))
+    return set_error(BSK_ERR_INVALID_ARG, "%s: null pointer", what);
+  a.x[0] = Q; a.x[1] = K;
+  a.y[0] = Q_out; a.y[1] = K_out;
+  a.token_stride[0] = q_token_stride; a.token_stride[1] = k_token_stride;
+  a.head_stride[0] = q_head_stride; a.head_stride[1] = k_head_stride;
+  a.heads[0] = heads; a.heads[1] = kv_heads;
+  a.w[0] = q_weight; a.w[1] = k_weight;
+  a.w_f32 = weight_f32 != 0 || dtype == 2;
+  a.positions = positions;
+  a.positions64 = position_bytes == 8;
+  a.axes = axes;
+  a.num_axes = num_axes;
+  a.inv_freq = inv_freq;
+  a.tokens = tokens;
+  a.dim = dim;
+  a.rotary_dim = rotary_dim;
+  a.scale = scale;
+  a.eps = eps;
+  return BSK_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int bsk_rotary(int dtype, const void* Q, int64_t q_token_stride, int64_t q_head_stride, void* Q_out, int heads,
+               const void* K, int64_t k_token_stride, int64_t k_head_stride, void* K_out, int kv_heads,
+               const void* positions, int position_bytes, const float* inv_freq, int tokens, int dim, int rotary_dim,
+               int interleaved, float scale, int backward, void* stream) {
+  return rotary(dtype, Q, q_token_stride, q_head_stride, Q_out, heads, K, k_token_stride, k_head_stride, K_out, kv_heads, positions,
+                position_bytes, nullptr, 1, inv_freq, tokens, dim, rotary_dim, interleaved, scale, backward, stream);
+}
+
+int bsk_rotary_axes(int dtype, const void* Q, int64_t q_token_stride, int64_t q_head_stride, void* Q_out, int heads,
+                    const void* K, int64_t k_token_stride, int64_t k_head_stride, void* K_out, int kv_heads,
+                    const void* positions, int position_bytes, const int32_t* axes, int num_axes, const float* inv_freq,
+                    int tokens, int dim, int rotary_dim, int interleaved, float scale, int backward, void* stream) {
+  if (tokens > 0 && !axes) return set_error(BSK_ERR_INVALID_ARG, "rotary: null pointer");
+  return rotary(dtype, Q, q_token_stride, q_head_stride, Q_out, heads, K, k_token_stride, k_head_stride, K_out, kv_heads, positions,
+                position_bytes, axes, num_axes, inv_freq, tokens, dim, rotary_dim, interleaved, scale, backward, stream);
+}
+
+int bsk_qk_norm_rotary(int dtype, const void* Q, int64_t q_token_stride, int64_t q_head_stride, void* Q_out, int heads,
+                       const void* K, int64_t k_token_stride, int64_t k_head_stride, void* K_out, int kv_heads,
+                       const void* q_weight, const void* k_weight, int weight_f32, const void* positions, int position_bytes,
+                       const int32_t* axes, int num_axes, const float* inv_freq, int tokens, int dim, int rotary_dim,
+                       int interleaved, float scale, float eps, void* stream) {
+  bsk::NormRotaryArgs a{};
+  if (int rc = norm_rotary_args("qk_norm_rotary", a, dtype, Q, q_token_stride, q_head_stride, Q_out, heads, K, k_token_stride,
+                                k_head_stride, K_out, kv_heads, q_weight, k_weight, weight_f32, positions, position_bytes, axes,
+                                num_axes, inv_freq, tokens, dim, rotary_dim, scale, eps))
+    return rc;
+  DeviceState* st;
+  if (int rc = device_state(&st)) return rc;
+  if (tokens == 0 || (heads == 0 && kv_heads == 0)) return BSK_OK;
+  a.err = st->err_word;
+  const cudaError_t e = bsk::norm_rotary_fwd(dtype, interleaved != 0, a, st->sm_count, static_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? BSK_OK : cuda_fail(e, "qk_norm_rotary launch");
+}
+
+int64_t bsk_qk_norm_rotary_workspace_bytes(int tokens, int heads, int kv_heads, int dim) {
+  if (tokens < 0 || heads < 0 || kv_heads < 0 || dim <= 0 || dim > bsk::kRotaryMaxDim)
+    return set_error(BSK_ERR_INVALID_ARG, "qk_norm_rotary_workspace_bytes: extent out of range");
+  DeviceState* st;
+  if (int rc = device_state(&st)) return rc;
+  return bsk::norm_rotary_partials(tokens, heads, kv_heads, dim, st->sm_count) * (int64_t)sizeof(float);
+}
+
+int bsk_qk_norm_rotary_bwd(int dtype, const void* dQ_out, int64_t dq_token_stride, int64_t dq_head_stride, const void* Q,
+                           int64_t q_token_stride, int64_t q_head_stride, void* dQ, int heads, const void* dK_out,
+                           int64_t dk_token_stride, int64_t dk_head_stride, const void* K, int64_t k_token_stride,
+                           int64_t k_head_stride, void* dK, int kv_heads, const void* q_weight, const void* k_weight,
+                           int weight_f32, void* dq_weight, void* dk_weight, const void* positions, int position_bytes,
+                           const int32_t* axes, int num_axes, const float* inv_freq, int tokens, int dim, int rotary_dim,
+                           int interleaved, float scale, float eps, void* workspace, int64_t workspace_bytes, void* stream) {
+  const char* what = "qk_norm_rotary_bwd";
+  bsk::NormRotaryArgs a{};
+  if (int rc = norm_rotary_args(what, a, dtype, Q, q_token_stride, q_head_stride, dQ, heads, K, k_token_stride, k_head_stride, dK,
+                                kv_heads, q_weight, k_weight, weight_f32, positions, position_bytes, axes, num_axes, inv_freq,
+                                tokens, dim, rotary_dim, scale, eps))
+    return rc;
+  if (tokens > 0 && ((heads && !dQ_out) || (kv_heads && !dK_out))) return set_error(BSK_ERR_INVALID_ARG, "%s: null pointer", what);
+  DeviceState* st;
+  if (int rc = device_state(&st)) return rc;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (tokens == 0) {  // sums of nothing
+    const int64_t bytes = (int64_t)dim * (a.w_f32 || weight_f32 || dtype == 2 ? 4 : 2);
+    cudaError_t e = dq_weight ? cudaMemsetAsync(dq_weight, 0, bytes, s) : cudaSuccess;
+    if (e == cudaSuccess && dk_weight) e = cudaMemsetAsync(dk_weight, 0, bytes, s);
+    return e == cudaSuccess ? BSK_OK : cuda_fail(e, what);
+  }
+  if (heads == 0 && kv_heads == 0) return BSK_OK;
+  const int64_t need = bsk::norm_rotary_partials(tokens, heads, kv_heads, dim, st->sm_count) * (int64_t)sizeof(float);
+  if (workspace_bytes < need || !workspace || !aligned16(workspace))
+    return set_error(BSK_ERR_INVALID_ARG, "%s: 16-byte aligned workspace of %lld bytes needed", what, (long long)need);
+  a.dy[0] = dQ_out; a.dy[1] = dK_out;
+  a.dy_token_stride[0] = dq_token_stride; a.dy_token_stride[1] = dk_token_stride;
+  a.dy_head_stride[0] = dq_head_stride; a.dy_head_stride[1] = dk_head_stride;
+  a.partial = static_cast<float*>(workspace);
+  a.err = st->err_word;
+  const cudaError_t e = bsk::norm_rotary_bwd(dtype, interleaved != 0, a, heads ? dq_weight : nullptr, kv_heads ? dk_weight : nullptr,
+                                             st->sm_count, s);
+  return e == cudaSuccess ? BSK_OK : cuda_fail(e, "qk_norm_rotary_bwd launch");
 }
 
 }  // extern "C"
@@ -2074,6 +2202,28 @@ int bsk_kv_cache_gather(int dtype, const void* k_cache, const void* v_cache, int
   using namespace bsk;
   BSK_BY_TYPE(kv_cache_gather_kernel, dtype == 1, dim, cache_e4m3 != 0, <<<grid, kCacheThreads, 0, s>>>(a));
   return launch_status("kv_cache_gather launch");
+}
+
+int bsk_kv_cache_plan(const int32_t* kv_lens, const int32_t* new_lens, int batch, int32_t* block_table, int64_t table_stride,
+                      int table_width, const int32_t* free_pages, int num_free, const int32_t* free_count, int page_size,
+                      int64_t* slots, int32_t* positions, int tokens, int32_t* cu_seqlens, int32_t* kv_lens_out,
+                      int32_t* free_count_out, void* stream) {
+  const char* what = "kv_cache_plan";
+  if (batch < 0 || tokens < 0 || table_width < 0 || num_free < 0 || table_stride < 0)
+    return set_error(BSK_ERR_INVALID_ARG, "%s: negative extent", what);
+  if (page_size < 1) return set_error(BSK_ERR_INVALID_ARG, "%s: page size must be positive, got %d", what, page_size);
+  if (!free_count || !cu_seqlens || !free_count_out || (batch > 0 && (!kv_lens || !new_lens || !kv_lens_out)) ||
+      (batch > 0 && table_width > 0 && !block_table) || (num_free > 0 && !free_pages) || (tokens > 0 && (!slots || !positions)))
+    return set_error(BSK_ERR_INVALID_ARG, "%s: null pointer", what);
+  if (batch > 1 && table_stride < table_width)
+    return set_error(BSK_ERR_INVALID_ARG, "%s: rows of the block table overlap", what);
+  DeviceState* st;
+  if (int rc = device_state(&st)) return rc;
+  const bsk::KvPlanArgs a{kv_lens, new_lens, block_table, table_stride, free_pages, free_count, slots, positions, cu_seqlens,
+                          kv_lens_out, free_count_out, batch, table_width, num_free, page_size, tokens, st->err_word};
+  const unsigned grid = tokens > 0 ? (unsigned)(((int64_t)tokens + bsk::kKvPlanTokens - 1) / bsk::kKvPlanTokens) : 1u;
+  bsk::kv_plan_kernel<<<grid, bsk::kKvPlanThreads, 0, static_cast<cudaStream_t>(stream)>>>(a);
+  return launch_status("kv_cache_plan launch");
 }
 
 }  // extern "C"

@@ -9,7 +9,7 @@ libbsk_sm100.so. There is no CPU fallback: CPU tensors raise ``ValueError`` (as 
 from __future__ import annotations
 
 import math
-from typing import Optional, Tuple
+from typing import Optional, Sequence, Tuple
 
 import torch
 
@@ -431,16 +431,45 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: Optional
     return inv_freq.to(torch.float32).to(device if device is not None else "cpu"), scale
 
 
+def rotary_axes(sections: Sequence[int], cycle: bool = False, device=None) -> torch.Tensor:
+    """Which axis each pair takes, for ``axes`` of :func:`rotary_embedding` and :func:`qk_norm_rotary`: int32 [sum(sections)] on
+    ``device``. sections[a] pairs take axis a: one after the other (16, 24, 24: the first 16 pairs axis 0, the next 24 axis 1,
+    ..), or with ``cycle`` the axes in turn, 0, 1, 2, 0, 1, 2, .., where an axis that has its pairs is passed over."""
+    left = [int(n) for n in sections]
+    if not left or min(left) < 0 or sum(left) < 1:
+        raise ValueError(f"rotary_axes: sections must be counts of pairs, one at least positive, got {tuple(sections)}")
+    if cycle:
+        order = [a for turn in range(max(left)) for a, n in enumerate(left) if turn < n]
+    else:
+        order = [a for a, n in enumerate(left) for _ in range(n)]
+    return torch.tensor(order, dtype=torch.int32, device=device if device is not None else "cpu")
+
+
 def rotary_embedding(Q: torch.Tensor, K: Optional[torch.Tensor], positions: torch.Tensor, inv_freq: torch.Tensor,
-                     interleaved: bool = False, scale: float = 1.0):
+                     interleaved: bool = False, scale: float = 1.0, axes: Optional[torch.Tensor] = None):
     """Rotary positions of Q [tokens, heads, dim] and K [tokens, kv_heads, dim] (K may be None) in one launch; returns
     new contiguous (Q', K'). fp16, bf16 or fp32; any strides with a unit inner stride are read in place.
 
     Pair i of a head -- elements (i, i + r/2), or (2i, 2i+1) with ``interleaved`` -- turns by positions[t] * inv_freq[i]
     and is multiplied by ``scale``; r = 2 * len(inv_freq), elements from r on are copied unchanged (and unscaled).
     positions: int32 or int64 [tokens], any value (angles are exact to fp32 at every one of them); inv_freq: float32 (see
-    :func:`rotary_frequencies`). Differentiable (once, in reverse mode) in Q and K."""
-    return _C().rotary_embedding(Q, K, positions, inv_freq, interleaved, scale)
+    :func:`rotary_frequencies`). Differentiable (once, in reverse mode) in Q and K.
+    axes (int32 or int64 [len(inv_freq)], see :func:`rotary_axes`): several axes, time, height and width of patches say:
+    positions are then [number of axes, tokens] and pair i turns by positions[axes[i], t] * inv_freq[i]. An axis out of range
+    counts as the nearest and is reported by :func:`synchronize_and_check`."""
+    return _C().rotary_embedding(Q, K, positions, inv_freq, interleaved, scale, axes)
+
+
+def qk_norm_rotary(Q: torch.Tensor, K: Optional[torch.Tensor], q_weight: torch.Tensor, k_weight: Optional[torch.Tensor],
+                   positions: torch.Tensor, inv_freq: torch.Tensor, interleaved: bool = False, scale: float = 1.0,
+                   eps: float = 1e-6, axes: Optional[torch.Tensor] = None):
+    """RMS norm of each head of Q and K, then their rotary positions, in one pass; returns new contiguous (Q', K').
+
+    z = x / sqrt(mean(x^2) + eps) * weight over a head's dim elements, then z turned as by :func:`rotary_embedding`, whose
+    arguments (and types, strides, several axes) apply. q_weight and k_weight: [dim] of the rows' dtype or float32 (K and
+    k_weight may be None). fp32 inside, rounded once; eps at least 1e-30. Differentiable (once, in reverse mode) in Q, K and the
+    weights (deterministic, no atomics)."""
+    return _C().qk_norm_rotary(Q, K, q_weight, k_weight, positions, inv_freq, interleaved, scale, eps, axes)
 
 
 # ----------------------------------------------------------------------------------------- paged key/value cache
@@ -466,6 +495,21 @@ def kv_cache_gather(k_cache: torch.Tensor, v_cache: torch.Tensor, slots: torch.T
     if dtype not in (torch.float16, torch.bfloat16):
         raise ValueError("kv_cache_gather: dtype must be torch.float16 or torch.bfloat16")
     return _C().kv_cache_gather(k_cache, v_cache, slots, dtype == torch.float16, k_scale, v_scale)
+
+
+def kv_cache_plan(kv_lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch.Tensor, free_pages: torch.Tensor,
+                  free_count: torch.Tensor, page_size: int, tokens: int):
+    """A serving step's bookkeeping on the device: where the new tokens of all requests go, and the pages that they open.
+
+    kv_lens, new_lens: int32 or int64 [batch], cached and new tokens of each request; block_table: int32 [batch, width], its
+    pages. free_pages: int32, a stack of which the first free_count[0] (int32 [1]) are free; pages are taken from its end, in
+    the order of the requests and of the positions, and entered in block_table in place. tokens: rows of the step, at least the
+    sum of new_lens. Returns (slots int64 [tokens], positions int32 [tokens], cu_seqlens int32 [batch + 1], kv_lens int32
+    [batch], free_count int32 [1]) for :func:`qk_norm_rotary`, :func:`kv_cache_append`, :func:`attention_paged` and the next
+    step; rows behind the last request's have slot -1 and position 0. Nothing synchronises, and nothing but block_table is
+    changed, so a call may be repeated. Reported by :func:`synchronize_and_check`: lengths that are negative or pass the table or
+    ``tokens``, and pages that are not there (slot -1)."""
+    return _C().kv_cache_plan(kv_lens, new_lens, block_table, free_pages, free_count, page_size, tokens)
 
 
 # ----------------------------------------------------------------------------------------- packed and paged attention

@@ -2,6 +2,7 @@
 #include "norm_rotary.h"
 
 #include <algorithm>
+#include <atomic>
 
 namespace bsk {
 namespace {
@@ -12,44 +13,73 @@ int lanes_for(int units) {
   return g;
 }
 
-// Blocks that the backward gives Q (w = 0) and K: about two rounds of what an SM holds, by their shares of the heads.
-int bwd_blocks(const int (&heads)[2], int w, int sm_count) {
-  if (!heads[w]) return 0;
-  const int64_t all = (int64_t)heads[0] + heads[1];
-  return (int)std::max<int64_t>(1, (int64_t)4 * sm_count * heads[w] / all);
-}
-
-template <class T, int kVec, int kUnits, bool kInter>
-cudaError_t launch(NormRotaryArgs& a, bool backward, int sm_count, cudaStream_t s) {
-  a.units = a.dim / (2 * kVec);
-  a.group = lanes_for((a.units + kUnits - 1) / kUnits);
-  const int groups = kNormThreads / a.group;
-  // A row's lanes keep to one token. Few tokens: as many of its heads at once as there are groups, so that a token takes one
-  // step; many: four heads a group (the loads of a batch, forward), and the groups left over take other tokens.
-  const bool few = a.tokens <= 4 * sm_count;
-  if (!backward) {
-    const int all = a.heads[0] + a.heads[1];
-    a.at_once[0] = std::min(groups, few ? all : (all + kNormBatch - 1) / kNormBatch);
-    a.per_block[0] = few ? 1 : groups / a.at_once[0];
-    const int64_t grid = ((int64_t)a.tokens + a.per_block[0] - 1) / a.per_block[0];
-    norm_rotary_kernel<T, kVec, kUnits, kInter>
-        <<<(unsigned)grid, kNormThreads, a.per_block[0] * (a.rotary_dim / 2) * sizeof(float2), s>>>(a);
-    return cudaGetLastError();
+// Launch of a kernel that takes more shared memory than the default limit, raised on its first call on a device (`ready`).
+template <class K>
+cudaError_t run(K kernel, std::atomic<uint64_t>& ready, int most, int grid, int smem, const NormRotaryArgs& a, cudaStream_t s) {
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  if (e != cudaSuccess) return e;
+  const uint64_t bit = uint64_t{1} << (device & 63);
+  if (!(ready.load(std::memory_order_acquire) & bit)) {
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+    if (e != cudaSuccess) return e;
+    ready.fetch_or(bit, std::memory_order_release);
   }
-  for (int w = 0; w < 2; ++w) {
-    a.at_once[w] = std::max(1, std::min(groups, few ? a.heads[w] : (a.heads[w] + 3) / 4));
-    a.per_block[w] = few ? 1 : groups / a.at_once[w];
-  }
-  a.blocks_q = bwd_blocks(a.heads, 0, sm_count);
-  const int grid = a.blocks_q + bwd_blocks(a.heads, 1, sm_count);
-  // (angles of per_block tokens, or the groups' sums: both fit)
-  norm_rotary_bwd_kernel<T, kVec, kUnits, kInter><<<grid, kNormThreads, groups * a.dim * sizeof(float), s>>>(a);
+  kernel<<<grid, kNormThreads, smem, s>>>(a);
   return cudaGetLastError();
 }
 
+// Blocks that Q (w = 0) and K get of `per_sm` on each SM, by what their rows and a token's angles cost (the angles about what
+// six heads do), and no more than there are chunks.
+int blocks_of(const int (&heads)[2], int w, int per_sm, int64_t chunks, int sm_count) {
+  if (!heads[w]) return 0;
+  const auto cost = [&](int i) { return heads[i] ? (int64_t)heads[i] + 6 : 0; };
+  return (int)std::max<int64_t>(1, std::min(chunks, per_sm * sm_count * cost(w) / (cost(0) + cost(1))));
+}
+
+template <class T, int kVec, int kUnits, bool kInter, int kLanes, bool kBackward>
+cudaError_t launch(NormRotaryArgs& a, int sm_count, cudaStream_t s) {
+  using Sh = NormShape<T, kVec, kUnits, kBackward>;
+  const int groups = kNormThreads / a.group;
+  // A row's lanes keep to one token. Few tokens: as many of its heads at once as there are groups, so that a token takes one
+  // step; many: four heads a group, and the groups left over take other tokens.
+  const bool few = a.tokens <= 4 * sm_count;
+  int grid = 0;
+  for (int w = 0; w < 2; ++w) {
+    a.at_once[w] = std::max(1, std::min(groups, few ? a.heads[w] : (a.heads[w] + 3) / 4));
+    a.per_block[w] = few ? 1 : groups / a.at_once[w];
+    grid += blocks_of(a.heads, w, Sh::kBlocksPerSm, ((int64_t)a.tokens + a.per_block[w] - 1) / a.per_block[w], sm_count);
+    if (w == 0) a.blocks_q = grid;
+  }
+  a.grid = grid;
+  static std::atomic<uint64_t> ready{0};
+  if constexpr (kBackward)
+    return run(norm_rotary_bwd_kernel<T, kVec, kUnits, kInter, kLanes>, ready, Sh::kMostSmem, grid, Sh::smem_bytes(a), a, s);
+  else
+    return run(norm_rotary_kernel<T, kVec, kUnits, kInter, kLanes>, ready, Sh::kMostSmem, grid, Sh::smem_bytes(a), a, s);
+}
+
+// The lanes of a row are a power of two; for 16-byte pieces their number is known to the compiler (whose sums it unrolls).
+template <class T, int kVec, int kUnits, bool kInter, bool kBackward>
+cudaError_t launch_lanes(NormRotaryArgs& a, int sm_count, cudaStream_t s) {
+  a.units = a.dim / (2 * kVec);
+  a.group = lanes_for((a.units + kUnits - 1) / kUnits);
+  if constexpr (kVec * sizeof(T) == 16 && kUnits == 1) {
+    a.group = std::max(a.group, 4);
+    if (a.group == 4) return launch<T, kVec, kUnits, kInter, 4, kBackward>(a, sm_count, s);
+    if (a.group == 8) return launch<T, kVec, kUnits, kInter, 8, kBackward>(a, sm_count, s);
+    if (a.group == 16) return launch<T, kVec, kUnits, kInter, 16, kBackward>(a, sm_count, s);
+    return launch<T, kVec, kUnits, kInter, 32, kBackward>(a, sm_count, s);
+  } else {
+    return launch<T, kVec, kUnits, kInter, 0, kBackward>(a, sm_count, s);
+  }
+}
+
 template <class T, int kVec, int kUnits>
-cudaError_t launch(NormRotaryArgs& a, bool inter, bool backward, int sm_count, cudaStream_t s) {
-  return inter ? launch<T, kVec, kUnits, true>(a, backward, sm_count, s) : launch<T, kVec, kUnits, false>(a, backward, sm_count, s);
+cudaError_t launch_any(NormRotaryArgs& a, bool inter, bool backward, int sm_count, cudaStream_t s) {
+  if (backward)
+    return inter ? launch_lanes<T, kVec, kUnits, true, true>(a, sm_count, s) : launch_lanes<T, kVec, kUnits, false, true>(a, sm_count, s);
+  return inter ? launch_lanes<T, kVec, kUnits, true, false>(a, sm_count, s) : launch_lanes<T, kVec, kUnits, false, false>(a, sm_count, s);
 }
 
 // Whether every row can be read and written in pieces of kVec elements, `bytes` wide.
@@ -75,14 +105,14 @@ cudaError_t pick(NormRotaryArgs& a, bool inter, bool backward, int sm_count, cud
   a.aligned32 = fits(a, inter, backward, kWide, kElem, 32);
   if (fits(a, inter, backward, kWide, kElem, 16)) {
     if constexpr (kElem == 4)
-      if (a.dim > 2 * kWide * 32) return launch<T, kWide, 2>(a, inter, backward, sm_count, s);
-    return launch<T, kWide, 1>(a, inter, backward, sm_count, s);
+      if (a.dim > 2 * kWide * 32) return launch_any<T, kWide, 2>(a, inter, backward, sm_count, s);
+    return launch_any<T, kWide, 1>(a, inter, backward, sm_count, s);
   }
   a.aligned32 = 0;
   if constexpr (kElem == 2)
     if (fits(a, inter, backward, 2, kElem, 4))
-      return a.dim <= 128 ? launch<T, 2, 1>(a, inter, backward, sm_count, s) : launch<T, 2, 4>(a, inter, backward, sm_count, s);
-  return launch<T, 1, 8>(a, inter, backward, sm_count, s);
+      return a.dim <= 128 ? launch_any<T, 2, 1>(a, inter, backward, sm_count, s) : launch_any<T, 2, 4>(a, inter, backward, sm_count, s);
+  return launch_any<T, 1, 8>(a, inter, backward, sm_count, s);
 }
 
 cudaError_t by_type(int dtype, bool inter, NormRotaryArgs& a, bool backward, int sm_count, cudaStream_t s) {
@@ -108,8 +138,8 @@ cudaError_t launch_weights(const NormWeightArgs& n, cudaStream_t s) {
 }  // namespace
 
 int64_t norm_rotary_partials(int tokens, int heads, int kv_heads, int dim, int sm_count) {
-  const int h[2] = {heads, kv_heads};
-  return (int64_t)(bwd_blocks(h, 0, sm_count) + bwd_blocks(h, 1, sm_count)) * dim;
+  // (no kernel has more than two blocks on an SM, and Q and K get one each at least)
+  return tokens > 0 ? ((int64_t)2 * sm_count + 2) * dim : 0;
 }
 
 cudaError_t norm_rotary_fwd(int dtype, bool interleaved, NormRotaryArgs a, int sm_count, cudaStream_t s) {
@@ -123,8 +153,8 @@ cudaError_t norm_rotary_bwd(int dtype, bool interleaved, NormRotaryArgs a, void*
   n.partial = a.partial;
   n.dw[0] = dwq;
   n.dw[1] = dwk;
-  n.count[0] = n.first[1] = bwd_blocks(a.heads, 0, sm_count);
-  n.count[1] = bwd_blocks(a.heads, 1, sm_count);
+  n.count[0] = n.first[1] = a.blocks_q;
+  n.count[1] = a.grid - a.blocks_q;
   n.dim = a.dim;
   n.w_f32 = a.w_f32;
   if (dtype == 0) return launch_weights<__nv_bfloat16>(n, s);

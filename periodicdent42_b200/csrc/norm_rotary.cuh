@@ -18,13 +18,15 @@
 
 #include <type_traits>
 
+#include "gemm_sm100.cuh"
+#include "bsattn_bwd_sm100.cuh"
 #include "rotary.cuh"
 
 namespace bsk {
 
 constexpr int kNormThreads = 256;
-constexpr int kNormBatch = 4;      // rows of a thread in flight, forward
-constexpr int kNormBatchBwd = 2;   // backward: rows of x and of dy
+constexpr int kNormBatch = 4;     // rows of a thread's step, forward
+constexpr int kNormBatchBwd = 2;  // backward: rows of x and of dy
 
 struct NormRotaryArgs {
   const void* x[2];                // Q, K (either may be absent: 0 heads)
@@ -44,9 +46,9 @@ struct NormRotaryArgs {
   float scale, eps;
   int aligned32;                   // every row starts at a multiple of 32 bytes
   int group, units;                // lanes and units of a row
-  int at_once[2], per_block[2];    // heads of a token side by side, tokens of a block (forward: [0], for Q and K together)
-  float* partial;                  // backward: [blocks of Q, then of K][dim]
-  int blocks_q;
+  int at_once[2], per_block[2];    // heads of a token side by side, tokens of a chunk
+  int grid, blocks_q;              // blocks, and those of them that take Q; the others take K
+  float* partial;                  // backward: [blocks][dim]
   uint32_t* err;
 };
 
@@ -54,41 +56,177 @@ struct NormRotaryArgs {
 template <int kVec, bool kInter>
 struct NormUnit {
   int e0, e1, pair;
-  bool turned, live, joined;  // joined: the two pieces are neighbours
+  bool turned, live;
   __device__ __forceinline__ NormUnit(int u, int units, int half) {
     live = u < units;
     pair = live ? u * kVec : 0;
     turned = live && pair < half;
-    joined = kInter || !turned;
+    const bool joined = kInter || !turned;
     e0 = joined ? 2 * pair : pair;
     e1 = joined ? e0 + kVec : pair + half;
   }
 };
 
+// Arithmetic on N floats, two at a time where N is even (one instruction for both).
+template <int N>
+__device__ __forceinline__ void v_mul(float (&d)[N], const float (&a)[N], const float (&b)[N]) {
+  if constexpr (N % 2 == 0) {
+#pragma unroll
+    for (int k = 0; k < N; k += 2) f2_unpack(f2_mul(f2_pack(a[k], a[k + 1]), f2_pack(b[k], b[k + 1])), d[k], d[k + 1]);
+  } else {
+#pragma unroll
+    for (int k = 0; k < N; ++k) d[k] = a[k] * b[k];
+  }
+}
+template <int N>
+__device__ __forceinline__ void v_scale(float (&d)[N], float c) {
+  if constexpr (N % 2 == 0) {
+#pragma unroll
+    for (int k = 0; k < N; k += 2) f2_unpack(f2_mul(f2_pack(d[k], d[k + 1]), f2_pack(c, c)), d[k], d[k + 1]);
+  } else {
+#pragma unroll
+    for (int k = 0; k < N; ++k) d[k] *= c;
+  }
+}
+// d = a b + c
+template <int N>
+__device__ __forceinline__ void v_fma(float (&d)[N], const float (&a)[N], const float (&b)[N], const float (&c)[N]) {
+  if constexpr (N % 2 == 0) {
+#pragma unroll
+    for (int k = 0; k < N; k += 2)
+      f2_unpack(f2_fma(f2_pack(a[k], a[k + 1]), f2_pack(b[k], b[k + 1]), f2_pack(c[k], c[k + 1])), d[k], d[k + 1]);
+  } else {
+#pragma unroll
+    for (int k = 0; k < N; ++k) d[k] = fmaf(a[k], b[k], c[k]);
+  }
+}
+// d = c - a b
+template <int N>
+__device__ __forceinline__ void v_nfma(float (&d)[N], const float (&a)[N], const float (&b)[N], const float (&c)[N]) {
+  float m[N];
+#pragma unroll
+  for (int k = 0; k < N; ++k) m[k] = -b[k];
+  v_fma(d, a, m, c);
+}
+// d = a c + b
+template <int N>
+__device__ __forceinline__ void v_axpy(float (&d)[N], const float (&a)[N], float c, const float (&b)[N]) {
+  if constexpr (N % 2 == 0) {
+#pragma unroll
+    for (int k = 0; k < N; k += 2)
+      f2_unpack(f2_fma(f2_pack(a[k], a[k + 1]), f2_pack(c, c), f2_pack(b[k], b[k + 1])), d[k], d[k + 1]);
+  } else {
+#pragma unroll
+    for (int k = 0; k < N; ++k) d[k] = fmaf(a[k], c, b[k]);
+  }
+}
+// A unit's elements, the pairs' first ones and second ones (of a part that is not turned: the even and the odd ones, or the
+// two pieces; it makes no difference there).
+template <int kVec>
+struct Halves {
+  float a[kVec], b[kVec];
+};
+
+template <int kVec>
+__device__ __forceinline__ float dot(const Halves<kVec>& x, const Halves<kVec>& y) {
+  float s;
+  if constexpr (kVec % 2 == 0) {
+    uint64_t sa = 0, sb = 0;
+#pragma unroll
+    for (int k = 0; k < kVec; k += 2) {
+      sa = f2_fma(f2_pack(x.a[k], x.a[k + 1]), f2_pack(y.a[k], y.a[k + 1]), sa);
+      sb = f2_fma(f2_pack(x.b[k], x.b[k + 1]), f2_pack(y.b[k], y.b[k + 1]), sb);
+    }
+    float lo, hi;
+    f2_unpack(f2_add(sa, sb), lo, hi);
+    s = lo + hi;
+  } else {
+    s = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kVec; ++k) s = fmaf(x.b[k], y.b[k], fmaf(x.a[k], y.a[k], s));
+  }
+  return s;
+}
+
+// Element k of the halves' a (b) is element `first` (`second`) of the unit's two pieces, one behind the other.
+template <int kVec, bool kInter>
+__device__ __forceinline__ constexpr int first_of(int k) { return kInter ? 2 * k : k; }
+template <int kVec, bool kInter>
+__device__ __forceinline__ constexpr int second_of(int k) { return kInter ? 2 * k + 1 : kVec + k; }
+
+template <class T, int kVec, bool kInter>
+__device__ __forceinline__ void unpack_pieces(const Pack<T, kVec>& p, const Pack<T, kVec>& q, Halves<kVec>& f) {
+#pragma unroll
+  for (int k = 0; k < kVec; ++k) {
+    constexpr int n = kVec;
+    const int i = first_of<kVec, kInter>(k), j = second_of<kVec, kInter>(k);
+    f.a[k] = to_f32<T>(i < n ? p.v[i % n] : q.v[i % n]);
+    f.b[k] = to_f32<T>(j < n ? p.v[j % n] : q.v[j % n]);
+  }
+}
+
+template <class T, int kVec, bool kInter>
+__device__ __forceinline__ void pack_pieces(const Halves<kVec>& f, Pack<T, kVec>& p, Pack<T, kVec>& q) {
+  float e[2 * kVec];
+#pragma unroll
+  for (int k = 0; k < kVec; ++k) {
+    e[first_of<kVec, kInter>(k)] = f.a[k];
+    e[second_of<kVec, kInter>(k)] = f.b[k];
+  }
+  if constexpr (sizeof(T) == 2 && kVec % 2 == 0) {
+    constexpr bool kF16 = std::is_same<T, __half>::value;
+    uint32_t w[kVec];
+#pragma unroll
+    for (int k = 0; k < kVec; ++k) w[k] = pack2<kF16>(e[2 * k], e[2 * k + 1]);
+    memcpy(&p, w, sizeof(p));
+    memcpy(&q, w + kVec / 2, sizeof(q));
+  } else {
+#pragma unroll
+    for (int k = 0; k < kVec; ++k) {
+      p.v[k] = from_f32<T>(e[k]);
+      q.v[k] = from_f32<T>(e[kVec + k]);
+    }
+  }
+}
+
+// Sines and cosines of a unit's pairs, times the scale.
+template <int kVec>
+struct Turn {
+  float c[kVec], s[kVec];
+};
+// dz = R^T dy
+template <int kVec>
+__device__ __forceinline__ void turn_back(Halves<kVec>& f, const Turn<kVec>& r) {
+  float u[kVec], w[kVec];
+  v_mul(u, f.b, r.s);
+  v_mul(w, f.b, r.c);
+  v_fma(u, f.a, r.c, u);
+  v_nfma(f.b, f.a, r.s, w);
+#pragma unroll
+  for (int k = 0; k < kVec; ++k) f.a[k] = u[k];
+}
+
+// A unit's two pieces: neighbours in the interleaved layout, one access where rows start at multiples of 32 bytes.
+template <bool kInter, class T, class P>
+__device__ __forceinline__ void store_pieces(T* y, int apart, int aligned32, const P& p, const P& q) {
+  if constexpr (kInter) {
+    store_pair(y, y + apart, aligned32 != 0, p, q);
+  } else {
+    *reinterpret_cast<P*>(y) = p;
+    *reinterpret_cast<P*>(y + apart) = q;
+  }
+}
+
+// Sum over a row's lanes; kLanes 0: `group` of them.
+template <int kLanes>
 __device__ __forceinline__ float group_sum(float v, int group) {
-  for (int o = group >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  if constexpr (kLanes > 0) {
+#pragma unroll
+    for (int o = kLanes / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  } else {
+    for (int o = group >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  }
   return v;
-}
-
-template <class T, int kVec>
-__device__ __forceinline__ void unpack_pieces(const Pack<T, kVec>& p, const Pack<T, kVec>& q, float (&f)[2 * kVec]) {
-#pragma unroll
-  for (int k = 0; k < kVec; ++k) {
-    f[k] = to_f32<T>(p.v[k]);
-    f[kVec + k] = to_f32<T>(q.v[k]);
-  }
-}
-
-// Turned pairs of a unit in place: (a, b) -> (a c - b s, a s + b c); kBack: the other way.
-template <int kVec, bool kInter, bool kBack>
-__device__ __forceinline__ void turn_pieces(float (&f)[2 * kVec], const float2 (&rot)[kVec]) {
-#pragma unroll
-  for (int k = 0; k < kVec; ++k) {
-    const int ia = kInter ? 2 * k : k, ib = kInter ? 2 * k + 1 : kVec + k;
-    const float va = f[ia], vb = f[ib], c = rot[k].x, s = kBack ? -rot[k].y : rot[k].y;
-    f[ia] = va * c - vb * s;
-    f[ib] = va * s + vb * c;
-  }
 }
 
 template <class T>
@@ -96,265 +234,431 @@ __device__ __forceinline__ float weight_at(const NormRotaryArgs& a, int w, int e
   return a.w_f32 ? __ldg(static_cast<const float*>(a.w[w]) + e) : to_f32<T>(static_cast<const T*>(a.w[w])[e]);
 }
 
-// (cos, sin) * scale of `count` tokens from t0 on: [token][pair].
-__device__ __forceinline__ void norm_angles(const NormRotaryArgs& a, int64_t t0, int count, float2* rot) {
+// Weights in shared memory as the lanes take them: 16 bytes of a unit (8 for kVec 1) beside those of the next, so that the
+// lanes of a row read neighbouring ones.
+template <int kVec>
+struct WeightChunk {
+  static constexpr int kFloats = kVec == 1 ? 2 : 4, kChunks = 2 * kVec / kFloats;
+  using V = typename std::conditional<kVec == 1, float2, float4>::type;
+};
+template <class T, int kVec, bool kInter>
+__device__ __forceinline__ void stage_weights(const NormRotaryArgs& a, int w, float* dst) {
+  using C = WeightChunk<kVec>;
   const int half = a.rotary_dim / 2;
-  for (int i = threadIdx.x; i < count * half; i += kNormThreads) {
-    const int it = i / half, pair = i - it * half;
+  for (int i = threadIdx.x; i < a.dim; i += kNormThreads) {
+    const int x = i % C::kFloats, u = i / C::kFloats % a.units, c = i / C::kFloats / a.units;
+    const int at = c * C::kFloats + x;  // of the unit's halves: a, then b
+    const NormUnit<kVec, kInter> unit(u, a.units, half);
+    const int e = at < kVec ? first_of<kVec, kInter>(at) : second_of<kVec, kInter>(at - kVec);
+    dst[i] = weight_at<T>(a, w, e < kVec ? unit.e0 + e : unit.e1 + e - kVec);
+  }
+}
+template <int kVec>
+__device__ __forceinline__ void read_weights(const float* src, int unit, int units, Halves<kVec>& f) {
+  using C = WeightChunk<kVec>;
+  float v[2 * kVec];
+#pragma unroll
+  for (int c = 0; c < C::kChunks; ++c) {
+    const typename C::V x = reinterpret_cast<const typename C::V*>(src)[c * units + unit];
+    memcpy(v + c * C::kFloats, &x, sizeof(x));
+  }
+#pragma unroll
+  for (int k = 0; k < kVec; ++k) {
+    f.a[k] = v[k];
+    f.b[k] = v[kVec + k];
+  }
+}
+
+// (cos, sin) * scale of `count` tokens from t0 on: [token][pair]. Element threadIdx.x is pair `pair0` of token `it0`.
+__device__ __forceinline__ void norm_angles(const NormRotaryArgs& a, int64_t t0, int count, int it0, int pair0, float2* rot) {
+  const int half = a.rotary_dim / 2, tokens = kNormThreads / half, pairs = kNormThreads % half;
+  for (int it = it0, pair = pair0, i = threadIdx.x; it < count; i += kNormThreads) {
     const int64_t at = position_of(a.positions, a.positions64, a.axes, a.num_axes, a.tokens, t0 + it, pair, a.err);
     float s, c;
     sincospif(2.0f * static_cast<float>(turn_fraction(at, a.inv_freq[pair])), &s, &c);
     rot[i] = make_float2(c * a.scale, s * a.scale);
+    it += tokens;
+    pair += pairs;
+    if (pair >= half) {
+      pair -= half;
+      ++it;
+    }
   }
 }
 
-// Rows whose squares pass fp32's range are scaled down by this first.
+// A row whose squares pass fp32's range is multiplied by this first.
 constexpr float kNormDown = 0x1p-100f;
 
-// kUnits units per lane: units group * p + lane for p < kUnits.
-template <class T, int kVec, int kUnits, bool kInter>
-__global__ void __launch_bounds__(kNormThreads) norm_rotary_kernel(const __grid_constant__ NormRotaryArgs a) {
-  extern __shared__ float2 rot_s[];
-  using P = Pack<T, kVec>;
-  using Unit = NormUnit<kVec, kInter>;
-  const int half = a.rotary_dim / 2;
-  const int64_t t0 = static_cast<int64_t>(blockIdx.x) * a.per_block[0];
-  const int nt = static_cast<int>(min(static_cast<int64_t>(a.per_block[0]), a.tokens - t0));
-  const int lane = threadIdx.x & (a.group - 1), g = threadIdx.x / a.group;
-  const int at_once = a.at_once[0], it = g / at_once, h0 = g - it * at_once;
-  const int all_heads = a.heads[0] + a.heads[1];
-  const int rows = it < nt ? all_heads : 0;
-  P p[kNormBatch][kUnits], q[kNormBatch][kUnits];
-  auto load = [&](int first) {
-#pragma unroll
-    for (int b = 0; b < kNormBatch; ++b) {
-      const int row = first + b * at_once;
-      const int w = row >= a.heads[0], h = w ? row - a.heads[0] : row;
-      const T* x = static_cast<const T*>(a.x[w]) + (t0 + it) * a.token_stride[w] + h * a.head_stride[w];
-#pragma unroll
-      for (int n = 0; n < kUnits; ++n) {
-        const Unit u(a.group * n + lane, a.units, half);
-        if (row < rows && u.live) {
-          load_pair(x + u.e0, x + u.e1, a.aligned32 && u.joined, p[b][n], q[b][n]);
-        } else {
-          p[b][n] = P{};
-          q[b][n] = P{};
-        }
-      }
-    }
-  };
-  load(h0);
-  norm_angles(a, t0, nt, rot_s);
-  __syncthreads();
-  float2 rot[kUnits][kVec];
-  float weight[2][kUnits][2 * kVec];
+template <int kVec, int kUnits, bool kInter>
+__device__ __forceinline__ void read_turns(const NormRotaryArgs& a, const float2* rot, int group, int lane, bool any,
+                                           Turn<kVec> (&t)[kUnits]) {
 #pragma unroll
   for (int n = 0; n < kUnits; ++n) {
-    const Unit u(a.group * n + lane, a.units, half);
+    const NormUnit<kVec, kInter> u(group * n + lane, a.units, a.rotary_dim / 2);
 #pragma unroll
-    for (int k = 0; k < kVec; ++k) rot[n][k] = u.turned && rows ? rot_s[it * half + u.pair + k] : make_float2(1.0f, 0.0f);
-#pragma unroll
-    for (int w = 0; w < 2; ++w)
-#pragma unroll
-      for (int k = 0; k < kVec; ++k) {
-        weight[w][n][k] = a.heads[w] && u.live ? weight_at<T>(a, w, u.e0 + k) : 0.0f;
-        weight[w][n][kVec + k] = a.heads[w] && u.live ? weight_at<T>(a, w, u.e1 + k) : 0.0f;
-      }
-  }
-  const float inv_dim = 1.0f / static_cast<float>(a.dim);
-  // (every lane of a warp takes part in every sum: the loop's length is the same for all)
-  const int rounds = (all_heads + kNormBatch * at_once - 1) / (kNormBatch * at_once);
-  for (int round = 0; round < rounds; ++round) {
-    const int first = h0 + round * kNormBatch * at_once;
-    if (round) load(first);
-#pragma unroll
-    for (int b = 0; b < kNormBatch; ++b) {
-      const int row = first + b * at_once;
-      const int w = row >= a.heads[0], h = w ? row - a.heads[0] : row;
-      float f[kUnits][2 * kVec], ss = 0.0f;
-#pragma unroll
-      for (int n = 0; n < kUnits; ++n) {
-        unpack_pieces<T, kVec>(p[b][n], q[b][n], f[n]);
-#pragma unroll
-        for (int k = 0; k < 2 * kVec; ++k) ss = fmaf(f[n][k], f[n][k], ss);
-      }
-      ss = group_sum(ss, a.group);
-      float eps = a.eps;
-      if constexpr (sizeof(T) != 2 || !std::is_same<T, __half>::value) {
-        const bool far = !(ss <= 3.0e38f);
-        if (__any_sync(0xffffffffu, far)) {
-          const float down = far ? kNormDown : 1.0f;
-          ss = 0.0f;
-#pragma unroll
-          for (int n = 0; n < kUnits; ++n)
-#pragma unroll
-            for (int k = 0; k < 2 * kVec; ++k) {
-              f[n][k] *= down;
-              ss = fmaf(f[n][k], f[n][k], ss);
-            }
-          ss = group_sum(ss, a.group);
-          if (far) eps = 0.0f;
-        }
-      }
-      const float inv = rsqrtf(fmaf(ss, inv_dim, eps));
-      if (row >= rows) continue;
-      T* y = static_cast<T*>(a.y[w]) + ((t0 + it) * a.heads[w] + h) * a.dim;
-#pragma unroll
-      for (int n = 0; n < kUnits; ++n) {
-        const Unit u(a.group * n + lane, a.units, half);
-        if (!u.live) continue;
-#pragma unroll
-        for (int k = 0; k < 2 * kVec; ++k) f[n][k] *= inv * (w ? weight[1][n][k] : weight[0][n][k]);
-        if (u.turned) turn_pieces<kVec, kInter, false>(f[n], rot[n]);
-        P po, qo;
-#pragma unroll
-        for (int k = 0; k < kVec; ++k) {
-          po.v[k] = from_f32<T>(f[n][k]);
-          qo.v[k] = from_f32<T>(f[n][kVec + k]);
-        }
-        store_pair(y + u.e0, y + u.e1, a.aligned32 && u.joined, po, qo);
-      }
+    for (int k = 0; k < kVec; ++k) {
+      const float2 r = u.turned && any ? rot[u.pair + k] : make_float2(1.0f, 0.0f);
+      t[n].c[k] = r.x;
+      t[n].s[k] = r.y;
     }
   }
 }
 
-template <class T, int kVec, int kUnits, bool kInter>
-__global__ void __launch_bounds__(kNormThreads) norm_rotary_bwd_kernel(const __grid_constant__ NormRotaryArgs a) {
-  extern __shared__ float2 rot_s[];  // (cos, sin) of a chunk's tokens; at the end the groups' sums of dw
-  ptx::grid_launch_dependents();
-  using P = Pack<T, kVec>;
-  using Unit = NormUnit<kVec, kInter>;
-  const int half = a.rotary_dim / 2;
-  const int w = static_cast<int>(blockIdx.x) >= a.blocks_q;
-  const int block = w ? blockIdx.x - a.blocks_q : blockIdx.x, blocks = w ? gridDim.x - a.blocks_q : a.blocks_q;
-  const int heads = a.heads[w];
-  const int lane = threadIdx.x & (a.group - 1), g = threadIdx.x / a.group, groups = kNormThreads / a.group;
-  const int at_once = a.at_once[w], tokens_per_block = a.per_block[w];
-  const int it = g / at_once, h0 = g - it * at_once;
-  const T* xs = static_cast<const T*>(a.x[w]);
-  const T* dys = static_cast<const T*>(a.dy[w]);
-  float weight[kUnits][2 * kVec], dw[kUnits][2 * kVec];
-#pragma unroll
-  for (int n = 0; n < kUnits; ++n) {
-    const Unit u(a.group * n + lane, a.units, half);
-#pragma unroll
-    for (int k = 0; k < kVec; ++k) {
-      weight[n][k] = u.live ? weight_at<T>(a, w, u.e0 + k) : 0.0f;
-      weight[n][kVec + k] = u.live ? weight_at<T>(a, w, u.e1 + k) : 0.0f;
-      dw[n][k] = dw[n][kVec + k] = 0.0f;
+// A thread's rows on their way: rings of kStages steps in shared memory, each of kPieces pieces of a thread's own, [step][piece]
+// [thread], so that nobody waits for another thread's. Pieces of 4 bytes and more are copied asynchronously.
+template <class P, int kPieces>
+struct NormRing {
+  static constexpr int kStepBytes = kPieces * kNormThreads * (int)sizeof(P);
+  static constexpr int kStages = kStepBytes <= 32768 ? 3 : 2;
+  static constexpr int kBytes = kStages * kStepBytes;
+  static constexpr bool kAsync = sizeof(P) >= 4;
+  static __device__ __forceinline__ uint8_t* at(uint8_t* ring, int stage, int piece) {
+    return ring + stage * kStepBytes + (piece * kNormThreads + threadIdx.x) * sizeof(P);
+  }
+  static __device__ __forceinline__ void fetch(uint8_t* dst, const void* src, bool live) {
+    if constexpr (kAsync) {
+      const uint32_t n = live ? sizeof(P) : 0u;  // 0: zeros, src is not read
+      if constexpr (sizeof(P) == 16)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(ptx::smem_u32(dst)), "l"(src), "r"(n) : "memory");
+      else
+        asm volatile("cp.async.ca.shared.global [%0], [%1], %3, %2;" ::"r"(ptx::smem_u32(dst)), "l"(src), "r"(n), "n"(sizeof(P)) : "memory");
+    } else {
+      *reinterpret_cast<P*>(dst) = live ? *static_cast<const P*>(src) : P{};
     }
   }
-  const float inv_dim = 1.0f / static_cast<float>(a.dim);
-  const int rounds = (heads + kNormBatchBwd * at_once - 1) / (kNormBatchBwd * at_once);
-  const int64_t chunks = (static_cast<int64_t>(a.tokens) + tokens_per_block - 1) / tokens_per_block;
-  for (int64_t chunk = block; chunk < chunks; chunk += blocks) {
-    const int64_t t0 = chunk * tokens_per_block, t = t0 + it;
-    const int nt = static_cast<int>(min(static_cast<int64_t>(tokens_per_block), a.tokens - t0));
-    const int rows = it < nt ? heads : 0;
-    P xp[kNormBatchBwd][kUnits], xq[kNormBatchBwd][kUnits], dp[kNormBatchBwd][kUnits], dq[kNormBatchBwd][kUnits];
-    auto load = [&](int first) {
+  static __device__ __forceinline__ void commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+  static __device__ __forceinline__ void wait() { asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory"); }
+};
+
+// Chunks of per_block tokens are walked with a stride of the blocks, a chunk's heads in rounds of kRows rows a thread; a step is a
+// round of a chunk. Where this thread's next step to be fetched, or to be worked on, stands.
+struct NormStep {
+  int64_t chunk;
+  int round, stage;
+  __device__ __forceinline__ void next(int rounds, int64_t blocks, int stages) {
+    if (++round == rounds) {
+      round = 0;
+      chunk += blocks;
+    }
+    if (++stage == stages) stage = 0;
+  }
+};
+
+// kUnits units per lane: units group * p + lane for p < kUnits. kLanes: the group's width, 0 where it is known at run time only.
+template <class T, int kVec, int kUnits, bool kBackward>
+struct NormShape {
+  using P = Pack<T, kVec>;
+  static constexpr int kRows = kBackward ? kNormBatchBwd : kNormBatch;
+  static constexpr int kTensors = kBackward ? 2 : 1;
+  using Ring = NormRing<P, kRows * kUnits * 2 * kTensors>;
+  static constexpr int kBlocksPerSm = kVec * sizeof(T) == 16 && kUnits == 1 ? 2 : 1;  // by registers and shared memory
+  static constexpr int kMostSmem = Ring::kBytes + 20 * 1024;
+  // the ring (at the end the groups' sums of dw), a chunk's angles, the weights
+  static __host__ __device__ int weights_at(const NormRotaryArgs& a) {
+    const int per_block = a.per_block[0] > a.per_block[1] ? a.per_block[0] : a.per_block[1];
+    const int loop = Ring::kBytes + per_block * (a.rotary_dim / 2) * (int)sizeof(float2);
+    const int sums = kBackward ? kNormThreads / a.group * a.dim * (int)sizeof(float) : 0;
+    return ((loop > sums ? loop : sums) + 15) / 16 * 16;
+  }
+  static int smem_bytes(const NormRotaryArgs& a) { return weights_at(a) + a.dim * (int)sizeof(float); }
+};
+
+// Blocks [0, blocks_q) take Q, the others K, each with the tokens blocks * per_block apart.
+struct NormBlock {
+  int w, heads, at_once, per_block, it, h0, rounds;
+  int64_t first, blocks, chunks;
+  __device__ __forceinline__ NormBlock(const NormRotaryArgs& a, int g, int rows_a_step) {
+    w = static_cast<int>(blockIdx.x) >= a.blocks_q;
+    first = w ? blockIdx.x - a.blocks_q : blockIdx.x;
+    blocks = w ? gridDim.x - a.blocks_q : a.blocks_q;
+    heads = a.heads[w];
+    at_once = a.at_once[w];
+    per_block = a.per_block[w];
+    it = g / at_once;
+    h0 = g - it * at_once;
+    rounds = (heads + rows_a_step * at_once - 1) / (rows_a_step * at_once);
+    chunks = (static_cast<int64_t>(a.tokens) + per_block - 1) / per_block;
+  }
+  // heads of this thread's token of a chunk, 0 where it has none
+  __device__ __forceinline__ int rows(const NormRotaryArgs& a, int64_t chunk) const {
+    return it < per_block && chunk * per_block + it < a.tokens ? heads : 0;
+  }
+};
+
+template <class T, int kVec, int kUnits, bool kInter, int kLanes>
+__global__ void __launch_bounds__(kNormThreads, NormShape<T, kVec, kUnits, false>::kBlocksPerSm)
+    norm_rotary_kernel(const __grid_constant__ NormRotaryArgs a) {
+  extern __shared__ float4 norm_smem[];
+  using P = Pack<T, kVec>;
+  using Sh = NormShape<T, kVec, kUnits, false>;
+  using Ring = typename Sh::Ring;
+  using Unit = NormUnit<kVec, kInter>;
+  uint8_t* ring = reinterpret_cast<uint8_t*>(norm_smem);
+  float2* rot = reinterpret_cast<float2*>(ring + Ring::kBytes);  // [tokens][pairs]
+  float* w_s = reinterpret_cast<float*>(ring + Sh::weights_at(a));
+  const int half = a.rotary_dim / 2, group = kLanes > 0 ? kLanes : a.group;
+  const int lane = threadIdx.x & (group - 1);
+  const NormBlock blk(a, threadIdx.x / group, kNormBatch);
+  const int w = blk.w;
+  const T* xs = static_cast<const T*>(a.x[w]);
+  const int64_t x_step = blk.at_once * a.head_stride[w], y_step = static_cast<int64_t>(blk.at_once) * a.dim;
+  NormStep ahead{blk.first, 0, 0};
+  auto fetch = [&]() {
+    if (ahead.chunk < blk.chunks) {
+      const int rows = blk.rows(a, ahead.chunk), h = blk.h0 + ahead.round * kNormBatch * blk.at_once;
+      const T* x0 = xs + (ahead.chunk * blk.per_block + blk.it) * a.token_stride[w] + h * a.head_stride[w];
 #pragma unroll
-      for (int b = 0; b < kNormBatchBwd; ++b) {
-        const int h = first + b * at_once;
-        const T* x = xs + t * a.token_stride[w] + h * a.head_stride[w];
-        const T* dy = dys + t * a.dy_token_stride[w] + h * a.dy_head_stride[w];
+      for (int n = 0; n < kUnits; ++n) {
+        const Unit u(group * n + lane, a.units, half);
+        const T* x = x0 + u.e0;  // (not read where the row or the unit is not there)
 #pragma unroll
-        for (int n = 0; n < kUnits; ++n) {
-          const Unit u(a.group * n + lane, a.units, half);
-          if (h < rows && u.live) {
-            load_pair(x + u.e0, x + u.e1, a.aligned32 && u.joined, xp[b][n], xq[b][n]);
-            load_pair(dy + u.e0, dy + u.e1, a.aligned32 && u.joined, dp[b][n], dq[b][n]);
-          } else {
-            xp[b][n] = xq[b][n] = dp[b][n] = dq[b][n] = P{};
-          }
+        for (int b = 0; b < kNormBatch; ++b, x += x_step) {
+          const bool live = h + b * blk.at_once < rows && u.live;
+          Ring::fetch(Ring::at(ring, ahead.stage, (b * kUnits + n) * 2), x, live);
+          Ring::fetch(Ring::at(ring, ahead.stage, (b * kUnits + n) * 2 + 1), x + (u.e1 - u.e0), live);
         }
       }
-    };
-    load(h0);
+    }
+    Ring::commit();
+    ahead.next(blk.rounds, blk.blocks, Ring::kStages);
+  };
+#pragma unroll
+  for (int i = 0; i < Ring::kStages - 1; ++i) fetch();
+  stage_weights<T, kVec, kInter>(a, w, w_s);
+  const float inv_dim = 1.0f / static_cast<float>(a.dim);
+  const int it0 = threadIdx.x / half, pair0 = threadIdx.x % half;
+  NormStep now{blk.first, 0, 0};
+  while (now.chunk < blk.chunks) {
+    const int64_t t0 = now.chunk * blk.per_block, t = t0 + blk.it;
+    const int rows = blk.rows(a, now.chunk);
     __syncthreads();  // the chunk before has read its angles
-    norm_angles(a, t0, nt, rot_s);
+    norm_angles(a, t0, static_cast<int>(min(static_cast<int64_t>(blk.per_block), a.tokens - t0)), it0, pair0, rot);
     __syncthreads();
-    float2 rot[kUnits][kVec];
+    // Turn and weights in one: (a, b) -> (a ac - b bs, a as + b bc)
+    Turn<kVec> ca[kUnits], cb[kUnits];
+    read_turns<kVec, kUnits, kInter>(a, rot + blk.it * half, group, lane, rows > 0, ca);
 #pragma unroll
     for (int n = 0; n < kUnits; ++n) {
-      const Unit u(a.group * n + lane, a.units, half);
-#pragma unroll
-      for (int k = 0; k < kVec; ++k) rot[n][k] = u.turned && rows ? rot_s[it * half + u.pair + k] : make_float2(1.0f, 0.0f);
+      Halves<kVec> weight;
+      const Unit u(group * n + lane, a.units, half);
+      read_weights<kVec>(w_s, u.live ? group * n + lane : 0, a.units, weight);
+      v_mul(cb[n].c, ca[n].c, weight.b);
+      v_mul(cb[n].s, ca[n].s, weight.b);
+      v_mul(ca[n].c, ca[n].c, weight.a);
+      v_mul(ca[n].s, ca[n].s, weight.a);
     }
-    for (int round = 0; round < rounds; ++round) {
-      const int first = h0 + round * kNormBatchBwd * at_once;
-      if (round) load(first);
+    // (every lane of a warp takes part in every sum: the loop's length is the same for all)
+    for (int round = 0; round < blk.rounds; ++round) {
+      fetch();
+      Ring::wait();
+      const int h = blk.h0 + round * kNormBatch * blk.at_once;
+      T* y = static_cast<T*>(a.y[w]) + (t * blk.heads + h) * a.dim;
 #pragma unroll
-      for (int b = 0; b < kNormBatchBwd; ++b) {
-        const int h = first + b * at_once;
-        float x[kUnits][2 * kVec], dz[kUnits][2 * kVec], ss = 0.0f, dot = 0.0f;
+      for (int b = 0; b < kNormBatch; ++b, y += y_step) {
+        Halves<kVec> f[kUnits];
+        float ss = 0.0f, eps = a.eps;
 #pragma unroll
         for (int n = 0; n < kUnits; ++n) {
-          const Unit u(a.group * n + lane, a.units, half);
-          unpack_pieces<T, kVec>(xp[b][n], xq[b][n], x[n]);
-          unpack_pieces<T, kVec>(dp[b][n], dq[b][n], dz[n]);
-          if (u.turned) turn_pieces<kVec, kInter, true>(dz[n], rot[n]);
-#pragma unroll
-          for (int k = 0; k < 2 * kVec; ++k) ss = fmaf(x[n][k], x[n][k], ss);
+          unpack_pieces<T, kVec, kInter>(*reinterpret_cast<const P*>(Ring::at(ring, now.stage, (b * kUnits + n) * 2)),
+                                         *reinterpret_cast<const P*>(Ring::at(ring, now.stage, (b * kUnits + n) * 2 + 1)), f[n]);
+          ss += dot(f[n], f[n]);
         }
-        ss = group_sum(ss, a.group);
-        float eps = a.eps, down = 1.0f;
-        if constexpr (sizeof(T) != 2 || !std::is_same<T, __half>::value) {
+        ss = group_sum<kLanes>(ss, group);
+        if constexpr (!std::is_same<T, __half>::value) {
           const bool far = !(ss <= 3.0e38f);
           if (__any_sync(0xffffffffu, far)) {
-            down = far ? kNormDown : 1.0f;
+            if (far) eps = 0.0f;
             ss = 0.0f;
 #pragma unroll
-            for (int n = 0; n < kUnits; ++n)
-#pragma unroll
-              for (int k = 0; k < 2 * kVec; ++k) {
-                x[n][k] *= down;
-                ss = fmaf(x[n][k], x[n][k], ss);
-              }
-            ss = group_sum(ss, a.group);
-            if (far) eps = 0.0f;
+            for (int n = 0; n < kUnits; ++n) {
+              v_scale(f[n].a, far ? kNormDown : 1.0f);
+              v_scale(f[n].b, far ? kNormDown : 1.0f);
+              ss += dot(f[n], f[n]);
+            }
+            ss = group_sum<kLanes>(ss, group);
           }
         }
         const float inv = rsqrtf(fmaf(ss, inv_dim, eps));
-#pragma unroll
-        for (int n = 0; n < kUnits; ++n)
-#pragma unroll
-          for (int k = 0; k < 2 * kVec; ++k) {
-            x[n][k] *= inv;  // xhat
-            dw[n][k] = fmaf(dz[n][k], x[n][k], dw[n][k]);
-            dz[n][k] *= weight[n][k];  // g
-            dot = fmaf(dz[n][k], x[n][k], dot);
-          }
-        dot = group_sum(dot, a.group) * inv_dim;
-        if (h >= rows) continue;
-        T* y = static_cast<T*>(a.y[w]) + (t * heads + h) * a.dim;
-        const float out = inv * down;
+        if (h + b * blk.at_once >= rows) continue;
 #pragma unroll
         for (int n = 0; n < kUnits; ++n) {
-          const Unit u(a.group * n + lane, a.units, half);
+          const Unit u(group * n + lane, a.units, half);
           if (!u.live) continue;
-          P po, qo;
-#pragma unroll
-          for (int k = 0; k < kVec; ++k) {
-            po.v[k] = from_f32<T>((dz[n][k] - x[n][k] * dot) * out);
-            qo.v[k] = from_f32<T>((dz[n][kVec + k] - x[n][kVec + k] * dot) * out);
+          Halves<kVec> y_f;
+          v_mul(y_f.a, f[n].a, ca[n].c);
+          v_mul(y_f.b, f[n].b, cb[n].c);
+          if (u.turned) {
+            v_nfma(y_f.a, f[n].b, cb[n].s, y_f.a);
+            v_fma(y_f.b, f[n].a, ca[n].s, y_f.b);
           }
-          store_pair(y + u.e0, y + u.e1, a.aligned32 && u.joined, po, qo);
+          v_scale(y_f.a, inv);
+          v_scale(y_f.b, inv);
+          P po, qo;
+          pack_pieces<T, kVec, kInter>(y_f, po, qo);
+          store_pieces<kInter>(y + u.e0, u.e1 - u.e0, a.aligned32, po, qo);
+        }
+      }
+      now.next(blk.rounds, blk.blocks, Ring::kStages);
+    }
+  }
+  asm volatile("cp.async.wait_all;" ::: "memory");
+}
+
+template <class T, int kVec, int kUnits, bool kInter, int kLanes>
+__global__ void __launch_bounds__(kNormThreads, NormShape<T, kVec, kUnits, true>::kBlocksPerSm)
+    norm_rotary_bwd_kernel(const __grid_constant__ NormRotaryArgs a) {
+  extern __shared__ float4 norm_smem[];
+  ptx::grid_launch_dependents();
+  using P = Pack<T, kVec>;
+  using Sh = NormShape<T, kVec, kUnits, true>;
+  using Ring = typename Sh::Ring;
+  using Unit = NormUnit<kVec, kInter>;
+  uint8_t* ring = reinterpret_cast<uint8_t*>(norm_smem);
+  float2* rot = reinterpret_cast<float2*>(ring + Ring::kBytes);  // [tokens][pairs]
+  float* w_s = reinterpret_cast<float*>(ring + Sh::weights_at(a));
+  const int half = a.rotary_dim / 2, group = kLanes > 0 ? kLanes : a.group;
+  const int lane = threadIdx.x & (group - 1), g = threadIdx.x / group, groups = kNormThreads / group;
+  const NormBlock blk(a, g, kNormBatchBwd);
+  const int w = blk.w;
+  const T* xs = static_cast<const T*>(a.x[w]);
+  const T* dys = static_cast<const T*>(a.dy[w]);
+  const int64_t x_step = blk.at_once * a.head_stride[w], dy_step = blk.at_once * a.dy_head_stride[w],
+                y_step = static_cast<int64_t>(blk.at_once) * a.dim;
+  NormStep ahead{blk.first, 0, 0};
+  auto fetch = [&]() {
+    if (ahead.chunk < blk.chunks) {
+      const int rows = blk.rows(a, ahead.chunk), h = blk.h0 + ahead.round * kNormBatchBwd * blk.at_once;
+      const int64_t t = ahead.chunk * blk.per_block + blk.it;
+      const T* x0 = xs + t * a.token_stride[w] + h * a.head_stride[w];
+      const T* dy0 = dys + t * a.dy_token_stride[w] + h * a.dy_head_stride[w];
+#pragma unroll
+      for (int n = 0; n < kUnits; ++n) {
+        const Unit u(group * n + lane, a.units, half);
+        const T* x = x0 + u.e0;  // (not read where the row or the unit is not there)
+        const T* dy = dy0 + u.e0;
+#pragma unroll
+        for (int b = 0; b < kNormBatchBwd; ++b, x += x_step, dy += dy_step) {
+          const bool live = h + b * blk.at_once < rows && u.live;
+          const int piece = (b * kUnits + n) * 4;
+          Ring::fetch(Ring::at(ring, ahead.stage, piece), x, live);
+          Ring::fetch(Ring::at(ring, ahead.stage, piece + 1), x + (u.e1 - u.e0), live);
+          Ring::fetch(Ring::at(ring, ahead.stage, piece + 2), dy, live);
+          Ring::fetch(Ring::at(ring, ahead.stage, piece + 3), dy + (u.e1 - u.e0), live);
         }
       }
     }
+    Ring::commit();
+    ahead.next(blk.rounds, blk.blocks, Ring::kStages);
+  };
+#pragma unroll
+  for (int i = 0; i < Ring::kStages - 1; ++i) fetch();
+  stage_weights<T, kVec, kInter>(a, w, w_s);
+  Halves<kVec> dw[kUnits];
+#pragma unroll
+  for (int n = 0; n < kUnits; ++n)
+#pragma unroll
+    for (int k = 0; k < kVec; ++k) dw[n].a[k] = dw[n].b[k] = 0.0f;
+  const float inv_dim = 1.0f / static_cast<float>(a.dim);
+  const int it0 = threadIdx.x / half, pair0 = threadIdx.x % half;
+  NormStep now{blk.first, 0, 0};
+  while (now.chunk < blk.chunks) {
+    const int64_t t0 = now.chunk * blk.per_block, t = t0 + blk.it;
+    const int rows = blk.rows(a, now.chunk);
+    __syncthreads();  // the chunk before has read its angles
+    norm_angles(a, t0, static_cast<int>(min(static_cast<int64_t>(blk.per_block), a.tokens - t0)), it0, pair0, rot);
+    __syncthreads();
+    Turn<kVec> turn[kUnits];
+    read_turns<kVec, kUnits, kInter>(a, rot + blk.it * half, group, lane, rows > 0, turn);
+    for (int round = 0; round < blk.rounds; ++round) {
+      fetch();
+      Ring::wait();
+      const int h = blk.h0 + round * kNormBatchBwd * blk.at_once;
+      T* y = static_cast<T*>(a.y[w]) + (t * blk.heads + h) * a.dim;
+#pragma unroll
+      for (int b = 0; b < kNormBatchBwd; ++b, y += y_step) {
+        // dx = (g - x (sum(g x) / (dim rms^2))) / rms: both sums of a row at once
+        Halves<kVec> x[kUnits], dz[kUnits];
+        float ss = 0.0f, gx = 0.0f, eps = a.eps, down = 1.0f;
+        auto sums = [&]() {
+          ss = gx = 0.0f;
+#pragma unroll
+          for (int n = 0; n < kUnits; ++n) {
+            Halves<kVec> p, weight;
+            read_weights<kVec>(w_s, min(group * n + lane, a.units - 1), a.units, weight);
+            v_mul(p.a, dz[n].a, x[n].a);
+            v_mul(p.b, dz[n].b, x[n].b);
+            ss += dot(x[n], x[n]);
+            gx += dot(p, weight);
+          }
+          ss = group_sum<kLanes>(ss, group);
+          gx = group_sum<kLanes>(gx, group);
+        };
+#pragma unroll
+        for (int n = 0; n < kUnits; ++n) {
+          const Unit u(group * n + lane, a.units, half);
+          const int piece = (b * kUnits + n) * 4;
+          unpack_pieces<T, kVec, kInter>(*reinterpret_cast<const P*>(Ring::at(ring, now.stage, piece)),
+                                         *reinterpret_cast<const P*>(Ring::at(ring, now.stage, piece + 1)), x[n]);
+          unpack_pieces<T, kVec, kInter>(*reinterpret_cast<const P*>(Ring::at(ring, now.stage, piece + 2)),
+                                         *reinterpret_cast<const P*>(Ring::at(ring, now.stage, piece + 3)), dz[n]);
+          if (u.turned) turn_back<kVec>(dz[n], turn[n]);
+        }
+        sums();
+        if constexpr (!std::is_same<T, __half>::value) {
+          const bool far = !(ss <= 3.0e38f);
+          if (__any_sync(0xffffffffu, far)) {
+            if (far) {
+              down = kNormDown;
+              eps = 0.0f;
+            }
+#pragma unroll
+            for (int n = 0; n < kUnits; ++n) {
+              v_scale(x[n].a, down);
+              v_scale(x[n].b, down);
+            }
+            sums();
+          }
+        }
+        const float inv = rsqrtf(fmaf(ss, inv_dim, eps));
+        const float mean = gx * inv_dim * inv * inv, out = inv * down;
+        const bool live_row = h + b * blk.at_once < rows;
+#pragma unroll
+        for (int n = 0; n < kUnits; ++n) {
+          const Unit u(group * n + lane, a.units, half);
+          Halves<kVec> g_f, weight;
+          v_mul(g_f.a, dz[n].a, x[n].a);
+          v_mul(g_f.b, dz[n].b, x[n].b);
+          v_axpy(dw[n].a, g_f.a, inv, dw[n].a);
+          v_axpy(dw[n].b, g_f.b, inv, dw[n].b);
+          if (!live_row || !u.live) continue;
+          read_weights<kVec>(w_s, group * n + lane, a.units, weight);
+          v_mul(g_f.a, dz[n].a, weight.a);
+          v_mul(g_f.b, dz[n].b, weight.b);
+          v_axpy(g_f.a, x[n].a, -mean, g_f.a);
+          v_axpy(g_f.b, x[n].b, -mean, g_f.b);
+          v_scale(g_f.a, out);
+          v_scale(g_f.b, out);
+          P po, qo;
+          pack_pieces<T, kVec, kInter>(g_f, po, qo);
+          store_pieces<kInter>(y + u.e0, u.e1 - u.e0, a.aligned32, po, qo);
+        }
+      }
+      now.next(blk.rounds, blk.blocks, Ring::kStages);
+    }
   }
+  asm volatile("cp.async.wait_all;" ::: "memory");
   // the groups' sums, added in order
-  float* sums = reinterpret_cast<float*>(rot_s);
+  float* sums = reinterpret_cast<float*>(ring);
   __syncthreads();
 #pragma unroll
   for (int n = 0; n < kUnits; ++n) {
-    const Unit u(a.group * n + lane, a.units, half);
+    const Unit u(group * n + lane, a.units, half);
     if (!u.live) continue;
 #pragma unroll
     for (int k = 0; k < kVec; ++k) {
-      sums[g * a.dim + u.e0 + k] = dw[n][k];
-      sums[g * a.dim + u.e1 + k] = dw[n][kVec + k];
+      const int i = first_of<kVec, kInter>(k), j = second_of<kVec, kInter>(k);
+      sums[g * a.dim + (i < kVec ? u.e0 + i : u.e1 + i - kVec)] = dw[n].a[k];
+      sums[g * a.dim + (j < kVec ? u.e0 + j : u.e1 + j - kVec)] = dw[n].b[k];
     }
   }
   __syncthreads();

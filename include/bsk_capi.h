@@ -490,8 +490,9 @@ int bsk_attention_varlen_bwd(int dtype, const void* dO, int64_t do_token_stride,
 
 /*
  * The same attention with a sliding window (causal): a row at position p sees the keys at positions p - window + 1 .. p
- * and the first `sinks` ones (0 .. sinks - 1, up to p). window >= 1, sinks >= 0; otherwise as the functions above, their
- * workspaces included. The work is that of the keys that are seen: key blocks that no row of a tile sees are not read. Over a
+ * and the first `sinks` ones (0 .. sinks - 1, up to p). window >= 1, sinks >= 0; otherwise as the functions above. The packed
+ * form's workspace size is bsk_attention_varlen_window_workspace_bytes (it depends on the current device), the paged form's as
+ * above. The work is that of the keys that are seen: key blocks that no row of a tile sees are not read. Over a
  * paged cache, pages wholly outside what a sequence's new tokens see are neither read nor looked up (their table entries may
  * hold anything). A non-finite V may reach rows that have left it behind by fewer than 256 tokens, as it may those before it.
  */
@@ -501,6 +502,8 @@ int bsk_attention_paged_window(int dtype, const void* Q, int64_t q_token_stride,
                                const int32_t* cu_seqlens, void* O, int tokens, int batch, int heads, int kv_heads, int dim,
                                int num_pages, int page_size, float scale, int window, int sinks, void* workspace,
                                int64_t workspace_bytes, void* stream);
+int64_t bsk_attention_varlen_window_workspace_bytes(int tokens, int batch, int heads, int kv_heads, int dim, int window, int sinks,
+                                                    int backward);
 int bsk_attention_varlen_window_fwd(int dtype, const void* Q, int64_t q_token_stride, int64_t q_head_stride, const void* K,
                                     int64_t k_token_stride, int64_t k_head_stride, const void* V, int64_t v_token_stride,
                                     int64_t v_head_stride, const int32_t* cu_seqlens, void* O, float* lse, int tokens,

@@ -103,6 +103,7 @@ SIGNATURES = {
                                         _vp]),
     "bsk_attention_paged_window": (_i32, [_i32, _vp, _i64, _i64, _vp, _vp, _i32, _vp, _vp, _vp, _i64, _i32, _vp, _vp, _vp, _i32,
                                           _i32, _i32, _i32, _i32, _i32, _i32, _f32, _i32, _i32, _vp, _i64, _vp]),
+    "bsk_attention_varlen_window_workspace_bytes": (_i64, [_i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32]),
     "bsk_attention_varlen_window_fwd": (_i32, [_i32, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _i32,
                                                _i32, _i32, _i32, _i32, _f32, _i32, _i32, _vp, _i64, _vp]),
     "bsk_attention_varlen_window_bwd": (_i32, [_i32, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp,

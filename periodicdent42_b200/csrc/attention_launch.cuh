@@ -94,7 +94,7 @@ cudaError_t launch_overlapped(void (*kernel)(KArgs...), dim3 grid, int threads, 
 
 template <int kKind, bool kWin>
 cudaError_t varattn_fwd_launch(bool f16, int dim, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
-                               const VarFwdArgs& a, unsigned grid, cudaStream_t s) {
+                               const VarFwdArgsOf<kWin>& a, unsigned grid, cudaStream_t s) {
   if (f16 && dim == 128)
     return launch_overlapped(varattn_fwd_kernel<true, 128, kKind, kWin>, grid, kAttnThreads,
                              VarShape<true, 128, kKind>::kSmemBytes, s, tq, tk, tv, a);
@@ -111,26 +111,32 @@ cudaError_t varattn_fwd_launch(bool f16, int dim, const CUtensorMap& tq, const C
 // Statistics (and work lists), then dK / dV, then dQ.
 struct VarBwdGrids {
   unsigned prep, dkdv, dq;
+  unsigned splits;  // kWin: split key blocks at most (0: none is split)
 };
 template <bool kF16, int kD, bool kWin>
-cudaError_t varattn_bwd_launch_one(const VarPrepArgs& p, const VarBwdArgs& a, const CUtensorMap& tq, const CUtensorMap& tk,
+cudaError_t varattn_bwd_launch_one(const VarPrepArgs& p, const VarBwdArgs& a, [[maybe_unused]] const VarJoinArgs& j, const CUtensorMap& tq, const CUtensorMap& tk,
                                    const CUtensorMap& tv, const CUtensorMap& tdo, const VarBwdGrids& g, cudaStream_t s) {
   varattn_bwd_prep_kernel<kF16, kD><<<g.prep, kPlanThreads, 0, s>>>(p);
   cudaError_t e = launch_overlapped(varattn_bwd_dkdv_kernel<kF16, kD, kWin>, g.dkdv, kBwdThreads,
                                     BwdDkdvShape<kF16, kD>::kSmemBytes, s, tq, tk, tv, tdo, a);
   if (e != cudaSuccess) return e;
-  return launch_overlapped(varattn_bwd_dq_kernel<kF16, kD, kWin>, g.dq, kBwdThreads, BwdDqShape<kF16, kD>::kSmemBytes, s, tq, tk,
-                           tv, tdo, a);
+  e = launch_overlapped(varattn_bwd_dq_kernel<kF16, kD, kWin>, g.dq, kBwdThreads, BwdDqShape<kF16, kD>::kSmemBytes, s, tq, tk, tv,
+                        tdo, a);
+  if constexpr (kWin)
+    if (e == cudaSuccess && g.splits)
+      e = launch_overlapped(varattn_bwd_join_kernel<kF16, kD>, dim3(g.splits, j.kv_heads, kVarBlk / kJoinRows), kJoinRows * kD / 2, 0, s,
+                            j);
+  return e;
 }
 template <bool kWin>
-cudaError_t varattn_bwd_launch(bool f16, int dim, const VarPrepArgs& p, const VarBwdArgs& a, const CUtensorMap& tq,
+cudaError_t varattn_bwd_launch(bool f16, int dim, const VarPrepArgs& p, const VarBwdArgs& a, const VarJoinArgs& j, const CUtensorMap& tq,
                                const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& tdo, const VarBwdGrids& g,
                                cudaStream_t s) {
   if (f16)
-    return dim == 128 ? varattn_bwd_launch_one<true, 128, kWin>(p, a, tq, tk, tv, tdo, g, s)
-                      : varattn_bwd_launch_one<true, 64, kWin>(p, a, tq, tk, tv, tdo, g, s);
-  return dim == 128 ? varattn_bwd_launch_one<false, 128, kWin>(p, a, tq, tk, tv, tdo, g, s)
-                    : varattn_bwd_launch_one<false, 64, kWin>(p, a, tq, tk, tv, tdo, g, s);
+    return dim == 128 ? varattn_bwd_launch_one<true, 128, kWin>(p, a, j, tq, tk, tv, tdo, g, s)
+                      : varattn_bwd_launch_one<true, 64, kWin>(p, a, j, tq, tk, tv, tdo, g, s);
+  return dim == 128 ? varattn_bwd_launch_one<false, 128, kWin>(p, a, j, tq, tk, tv, tdo, g, s)
+                    : varattn_bwd_launch_one<false, 64, kWin>(p, a, j, tq, tk, tv, tdo, g, s);
 }
 
 // Rows per tile (8 * nq), tiles, CTAs per tile, and whether a CTA has its SM to itself.

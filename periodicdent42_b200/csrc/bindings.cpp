@@ -580,11 +580,14 @@ torch::Tensor attention_paged(torch::Tensor Q, torch::Tensor k_cache, torch::Ten
   return O;
 }
 
-torch::Tensor varlen_workspace(const torch::Tensor& Q, int64_t batch, int64_t kv_heads, bool backward) {
-  const int64_t n = bsk_attention_varlen_workspace_bytes(static_cast<int>(Q.size(0)), static_cast<int>(batch),
-                                                         static_cast<int>(Q.size(1)), static_cast<int>(kv_heads),
-                                                         static_cast<int>(Q.size(2)), backward);
-  TORCH_CHECK(n >= 0, "bsk_attention_varlen_workspace_bytes failed: ", bsk_last_error());
+torch::Tensor varlen_workspace(const torch::Tensor& Q, int64_t batch, int64_t kv_heads, int64_t window, int64_t sinks, bool backward) {
+  const int tokens = static_cast<int>(Q.size(0)), heads = static_cast<int>(Q.size(1)), dim = static_cast<int>(Q.size(2));
+  const int64_t n = window > 0 ? bsk_attention_varlen_window_workspace_bytes(tokens, static_cast<int>(batch), heads,
+                                                                             static_cast<int>(kv_heads), dim, static_cast<int>(window),
+                                                                             static_cast<int>(sinks), backward)
+                               : bsk_attention_varlen_workspace_bytes(tokens, static_cast<int>(batch), heads,
+                                                                      static_cast<int>(kv_heads), dim, backward);
+  TORCH_CHECK(n >= 0, "attention_varlen: workspace size failed: ", bsk_last_error());
   return torch::empty({n}, Q.options().dtype(torch::kUInt8));
 }
 
@@ -613,7 +616,7 @@ std::tuple<torch::Tensor, torch::Tensor> attention_varlen_fwd(torch::Tensor Q, t
   const Rows q = as_rows(Q), k = as_rows(K), v = as_rows(V);
   auto O = torch::empty({Q.size(0), Q.size(1), Q.size(2)}, Q.options());
   auto lse = torch::empty({want_lse ? Q.size(0) : 0, Q.size(1)}, Q.options().dtype(torch::kFloat32));
-  auto ws = varlen_workspace(Q, batch, K.size(1), false);
+  auto ws = varlen_workspace(Q, batch, K.size(1), window, sinks, false);
   float* const lse_ptr = want_lse ? lse.data_ptr<float>() : nullptr;
   const int tokens = static_cast<int>(Q.size(0)), n = narrow(batch, op, "batch"), heads = static_cast<int>(Q.size(1)),
             kv_heads = static_cast<int>(K.size(1)), dim = static_cast<int>(Q.size(2));
@@ -654,7 +657,7 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> attention_varlen_bwd(tor
   auto dQ = torch::empty({Q.size(0), Q.size(1), Q.size(2)}, Q.options());
   auto dK = torch::empty({K.size(0), K.size(1), K.size(2)}, K.options());
   auto dV = torch::empty_like(dK);
-  auto ws = varlen_workspace(Q, batch, K.size(1), true);
+  auto ws = varlen_workspace(Q, batch, K.size(1), window, sinks, true);
   const int tokens = static_cast<int>(Q.size(0)), n = narrow(batch, op, "batch"), heads = static_cast<int>(Q.size(1)),
             kv_heads = static_cast<int>(K.size(1)), dim = static_cast<int>(Q.size(2));
   if (window > 0)

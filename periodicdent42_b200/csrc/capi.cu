@@ -2334,6 +2334,29 @@ int64_t varlen_workspace(int64_t tokens, int64_t batch, int heads, int kv_heads,
   return plan + plan_bytes(tokens, batch, bsk::kVarBlk) + bsk::plan_slots(tokens, batch, tt) * kv_heads * 1024;
 }
 
+// What the backward needs beside that for key blocks with sinks, which are split along their query tiles: a list with room for
+// the pieces, the split blocks and the pieces' fp32 rows. A sequence has at most win_sink_blocks of them, each of at most its tiles / plan_window_tiles + 1 pieces.
+struct KeySplitPlan {
+  int64_t pieces;  // 0: nothing is split
+  int64_t list_at, splits_at, rows_at, total;
+};
+KeySplitPlan key_split_plan(int64_t at, int64_t tokens, int64_t batch, int heads, int kv_heads, int dim, Window win, int sm_count) {
+  KeySplitPlan p{};
+  p.list_at = p.splits_at = p.rows_at = p.total = at;
+  if (!win.window || !win.sinks) return p;
+  const int64_t tt = bsk::kVarBlk / (heads / kv_heads), slots = bsk::plan_slots(tokens, batch, tt);
+  // Up to four windows' worth of tiles in one entry is no more than a few others after it (ten sequences of 1 .. 255 tokens,
+  // window 64: the join's launch alone cost 3 us).
+  if (tokens / tt + 1 <= 4 * bsk::plan_window_tiles(win.window, tt)) return p;
+  const int64_t by_list = bsk::plan_pieces(bsk::kPlanKeyShares * sm_count, kv_heads);
+  const int64_t by_length = bsk::win_sink_blocks(win.sinks) * (slots / bsk::plan_window_tiles(win.window, tt) + batch);
+  p.pieces = by_list < by_length ? by_list : by_length;
+  p.splits_at = at + 16 + (bsk::plan_slots(tokens, batch, bsk::kVarBlk) + p.pieces) * (int64_t)sizeof(bsk::VarItem);
+  p.rows_at = (p.splits_at + p.pieces * (int64_t)sizeof(bsk::VarSplit) + 31) / 32 * 32;
+  p.total = p.rows_at + p.pieces * kv_heads * bsk::kVarBlk * 2 * dim * 4 + 32;  // (+ 32: rows start 32-byte aligned)
+  return p;
+}
+
 int attention_paged(int dtype, const void* Q, int64_t q_token_stride, int64_t q_head_stride, const void* k_cache,
                     const void* v_cache, int cache_e4m3, const float* k_scale, const float* v_scale,
                     const int32_t* block_table, int64_t table_stride, int table_width, const int32_t* kv_lens,
@@ -2414,10 +2437,11 @@ int attention_paged(int dtype, const void* Q, int64_t q_token_stride, int64_t q_
     p.window = win.window;
     p.sinks = win.sinks;
     p.split_ctas = w.split_ctas;
+    p.min_piece = bsk::kPlanMinPiece;
     p.kv_heads = kv_heads;
     p.splits = reinterpret_cast<bsk::VarSplit*>(ws + w.splits_at);
     plan_launch(p, workspace, *st, s);
-    bsk::VarFwdArgs f{};
+    bsk::VarFwdWindowArgs f{};
     f.O = O;
     f.count = reinterpret_cast<const int*>(ws);
     f.items = reinterpret_cast<const bsk::VarItem*>(ws + w.items_at);
@@ -2514,7 +2538,7 @@ int attention_varlen_fwd(int dtype, const void* Q, int64_t q_token_stride, int64
   p.window = win.window;
   p.sinks = win.sinks;
   plan_launch(p, workspace, *st, s);
-  bsk::VarFwdArgs f{};
+  bsk::VarFwdWindowArgs f{};
   f.O = O;
   f.lse = lse;
   f.count = static_cast<const int*>(workspace);
@@ -2560,8 +2584,13 @@ int attention_varlen_bwd(int dtype, const void* dO, int64_t do_token_stride, int
   win = window_within(win, tokens);
   if (win.window)
     if (int rc = window_ready(*st)) return rc;
+  const KeySplitPlan ks = key_split_plan((varlen_workspace(tokens, batch, heads, kv_heads, dim, true) + 15) / 16 * 16, tokens, batch,
+                                         heads, kv_heads, dim, win, st->sm_count);
+  if (ks.pieces && workspace_bytes < ks.total)
+    return set_error(BSK_ERR_INVALID_ARG, "%s: workspace of %lld bytes needed", what, (long long)ks.total);
   const int group = heads / kv_heads, tt = bsk::kVarBlk / group;
   const int64_t slots = bsk::plan_slots(tokens, batch, tt), key_slots = bsk::plan_slots(tokens, batch, bsk::kVarBlk);
+  const int64_t key_items = key_slots + ks.pieces;
   if (!plan_fits(tokens, batch, tt, kv_heads)) return set_error(BSK_ERR_UNSUPPORTED, "%s: too many rows", what);
   const bool f16 = dtype == 1;
   CUtensorMap tq, tk, tv, tdo;
@@ -2583,9 +2612,16 @@ int attention_varlen_bwd(int dtype, const void* dO, int64_t do_token_stride, int
     a.window = win.window;
     a.sinks = win.sinks;
     a.keys = i;
-    a.tile_slots = 1;
-    a.count = reinterpret_cast<int*>(i ? ws_keys : ws);
-    a.items = reinterpret_cast<bsk::VarItem*>((i ? ws_keys : ws) + 16);
+    a.tile_slots = i == 0;
+    char* list = i == 0 ? ws : ks.pieces ? ws + ks.list_at : ws_keys;
+    if (i == 1 && ks.pieces) {
+      a.split_ctas = bsk::kPlanKeyShares * st->sm_count;
+      a.min_piece = (int)bsk::plan_window_tiles(win.window, tt);
+      a.kv_heads = kv_heads;
+      a.splits = reinterpret_cast<bsk::VarSplit*>(ws + ks.splits_at);
+    }
+    a.count = reinterpret_cast<int*>(list);
+    a.items = reinterpret_cast<bsk::VarItem*>(list + 16);
     a.err = st->err_word;
   }
   p.dO = dO;
@@ -2620,10 +2656,13 @@ int attention_varlen_bwd(int dtype, const void* dO, int64_t do_token_stride, int
   const int64_t spread = 2 * (int64_t)st->sm_count / slots;
   p.head_groups = (int)(spread < 1 ? 1 : spread > kv_heads ? kv_heads : spread);
   const bsk::VarBwdGrids g{(unsigned)(2 + slots * p.head_groups),
-                           (unsigned)(key_slots * kv_heads < st->sm_count ? key_slots * kv_heads : st->sm_count),
-                           (unsigned)(slots * kv_heads < st->sm_count ? slots * kv_heads : st->sm_count)};
-  const cudaError_t e = win.window ? bsk::window_bwd(f16, dim, p, a, tq, tk, tv, tdo, g, s)
-                                   : bsk::varattn_bwd_launch<false>(f16, dim, p, a, tq, tk, tv, tdo, g, s);
+                           (unsigned)(key_items * kv_heads < st->sm_count ? key_items * kv_heads : st->sm_count),
+                           (unsigned)(slots * kv_heads < st->sm_count ? slots * kv_heads : st->sm_count),
+                           (unsigned)(ks.pieces ? ks.pieces / 2 + 1 : 0)};
+  a.part = reinterpret_cast<float*>((reinterpret_cast<uintptr_t>(ws + ks.rows_at) + 31) & ~uintptr_t(31));
+  const bsk::VarJoinArgs j{dK, dV, a.part, p.plan[1].splits, p.plan[1].count, kv_heads, scale};
+  const cudaError_t e = win.window ? bsk::window_bwd(f16, dim, p, a, j, tq, tk, tv, tdo, g, s)
+                                   : bsk::varattn_bwd_launch<false>(f16, dim, p, a, j, tq, tk, tv, tdo, g, s);
   if (e != cudaSuccess) return cuda_fail(e, "attention_varlen_bwd launch");
   return launch_status("attention_varlen_bwd launch");
 }
@@ -2675,6 +2714,19 @@ int bsk_attention_varlen_fwd(int dtype, const void* Q, int64_t q_token_stride, i
   return attention_varlen_fwd(dtype, Q, q_token_stride, q_head_stride, K, k_token_stride, k_head_stride, V, v_token_stride,
                               v_head_stride, cu_seqlens, O, lse, tokens, batch, heads, kv_heads, dim, scale, causal, Window{},
                               workspace, workspace_bytes, stream);
+}
+
+int64_t bsk_attention_varlen_window_workspace_bytes(int tokens, int batch, int heads, int kv_heads, int dim, int window, int sinks,
+                                                    int backward) {
+  const char* what = "attention_varlen_window_workspace_bytes";
+  if (int rc = heads_checks(what, 0, tokens, batch, heads, kv_heads, dim, 1.0f)) return rc;
+  if (int rc = window_checks(what, window, sinks)) return rc;
+  const int64_t base = varlen_workspace(tokens, batch, heads, kv_heads, dim, backward != 0);
+  const Window win = window_within(Window{window, sinks}, tokens);
+  if (!backward || !win.window || !win.sinks) return base;
+  DeviceState* st;
+  if (int rc = device_state(&st)) return rc;
+  return key_split_plan((base + 15) / 16 * 16, tokens, batch, heads, kv_heads, dim, win, st->sm_count).total;
 }
 
 int bsk_attention_varlen_window_fwd(int dtype, const void* Q, int64_t q_token_stride, int64_t q_head_stride, const void* K,

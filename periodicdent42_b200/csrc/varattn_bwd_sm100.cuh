@@ -41,6 +41,7 @@ struct VarBwdArgs {
   float scale;           // softmax scale
   float scale_log2;      // scale * log2(e)
   int window, sinks;     // kWin: a row at position p sees keys (p - window, p] and [0, sinks)
+  float* part;           // kWin: pieces of split key blocks, [pieces][kv heads][128 keys][dV | dK, unscaled]
   uint32_t* err;
   uint64_t timeout_ns;
 };
@@ -78,6 +79,21 @@ __device__ __forceinline__ void write_acc_half_if(uint32_t t_row, int x, uint16_
     ptx::tmem_ld_32x32b_x32(t_row + col, u);
     ptx::tmem_wait_ld();
     if (live) store_row_half<kF16>(row_out + col, u, mul);
+    __syncwarp();
+  }
+}
+
+// The same into a piece's fp32 rows.
+template <int kD>
+__device__ __forceinline__ void write_acc_half_f32(uint32_t t_row, int x, float* row_out) {
+#pragma unroll 1
+  for (int cc = 0; cc < kD / 64; ++cc) {
+    const int col = x * (kD / 2) + cc * 32;
+    uint32_t u[32];
+    ptx::tmem_ld_32x32b_x32(t_row + col, u);
+    ptx::tmem_wait_ld();
+#pragma unroll
+    for (int i = 0; i < 32; i += 8) st_global_v8(row_out + col + i, u + i);
     __syncwarp();
   }
 }
@@ -879,8 +895,14 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       if (!ok) break;
       ++acc_cnt;
       ptx::tc_fence_after();
-      write_acc_half_if<kF16, kD>(tmem_base + lane_off + T_DV, x, dv_row, 1.0f, live);
-      write_acc_half_if<kF16, kD>(tmem_base + lane_off + T_DK, x, dk_row, a.scale, live);
+      if (kWin && it.part >= 0) {
+        float* row = a.part + ((static_cast<int64_t>(it.part) * a.kv_heads + hkv) * kVarBlk + r) * 2 * kD;
+        write_acc_half_f32<kD>(tmem_base + lane_off + T_DV, x, row);
+        write_acc_half_f32<kD>(tmem_base + lane_off + T_DK, x, row + kD);
+      } else {
+        write_acc_half_if<kF16, kD>(tmem_base + lane_off + T_DV, x, dv_row, 1.0f, live);
+        write_acc_half_if<kF16, kD>(tmem_base + lane_off + T_DK, x, dk_row, a.scale, live);
+      }
       ptx::tc_fence_before();
       __syncwarp();
       if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(acc_empty));
@@ -891,6 +913,45 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   __syncthreads();
   ptx::tc_fence_after();
   if (warp == 1) ptx::tmem_dealloc(tmem_base, kAttnTmemCols);
+}
+
+// Pieces of split key blocks -> dV and dK: sums in the pieces' order, one rounding. Block (split block, kv head, 16 keys); a
+// thread adds up four neighbouring columns. Reads each partial result once, from L2.
+struct VarJoinArgs {
+  void* dK;
+  void* dV;
+  const float* part;
+  const VarSplit* splits;
+  const int* count;  // [1]: split key blocks
+  int kv_heads;
+  float scale;
+};
+constexpr int kJoinRows = 16;
+
+template <bool kF16, int kD>
+__global__ void __launch_bounds__(kJoinRows * kD / 2) varattn_bwd_join_kernel(const VarJoinArgs a) {
+  ptx::grid_dependency_wait();
+  if (static_cast<int>(blockIdx.x) >= a.count[1]) return;
+  const VarSplit sp = a.splits[blockIdx.x];
+  const int hkv = blockIdx.y, r = blockIdx.z * kJoinRows + threadIdx.x / (kD / 2), c = threadIdx.x % (kD / 2);
+  if (r >= sp.ntok) return;
+  const float4* p = reinterpret_cast<const float4*>(
+      a.part + ((static_cast<int64_t>(sp.first) * a.kv_heads + hkv) * kVarBlk + r) * 2 * kD) + c;
+  const int64_t step = static_cast<int64_t>(a.kv_heads) * kVarBlk * kD / 2;
+  float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+  for (int i = 0; i < sp.n; ++i) {
+    const float4 v = __ldg(p + i * step);
+    acc.x += v.x;
+    acc.y += v.y;
+    acc.z += v.z;
+    acc.w += v.w;
+  }
+  const bool is_dk = c >= kD / 4;
+  const float mul = is_dk ? a.scale : 1.0f;
+  uint16_t* out = static_cast<uint16_t*>(is_dk ? a.dK : a.dV) + (static_cast<int64_t>(sp.row0 + r) * a.kv_heads + hkv) * kD;
+  reinterpret_cast<uint2*>(out)[c % (kD / 4)] =
+      make_uint2(pack2<kF16>(acc.x * mul, acc.y * mul), pack2<kF16>(acc.z * mul, acc.w * mul));
 }
 
 }  // namespace bsk

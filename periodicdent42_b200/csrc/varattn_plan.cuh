@@ -7,7 +7,10 @@
 // length is arbitrary and changes no result, since an entry's arithmetic depends on the entry alone.
 //
 // Where there are few entries for the GPU (a small chunk over a long cache), long ones are split along their keys; the
-// pieces' results meet in a second kernel (varattn_combine_kernel).
+// pieces' results meet in a second kernel (varattn_combine_kernel). With a window, the key blocks that hold sinks are seen by
+// all tiles of their sequence, the others by a window's worth: in the backward's list of key blocks the long ones are split
+// along their query tiles (varattn_bwd_join_kernel), since the zigzag gives every CTA the same number of entries (packed
+// sequences of 8192 .. 596 tokens, window 1024, 4 sinks, 32 / 8 heads, D 128: dK / dV 1155 us whole, 624 in pieces).
 //
 // Tiles are numbered without a scan: tile j of sequence i is slot cu[i] / TT + i + j (sequences never overlap in it: the
 // next one's first slot is at least ceil(n_i / TT) further). Slots from cu[batch] / TT + batch on cover the rows behind the
@@ -32,7 +35,7 @@ struct __align__(16) VarItem {
   int kv_len;  // keys of the sequence
   int pos0;    // position of the tile's first token (first key of the block, for dK / dV)
   int b0, b1;  // key blocks [b0, b1) (query tiles, for dK / dV)
-  int part;    // index of a split entry's piece, -1 for a whole entry (in the backward's lists: slot of the tile)
+  int part;    // index of a split entry's piece, -1 for a whole entry (in the backward's list of query tiles: slot of the tile)
 };
 
 // An entry that was split along its keys: pieces [first, first + n) hold its partial results.
@@ -46,8 +49,9 @@ struct PlanArgs {
   int64_t kv_room;     // keys that a block table row has room for
   int tokens, batch, tt, causal;
   int keys;            // 1: entries are key blocks
-  int tile_slots;      // 1: entries carry their slot in `part` (nothing is split)
+  int tile_slots;      // 1: entries carry their slot in `part` (and are not split)
   int split_ctas;      // > 0: entries may be split along their keys to give this many CTAs work (kv_heads items an entry)
+  int min_piece;       // and are left whole up to this length
   int kv_heads;
   int window, sinks;   // window > 0 (causal): a row at position p sees keys (p - window, p] and [0, sinks)
   VarItem* items;
@@ -60,6 +64,10 @@ struct PlanArgs {
 // ceil(n / L) < 2 n / L pieces.
 __host__ __device__ inline int plan_pieces(int split_ctas, int kv_heads) { return 2 * split_ctas / kv_heads + 1; }
 constexpr int kPlanMinPiece = 4;  // key blocks: shorter pieces cost more in partial results than they save
+// The backward's key blocks are split for this many times the CTAs: a piece is then a quarter of a CTA's share at least.
+constexpr int kPlanKeyShares = 4;
+// Query tiles that see a key block without sinks, at most.
+__host__ __device__ inline int64_t plan_window_tiles(int64_t window, int64_t tt) { return (window + kVarBlk - 2) / tt + 2; }
 
 // Slots that a launch reserves for `tokens` rows of `batch` sequences in tiles of tt.
 __host__ __device__ inline int64_t plan_slots(int64_t tokens, int64_t batch, int64_t tt) { return tokens / tt + batch + 1; }
@@ -152,7 +160,7 @@ __device__ __forceinline__ void build_plan(const PlanArgs& a) {
       // A CTA's even share of the work; with fewer items than CTAs, the shortest pieces that leave one per CTA (else some
       // CTAs would get two pieces, and the rest wait).
       long long l = max((static_cast<long long>(work) * a.kv_heads + a.split_ctas - 1) / a.split_ctas,
-                        static_cast<long long>(kPlanMinPiece));
+                        static_cast<long long>(a.min_piece));
       const int n = n_live;
       if (n <= kFew && static_cast<int64_t>(n) * a.kv_heads < a.split_ctas)
         while (true) {
@@ -202,7 +210,8 @@ __device__ __forceinline__ void build_plan(const PlanArgs& a) {
       continue;
     }
     const int first = atomicAdd(&n_part, p), b0 = it.b0;
-    a.splits[atomicAdd(&n_split, 1)] = {it.row0, it.ntok, first, p};
+    if (a.keys) a.splits[atomicAdd(&n_split, 1)] = {it.row0 + it.pos0, min(kVarBlk, it.kv_len - it.pos0), first, p};
+    else a.splits[atomicAdd(&n_split, 1)] = {it.row0, it.ntok, first, p};
     for (int j = 0; j < p; ++j) {
       it.b0 = b0 + static_cast<int>(static_cast<int64_t>(n) * j / p);
       it.b1 = b0 + static_cast<int>(static_cast<int64_t>(n) * (j + 1) / p);

@@ -42,6 +42,8 @@
 // group.
 #pragma once
 
+#include <type_traits>
+
 #include "bsattn_bwd_sm100.cuh"
 #include "varattn_plan.cuh"
 
@@ -108,10 +110,21 @@ struct VarFwdArgs {
   const float* v_scale;
   int heads, kv_heads, group, causal;
   float scale_log2;
-  int window, sinks;    // kWin: a row at position p sees keys (p - window, p] and [0, sinks)
   uint32_t* err;
   uint64_t timeout_ns;
 };
+// The kernels with a window (kWin) take two more. (Added to the arguments of the others, eight bytes changed the compiler's
+// allocation: 84 bytes of spills over e4m3 caches, where there are none.)
+struct VarFwdWindowArgs : VarFwdArgs {
+  int window, sinks;    // a row at position p sees keys (p - window, p] and [0, sinks)
+};
+template <bool kWin>
+using VarFwdArgsOf = typename std::conditional<kWin, VarFwdWindowArgs, VarFwdArgs>::type;
+struct VarWindow {
+  int window, sinks;
+};
+__device__ __forceinline__ VarWindow window_of(const VarFwdArgs&) { return {0, 0}; }
+__device__ __forceinline__ VarWindow window_of(const VarFwdWindowArgs& a) { return {a.window, a.sinks}; }
 
 // Bits [0, n) of a word.
 __device__ __forceinline__ uint32_t bits_below(int n) { return n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1u; }
@@ -141,7 +154,7 @@ __device__ __forceinline__ int range_top(const int* top, uint32_t segs, int firs
 template <bool kF16, int kD, int kKind, bool kWin = false>
 __global__ void __launch_bounds__(kAttnThreads, 1)
     varattn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
-                       const __grid_constant__ CUtensorMap tmV, const VarFwdArgs a) {
+                       const __grid_constant__ CUtensorMap tmV, const VarFwdArgsOf<kWin> a) {
   using Sh = VarShape<kF16, kD, kKind>;
   constexpr bool kPaged = kKind != kPacked, kE4m3 = kKind == kCacheE4m3;
   constexpr bool kOpF16 = kF16 || kE4m3;  // type of the products' operands
@@ -259,12 +272,13 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     return true;
   };
   // Key block of entry b of the item's list (see win_skip), and whether some row of the tile sees some key of [key, key + n).
-  const int sink_blocks = kWin ? win_sink_blocks(a.sinks) : 0;
+  const int window = window_of(a).window, sinks = window_of(a).sinks;
+  const int sink_blocks = kWin ? win_sink_blocks(sinks) : 0;
   auto block_of = [&](const VarItem& it, int b) -> int {
-    return kWin && b >= sink_blocks ? b + win_skip(it.pos0, a.window, a.sinks) : b;
+    return kWin && b >= sink_blocks ? b + win_skip(it.pos0, window, sinks) : b;
   };
   auto in_reach = [&](const VarItem& it, int key, int n) -> bool {
-    return !kWin || key < a.sinks || key + n > max(it.pos0, 0) - a.window + 1;
+    return !kWin || key < sinks || key + n > max(it.pos0, 0) - window + 1;
   };
   // Keys of the sequence in the item's last block: below 128 its V tile holds foreign rows.
   auto tail_rows = [&](const VarItem& it) { return it.kv_len - block_of(it, it.b1 - 1) * kVarBlk; };
@@ -314,12 +328,12 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       };
       auto push = [&](const CUtensorMap* m, const VarItem& it, int hkv, int b, bool is_v, int row) -> bool {
         if (!wait(&ring_empty[slot], slot_phase ^ 1, 2)) return false;
-        const bool foreign = !kE4m3 && is_v && it.kv_len - b * kVarBlk < kVarBlk;
+        const bool foreign = !kE4m3 && is_v && b == it.b1 - 1 && tail_rows(it) < kVarBlk;
         const uint32_t fb = ptx::smem_u32(foreign ? &raw_full[slot] : &ring_full[slot]);
         uint32_t dst = kv0 + slot * (kE4m3 ? Sh::kStageBytes : kTile);
         if (kPaged) dst += lane * (kE4m3 ? box_rows * kD : (box_rows >> 3) * kGroupPitch);
         if (lane == 0) {
-          const int boxes = kPaged ? min(pages_per_blk, (it.kv_len - b * kVarBlk + box_rows - 1) / box_rows) : 1;
+          const int boxes = kPaged ? min(pages_per_blk, (it.kv_len - block_of(it, b) * kVarBlk + box_rows - 1) / box_rows) : 1;
           ptx::mbar_arrive_expect_tx(fb, boxes * box_rows * kD * (kE4m3 ? 1 : 2));
         }
         if constexpr (kE4m3) {
@@ -353,21 +367,19 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
             ptx::tma_load_3d(ptx::smem_u32(sQ) + qbuf * kTile + c * kAttnChunk, &tmQ, qf, 64 * c, hkv * group, it.row0);
         }
         ++q_issued;
-        int row = 0, prev = 0, before = 0;
-        for (int x = it.b0; x < it.b1 && ok; ++x) {
-          const int b = block_of(it, x);
+        int row = 0, prev = 0;
+        for (int b = it.b0; b < it.b1 && ok; ++b) {
           if constexpr (kPaged) {
-            row = row_of(it, b, ahead);
-            if (x + 1 < it.b1) ahead = entry(it, block_of(it, x + 1));
+            row = row_of(it, block_of(it, b), ahead);
+            if (b + 1 < it.b1) ahead = entry(it, block_of(it, b + 1));
           } else {
-            row = it.src + b * kVarBlk;
+            row = it.src + block_of(it, b) * kVarBlk;
           }
           ok = push(&tmK, it, hkv, b, false, row);
-          if (ok && x > it.b0) ok = push(&tmV, it, hkv, before, true, prev);
+          if (ok && b > it.b0) ok = push(&tmV, it, hkv, b - 1, true, prev);
           prev = row;
-          before = b;
         }
-        if (ok) ok = push(&tmV, it, hkv, before, true, prev);
+        if (ok) ok = push(&tmV, it, hkv, it.b1 - 1, true, prev);
       }
     }
     if (lane == 0) {  // drain loads still in flight
@@ -625,13 +637,13 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       const int limit = a.causal ? it.pos0 + tok + 1 : it.kv_len;
       const int clear = (a.causal ? it.pos0 + 1 : it.kv_len) >> 7;
       // a window also masks keys before `lo` (the sinks apart); key blocks that start before `lo_all` have such keys for some row
-      const int lo = max(it.pos0 + tok, 0) - a.window + 1, lo_all = max(it.pos0 + tt, 0) - a.window;
+      const int lo = max(it.pos0 + tok, 0) - window + 1, lo_all = max(it.pos0 + tt, 0) - window;
       float m_run = -INFINITY, l_run = 0.0f;
       int own = kScaleLow, ref = kScaleLow;  // e4m3 with a window: largest value scale that the row has seen, and its reference
       const uint32_t tO = tO0 + 128 * (rows & 1);
       for (int j = 0; j < n; ++j, ++g) {
         const int kb = block_of(it, it.b0 + j);
-        const bool cut = kWin && (kb >= clear || (kb * kVarBlk < lo_all && (kb + 1) * kVarBlk > a.sinks));
+        const bool cut = kWin && (kb >= clear || (kb * kVarBlk < lo_all && (kb + 1) * kVarBlk > sinks));
         const uint32_t b = g & 1;
         const uint32_t tS = tmem_base + 128 * b + lane_off;
         if constexpr (kE4m3) {
@@ -663,7 +675,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         if constexpr (kWin) {
           if (cut) {
             const int base = kb * kVarBlk + 64 * h;
-            const uint32_t seen[2] = {seen_bits(base, limit, lo, a.sinks), seen_bits(base + 32, limit, lo, a.sinks)};
+            const uint32_t seen[2] = {seen_bits(base, limit, lo, sinks), seen_bits(base + 32, limit, lo, sinks)};
 #pragma unroll
             for (int i = 0; i < 64; ++i)
               if (!(seen[i >> 5] >> (i & 31) & 1)) v[i] = -INFINITY;
@@ -705,7 +717,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
           if (cut) {
             const int base = kb * kVarBlk, end = min(limit - base, kVarBlk);
             own = max(own, max(range_top(v_top + 128 * b, segs, max(lo - base, 0), end),
-                               range_top(v_top + 128 * b, segs, 0, min(a.sinks - base, end))));
+                               range_top(v_top + 128 * b, segs, 0, min(sinks - base, end))));
           } else {
             const uint32_t two = __vmaxu2(segs & 0x00ff00ffu, (segs >> 8) & 0x00ff00ffu);
             own = max(own, static_cast<int>(max(two & 0xffffu, two >> 16)));

@@ -139,12 +139,11 @@ cudaError_t varattn_bwd_launch(bool f16, int dim, const VarPrepArgs& p, const Va
                     : varattn_bwd_launch_one<false, 64, kWin>(p, a, j, tq, tk, tv, tdo, g, s);
 }
 
-// Rows per tile (8 * nq), tiles, CTAs per tile, and whether a CTA has its SM to itself.
+// Rows per tile (8 * nq), tiles, CTAs per tile and warps per CTA.
 struct PagedGrid {
   int nq;
   unsigned tiles;
-  int cluster;
-  bool alone;
+  int cluster, warps;
 };
 template <bool kF16, int kD, bool kFp8, int kNQ, bool kWin>
 cudaError_t paged_decode_launch_rows(const PagedArgs& a, const PagedGrid& g, cudaStream_t s) {
@@ -155,9 +154,8 @@ cudaError_t paged_decode_launch_rows(const PagedArgs& a, const PagedGrid& g, cud
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.gridDim = dim3(g.tiles * g.cluster, a.kv_heads, 1);
   using Sh = PagedShape<kD, kFp8, kNQ>;
-  const int warps = g.alone ? Sh::kMaxWarps : 4;
-  cfg.blockDim = dim3(32 * warps, 1, 1);
-  cfg.dynamicSmemBytes = Sh::smem_bytes(warps);
+  cfg.blockDim = dim3(32 * g.warps, 1, 1);
+  cfg.dynamicSmemBytes = Sh::smem_bytes(g.warps);
   cfg.stream = s;
   cfg.attrs = attr;
   cfg.numAttrs = 1;

@@ -501,9 +501,20 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor, torch::Tensor, torch::Te
   const int rows = narrow(tokens, op, "tokens");
   const auto pages = free_pages.contiguous();
   const auto i32 = block_table.options();
-  auto slots = torch::empty({tokens}, i32.dtype(torch::kInt64));
-  auto positions = torch::empty({tokens}, i32), cu = torch::empty({batch + 1}, i32), lens = torch::empty({batch}, i32),
-       left = torch::empty({1}, i32);
+  // one allocation, whose parts the results are (each allocation costs the host 0.8 us, all else of the call 5)
+  const auto buffer = torch::empty({2 * tokens + tokens + 2 * batch + 2}, i32);
+  int64_t used = 0;  // 4-byte words
+  const auto part = [&](int64_t n, at::ScalarType type) {
+    const int64_t bytes = at::elementSize(type);
+    auto t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(buffer.storage()), buffer.key_set(), at::scalarTypeToTypeMeta(type));
+    t.unsafeGetTensorImpl()->set_sizes_contiguous({n});
+    t.unsafeGetTensorImpl()->set_storage_offset(used * 4 / bytes);
+    used += n * bytes / 4;
+    return t;
+  };
+  const auto slots = part(tokens, torch::kInt64);
+  const auto positions = part(tokens, torch::kInt32), cu = part(batch + 1, torch::kInt32), lens = part(batch, torch::kInt32),
+             left = part(1, torch::kInt32);
   check_rc(bsk_kv_cache_plan(kv.data_ptr<int32_t>(), n.data_ptr<int32_t>(), narrow(batch, op, "batch"), block_table.data_ptr<int32_t>(),
                              batch > 1 ? block_table.stride(0) : width, narrow(width, op, "table width"), pages.data_ptr<int32_t>(),
                              narrow(pages.size(0), op, "free pages"), free_count.data_ptr<int32_t>(), narrow(page_size, op, "page_size"),

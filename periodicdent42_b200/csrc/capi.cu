@@ -1969,6 +1969,28 @@ int rotary(int dtype, const void* Q, int64_t q_token_stride, int64_t q_head_stri
   if (!positions || !inv_freq || (heads && (!Q || !Q_out)) || (kv_heads && (!K || !K_out)))
     return set_error(BSK_ERR_INVALID_ARG, "%s: null pointer", what);
   if (int rc = device_state(&st)) return rc;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (axes) {
+    bsk::NormRotaryArgs n{};
+    n.x[0] = Q; n.x[1] = K;
+    n.y[0] = Q_out; n.y[1] = K_out;
+    n.token_stride[0] = q_token_stride; n.token_stride[1] = k_token_stride;
+    n.head_stride[0] = q_head_stride; n.head_stride[1] = k_head_stride;
+    n.heads[0] = heads; n.heads[1] = kv_heads;
+    n.positions = positions;
+    n.positions64 = position_bytes == 8;
+    n.axes = axes;
+    n.num_axes = num_axes;
+    n.inv_freq = inv_freq;
+    n.tokens = tokens;
+    n.dim = dim;
+    n.rotary_dim = rotary_dim;
+    n.scale = scale;
+    n.sign = backward ? -1.0f : 1.0f;
+    n.err = st->err_word;
+    const cudaError_t e = bsk::rotary_axes_turn(dtype, interleaved != 0, n, st->sm_count, s);
+    return e == cudaSuccess ? BSK_OK : cuda_fail(e, "rotary launch");
+  }
   bsk::RotaryArgs a{};
   a.x[0] = Q; a.x[1] = K;
   a.y[0] = Q_out; a.y[1] = K_out;
@@ -1977,16 +1999,12 @@ int rotary(int dtype, const void* Q, int64_t q_token_stride, int64_t q_head_stri
   a.heads[0] = heads; a.heads[1] = kv_heads;
   a.positions = positions;
   a.positions64 = position_bytes == 8;
-  a.axes = axes;
-  a.num_axes = num_axes;
-  a.err = st->err_word;
   a.inv_freq = inv_freq;
   a.tokens = tokens;
   a.dim = dim;
   a.rotary_dim = rotary_dim;
   a.scale = scale;
   a.sign = backward ? -1.0f : 1.0f;
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (dtype == 0) return rotary_pick<__nv_bfloat16>(a, interleaved != 0, *st, s);
   if (dtype == 1) return rotary_pick<__half>(a, interleaved != 0, *st, s);
   return rotary_pick<float>(a, interleaved != 0, *st, s);
@@ -2491,10 +2509,25 @@ int attention_paged(int dtype, const void* Q, int64_t q_token_stride, int64_t q_
   const int64_t most_keys = win.window && reach < room ? reach : room;
   int cluster = 1;
   while (cluster < 8 && items * cluster * 2 <= (int64_t)2 * st->sm_count && most_keys >= (int64_t)cluster * 256) cluster *= 2;
-  if (cluster == 1 && items <= (int64_t)4 * st->sm_count && most_keys >= 2048) cluster = 2;
-  const bool alone = items * cluster <= st->sm_count;
+  if (!win.window && cluster == 1 && items <= (int64_t)4 * st->sm_count && most_keys >= 2048) cluster = 2;
+  int warps = items * cluster <= st->sm_count ? bsk::paged_max_warps(nq) : 4;
+  // With a window the tiles are of one length, so that the CTAs of an SM (12 warps' worth of registers) end together: warps by
+  // how many rounds the tiles take then, each a piece of 1 / warps of a tile's keys and a start. Measured (us; 4, 3 and 2 warps;
+  // sequences x window): e4m3 64x1024 42, 39, 39; 96x1024 51, 58, 47; 200x256 43, 46, 36; 64x4096 109, 102, 121;
+  // bf16 64x1024 58, 49, 47; 128x512 56, 53, 60; 64x128 17, 14, 12.
+  if (win.window && nq == 1 && cluster == 1 && items > st->sm_count) {
+    double least = 1e30;
+    for (int n = 4; n >= 2; --n) {
+      const int64_t slots = (int64_t)(bsk::paged_max_warps(nq) / n) * st->sm_count;
+      const double time = (double)((items + slots - 1) / slots) * (1.0 / n + 0.02);
+      if (time < least) {
+        least = time;
+        warps = n;
+      }
+    }
+  }
   if (tiles * cluster >= (int64_t)1 << 31) return set_error(BSK_ERR_UNSUPPORTED, "%s: too many rows", what);
-  const bsk::PagedGrid g{nq, (unsigned)tiles, cluster, alone};
+  const bsk::PagedGrid g{nq, (unsigned)tiles, cluster, warps};
   const cudaError_t e = win.window ? bsk::window_decode(dtype == 1, dim, cache_e4m3 != 0, a, g, s)
                                    : bsk::paged_decode_launch<false>(dtype == 1, dim, cache_e4m3 != 0, a, g, s);
   if (e != cudaSuccess) return cuda_fail(e, "attention_paged launch");

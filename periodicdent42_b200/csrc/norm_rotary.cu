@@ -37,9 +37,11 @@ int blocks_of(const int (&heads)[2], int w, int per_sm, int64_t chunks, int sm_c
   return (int)std::max<int64_t>(1, std::min(chunks, per_sm * sm_count * cost(w) / (cost(0) + cost(1))));
 }
 
-template <class T, int kVec, int kUnits, bool kInter, int kLanes, bool kBackward>
+enum class Pass { kForward, kBackward, kTurn };  // kTurn: the rotation alone
+
+template <class T, int kVec, int kUnits, bool kInter, int kLanes, Pass kPass>
 cudaError_t launch(NormRotaryArgs& a, int sm_count, cudaStream_t s) {
-  using Sh = NormShape<T, kVec, kUnits, kBackward>;
+  using Sh = NormShape<T, kVec, kUnits, kPass == Pass::kBackward>;
   const int groups = kNormThreads / a.group;
   // A row's lanes keep to one token. Few tokens: as many of its heads at once as there are groups, so that a token takes one
   // step; many: four heads a group, and the groups left over take other tokens.
@@ -53,33 +55,38 @@ cudaError_t launch(NormRotaryArgs& a, int sm_count, cudaStream_t s) {
   }
   a.grid = grid;
   static std::atomic<uint64_t> ready{0};
-  if constexpr (kBackward)
+  if constexpr (kPass == Pass::kBackward)
     return run(norm_rotary_bwd_kernel<T, kVec, kUnits, kInter, kLanes>, ready, Sh::kMostSmem, grid, Sh::smem_bytes(a), a, s);
   else
-    return run(norm_rotary_kernel<T, kVec, kUnits, kInter, kLanes>, ready, Sh::kMostSmem, grid, Sh::smem_bytes(a), a, s);
+    return run(norm_rotary_kernel<T, kVec, kUnits, kInter, kLanes, kPass == Pass::kForward>, ready, Sh::kMostSmem, grid,
+               Sh::smem_bytes(a), a, s);
 }
 
 // The lanes of a row are a power of two; for 16-byte pieces their number is known to the compiler (whose sums it unrolls).
-template <class T, int kVec, int kUnits, bool kInter, bool kBackward>
+template <class T, int kVec, int kUnits, bool kInter, Pass kPass>
 cudaError_t launch_lanes(NormRotaryArgs& a, int sm_count, cudaStream_t s) {
   a.units = a.dim / (2 * kVec);
   a.group = lanes_for((a.units + kUnits - 1) / kUnits);
-  if constexpr (kVec * sizeof(T) == 16 && kUnits == 1) {
+  if constexpr (kVec * sizeof(T) == 16 && kUnits == 1 && kPass != Pass::kTurn) {
     a.group = std::max(a.group, 4);
-    if (a.group == 4) return launch<T, kVec, kUnits, kInter, 4, kBackward>(a, sm_count, s);
-    if (a.group == 8) return launch<T, kVec, kUnits, kInter, 8, kBackward>(a, sm_count, s);
-    if (a.group == 16) return launch<T, kVec, kUnits, kInter, 16, kBackward>(a, sm_count, s);
-    return launch<T, kVec, kUnits, kInter, 32, kBackward>(a, sm_count, s);
+    if (a.group == 4) return launch<T, kVec, kUnits, kInter, 4, kPass>(a, sm_count, s);
+    if (a.group == 8) return launch<T, kVec, kUnits, kInter, 8, kPass>(a, sm_count, s);
+    if (a.group == 16) return launch<T, kVec, kUnits, kInter, 16, kPass>(a, sm_count, s);
+    return launch<T, kVec, kUnits, kInter, 32, kPass>(a, sm_count, s);
   } else {
-    return launch<T, kVec, kUnits, kInter, 0, kBackward>(a, sm_count, s);
+    return launch<T, kVec, kUnits, kInter, 0, kPass>(a, sm_count, s);
   }
 }
 
+template <class T, int kVec, int kUnits, Pass kPass>
+cudaError_t launch_layout(NormRotaryArgs& a, bool inter, int sm_count, cudaStream_t s) {
+  return inter ? launch_lanes<T, kVec, kUnits, true, kPass>(a, sm_count, s) : launch_lanes<T, kVec, kUnits, false, kPass>(a, sm_count, s);
+}
 template <class T, int kVec, int kUnits>
-cudaError_t launch_any(NormRotaryArgs& a, bool inter, bool backward, int sm_count, cudaStream_t s) {
-  if (backward)
-    return inter ? launch_lanes<T, kVec, kUnits, true, true>(a, sm_count, s) : launch_lanes<T, kVec, kUnits, false, true>(a, sm_count, s);
-  return inter ? launch_lanes<T, kVec, kUnits, true, false>(a, sm_count, s) : launch_lanes<T, kVec, kUnits, false, false>(a, sm_count, s);
+cudaError_t launch_any(NormRotaryArgs& a, bool inter, Pass pass, int sm_count, cudaStream_t s) {
+  if (pass == Pass::kTurn) return launch_layout<T, kVec, kUnits, Pass::kTurn>(a, inter, sm_count, s);
+  if (pass == Pass::kBackward) return launch_layout<T, kVec, kUnits, Pass::kBackward>(a, inter, sm_count, s);
+  return launch_layout<T, kVec, kUnits, Pass::kForward>(a, inter, sm_count, s);
 }
 
 // Whether every row can be read and written in pieces of kVec elements, `bytes` wide.
@@ -100,25 +107,26 @@ bool fits(const NormRotaryArgs& a, bool inter, bool backward, int vec, int elem,
 // 16-byte pieces where rows and halves allow them, else 4-byte ones, else single elements (dim 80, 40 elements turned, bf16:
 // half of a pair's elements starts at a multiple of 40 bytes).
 template <class T>
-cudaError_t pick(NormRotaryArgs& a, bool inter, bool backward, int sm_count, cudaStream_t s) {
+cudaError_t pick(NormRotaryArgs& a, bool inter, Pass pass, int sm_count, cudaStream_t s) {
+  const bool backward = pass == Pass::kBackward;
   constexpr int kWide = 16 / sizeof(T), kElem = sizeof(T);
   a.aligned32 = fits(a, inter, backward, kWide, kElem, 32);
   if (fits(a, inter, backward, kWide, kElem, 16)) {
     if constexpr (kElem == 4)
-      if (a.dim > 2 * kWide * 32) return launch_any<T, kWide, 2>(a, inter, backward, sm_count, s);
-    return launch_any<T, kWide, 1>(a, inter, backward, sm_count, s);
+      if (a.dim > 2 * kWide * 32) return launch_any<T, kWide, 2>(a, inter, pass, sm_count, s);
+    return launch_any<T, kWide, 1>(a, inter, pass, sm_count, s);
   }
   a.aligned32 = 0;
   if constexpr (kElem == 2)
     if (fits(a, inter, backward, 2, kElem, 4))
-      return a.dim <= 128 ? launch_any<T, 2, 1>(a, inter, backward, sm_count, s) : launch_any<T, 2, 4>(a, inter, backward, sm_count, s);
-  return launch_any<T, 1, 8>(a, inter, backward, sm_count, s);
+      return a.dim <= 128 ? launch_any<T, 2, 1>(a, inter, pass, sm_count, s) : launch_any<T, 2, 4>(a, inter, pass, sm_count, s);
+  return launch_any<T, 1, 8>(a, inter, pass, sm_count, s);
 }
 
-cudaError_t by_type(int dtype, bool inter, NormRotaryArgs& a, bool backward, int sm_count, cudaStream_t s) {
-  if (dtype == 0) return pick<__nv_bfloat16>(a, inter, backward, sm_count, s);
-  if (dtype == 1) return pick<__half>(a, inter, backward, sm_count, s);
-  return pick<float>(a, inter, backward, sm_count, s);
+cudaError_t by_type(int dtype, bool inter, NormRotaryArgs& a, Pass pass, int sm_count, cudaStream_t s) {
+  if (dtype == 0) return pick<__nv_bfloat16>(a, inter, pass, sm_count, s);
+  if (dtype == 1) return pick<__half>(a, inter, pass, sm_count, s);
+  return pick<float>(a, inter, pass, sm_count, s);
 }
 
 template <class T>
@@ -143,11 +151,17 @@ int64_t norm_rotary_partials(int tokens, int heads, int kv_heads, int dim, int s
 }
 
 cudaError_t norm_rotary_fwd(int dtype, bool interleaved, NormRotaryArgs a, int sm_count, cudaStream_t s) {
-  return by_type(dtype, interleaved, a, false, sm_count, s);
+  a.sign = 1.0f;
+  return by_type(dtype, interleaved, a, Pass::kForward, sm_count, s);
+}
+
+cudaError_t rotary_axes_turn(int dtype, bool interleaved, NormRotaryArgs a, int sm_count, cudaStream_t s) {
+  return by_type(dtype, interleaved, a, Pass::kTurn, sm_count, s);
 }
 
 cudaError_t norm_rotary_bwd(int dtype, bool interleaved, NormRotaryArgs a, void* dwq, void* dwk, int sm_count, cudaStream_t s) {
-  cudaError_t e = by_type(dtype, interleaved, a, true, sm_count, s);
+  a.sign = 1.0f;
+  cudaError_t e = by_type(dtype, interleaved, a, Pass::kBackward, sm_count, s);
   if (e != cudaSuccess || (!dwq && !dwk)) return e;
   NormWeightArgs n{};
   n.partial = a.partial;

@@ -7,6 +7,9 @@
 // Everything is fp32 from the loads on; y and dx are rounded once, dw after its sum. The squares of a row may pass fp32's range
 // (bf16 and fp32 rows beyond 10^19): then the row is multiplied by 2^-100 first, which changes its rms alone.
 //
+// The same kernel without the norm (kNorm) turns by positions on several axes. (The one-axis rotation has rotary.cuh's kernel,
+// whose results it keeps bit for bit where all axes agree.)
+//
 // A row is held by a group of 4 .. 32 lanes, each with its pairs' both elements, so the two sums of a row are shuffles and the
 // row is read once. A group keeps to one token: the angles' sines and cosines and the weights stay in its lanes' registers for
 // all of its heads, of which kNormBatch rows are loaded before any is used (and before the angles are taken). The backward
@@ -43,7 +46,7 @@ struct NormRotaryArgs {
   int num_axes;
   const float* inv_freq;
   int tokens, dim, rotary_dim;
-  float scale, eps;
+  float scale, sign, eps;          // sign: of the angles
   int aligned32;                   // every row starts at a multiple of 32 bytes
   int group, units;                // lanes and units of a row
   int at_once[2], per_block[2];    // heads of a token side by side, tokens of a chunk
@@ -276,7 +279,7 @@ __device__ __forceinline__ void norm_angles(const NormRotaryArgs& a, int64_t t0,
     const int64_t at = position_of(a.positions, a.positions64, a.axes, a.num_axes, a.tokens, t0 + it, pair, a.err);
     float s, c;
     sincospif(2.0f * static_cast<float>(turn_fraction(at, a.inv_freq[pair])), &s, &c);
-    rot[i] = make_float2(c * a.scale, s * a.scale);
+    rot[i] = make_float2(c * a.scale, a.sign * s * a.scale);
     it += tokens;
     pair += pairs;
     if (pair >= half) {
@@ -385,7 +388,8 @@ struct NormBlock {
   }
 };
 
-template <class T, int kVec, int kUnits, bool kInter, int kLanes>
+// kNorm: else the rotation alone (without weights, eps and the norm; the part that is not turned is copied).
+template <class T, int kVec, int kUnits, bool kInter, int kLanes, bool kNorm>
 __global__ void __launch_bounds__(kNormThreads, NormShape<T, kVec, kUnits, false>::kBlocksPerSm)
     norm_rotary_kernel(const __grid_constant__ NormRotaryArgs a) {
   extern __shared__ float4 norm_smem[];
@@ -424,7 +428,7 @@ __global__ void __launch_bounds__(kNormThreads, NormShape<T, kVec, kUnits, false
   };
 #pragma unroll
   for (int i = 0; i < Ring::kStages - 1; ++i) fetch();
-  stage_weights<T, kVec, kInter>(a, w, w_s);
+  if constexpr (kNorm) stage_weights<T, kVec, kInter>(a, w, w_s);
   const float inv_dim = 1.0f / static_cast<float>(a.dim);
   const int it0 = threadIdx.x / half, pair0 = threadIdx.x % half;
   NormStep now{blk.first, 0, 0};
@@ -434,18 +438,22 @@ __global__ void __launch_bounds__(kNormThreads, NormShape<T, kVec, kUnits, false
     __syncthreads();  // the chunk before has read its angles
     norm_angles(a, t0, static_cast<int>(min(static_cast<int64_t>(blk.per_block), a.tokens - t0)), it0, pair0, rot);
     __syncthreads();
-    // Turn and weights in one: (a, b) -> (a ac - b bs, a as + b bc)
+    // Turn and weights in one: (a, b) -> (a ac + b bs, a as + b bc), bs with the other sign
     Turn<kVec> ca[kUnits], cb[kUnits];
     read_turns<kVec, kUnits, kInter>(a, rot + blk.it * half, group, lane, rows > 0, ca);
 #pragma unroll
     for (int n = 0; n < kUnits; ++n) {
-      Halves<kVec> weight;
-      const Unit u(group * n + lane, a.units, half);
-      read_weights<kVec>(w_s, u.live ? group * n + lane : 0, a.units, weight);
-      v_mul(cb[n].c, ca[n].c, weight.b);
-      v_mul(cb[n].s, ca[n].s, weight.b);
-      v_mul(ca[n].c, ca[n].c, weight.a);
-      v_mul(ca[n].s, ca[n].s, weight.a);
+      cb[n] = ca[n];
+      v_scale(cb[n].s, -1.0f);
+      if constexpr (kNorm) {
+        Halves<kVec> weight;
+        const Unit u(group * n + lane, a.units, half);
+        read_weights<kVec>(w_s, u.live ? group * n + lane : 0, a.units, weight);
+        v_mul(cb[n].c, cb[n].c, weight.b);
+        v_mul(cb[n].s, cb[n].s, weight.b);
+        v_mul(ca[n].c, ca[n].c, weight.a);
+        v_mul(ca[n].s, ca[n].s, weight.a);
+      }
     }
     // (every lane of a warp takes part in every sum: the loop's length is the same for all)
     for (int round = 0; round < blk.rounds; ++round) {
@@ -461,10 +469,10 @@ __global__ void __launch_bounds__(kNormThreads, NormShape<T, kVec, kUnits, false
         for (int n = 0; n < kUnits; ++n) {
           unpack_pieces<T, kVec, kInter>(*reinterpret_cast<const P*>(Ring::at(ring, now.stage, (b * kUnits + n) * 2)),
                                          *reinterpret_cast<const P*>(Ring::at(ring, now.stage, (b * kUnits + n) * 2 + 1)), f[n]);
-          ss += dot(f[n], f[n]);
+          if constexpr (kNorm) ss += dot(f[n], f[n]);
         }
-        ss = group_sum<kLanes>(ss, group);
-        if constexpr (!std::is_same<T, __half>::value) {
+        if constexpr (kNorm) ss = group_sum<kLanes>(ss, group);
+        if constexpr (kNorm && !std::is_same<T, __half>::value) {
           const bool far = !(ss <= 3.0e38f);
           if (__any_sync(0xffffffffu, far)) {
             if (far) eps = 0.0f;
@@ -485,16 +493,26 @@ __global__ void __launch_bounds__(kNormThreads, NormShape<T, kVec, kUnits, false
           const Unit u(group * n + lane, a.units, half);
           if (!u.live) continue;
           Halves<kVec> y_f;
-          v_mul(y_f.a, f[n].a, ca[n].c);
-          v_mul(y_f.b, f[n].b, cb[n].c);
-          if (u.turned) {
-            v_nfma(y_f.a, f[n].b, cb[n].s, y_f.a);
-            v_fma(y_f.b, f[n].a, ca[n].s, y_f.b);
-          }
-          v_scale(y_f.a, inv);
-          v_scale(y_f.b, inv);
           P po, qo;
-          pack_pieces<T, kVec, kInter>(y_f, po, qo);
+          if (u.turned) {
+            v_mul(y_f.a, f[n].b, cb[n].s);
+            v_fma(y_f.a, f[n].a, ca[n].c, y_f.a);
+            v_mul(y_f.b, f[n].b, cb[n].c);
+            v_fma(y_f.b, f[n].a, ca[n].s, y_f.b);
+          } else if constexpr (kNorm) {
+            v_mul(y_f.a, f[n].a, ca[n].c);
+            v_mul(y_f.b, f[n].b, cb[n].c);
+          }
+          if constexpr (kNorm) {
+            v_scale(y_f.a, inv);
+            v_scale(y_f.b, inv);
+          }
+          if (kNorm || u.turned) {
+            pack_pieces<T, kVec, kInter>(y_f, po, qo);
+          } else {
+            po = *reinterpret_cast<const P*>(Ring::at(ring, now.stage, (b * kUnits + n) * 2));
+            qo = *reinterpret_cast<const P*>(Ring::at(ring, now.stage, (b * kUnits + n) * 2 + 1));
+          }
           store_pieces<kInter>(y + u.e0, u.e1 - u.e0, a.aligned32, po, qo);
         }
       }

@@ -14,5 +14,8 @@ __attribute__((visibility("hidden"))) cudaError_t norm_rotary_fwd(int dtype, boo
                                                                   cudaStream_t s);
 __attribute__((visibility("hidden"))) cudaError_t norm_rotary_bwd(int dtype, bool interleaved, NormRotaryArgs a, void* dwq, void* dwk,
                                                                   int sm_count, cudaStream_t s);
+// The rotation alone, a.sign the sign of the angles (-1: the gradient).
+__attribute__((visibility("hidden"))) cudaError_t rotary_axes_turn(int dtype, bool interleaved, NormRotaryArgs a, int sm_count,
+                                                                   cudaStream_t s);
 
 }  // namespace bsk

@@ -152,6 +152,8 @@ __device__ __forceinline__ float log2f_approx(float x) {
   return y;
 }
 
+__host__ __device__ constexpr int paged_max_warps(int nq) { return nq == 1 ? 12 : 8; }  // by registers
+
 template <int kD, bool kFp8, int kNQ>
 struct PagedShape {
   static constexpr int kRows = 8 * kNQ;                             // query rows of a tile
@@ -162,7 +164,7 @@ struct PagedShape {
   static constexpr int kStage = kPagedStageBytes + kScaleBytes;
   static constexpr int kWarpBytes = kPagedStages * kStage;
   static constexpr int kPitch = kD + 4;  // floats per row of the merge area: neighbouring rows in different banks
-  static constexpr int kMaxWarps = kNQ == 1 ? 12 : 8;  // by registers
+  static constexpr int kMaxWarps = paged_max_warps(kNQ);
   static constexpr int smem_bytes(int warps) {
     const int merge = (warps + 1) * kRows * (kPitch + 4) * 4;
     return warps * kWarpBytes > merge ? warps * kWarpBytes : merge;

@@ -12,9 +12,6 @@
 // 64-bit number: the fraction is exact to 2^-43 of a turn for every 64-bit position. The rotation itself is fp32 and each
 // result is rounded once.
 //
-// Several axes (time, height, width of an image's or a video's patches): pair i turns by the position on axis axes[i], read from
-// positions [num_axes, tokens]. An axis outside that range counts as the nearest and is reported.
-//
 // Bound: HBM, each row is read and written once. The angles cost one double product and one sincospif per (token,
 // pair): they are taken once per token by the block, kept in shared memory and used by all heads of Q and K. The rows of
 // a block (its tokens' heads of Q, then of K) are dealt out to groups of threads, a thread keeping its place within the
@@ -41,11 +38,8 @@ struct RotaryArgs {
   void* y[2];             // contiguous [tokens, heads, dim]
   int64_t token_stride[2], head_stride[2];  // of x, in elements
   int heads[2];
-  const void* positions;  // int32 or int64 [tokens], or [num_axes, tokens]
+  const void* positions;  // int32 or int64 [tokens]
   int positions64;
-  const int* axes;        // [rotary_dim / 2] axis of each pair, nullptr: one axis
-  int num_axes;
-  uint32_t* err;
   const float* inv_freq;  // [rotary_dim / 2]
   int tokens, dim, rotary_dim;
   float scale, sign;
@@ -82,7 +76,8 @@ __device__ __forceinline__ double turn_fraction(int64_t position, float frequenc
   return (t - rint(t)) + (t_low - rint(t_low));
 }
 
-// Position of token t on pair i's axis.
+// Position of token t on pair i's axis, for several of them: positions [num_axes, tokens], pair i takes axes[i]. An axis out of
+// range counts as the nearest and is reported. axes nullptr: one axis.
 __device__ __forceinline__ int64_t position_of(const void* positions, int positions64, const int* axes, int num_axes, int tokens,
                                                int64_t t, int i, uint32_t* err) {
   if (axes) {
@@ -166,7 +161,7 @@ __global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const __grid_con
   load(g0);
   for (int i = threadIdx.x; i < nt * half; i += kRotaryThreads) {
     const int64_t t = t0 + i / half;
-    const int64_t at = position_of(a.positions, a.positions64, a.axes, a.num_axes, a.tokens, t, i % half, a.err);
+    const int64_t at = a.positions64 ? static_cast<const int64_t*>(a.positions)[t] : static_cast<const int*>(a.positions)[t];
     const double turn = turn_fraction(at, a.inv_freq[i % half]);
     float s, c;
     sincospif(2.0f * static_cast<float>(turn), &s, &c);

@@ -121,7 +121,7 @@ __global__ void __launch_bounds__(kPlanThreads) varattn_bwd_prep_kernel(const __
   constexpr int kTpr = kD / 8, kRowsAtOnce = kPlanThreads / kTpr;  // 64 or 128 rows
   const int slot = (blockIdx.x - 2) / a.head_groups, first = (blockIdx.x - 2) % a.head_groups;
   VarItem it;
-  if (!plan_item(a.plan[0], slot, it) || it.b1 <= it.b0) return;
+  if (!plan_item(a.plan[0], a.plan[0].cu, nullptr, slot, it) || it.b1 <= it.b0) return;
   const int c = threadIdx.x % kTpr;
 #pragma unroll
   for (int r0 = 0; r0 < kVarBlk; r0 += kRowsAtOnce) {

@@ -91,6 +91,54 @@ def test_steps_in_a_captured_graph(no_device_error, cuda_dev):
         _, _, _, kv, stack, table = pa.plan_steps(kv, new, table, stack, page, 20)
 
 
+def test_results_are_tensors_of_their_own(no_device_error, cuda_dev):
+    """In inference mode and out of it: results may be changed in place, and a change of one leaves the others."""
+    kv, new = [3, 0, 21], [2, 9, 1]
+    for mode in (torch.inference_mode, torch.enable_grad):
+        with mode():
+            t, table, stack = make(kv, new, 8, cuda_dev)
+            out = bsk.kv_cache_plan(**t, page_size=8, tokens=15)
+            keep = [x.tolist() for x in out]
+            for i, x in enumerate(out):
+                assert x.is_contiguous() and not x.requires_grad
+                x += 1
+                assert x.tolist() == [y + 1 for y in keep[i]]
+                x -= 1
+            assert [x.tolist() for x in out] == keep
+            check(out, t, kv, new, table, stack, 8, 15)
+
+
+def test_two_streams_at_once(no_device_error, cuda_dev):
+    """Calls of all the serving operators side by side on two streams give what they give one after the other."""
+    torch.manual_seed(0)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    f, _ = bsk.rotary_frequencies(64, device=cuda_dev)
+    w = torch.rand(64, device=cuda_dev).add(0.5).bfloat16()
+
+    def step(seed, lens):
+        t, _, _ = make(lens, [n % 7 + 1 for n in lens], 8, cuda_dev, seed=seed)
+        rows = sum(n % 7 + 1 for n in lens)
+        slots, pos, cu, kv, _ = bsk.kv_cache_plan(**t, page_size=8, tokens=rows)
+        g = torch.Generator(device=cuda_dev).manual_seed(seed)
+        q, k, v = (torch.randn(rows, h, 64, generator=g, device=cuda_dev).bfloat16() for h in (4, 2, 2))
+        pages = int(t["free_pages"].max()) + int(t["block_table"].max()) + 2
+        cache = [torch.randn(pages, 8, 2, 64, generator=g, device=cuda_dev).bfloat16() for _ in range(2)]
+        q, k = bsk.qk_norm_rotary(q, k, w, w, pos, f)
+        bsk.kv_cache_append(k, v, *cache, slots)
+        return bsk.attention_paged(q, *cache, t["block_table"], kv, cu, window=20, sinks=2)
+
+    jobs = [(1, [5, 90, 400]), (2, [33] * 40)]
+    want = [step(*j) for j in jobs]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(4):
+        for s, j in zip(streams, jobs):
+            with torch.cuda.stream(s):
+                got.append(step(*j))
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, want[i % 2]) for i, g in enumerate(got))
+
+
 def reported():
     with pytest.raises(RuntimeError):
         bsk.synchronize_and_check()

@@ -89,10 +89,10 @@ cudaError_t launch_any(NormRotaryArgs& a, bool inter, Pass pass, int sm_count, c
   return launch_layout<T, kVec, kUnits, Pass::kForward>(a, inter, sm_count, s);
 }
 
-// Whether every row can be read and written in pieces of kVec elements, `bytes` wide.
-bool fits(const NormRotaryArgs& a, bool inter, bool backward, int vec, int elem, int bytes) {
-  const int r = a.rotary_dim;
-  if ((a.dim - r) % (2 * vec) || (inter ? r % (2 * vec) : (r / 2) % vec)) return false;
+// Whether every row can be read and written in pieces of `vec` elements of `elem` bytes.
+bool fits(const NormRotaryArgs& a, bool inter, bool backward, int vec, int elem) {
+  const int r = a.rotary_dim, bytes = vec * elem;
+  if (a.dim % (2 * vec) || (inter ? r % vec : (r / 2) % vec)) return false;
   const auto on = [&](const void* p) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; };
   for (int w = 0; w < 2; ++w) {
     if (!a.heads[w]) continue;
@@ -104,22 +104,23 @@ bool fits(const NormRotaryArgs& a, bool inter, bool backward, int vec, int elem,
   return true;
 }
 
-// 16-byte pieces where rows and halves allow them, else 4-byte ones, else single elements (dim 80, 40 elements turned, bf16:
-// half of a pair's elements starts at a multiple of 40 bytes).
+// 16-byte pieces where rows and halves allow them, else 8- and 4-byte ones, else single elements (dim 80, 40 elements turned, bf16:
+// the second halves of the pairs start 40 bytes in, at a multiple of 8; 16383 tokens, 32 + 8 heads, with gradients: 253 us in
+// 8-byte pieces and four blocks on an SM, 677 us in 4-byte ones and one block).
 template <class T>
 cudaError_t pick(NormRotaryArgs& a, bool inter, Pass pass, int sm_count, cudaStream_t s) {
   const bool backward = pass == Pass::kBackward;
   constexpr int kWide = 16 / sizeof(T), kElem = sizeof(T);
-  a.aligned32 = fits(a, inter, backward, kWide, kElem, 32);
-  if (fits(a, inter, backward, kWide, kElem, 16)) {
+  if (fits(a, inter, backward, kWide, kElem)) {
     if constexpr (kElem == 4)
       if (a.dim > 2 * kWide * 32) return launch_any<T, kWide, 2>(a, inter, pass, sm_count, s);
     return launch_any<T, kWide, 1>(a, inter, pass, sm_count, s);
   }
-  a.aligned32 = 0;
-  if constexpr (kElem == 2)
-    if (fits(a, inter, backward, 2, kElem, 4))
+  if constexpr (kElem == 2) {
+    if (a.dim <= 256 && fits(a, inter, backward, 4, kElem)) return launch_any<T, 4, 1>(a, inter, pass, sm_count, s);
+    if (fits(a, inter, backward, 2, kElem))
       return a.dim <= 128 ? launch_any<T, 2, 1>(a, inter, pass, sm_count, s) : launch_any<T, 2, 4>(a, inter, pass, sm_count, s);
+  }
   return launch_any<T, 1, 8>(a, inter, pass, sm_count, s);
 }
 
@@ -146,8 +147,8 @@ cudaError_t launch_weights(const NormWeightArgs& n, cudaStream_t s) {
 }  // namespace
 
 int64_t norm_rotary_partials(int tokens, int heads, int kv_heads, int dim, int sm_count) {
-  // (no kernel has more than two blocks on an SM, and Q and K get one each at least)
-  return tokens > 0 ? ((int64_t)2 * sm_count + 2) * dim : 0;
+  // (Q and K get one block each at least)
+  return tokens > 0 ? ((int64_t)kNormMostBlocks * sm_count + 2) * dim : 0;
 }
 
 cudaError_t norm_rotary_fwd(int dtype, bool interleaved, NormRotaryArgs a, int sm_count, cudaStream_t s) {

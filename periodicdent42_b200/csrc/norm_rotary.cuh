@@ -10,13 +10,18 @@
 // The same kernel without the norm (kNorm) turns by positions on several axes. (The one-axis rotation has rotary.cuh's kernel,
 // whose results it keeps bit for bit where all axes agree.)
 //
-// A row is held by a group of 4 .. 32 lanes, each with its pairs' both elements, so the two sums of a row are shuffles and the
+// A row is held by a group of 1 .. 32 lanes, each with its pairs' both elements, so the two sums of a row are shuffles and the
 // row is read once. A group keeps to one token: the angles' sines and cosines and the weights stay in its lanes' registers for
-// all of its heads, of which kNormBatch rows are loaded before any is used (and before the angles are taken). The backward
-// gives Q and K blocks of their own, so that a thread adds up dw of one weight, walks the tokens with a fixed stride and
-// leaves one partial row of dw per block; a second kernel adds those up in a fixed order (no atomics).
+// all of its heads. The blocks are as many as fit on the SMs, some for Q and the others for K; each walks the tokens with a fixed
+// stride. Rows come through a ring of asynchronous copies in shared memory that each thread fills for itself, kNormBatch rows
+// (backward: kNormBatchBwd of x and of dy) a stage: the next stages, of the next token too, are on their way while one is used,
+// and no thread waits for another's. A thread adds up dw of its own weights and a block leaves one partial row; a second kernel
+// adds those up in a fixed order (no atomics).
 //
-// Bound: HBM, x read and y written once (backward: x and dy read, dx written).
+// Bound: HBM at first, x read and y written once (backward: x and dy read, dx written), then issue slots: the packed two-float
+// instructions halve the arithmetic, and what is left still takes about half of all slots. bf16, 16383 tokens, 32 + 8 heads of
+// 128: 70 us forward (4.8 TB/s; 50 % of the slots), 114 us backward (4.4 TB/s; 60 %); the rotation alone on three axes 68 us.
+// fp32: 275 us both ways (6.1 TB/s).
 #pragma once
 
 #include <type_traits>
@@ -28,6 +33,7 @@
 namespace bsk {
 
 constexpr int kNormThreads = 256;
+constexpr int kNormMostBlocks = 6;  // on an SM
 constexpr int kNormBatch = 4;     // rows of a thread's step, forward
 constexpr int kNormBatchBwd = 2;  // backward: rows of x and of dy
 
@@ -47,7 +53,6 @@ struct NormRotaryArgs {
   const float* inv_freq;
   int tokens, dim, rotary_dim;
   float scale, sign, eps;          // sign: of the angles
-  int aligned32;                   // every row starts at a multiple of 32 bytes
   int group, units;                // lanes and units of a row
   int at_once[2], per_block[2];    // heads of a token side by side, tokens of a chunk
   int grid, blocks_q;              // blocks, and those of them that take Q; the others take K
@@ -55,18 +60,30 @@ struct NormRotaryArgs {
   uint32_t* err;
 };
 
-// Unit u of a head: kVec pairs (or, in the part that is not turned, 2 kVec elements), as two pieces of kVec elements.
+// Unit u of a head: kVec pairs (or, in the part that is not turned, 2 kVec elements), as two pieces of kVec elements, each beside
+// the neighbouring lanes' ones. Half layout: the pairs' first elements and their second ones. Interleaved: kVec / 2 pairs from
+// either half of the head (single elements: a pair).
 template <int kVec, bool kInter>
 struct NormUnit {
-  int e0, e1, pair;
-  bool turned, live;
+  static constexpr int kFirst = kInter && kVec > 1 ? kVec / 2 : kVec;  // pairs of the first piece
+  int e0, e1, pair0, pair1;  // first elements of the pieces; the unit's pairs are pair0 + k, from k = kFirst on pair1 + k - kFirst
+  bool live, turned0, turned1;
   __device__ __forceinline__ NormUnit(int u, int units, int half) {
     live = u < units;
-    pair = live ? u * kVec : 0;
-    turned = live && pair < half;
-    const bool joined = kInter || !turned;
-    e0 = joined ? 2 * pair : pair;
-    e1 = joined ? e0 + kVec : pair + half;
+    const int n = live ? u : 0;
+    if constexpr (kInter && kVec > 1) {
+      e0 = n * kVec;
+      e1 = (units + n) * kVec;
+      pair0 = e0 / 2;
+      pair1 = e1 / 2;
+      turned0 = live && pair0 < half;
+      turned1 = live && pair1 < half;
+    } else {
+      pair0 = pair1 = n * kVec;
+      turned0 = turned1 = live && pair0 < half;
+      e0 = kInter || !turned0 ? 2 * pair0 : pair0;
+      e1 = kInter || !turned0 ? e0 + kVec : pair0 + half;
+    }
   }
 };
 
@@ -197,26 +214,59 @@ template <int kVec>
 struct Turn {
   float c[kVec], s[kVec];
 };
-// dz = R^T dy
-template <int kVec>
+// dz = R^T dy for pairs [kFrom, kTo)
+template <int kFrom, int kTo, int kVec>
 __device__ __forceinline__ void turn_back(Halves<kVec>& f, const Turn<kVec>& r) {
-  float u[kVec], w[kVec];
-  v_mul(u, f.b, r.s);
-  v_mul(w, f.b, r.c);
-  v_fma(u, f.a, r.c, u);
-  v_nfma(f.b, f.a, r.s, w);
+  constexpr int N = kTo - kFrom;
+  if constexpr (N > 0) {
+    float a[N], b[N], c[N], s[N], u[N], w[N];
 #pragma unroll
-  for (int k = 0; k < kVec; ++k) f.a[k] = u[k];
+    for (int k = 0; k < N; ++k) {
+      a[k] = f.a[kFrom + k];
+      b[k] = f.b[kFrom + k];
+      c[k] = r.c[kFrom + k];
+      s[k] = r.s[kFrom + k];
+    }
+    v_mul(u, b, s);
+    v_mul(w, b, c);
+    v_fma(u, a, c, u);
+    v_nfma(w, a, s, w);
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      f.a[kFrom + k] = u[k];
+      f.b[kFrom + k] = w[k];
+    }
+  }
 }
-
-// A unit's two pieces: neighbours in the interleaved layout, one access where rows start at multiples of 32 bytes.
-template <bool kInter, class T, class P>
-__device__ __forceinline__ void store_pieces(T* y, int apart, int aligned32, const P& p, const P& q) {
-  if constexpr (kInter) {
-    store_pair(y, y + apart, aligned32 != 0, p, q);
-  } else {
-    *reinterpret_cast<P*>(y) = p;
-    *reinterpret_cast<P*>(y + apart) = q;
+// y = (a ca.c + b cb.s, a ca.s + b cb.c) for pairs [kFrom, kTo); not turned: (a ca.c, b cb.c)
+template <int kFrom, int kTo, int kVec>
+__device__ __forceinline__ void turn_ahead(const Halves<kVec>& f, const Turn<kVec>& ca, const Turn<kVec>& cb, bool turned, Halves<kVec>& y) {
+  constexpr int N = kTo - kFrom;
+  if constexpr (N > 0) {
+    float a[N], b[N], ac[N], as[N], bc[N], bs[N], u[N], w[N];
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      a[k] = f.a[kFrom + k];
+      b[k] = f.b[kFrom + k];
+      ac[k] = ca.c[kFrom + k];
+      as[k] = ca.s[kFrom + k];
+      bc[k] = cb.c[kFrom + k];
+      bs[k] = cb.s[kFrom + k];
+    }
+    if (turned) {
+      v_mul(u, b, bs);
+      v_fma(u, a, ac, u);
+      v_mul(w, b, bc);
+      v_fma(w, a, as, w);
+    } else {
+      v_mul(u, a, ac);
+      v_mul(w, b, bc);
+    }
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      y.a[kFrom + k] = u[k];
+      y.b[kFrom + k] = w[k];
+    }
   }
 }
 
@@ -300,7 +350,9 @@ __device__ __forceinline__ void read_turns(const NormRotaryArgs& a, const float2
     const NormUnit<kVec, kInter> u(group * n + lane, a.units, a.rotary_dim / 2);
 #pragma unroll
     for (int k = 0; k < kVec; ++k) {
-      const float2 r = u.turned && any ? rot[u.pair + k] : make_float2(1.0f, 0.0f);
+      const bool second = k >= NormUnit<kVec, kInter>::kFirst, turned = second ? u.turned1 : u.turned0;
+      const int pair = second ? u.pair1 + k - NormUnit<kVec, kInter>::kFirst : u.pair0 + k;
+      const float2 r = turned && any ? rot[pair] : make_float2(1.0f, 0.0f);
       t[n].c[k] = r.x;
       t[n].s[k] = r.y;
     }
@@ -354,7 +406,8 @@ struct NormShape {
   static constexpr int kRows = kBackward ? kNormBatchBwd : kNormBatch;
   static constexpr int kTensors = kBackward ? 2 : 1;
   using Ring = NormRing<P, kRows * kUnits * 2 * kTensors>;
-  static constexpr int kBlocksPerSm = kVec * sizeof(T) == 16 && kUnits == 1 ? 2 : 1;  // by registers and shared memory
+  // by registers and shared memory: about as much on its way in an SM whatever a piece's size
+  static constexpr int kBlocksPerSm = kUnits > 1 ? 1 : 32 / (kVec * (int)sizeof(T)) < kNormMostBlocks ? 32 / (kVec * (int)sizeof(T)) : kNormMostBlocks;
   static constexpr int kMostSmem = Ring::kBytes + 20 * 1024;
   // the ring (at the end the groups' sums of dw), a chunk's angles, the weights
   static __host__ __device__ int weights_at(const NormRotaryArgs& a) {
@@ -494,26 +547,21 @@ __global__ void __launch_bounds__(kNormThreads, NormShape<T, kVec, kUnits, false
           if (!u.live) continue;
           Halves<kVec> y_f;
           P po, qo;
-          if (u.turned) {
-            v_mul(y_f.a, f[n].b, cb[n].s);
-            v_fma(y_f.a, f[n].a, ca[n].c, y_f.a);
-            v_mul(y_f.b, f[n].b, cb[n].c);
-            v_fma(y_f.b, f[n].a, ca[n].s, y_f.b);
-          } else if constexpr (kNorm) {
-            v_mul(y_f.a, f[n].a, ca[n].c);
-            v_mul(y_f.b, f[n].b, cb[n].c);
-          }
-          if constexpr (kNorm) {
-            v_scale(y_f.a, inv);
-            v_scale(y_f.b, inv);
-          }
-          if (kNorm || u.turned) {
+          if (kNorm || u.turned0 || u.turned1) {
+            turn_ahead<0, Unit::kFirst>(f[n], ca[n], cb[n], u.turned0, y_f);
+            turn_ahead<Unit::kFirst, kVec>(f[n], ca[n], cb[n], u.turned1, y_f);
+            if constexpr (kNorm) {
+              v_scale(y_f.a, inv);
+              v_scale(y_f.b, inv);
+            }
             pack_pieces<T, kVec, kInter>(y_f, po, qo);
-          } else {
-            po = *reinterpret_cast<const P*>(Ring::at(ring, now.stage, (b * kUnits + n) * 2));
-            qo = *reinterpret_cast<const P*>(Ring::at(ring, now.stage, (b * kUnits + n) * 2 + 1));
           }
-          store_pieces<kInter>(y + u.e0, u.e1 - u.e0, a.aligned32, po, qo);
+          if constexpr (!kNorm) {  // what is not turned is copied as it is
+            if (!u.turned0) po = *reinterpret_cast<const P*>(Ring::at(ring, now.stage, (b * kUnits + n) * 2));
+            if (!u.turned1) qo = *reinterpret_cast<const P*>(Ring::at(ring, now.stage, (b * kUnits + n) * 2 + 1));
+          }
+          *reinterpret_cast<P*>(y + u.e0) = po;
+          *reinterpret_cast<P*>(y + u.e1) = qo;
         }
       }
       now.next(blk.rounds, blk.blocks, Ring::kStages);
@@ -619,7 +667,8 @@ __global__ void __launch_bounds__(kNormThreads, NormShape<T, kVec, kUnits, true>
                                          *reinterpret_cast<const P*>(Ring::at(ring, now.stage, piece + 1)), x[n]);
           unpack_pieces<T, kVec, kInter>(*reinterpret_cast<const P*>(Ring::at(ring, now.stage, piece + 2)),
                                          *reinterpret_cast<const P*>(Ring::at(ring, now.stage, piece + 3)), dz[n]);
-          if (u.turned) turn_back<kVec>(dz[n], turn[n]);
+          if (u.turned0) turn_back<0, Unit::kFirst>(dz[n], turn[n]);
+          if (u.turned1) turn_back<Unit::kFirst, kVec>(dz[n], turn[n]);
         }
         sums();
         if constexpr (!std::is_same<T, __half>::value) {
@@ -658,7 +707,8 @@ __global__ void __launch_bounds__(kNormThreads, NormShape<T, kVec, kUnits, true>
           v_scale(g_f.b, out);
           P po, qo;
           pack_pieces<T, kVec, kInter>(g_f, po, qo);
-          store_pieces<kInter>(y + u.e0, u.e1 - u.e0, a.aligned32, po, qo);
+          *reinterpret_cast<P*>(y + u.e0) = po;
+          *reinterpret_cast<P*>(y + u.e1) = qo;
         }
       }
       now.next(blk.rounds, blk.blocks, Ring::kStages);

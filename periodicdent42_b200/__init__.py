@@ -13,6 +13,9 @@ functions and signatures, backed by hand-written tcgen05/TMA kernels behind a C 
     >>> Q, K = bsk.rotary_embedding(Q, K, positions, inv_freq)    # serving: rotary, cache, attention over the cache
     >>> bsk.kv_cache_append(K, V, k_cache, v_cache, slots, k_scale, v_scale)
     >>> O = bsk.attention_paged(Q, k_cache, v_cache, block_table, kv_lens, cu_seqlens, k_scale=k_scale, v_scale=v_scale)
+    >>> O = bsk.attention_varlen(Q, K, V, cu_seqlens, window=1024, sinks=4)      # also attention_paged
+    >>> Q, K = bsk.qk_norm_rotary(Q, K, q_weight, k_weight, positions, inv_freq) # RMS norm of each head, then rotary
+    >>> slots, positions, cu_seqlens, kv_lens, left = bsk.kv_cache_plan(kv_lens, new_lens, block_table, stack, left, 64, rows)
 """
 
 __version__ = "0.9.0+sm100a"

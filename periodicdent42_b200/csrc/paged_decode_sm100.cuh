@@ -26,6 +26,12 @@
 //   - the values' scales enter the exponent: w_j = 2^(s_j + log2 scale_j - m_w) with a running maximum m_w of its own, so
 //     the rounded weights span (0, 1] whatever the scales are, and O = sum_j w_j code_j 2^(m_w) beside l = sum_j p_j 2^m.
 //
+// A window with sinks (kWin): the pieces between the sinks' and the first that the tile's first row sees are left out of what is
+// dealt out; slots of keys that no row sees are not looked up, their copies are zeros. All tiles are then of one length, which
+// changes what is best for warps (see the launch): 64 sequences, window 1024, e4m3 cache: 40 us in a graph, 3.4 TB/s, where the
+// same rows without a window and uneven lengths run at 4.7. Bound there: a CTA's start and first copies (a warp has 11 stages
+// of 32 keys; long_scoreboard, issue 42 %).
+//
 // P (or w) is rounded to 16 bits for the second product (half a step: 2^-8 of a weight in bf16, 2^-11 in fp16, the
 // outputs' own rounding or finer); its sum is taken in fp32 before the rounding.
 #pragma once

@@ -33,13 +33,22 @@
 // wait for it. So the conversion's and the two issuers' loops are rolled (1024 new tokens over 30000, 32 / 8 heads, D 128:
 // 1047 us; when it was 1033: conversion unrolled 1126, issuers unrolled 1189, both 1203; 16-bit cache 555).
 //
+// A window with sinks (kWin: a row at position p sees keys (p - window, p] and [0, sinks)): a tile's list of key blocks is the
+// sinks' blocks and then those from the first one that its first row sees, so blocks that no row sees are neither copied nor
+// multiplied (32768 tokens, window 4096, 32 / 8 heads, D 128: 2.5 ms, 820 TFLOP/s; without a window 9.3). Three kinds of
+// blocks compare: the causal edge, the window's lower edge, the sinks' last. Over e4m3 caches a row's scale reference follows the
+// keys that this row sees: an unseen key's scale would push the row's own weights below fp16's range, so masked blocks take the
+// largest scale of the row's own range (range_top).
+//
 // P is rounded to the operands' type (half a step: 2^-8 of a weight in bf16, 2^-11 in fp16), its sums are fp32 and taken before.
 //
 // Bound: each key block's own chain of steps -- scores, maximum, exchange between the two warps of a row, exponentials, P, with
 // one query tile in flight per CTA; no pipe is at its limit (8192 tokens, 32 / 8 heads, D 128: tensor pipe 47 % of the time,
 // issue 49 %, XU 35 %, DRAM 3 %; 552 us in short runs, 646 when repeated under the power cap). Packing the group's heads into
 // the tile means a causal tile spans only TT tokens, so less of its last block is masked, and one K / V tile feeds the whole
-// group.
+// group. With the window above: tensor pipe 45 %, issue 49 %, XU 34 %; the two masked blocks of a tile's 34 make little of it, in
+// short windows they make most (8192 tokens, window 1024, 10 blocks a tile: 195 us at 80 us of products). Two query tiles in flight
+// (a thread a row of 128 keys, rows in one CTA by turns) were no faster: 2.4-2.5 ms for 2.2-2.5.
 #pragma once
 
 #include <type_traits>

@@ -1,6 +1,6 @@
 // Host side of the C ABI (include/bsk_capi.h): argument validation, per-device set-up, TMA tensor-map
-// encoding and kernel launches. Every kernel of the library is compiled here but those of window.cu; kernels get the device
-// error word below as an argument.
+// encoding and kernel launches. Every kernel of the library is compiled here but those of window.cu and norm_rotary.cu; kernels
+// get the device error word below as an argument.
 #include <cuda.h>
 #include <cuda_runtime.h>
 #include <cudaTypedefs.h>
@@ -2353,7 +2353,8 @@ int64_t varlen_workspace(int64_t tokens, int64_t batch, int heads, int kv_heads,
 }
 
 // What the backward needs beside that for key blocks with sinks, which are split along their query tiles: a list with room for
-// the pieces, the split blocks and the pieces' fp32 rows. A sequence has at most win_sink_blocks of them, each of at most its tiles / plan_window_tiles + 1 pieces.
+// the pieces, the split blocks and the pieces' fp32 rows. A sequence has at most win_sink_blocks of them, each of at most its tiles /
+// plan_window_tiles + 1 pieces.
 struct KeySplitPlan {
   int64_t pieces;  // 0: nothing is split
   int64_t list_at, splits_at, rows_at, total;

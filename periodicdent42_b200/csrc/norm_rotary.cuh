@@ -548,12 +548,12 @@ __global__ void __launch_bounds__(kNormThreads, NormShape<T, kVec, kUnits, false
           Halves<kVec> y_f;
           P po, qo;
           if (kNorm || u.turned0 || u.turned1) {
+            if constexpr (kNorm) {  // (before the turn: a large row times a large scale would pass fp32's range)
+              v_scale(f[n].a, inv);
+              v_scale(f[n].b, inv);
+            }
             turn_ahead<0, Unit::kFirst>(f[n], ca[n], cb[n], u.turned0, y_f);
             turn_ahead<Unit::kFirst, kVec>(f[n], ca[n], cb[n], u.turned1, y_f);
-            if constexpr (kNorm) {
-              v_scale(y_f.a, inv);
-              v_scale(y_f.b, inv);
-            }
             pack_pieces<T, kVec, kInter>(y_f, po, qo);
           }
           if constexpr (!kNorm) {  // what is not turned is copied as it is

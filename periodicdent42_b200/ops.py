@@ -468,7 +468,8 @@ def qk_norm_rotary(Q: torch.Tensor, K: Optional[torch.Tensor], q_weight: torch.T
     z = x / sqrt(mean(x^2) + eps) * weight over a head's dim elements, then z turned as by :func:`rotary_embedding`, whose
     arguments (and types, strides, several axes) apply. q_weight and k_weight: [dim] of the rows' dtype or float32 (K and
     k_weight may be None). fp32 inside, rounded once; eps at least 1e-30. Differentiable (once, in reverse mode) in Q, K and the
-    weights (deterministic, no atomics)."""
+    weights (deterministic, no atomics). Rows may be as large as their type holds; weight times scale, and in the backward a
+    row's elements times its gradient's, scale and weight, must stay within fp32's range."""
     return _C().qk_norm_rotary(Q, K, q_weight, k_weight, positions, inv_freq, interleaved, scale, eps, axes)
 
 
@@ -531,9 +532,9 @@ def attention_paged(Q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     their table entries hold anything.
     A row that sees no key is zero, and so are rows behind the last sequence. Stale contents of a page behind its
     sequence's end reach no row, NaN among them; a non-finite value inside a sequence may make rows of it NaN that see it
-    with weight zero or are masked for it, fewer than 256 tokens before it (or behind, where a window leaves it out). The softmax's
-    weights are rounded to Q's type for their product with V; over e4m3 caches they are weight times the value's scale, rounded to fp16. For serving: has no
-    gradient, and tensors that require one are refused outside torch.no_grad()."""
+    with weight zero or are masked for it, fewer than 256 tokens before it (or behind, where a window leaves it out). The
+    softmax's weights are rounded to Q's type for their product with V; over e4m3 caches they are weight times the value's scale,
+    rounded to fp16. For serving: has no gradient, and tensors that require one are refused outside torch.no_grad()."""
     if scale is None:
         scale = Q.shape[-1] ** -0.5 if Q.dim() and Q.shape[-1] else 1.0
     return _C().attention_paged(Q, k_cache, v_cache, block_table, kv_lens, cu_seqlens, scale, k_scale, v_scale,

@@ -73,6 +73,17 @@ def test_rows_of_every_size(no_device_error, cuda_dev, dtype):
     assert (got[0][0] == 0).all()
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("inter", [False, True])
+def test_large_rows_and_a_large_scale(no_device_error, cuda_dev, dtype, inter):
+    """Rows of 1e18 times a scale of 1e25 pass fp32's range, their results do not."""
+    f = bsk.rotary_frequencies(64, device=cuda_dev)[0]
+    q, k, qw, kw, _, _, pos = make(50, 4, 2, 128, dtype, cuda_dev, size=1e18)
+    for x, w, y in zip((q, k), (qw, kw), bsk.qk_norm_rotary(q, k, qw, kw, pos, f, interleaved=inter, scale=1e25)):
+        assert torch.isfinite(y).all()
+        assert pa.worst(y, *pa.norm_rotary64(x, w, pos, f, inter, 1e25, EPS)["y"]) <= 1.0
+
+
 @pytest.mark.parametrize("eps", [1e-30, 1e-3, 10.0])
 def test_eps(no_device_error, cuda_dev, eps):
     f = bsk.rotary_frequencies(64, device=cuda_dev)[0]

@@ -176,12 +176,27 @@ __device__ __forceinline__ constexpr int second_of(int k) { return kInter ? 2 * 
 
 template <class T, int kVec, bool kInter>
 __device__ __forceinline__ void unpack_pieces(const Pack<T, kVec>& p, const Pack<T, kVec>& q, Halves<kVec>& f) {
+  float e[2 * kVec];
+  if constexpr (std::is_same<T, __nv_bfloat16>::value && kVec % 2 == 0) {  // a shift and a mask for two elements
+    uint32_t w[kVec];
+    memcpy(w, &p, sizeof(p));
+    memcpy(w + kVec / 2, &q, sizeof(q));
+#pragma unroll
+    for (int k = 0; k < kVec; ++k) {
+      e[2 * k] = __uint_as_float(w[k] << 16);
+      e[2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u);
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < kVec; ++k) {
+      e[k] = to_f32<T>(p.v[k]);
+      e[kVec + k] = to_f32<T>(q.v[k]);
+    }
+  }
 #pragma unroll
   for (int k = 0; k < kVec; ++k) {
-    constexpr int n = kVec;
-    const int i = first_of<kVec, kInter>(k), j = second_of<kVec, kInter>(k);
-    f.a[k] = to_f32<T>(i < n ? p.v[i % n] : q.v[i % n]);
-    f.b[k] = to_f32<T>(j < n ? p.v[j % n] : q.v[j % n]);
+    f.a[k] = e[first_of<kVec, kInter>(k)];
+    f.b[k] = e[second_of<kVec, kInter>(k)];
   }
 }
 

@@ -29,36 +29,75 @@ cudaError_t run(K kernel, std::atomic<uint64_t>& ready, int most, int grid, int 
   return cudaGetLastError();
 }
 
-// Blocks that Q (w = 0) and K get of `per_sm` on each SM, by what their rows and a token's angles cost (the angles about what
-// six heads do), and no more than there are chunks.
-int blocks_of(const int (&heads)[2], int w, int per_sm, int64_t chunks, int sm_count) {
-  if (!heads[w]) return 0;
-  const auto cost = [&](int i) { return heads[i] ? (int64_t)heads[i] + 6 : 0; };
-  return (int)std::max<int64_t>(1, std::min(chunks, per_sm * sm_count * cost(w) / (cost(0) + cost(1))));
+enum class Pass { kForward, kBackward, kTurn };  // kTurn: the rotation alone
+
+// How a tensor's heads and tokens are dealt to a block's groups, and what a chunk of it costs.
+struct Deal {
+  int at_once, per_block;
+  int64_t chunks, cost;
+};
+// `most` heads of a token for each group. Costs in eighths of a row's, by the instructions counted for each: what a chunk takes
+// per thread beside its rows (angles and weights to registers), and an element of the angles.
+Deal deal(const NormRotaryArgs& a, int w, int groups, int rows, int most, Pass pass) {
+  const int at_once = std::max(1, std::min(groups, (a.heads[w] + most - 1) / most)), per_block = groups / at_once;
+  const int64_t steps = (a.heads[w] + rows * at_once - 1) / (rows * at_once);
+  const int64_t elements = ((int64_t)per_block * (a.rotary_dim / 2) + kNormThreads - 1) / kNormThreads;
+  const int chunk = pass == Pass::kForward ? 11 : pass == Pass::kBackward ? 3 : 5, angle = 6;
+  return {at_once, per_block, ((int64_t)a.tokens + per_block - 1) / per_block, steps * rows * 8 + chunk + elements * angle};
 }
 
-enum class Pass { kForward, kBackward, kTurn };  // kTurn: the rotation alone
+// The blocks of Q and of K out of `most` together, and how each is dealt: what ends first by the costs, where every block takes
+// whole chunks. Few tokens: as many heads of a token at once as there are groups, so that a token takes one step. Measured (us,
+// 16383 tokens, 32 + 8 heads of 128 with gradients; four heads a group and blocks by the heads / up to 8 / up to 16, by costs):
+// bf16 179 / 171 / 162, three axes without the norm 135 / 121 / 133 (long chunks of angles leave the copies idle), fp32 266 (four
+// heads by costs) / 291 / 299; 16 + 4 heads of 256 230 / 218 / 202; 4096 tokens 58 / 55 / 55, 2048 32 / 33 / 34.
+void deal_blocks(NormRotaryArgs& a, int groups, int rows, int most, int widest, bool few, Pass pass) {
+  if (few || !a.heads[0] || !a.heads[1]) {
+    const Deal d[2] = {deal(a, 0, groups, rows, few ? 1 : 8, pass), deal(a, 1, groups, rows, few ? 1 : 8, pass)};
+    int blocks[2] = {0, 0};
+    for (int w = 0; w < 2; ++w) {
+      a.at_once[w] = d[w].at_once;
+      a.per_block[w] = few ? 1 : d[w].per_block;
+      const int64_t chunks = few ? a.tokens : d[w].chunks, work[2] = {a.heads[0] ? a.heads[0] + 6 : 0, a.heads[1] ? a.heads[1] + 6 : 0};
+      if (a.heads[w]) blocks[w] = (int)std::max<int64_t>(1, std::min(chunks, most * work[w] / (work[0] + work[1])));
+    }
+    a.blocks_q = blocks[0];
+    a.grid = blocks[0] + blocks[1];
+    return;
+  }
+  int64_t least = INT64_MAX;
+  for (int i = 4; i <= widest; i *= 2)
+    for (int j = 4; j <= widest; j *= 2) {
+      const Deal q = deal(a, 0, groups, rows, i, pass), k = deal(a, 1, groups, rows, j, pass);
+      const double share = (double)(q.chunks * q.cost) / (double)(q.chunks * q.cost + k.chunks * k.cost);
+      const int64_t about = std::max<int64_t>(1, (int64_t)((double)most * share));
+      for (int64_t r = std::max<int64_t>(1, (q.chunks + about - 1) / about - 1), n = 0; n < 3; ++r, ++n) {  // rounds of Q
+        const int64_t blocks = (q.chunks + r - 1) / r, left = most - blocks;
+        if (left < 1) continue;
+        const int64_t time = std::max(r * q.cost, (k.chunks + left - 1) / left * k.cost);
+        if (time >= least) continue;
+        least = time;
+        a.at_once[0] = q.at_once;
+        a.at_once[1] = k.at_once;
+        a.per_block[0] = q.per_block;
+        a.per_block[1] = k.per_block;
+        a.blocks_q = (int)blocks;
+        a.grid = (int)(blocks + std::min(left, k.chunks));
+      }
+    }
+}
 
 template <class T, int kVec, int kUnits, bool kInter, int kLanes, Pass kPass>
 cudaError_t launch(NormRotaryArgs& a, int sm_count, cudaStream_t s) {
   using Sh = NormShape<T, kVec, kUnits, kPass == Pass::kBackward>;
-  const int groups = kNormThreads / a.group;
-  // A row's lanes keep to one token. Few tokens: as many of its heads at once as there are groups, so that a token takes one
-  // step; many: four heads a group, and the groups left over take other tokens.
-  const bool few = a.tokens <= 4 * sm_count;
-  int grid = 0;
-  for (int w = 0; w < 2; ++w) {
-    a.at_once[w] = std::max(1, std::min(groups, few ? a.heads[w] : (a.heads[w] + 3) / 4));
-    a.per_block[w] = few ? 1 : groups / a.at_once[w];
-    grid += blocks_of(a.heads, w, Sh::kBlocksPerSm, ((int64_t)a.tokens + a.per_block[w] - 1) / a.per_block[w], sm_count);
-    if (w == 0) a.blocks_q = grid;
-  }
-  a.grid = grid;
+  // (a row's lanes keep to one token)
+  constexpr int kWidest = sizeof(T) == 4 ? 4 : kPass == Pass::kTurn ? 8 : 16;
+  deal_blocks(a, kNormThreads / a.group, Sh::kRows, Sh::kBlocksPerSm * sm_count, kWidest, a.tokens <= 4 * sm_count, kPass);
   static std::atomic<uint64_t> ready{0};
   if constexpr (kPass == Pass::kBackward)
-    return run(norm_rotary_bwd_kernel<T, kVec, kUnits, kInter, kLanes>, ready, Sh::kMostSmem, grid, Sh::smem_bytes(a), a, s);
+    return run(norm_rotary_bwd_kernel<T, kVec, kUnits, kInter, kLanes>, ready, Sh::kMostSmem, a.grid, Sh::smem_bytes(a), a, s);
   else
-    return run(norm_rotary_kernel<T, kVec, kUnits, kInter, kLanes, kPass == Pass::kForward>, ready, Sh::kMostSmem, grid,
+    return run(norm_rotary_kernel<T, kVec, kUnits, kInter, kLanes, kPass == Pass::kForward>, ready, Sh::kMostSmem, a.grid,
                Sh::smem_bytes(a), a, s);
 }
 

@@ -19,9 +19,8 @@
 // adds those up in a fixed order (no atomics).
 //
 // Bound: HBM at first, x read and y written once (backward: x and dy read, dx written), then issue slots: the packed two-float
-// instructions halve the arithmetic, and what is left still takes about half of all slots. bf16, 16383 tokens, 32 + 8 heads of
-// 128: 70 us forward (4.8 TB/s; 50 % of the slots), 114 us backward (4.4 TB/s; 60 %); the rotation alone on three axes 68 us.
-// fp32: 275 us both ways (6.1 TB/s).
+// instructions halve the arithmetic, and what is left still takes about half of all slots. 16383 tokens, 32 + 8 heads of 128, us
+// (TB/s): bf16 forward 64 (5.2), both ways 163 (5.2); the rotation alone on three axes 60 (5.6); fp32 both ways 266 (6.3).
 #pragma once
 
 #include <type_traits>
@@ -337,22 +336,46 @@ __device__ __forceinline__ void read_weights(const float* src, int unit, int uni
   }
 }
 
-// (cos, sin) * scale of `count` tokens from t0 on: [token][pair]. Element threadIdx.x is pair `pair0` of token `it0`.
-__device__ __forceinline__ void norm_angles(const NormRotaryArgs& a, int64_t t0, int count, int it0, int pair0, float2* rot) {
-  const int half = a.rotary_dim / 2, tokens = kNormThreads / half, pairs = kNormThreads % half;
-  for (int it = it0, pair = pair0, i = threadIdx.x; it < count; i += kNormThreads) {
-    const int64_t at = position_of(a.positions, a.positions64, a.axes, a.num_axes, a.tokens, t0 + it, pair, a.err);
-    float s, c;
-    sincospif(2.0f * static_cast<float>(turn_fraction(at, a.inv_freq[pair])), &s, &c);
-    rot[i] = make_float2(c * a.scale, a.sign * s * a.scale);
-    it += tokens;
-    pair += pairs;
-    if (pair >= half) {
-      pair -= half;
-      ++it;
+// (cos, sin) * scale of a chunk's tokens, [token][pair], element i by thread i % kNormThreads. Where the pairs divide the threads
+// (dim 128: 64 of 256), a thread's pair is the same throughout and its rate is taken once; and most positions are small, exact in
+// 64 bits (both together: three axes, 16383 tokens, both ways, 144.6 us -> 134.7).
+struct NormAngles {
+  int it0, pair0;        // this thread's first token and pair
+  int tokens, pairs;     // what its next element is further
+  TurnRate rate;
+  int64_t start;         // of the positions of its axis
+  __device__ __forceinline__ NormAngles(const NormRotaryArgs& a) {
+    const int half = a.rotary_dim / 2;
+    it0 = threadIdx.x / half;
+    pair0 = threadIdx.x % half;
+    tokens = kNormThreads / half;
+    pairs = kNormThreads % half;
+    pick(a, pair0);
+  }
+  __device__ __forceinline__ void pick(const NormRotaryArgs& a, int pair) {
+    rate = turn_rate(a.inv_freq[pair]);
+    start = axis_start(a.axes, a.num_axes, a.tokens, pair, a.err);
+  }
+  __device__ __forceinline__ void take(const NormRotaryArgs& a, int64_t t0, int count, float2* rot) {
+    const int half = a.rotary_dim / 2;
+    for (int it = it0, pair = pair0, i = threadIdx.x; it < count; i += kNormThreads) {
+      if (pairs) pick(a, pair);
+      const int64_t t = start + t0 + it;
+      const int64_t at = a.positions64 ? static_cast<const int64_t*>(a.positions)[t] : static_cast<const int*>(a.positions)[t];
+      const int low = static_cast<int>(at);
+      const double turn = low == at ? turn_fraction(static_cast<double>(low), 0.0, rate) : turn_fraction(at, rate);
+      float s, c;
+      sincospif(2.0f * static_cast<float>(turn), &s, &c);
+      rot[i] = make_float2(c * a.scale, a.sign * s * a.scale);
+      it += tokens;
+      pair += pairs;
+      if (pair >= half) {
+        pair -= half;
+        ++it;
+      }
     }
   }
-}
+};
 
 // A row whose squares pass fp32's range is multiplied by this first.
 constexpr float kNormDown = 0x1p-100f;
@@ -498,13 +521,13 @@ __global__ void __launch_bounds__(kNormThreads, NormShape<T, kVec, kUnits, false
   for (int i = 0; i < Ring::kStages - 1; ++i) fetch();
   if constexpr (kNorm) stage_weights<T, kVec, kInter>(a, w, w_s);
   const float inv_dim = 1.0f / static_cast<float>(a.dim);
-  const int it0 = threadIdx.x / half, pair0 = threadIdx.x % half;
+  NormAngles angles(a);
   NormStep now{blk.first, 0, 0};
   while (now.chunk < blk.chunks) {
     const int64_t t0 = now.chunk * blk.per_block, t = t0 + blk.it;
     const int rows = blk.rows(a, now.chunk);
     __syncthreads();  // the chunk before has read its angles
-    norm_angles(a, t0, static_cast<int>(min(static_cast<int64_t>(blk.per_block), a.tokens - t0)), it0, pair0, rot);
+    angles.take(a, t0, static_cast<int>(min(static_cast<int64_t>(blk.per_block), a.tokens - t0)), rot);
     __syncthreads();
     // Turn and weights in one: (a, b) -> (a ac + b bs, a as + b bc), bs with the other sign
     Turn<kVec> ca[kUnits], cb[kUnits];
@@ -640,13 +663,13 @@ __global__ void __launch_bounds__(kNormThreads, NormShape<T, kVec, kUnits, true>
 #pragma unroll
     for (int k = 0; k < kVec; ++k) dw[n].a[k] = dw[n].b[k] = 0.0f;
   const float inv_dim = 1.0f / static_cast<float>(a.dim);
-  const int it0 = threadIdx.x / half, pair0 = threadIdx.x % half;
+  NormAngles angles(a);
   NormStep now{blk.first, 0, 0};
   while (now.chunk < blk.chunks) {
     const int64_t t0 = now.chunk * blk.per_block, t = t0 + blk.it;
     const int rows = blk.rows(a, now.chunk);
     __syncthreads();  // the chunk before has read its angles
-    norm_angles(a, t0, static_cast<int>(min(static_cast<int64_t>(blk.per_block), a.tokens - t0)), it0, pair0, rot);
+    angles.take(a, t0, static_cast<int>(min(static_cast<int64_t>(blk.per_block), a.tokens - t0)), rot);
     __syncthreads();
     Turn<kVec> turn[kUnits];
     read_turns<kVec, kUnits, kInter>(a, rot + blk.it * half, group, lane, rows > 0, turn);

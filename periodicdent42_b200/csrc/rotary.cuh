@@ -63,30 +63,39 @@ __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2hal
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-// position * frequency / 2 pi without its whole turns, in (-1, 1). Each number is a 64-bit one and what its rounding dropped.
-__device__ __forceinline__ double turn_fraction(int64_t position, float frequency) {
+// frequency / 2 pi, the turns per position: a 64-bit number and what its rounding dropped.
+struct TurnRate {
+  double g, g_low;
+};
+__device__ __forceinline__ TurnRate turn_rate(float frequency) {
   constexpr double kInv2Pi = 0.15915494309189535, kInv2PiLow = -9.839338337591243e-18;  // 1 / 2 pi to 107 bits
-  const double f = frequency;
-  const double g = f * kInv2Pi, g_low = fma(f, kInv2PiLow, fma(f, kInv2Pi, -g));  // turns per position
+  const double f = frequency, g = f * kInv2Pi;
+  return {g, fma(f, kInv2PiLow, fma(f, kInv2Pi, -g))};
+}
+// position * frequency / 2 pi without its whole turns, in (-1, 1). Each number is a 64-bit one and what its rounding dropped.
+__device__ __forceinline__ double turn_fraction(double p, double p_low, const TurnRate& r) {
+  const double t = p * r.g, t_low = fma(p_low, r.g, fma(p, r.g_low, fma(p, r.g, -t)));
+  return (t - rint(t)) + (t_low - rint(t_low));
+}
+__device__ __forceinline__ double turn_fraction(int64_t position, const TurnRate& r) {
   const double p = static_cast<double>(position);
   // (positions above 2^53; the largest ones round to 2^63, which no int64 holds)
   const double p_low = p < 0x1p63 ? static_cast<double>(position - static_cast<int64_t>(p))
                                   : static_cast<double>(position - INT64_MAX) - 1.0;
-  const double t = p * g, t_low = fma(p_low, g, fma(p, g_low, fma(p, g, -t)));
-  return (t - rint(t)) + (t_low - rint(t_low));
+  return turn_fraction(p, p_low, r);
+}
+__device__ __forceinline__ double turn_fraction(int64_t position, float frequency) {
+  return turn_fraction(position, turn_rate(frequency));
 }
 
-// Position of token t on pair i's axis, for several of them: positions [num_axes, tokens], pair i takes axes[i]. An axis out of
-// range counts as the nearest and is reported. axes nullptr: one axis.
-__device__ __forceinline__ int64_t position_of(const void* positions, int positions64, const int* axes, int num_axes, int tokens,
-                                               int64_t t, int i, uint32_t* err) {
-  if (axes) {
-    const int axis = __ldg(axes + i);
-    const int held = min(max(axis, 0), num_axes - 1);
-    if (held != axis) atomicCAS(err, 0u, kErrBounds | (kKidRotary << 8) | (1u << 16));
-    t += static_cast<int64_t>(held) * tokens;
-  }
-  return positions64 ? static_cast<const int64_t*>(positions)[t] : static_cast<const int*>(positions)[t];
+// Where the positions of pair i's axis begin, for several axes: positions [num_axes, tokens], pair i takes axes[i]. An axis out
+// of range counts as the nearest and is reported. axes nullptr: one axis.
+__device__ __forceinline__ int64_t axis_start(const int* axes, int num_axes, int tokens, int i, uint32_t* err) {
+  if (!axes) return 0;
+  const int axis = __ldg(axes + i);
+  const int held = min(max(axis, 0), num_axes - 1);
+  if (held != axis) atomicCAS(err, 0u, kErrBounds | (kKidRotary << 8) | (1u << 16));
+  return static_cast<int64_t>(held) * tokens;
 }
 
 template <class T, int N>

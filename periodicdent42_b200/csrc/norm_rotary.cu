@@ -144,8 +144,8 @@ bool fits(const NormRotaryArgs& a, bool inter, bool backward, int vec, int elem)
 }
 
 // 16-byte pieces where rows and halves allow them, else 8- and 4-byte ones, else single elements (dim 80, 40 elements turned, bf16:
-// the second halves of the pairs start 40 bytes in, at a multiple of 8; 16383 tokens, 32 + 8 heads, with gradients: 253 us in
-// 8-byte pieces and four blocks on an SM, 677 us in 4-byte ones and one block).
+// the second halves of the pairs start 40 bytes in, at a multiple of 8; 16383 tokens, 32 + 8 heads, with gradients: 223 us in
+// 8-byte pieces and four blocks on an SM; when it was 253, 677 us in 4-byte ones and one block).
 template <class T>
 cudaError_t pick(NormRotaryArgs& a, bool inter, Pass pass, int sm_count, cudaStream_t s) {
   const bool backward = pass == Pass::kBackward;

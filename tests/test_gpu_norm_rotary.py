@@ -73,6 +73,20 @@ def test_rows_of_every_size(no_device_error, cuda_dev, dtype):
     assert (got[0][0] == 0).all()
 
 
+@pytest.mark.parametrize("T,H,G,D,r", [(593, 1, 64, 64, 64), (593, 64, 1, 64, 32), (20000, 2, 1, 6, 4), (4097, 16, 16, 96, 96),
+                                       (1777, 1, 1, 512, 512), (2500, 33, 7, 128, 128)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_heads_and_tokens_of_many_proportions(no_device_error, cuda_dev, dtype, T, H, G, D, r):
+    """How heads and tokens are dealt to blocks follows the costs of Q and K: few heads beside many, odd ones, alone."""
+    f = bsk.rotary_frequencies(r, device=cuda_dev)[0]
+    x = make(T, H, G, D, dtype, cuda_dev, torch.float32, seed=H + G)
+    got = grads(*x, f)
+    check(got, *x, f)
+    for i, j in ((0, 2), (1, 3)):  # each alone is dealt in another way
+        with torch.no_grad():
+            assert torch.equal(bsk.qk_norm_rotary(x[i], None, x[j], None, x[6], f)[0], got[i])
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("inter", [False, True])
 def test_large_rows_and_a_large_scale(no_device_error, cuda_dev, dtype, inter):

@@ -12,7 +12,8 @@
 // TMA producer, warp 1 MMA issuer, warps 4-11 two warpgroups that each take 64 columns of the 128 x 128 score tiles, P kept
 // in fp32 registers between its use for dV and for dS; P^T and dS^T / dS are rounded to the inputs' type for the second
 // products (half a step: 2^-8 of a weight in bf16, 2^-11 in fp16, as the results' own rounding; gradients come out
-// 1.5 times as far from the 64-bit ones, normwise, as results rounded once). What differs:
+// 1.5 times as far from the 64-bit ones, normwise, as results rounded once; with windows of a few keys up to 1.8 times, since
+// Delta takes the rounded O and fewer keys' dS average that out). What differs:
 //   - masks go by position: keys behind a row (causal) or behind the sequence's end get P = 0;
 //   - rows of a tile that are not the sequence's own (behind its end, or the 128 mod group rows that no copy fills) would
 //     enter the sums as 0 x their value, so warp 2 sets them to zero in shared memory between the copy's arrival and the

@@ -799,9 +799,14 @@ struct NormRotary : public torch::autograd::Function<NormRotary> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto s = ctx->get_saved_variables();
     const auto opt = [](const torch::Tensor& t) { return t.defined() ? OptTensor(t) : std::nullopt; };
+    // Which of Q, K, q_weight, k_weight ask for a gradient. needs_input_grad counts the tensors that were given: without K and
+    // k_weight, q_weight is the second one.
+    const bool with_k = s[1].defined();
+    const bool need[4] = {ctx->needs_input_grad(0), with_k && ctx->needs_input_grad(1), ctx->needs_input_grad(with_k ? 2 : 1),
+                          with_k && ctx->needs_input_grad(3)};
     // only the halves that something asks for
-    const bool need_q = (ctx->needs_input_grad(0) || ctx->needs_input_grad(2)) && grads[0].defined();
-    const bool need_k = grads.size() > 1 && (ctx->needs_input_grad(1) || ctx->needs_input_grad(3)) && grads[1].defined();
+    const bool need_q = (need[0] || need[2]) && grads[0].defined();
+    const bool need_k = grads.size() > 1 && (need[1] || need[3]) && grads[1].defined();
     variable_list out(10);
     if (need_q || need_k) {
       at::AutoGradMode no_grad(false);
@@ -809,7 +814,7 @@ struct NormRotary : public torch::autograd::Function<NormRotary> {
                                opt(s[1]), s[2], opt(s[3]), s[4], s[5], opt(s[6]), ctx->saved_data["interleaved"].toBool(),
                                ctx->saved_data["scale"].toDouble(), ctx->saved_data["eps"].toDouble());
       for (int i = 0; i < 4; ++i)
-        if (ctx->needs_input_grad(i)) out[i] = d[i];
+        if (need[i]) out[i] = d[i];
     }
     return once(std::move(out), "qk_norm_rotary");
   }

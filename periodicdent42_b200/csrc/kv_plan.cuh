@@ -113,7 +113,8 @@ static __global__ void __launch_bounds__(kKvPlanThreads) kv_plan_kernel(const Kv
     const int chunk_end = static_cast<int>(min(tokens_before, static_cast<int64_t>(a.tokens)));
     __syncthreads();
     const int stop = min(row1, chunk_end);
-    for (int row = done + threadIdx.x; row < stop; row += kKvPlanThreads) {
+    for (uint32_t x = done + threadIdx.x; x < static_cast<uint32_t>(stop); x += kKvPlanThreads) {  // (passes 2^31 near the last row)
+      const int row = static_cast<int>(x);
       int lo = 0, hi = count;  // the last request that begins at or before the row (those without tokens begin where the next does)
       while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
@@ -141,9 +142,9 @@ static __global__ void __launch_bounds__(kKvPlanThreads) kv_plan_kernel(const Kv
     done = max(done, stop);
     __syncthreads();
   }
-  for (int row = done + threadIdx.x; row < row1; row += kKvPlanThreads) {  // padding
-    a.slots[row] = -1;
-    a.positions[row] = 0;
+  for (uint32_t x = done + threadIdx.x; x < static_cast<uint32_t>(row1); x += kKvPlanThreads) {  // padding
+    a.slots[x] = -1;
+    a.positions[x] = 0;
   }
   if (lead && threadIdx.x == 0) {
     if (tokens_before > a.tokens) kv_plan_flag(a.err, 4);

@@ -55,6 +55,10 @@ int cuda_fail(cudaError_t e, const char* what) {
 
 constexpr int kMaxDevices = 64;
 
+// The attention and plan kernels count sequences and work items in signed 32 bits, by steps of up to 1024; the step behind the
+// last one must not pass 2^31 either.
+constexpr int kMostSequences = INT32_MAX - (1 << 17);
+
 struct DeviceState {
   std::atomic<bool> counted{false};
   std::once_flag once;
@@ -2230,6 +2234,7 @@ int bsk_kv_cache_plan(const int32_t* kv_lens, const int32_t* new_lens, int batch
   if (batch < 0 || tokens < 0 || table_width < 0 || num_free < 0 || table_stride < 0)
     return set_error(BSK_ERR_INVALID_ARG, "%s: negative extent", what);
   if (page_size < 1) return set_error(BSK_ERR_INVALID_ARG, "%s: page size must be positive, got %d", what, page_size);
+  if (batch > kMostSequences) return set_error(BSK_ERR_UNSUPPORTED, "%s: at most 2^31 - 2^17 - 1 requests", what);
   if (!free_count || !cu_seqlens || !free_count_out || (batch > 0 && (!kv_lens || !new_lens || !kv_lens_out)) ||
       (batch > 0 && table_width > 0 && !block_table) || (num_free > 0 && !free_pages) || (tokens > 0 && (!slots || !positions)))
     return set_error(BSK_ERR_INVALID_ARG, "%s: null pointer", what);
@@ -2258,6 +2263,7 @@ int heads_checks(const char* what, int dtype, int tokens, int batch, int heads, 
   if (heads / kv_heads > 128)
     return set_error(BSK_ERR_UNSUPPORTED, "%s: at most 128 heads per kv head, got %d", what, heads / kv_heads);
   if (kv_heads > 65535) return set_error(BSK_ERR_UNSUPPORTED, "%s: at most 65535 kv heads", what);
+  if (batch > kMostSequences) return set_error(BSK_ERR_UNSUPPORTED, "%s: at most 2^31 - 2^17 - 1 sequences", what);
   if (!(scale > 0.0f) || !(scale < 1e30f)) return set_error(BSK_ERR_INVALID_ARG, "%s: scale must be positive and finite", what);
   return BSK_OK;
 }
@@ -2267,8 +2273,9 @@ int64_t plan_bytes(int64_t tokens, int64_t batch, int64_t tt) {
   return 16 + bsk::plan_slots(tokens, batch, tt) * (int64_t)sizeof(bsk::VarItem);
 }
 
+// (with up to 8 pieces an SM, and one a kv head, beside the slots)
 bool plan_fits(int64_t tokens, int64_t batch, int64_t tt, int64_t kv_heads) {
-  return bsk::plan_slots(tokens, batch, tt) * kv_heads < (int64_t)1 << 31;
+  return bsk::plan_slots(tokens, batch, tt) * kv_heads <= kMostSequences;
 }
 
 void plan_launch(bsk::PlanArgs a, void* ws, const DeviceState& st, cudaStream_t s) {
@@ -2542,6 +2549,8 @@ int attention_varlen_fwd(int dtype, const void* Q, int64_t q_token_stride, int64
                          int64_t workspace_bytes, void* stream) {
   const char* what = "attention_varlen_fwd";
   if (int rc = heads_checks(what, dtype, tokens, batch, heads, kv_heads, dim, scale)) return rc;
+  const int group = heads / kv_heads, tt = bsk::kVarBlk / group;
+  if (!plan_fits(tokens, batch, tt, kv_heads)) return set_error(BSK_ERR_UNSUPPORTED, "%s: too many rows or sequences", what);
   DeviceState* st;
   if (tokens == 0) return device_state(&st);
   const int64_t need = varlen_workspace(tokens, batch, heads, kv_heads, dim, false);
@@ -2555,8 +2564,6 @@ int attention_varlen_fwd(int dtype, const void* Q, int64_t q_token_stride, int64
   win = window_within(win, tokens);
   if (win.window)
     if (int rc = window_ready(*st)) return rc;
-  const int group = heads / kv_heads, tt = bsk::kVarBlk / group;
-  if (!plan_fits(tokens, batch, tt, kv_heads)) return set_error(BSK_ERR_UNSUPPORTED, "%s: too many rows", what);
   const bool f16 = dtype == 1;
   CUtensorMap tq, tk, tv;
   if (int rc = make_map3(&tq, f16, Q, dim, heads, tokens, q_head_stride * 2, q_token_stride * 2, group, tt, "Q")) return rc;
@@ -2603,6 +2610,8 @@ int attention_varlen_bwd(int dtype, const void* dO, int64_t do_token_stride, int
                          int64_t workspace_bytes, void* stream) {
   const char* what = "attention_varlen_bwd";
   if (int rc = heads_checks(what, dtype, tokens, batch, heads, kv_heads, dim, scale)) return rc;
+  const int group = heads / kv_heads, tt = bsk::kVarBlk / group;
+  if (!plan_fits(tokens, batch, tt, kv_heads)) return set_error(BSK_ERR_UNSUPPORTED, "%s: too many rows or sequences", what);
   DeviceState* st;
   if (tokens == 0) return device_state(&st);
   const int64_t need = varlen_workspace(tokens, batch, heads, kv_heads, dim, true);
@@ -2622,10 +2631,8 @@ int attention_varlen_bwd(int dtype, const void* dO, int64_t do_token_stride, int
                                          heads, kv_heads, dim, win, st->sm_count);
   if (ks.pieces && workspace_bytes < ks.total)
     return set_error(BSK_ERR_INVALID_ARG, "%s: workspace of %lld bytes needed", what, (long long)ks.total);
-  const int group = heads / kv_heads, tt = bsk::kVarBlk / group;
   const int64_t slots = bsk::plan_slots(tokens, batch, tt), key_slots = bsk::plan_slots(tokens, batch, bsk::kVarBlk);
   const int64_t key_items = key_slots + ks.pieces;
-  if (!plan_fits(tokens, batch, tt, kv_heads)) return set_error(BSK_ERR_UNSUPPORTED, "%s: too many rows", what);
   const bool f16 = dtype == 1;
   CUtensorMap tq, tk, tv, tdo;
   if (int rc = make_map3(&tq, f16, Q, dim, heads, tokens, q_head_stride * 2, q_token_stride * 2, group, tt, "Q")) return rc;

@@ -494,7 +494,9 @@ int bsk_attention_varlen_bwd(int dtype, const void* dO, int64_t do_token_stride,
  * form's workspace size is bsk_attention_varlen_window_workspace_bytes (it depends on the current device), the paged form's as
  * above. The work is that of the keys that are seen: key blocks that no row of a tile sees are not read. Over a
  * paged cache, pages wholly outside what a sequence's new tokens see are neither read nor looked up (their table entries may
- * hold anything). A non-finite V may reach rows that have left it behind by fewer than 256 tokens, as it may those before it.
+ * hold anything). A non-finite V may reach rows that have left it behind by fewer than 256 tokens, as it may those before it;
+ * so may a non-finite K or V reach dQ, and Q or dO the gradients of K and V: with sinks also those of all keys in the blocks of
+ * 128 keys that hold sinks, from every later row.
  */
 int bsk_attention_paged_window(int dtype, const void* Q, int64_t q_token_stride, int64_t q_head_stride, const void* k_cache,
                                const void* v_cache, int cache_e4m3, const float* k_scale, const float* v_scale,

@@ -62,10 +62,10 @@ __device__ __forceinline__ bool var_item(const VarItem* items, int n_items, int 
 template <int kD>
 __device__ __forceinline__ void zero_rows_warp(uint8_t* tile, int first, int end) {
   constexpr int kPer = kD / 8;
-  for (int i = ptx::lane_id(); i < (end - first) * kPer; i += 32) {
-    const int r = first + i / kPer, c = i % kPer;
-    *reinterpret_cast<uint4*>(tile + (c >> 3) * kAttnChunk + r * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
-  }
+  const int lane = ptx::lane_id();
+  uint8_t* piece = tile + ((lane % kPer) >> 3) * kAttnChunk + (lane & 7) * 16;  // this lane's, of row 0
+#pragma unroll 4
+  for (int r = first + lane / kPer; r < end; r += 32 / kPer) *reinterpret_cast<uint4*>(piece + r * 128) = make_uint4(0, 0, 0, 0);
   ptx::fence_proxy_async_smem();
   __syncwarp();
 }
@@ -258,6 +258,13 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     return kWin && b >= sink_blocks ? b + win_skip(it.pos0, a.window, a.sinks) : b;
   };
 
+  // Rows [sinks_end, gap_end) of entry b's K: keys beside the sinks that the window leaves out for the whole tile. dS = 0 would not
+  // stop a NaN in them (in V it would: dS of a masked key is replaced).
+  const int sinks_end = kWin && a.sinks % kVarBlk ? a.sinks % kVarBlk : kVarBlk;
+  auto gap_end = [&](const VarItem& it, int b) -> int {
+    return kWin && b == sink_blocks - 1 ? min(it.pos0 - a.window + 1 - b * kVarBlk, kVarBlk) : 0;
+  };
+
   if (warp == 0) {
     // ------------------------------------------------------------------ TMA producer (one thread)
     if (lane == 0) {
@@ -293,7 +300,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         for (int x = it.b0; x < it.b1 && ok; ++x) {
           const int b = block_of(it, x), row = it.src + b * kVarBlk;
           const bool foreign = it.kv_len - b * kVarBlk < kVarBlk;
-          ok = push(&tmK, hkv, row, foreign) && push(&tmV, hkv, row, foreign);
+          ok = push(&tmK, hkv, row, foreign || (kWin && gap_end(it, x) > sinks_end)) && push(&tmV, hkv, row, foreign);
         }
       }
       WaitCtl dctl = ctl;
@@ -396,16 +403,22 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     for (int k = 0; ok && item_at(k, it, hkv); ++k) {
       const int n = it.b1 - it.b0;
       if (n <= 0) continue;
-      const int live = it.kv_len - block_of(it, it.b1 - 1) * kVarBlk;
-      if (live < kVarBlk)
-        for (int w = 0; w < 2 && ok; ++w) {  // the item's last K tile and its last V tile
-          const uint32_t sl = (seq + 2 * n - 2 + w) % kSlots;
+      // the K tile of the last sinks' block, where some of its keys are left out, and the item's last K tile and last V tile
+      for (int y = kWin ? 0 : 1; y < 2 && ok; ++y) {
+        const int b = y ? it.b1 - 1 : sink_blocks - 1;
+        if (kWin && !y && (b < it.b0 || b >= it.b1 - 1)) continue;
+        const int live = y ? it.kv_len - block_of(it, b) * kVarBlk : kVarBlk, gap = gap_end(it, b);
+        for (int w = 0; w < 2 && ok; ++w) {
+          if (live >= kVarBlk && (!kWin || w || gap <= sinks_end)) continue;
+          const uint32_t sl = (seq + 2 * (b - it.b0) + w) % kSlots;
           ok = warp_wait_bounded_hint<kBwdSuspendNs>(ptx::smem_u32(&raw_full[sl]), (phases >> sl) & 1, ctl, 30);
           if (!ok) break;
           phases ^= 1u << sl;
+          if (kWin && !w) zero_rows_warp<kD>(sKV + sl * kTile, sinks_end, gap);
           zero_rows_warp<kD>(sKV + sl * kTile, live, kVarBlk);
           if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&kv_full[sl]));
         }
+      }
       seq += 2 * n;
     }
   } else if (warp >= 4) {

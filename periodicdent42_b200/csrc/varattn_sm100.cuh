@@ -17,7 +17,8 @@
 //     compare. A row without any key keeps its maximum at -inf and is written as zero.
 //   - The last block of a sequence may hold foreign rows (the next sequence's, or stale page contents, NaN among them). Their
 //     scores are replaced, but P = 0 does not stop a NaN in V: warp 3 sets those V rows to zero in shared memory between the
-//     copy's arrival and the PV product (only such blocks take this detour).
+//     copy's arrival and the PV product (only such blocks take this detour, and with a window the sinks' last one, whose keys
+//     beside the sinks the tile may have left behind).
 //
 // e4m3 caches (kKind 2): both products are fp16 products. Warps 12-15, which otherwise only write results, convert: codes
 // arrive by the same copies in a staging ring, a thread takes a key's row and writes it as fp16 (one instruction for two
@@ -291,6 +292,15 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
   };
   // Keys of the sequence in the item's last block: below 128 its V tile holds foreign rows.
   auto tail_rows = [&](const VarItem& it) { return it.kv_len - block_of(it, it.b1 - 1) * kVarBlk; };
+  // A window leaves out keys beside the sinks, in their last block: rows [sinks_end, gap_end) of entry b are seen by no row of the
+  // tile. They are foreign rows too, however far the tile is from them. (Pages that no row sees are zeros already; e4m3: unseen
+  // keys are converted to zeros one by one.)
+  const int sinks_end = kWin && sinks % kVarBlk ? sinks % kVarBlk : kVarBlk;
+  const int gap_box = kKind == kCache16 ? min(1 << a.page_shift, kVarBlk) : kVarBlk;
+  const int gap_most = (sinks_end + gap_box - 1) / gap_box * gap_box;
+  auto gap_end = [&](const VarItem& it, int b) -> int {
+    return kWin && b == sink_blocks - 1 ? min(max(it.pos0, 0) - window + 1 - b * kVarBlk, gap_most) : 0;
+  };
   // e4m3: the first block that may be the last one that some row sees keys of: that of the first token's own key, or the item's
   // last. The blocks before it are seen whole by every row that sees any key.
   auto first_edge = [](const VarItem& it) { return min(it.pos0 >> 7, it.b1 - 1); };
@@ -337,7 +347,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       };
       auto push = [&](const CUtensorMap* m, const VarItem& it, int hkv, int b, bool is_v, int row) -> bool {
         if (!wait(&ring_empty[slot], slot_phase ^ 1, 2)) return false;
-        const bool foreign = !kE4m3 && is_v && b == it.b1 - 1 && tail_rows(it) < kVarBlk;
+        const bool foreign = !kE4m3 && is_v && ((b == it.b1 - 1 && tail_rows(it) < kVarBlk) || (kWin && gap_end(it, b) > sinks_end));
         const uint32_t fb = ptx::smem_u32(foreign ? &raw_full[slot] : &ring_full[slot]);
         uint32_t dst = kv0 + slot * (kE4m3 ? Sh::kStageBytes : kTile);
         if (kPaged) dst += lane * (kE4m3 ? box_rows * kD : (box_rows >> 3) * kGroupPitch);
@@ -576,19 +586,26 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     for (int k = 0; !kE4m3 && ok && item_at(k, it, hkv); ++k) {
       const int n = it.b1 - it.b0;
       if (n <= 0) continue;
-      const int live = tail_rows(it);
-      if (live < kVarBlk) {
-        const uint32_t sl = (seq + 2 * n - 1) % kSlots;  // the item's last V tile
+      // V tiles of the last sinks' block, where some of its keys are left out, and of the item's last block
+      for (int x = kWin ? 0 : 1; x < 2; ++x) {
+        const int b = x ? it.b1 - 1 : sink_blocks - 1;
+        if (kWin && !x && (b < it.b0 || b >= it.b1 - 1)) continue;
+        const int live = x ? tail_rows(it) : kVarBlk, gap = gap_end(it, b);
+        if (live >= kVarBlk && (!kWin || gap <= sinks_end)) continue;
+        const uint32_t sl = (seq + (x ? 2 * n - 1 : attn_v_pos(b - it.b0, n))) % kSlots;
         ok = warp_wait_bounded<false, 256>(ptx::smem_u32(&raw_full[sl]), (phases >> sl) & 1, ctl, 30);
         if (!ok) break;
         phases ^= 1u << sl;
         uint8_t* tile = sKV + sl * kTile;
         constexpr int kPer = Sh::kChunks * 8;  // 16-byte pieces per row (a row's swizzle stays within its 128 bytes)
-        for (int i = lane; i < (kVarBlk - live) * kPer; i += 32) {
-          const int r = live + i / kPer, c = i % kPer;
-          *reinterpret_cast<uint4*>(tile + (r >> 3) * kGroupPitch + (c >> 3) * kChunkPitch + (r & 7) * 128 + (c & 7) * 16) =
-              make_uint4(0, 0, 0, 0);
-        }
+        uint8_t* piece = tile + ((lane % kPer) >> 3) * kChunkPitch + (lane & 7) * 16;  // this lane's, of row 0
+        auto zero = [&](int first, int end) {
+#pragma unroll 4
+          for (int r = first + lane / kPer; r < end; r += 32 / kPer)
+            *reinterpret_cast<uint4*>(piece + (r >> 3) * kGroupPitch + (r & 7) * 128) = make_uint4(0, 0, 0, 0);
+        };
+        if constexpr (kWin) zero(sinks_end, gap);
+        zero(live, kVarBlk);
         ptx::fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&kv_full[sl]));

@@ -562,8 +562,9 @@ def attention_varlen(Q: torch.Tensor, K: torch.Tensor, V: torch.Tensor, cu_seqle
     first ``sinks`` ones; the work is that of the tokens that are seen.
     Sequences do not reach one another, non-finite values included; inside one, a non-finite row of V may make rows NaN
     that are masked for it, fewer than 256 tokens before it (or behind, where a window leaves it out), and a
-    non-finite row of K or V the same rows of dQ, of Q or dO those keys' dK and dV. Differentiable (once, in reverse mode) in Q,
-    K and V (deterministic, no atomics). The softmax's weights and, for the gradients, dS are rounded to Q's type for their products."""
+    non-finite row of K or V the same rows of dQ, of Q or dO those keys' dK and dV (with sinks, also those of all keys in the
+    blocks of 128 that hold sinks, which all later rows see). Differentiable (once, in reverse mode) in Q, K and V (deterministic,
+    no atomics). The softmax's weights and, for the gradients, dS are rounded to Q's type for their products."""
     if scale is None:
         scale = Q.shape[-1] ** -0.5 if Q.dim() and Q.shape[-1] else 1.0
     return _C().attention_varlen(Q, K, V, cu_seqlens, scale, causal, _window("attention_varlen", window), sinks)

@@ -36,7 +36,8 @@
 //
 // A window with sinks (kWin: a row at position p sees keys (p - window, p] and [0, sinks)): a tile's list of key blocks is the
 // sinks' blocks and then those from the first one that its first row sees, so blocks that no row sees are neither copied nor
-// multiplied (32768 tokens, window 4096, 32 / 8 heads, D 128: 2.5 ms, 820 TFLOP/s; without a window 9.3). Three kinds of
+// multiplied (32768 tokens, window 4096, 32 / 8 heads, D 128: 2.18 ms, 944 TFLOP/s, at full clocks, without a window 8.54; repeated
+// under the power cap 2.56 and 10.0). Three kinds of
 // blocks compare: the causal edge, the window's lower edge, the sinks' last. Over e4m3 caches a row's scale reference follows the
 // keys that this row sees: an unseen key's scale would push the row's own weights below fp16's range, so masked blocks take the
 // largest scale of the row's own range (range_top).
@@ -48,8 +49,8 @@
 // issue 49 %, XU 35 %, DRAM 3 %; 552 us in short runs, 646 when repeated under the power cap). Packing the group's heads into
 // the tile means a causal tile spans only TT tokens, so less of its last block is masked, and one K / V tile feeds the whole
 // group. With the window above: tensor pipe 45 %, issue 49 %, XU 34 %; the two masked blocks of a tile's 34 make little of it, in
-// short windows they make most (8192 tokens, window 1024, 10 blocks a tile: 195 us at 80 us of products). Two query tiles in flight
-// (a thread a row of 128 keys, rows in one CTA by turns) were no faster: 2.4-2.5 ms for 2.2-2.5.
+// short windows they make most (8192 tokens, window 1024, 10 blocks a tile: 200 us at 80 us of products). Two query tiles in flight
+// (a thread a row of 128 keys, rows in one CTA by turns) were no faster: 2.4-2.5 ms for 2.2-2.5, each as the clock was.
 #pragma once
 
 #include <type_traits>
@@ -294,7 +295,8 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
   auto tail_rows = [&](const VarItem& it) { return it.kv_len - block_of(it, it.b1 - 1) * kVarBlk; };
   // A window leaves out keys beside the sinks, in their last block: rows [sinks_end, gap_end) of entry b are seen by no row of the
   // tile. They are foreign rows too, however far the tile is from them. (Pages that no row sees are zeros already; e4m3: unseen
-  // keys are converted to zeros one by one.)
+  // keys are converted to zeros one by one.) Five packed sequences, window 1024, 4 sinks: 343 us without this, 350; leaving steps of
+  // 16 such keys out of the product instead of setting them to zero took 380.
   const int sinks_end = kWin && sinks % kVarBlk ? sinks % kVarBlk : kVarBlk;
   const int gap_box = kKind == kCache16 ? min(1 << a.page_shift, kVarBlk) : kVarBlk;
   const int gap_most = (sinks_end + gap_box - 1) / gap_box * gap_box;

@@ -428,6 +428,7 @@ int bsk_kv_cache_gather(int dtype, const void* k_cache, const void* v_cache, int
  * Each of these sets the device error word: a negative length (counts as 0); new tokens beyond a row of the table (slot -1) or
  * beyond `tokens` rows (left out); no page left, or a request's own entry negative (slot -1, and the entry of a page not found
  * becomes -1); free_count outside [0, num_free] (counts as the nearest). Outputs may not overlap inputs.
+ * At most 2^31 - 2^17 - 1 requests.
  * No reference counterpart.
  */
 int bsk_kv_cache_plan(const int32_t* kv_lens, const int32_t* new_lens, int batch, int32_t* block_table, int64_t table_stride,
@@ -437,7 +438,7 @@ int bsk_kv_cache_plan(const int32_t* kv_lens, const int32_t* new_lens, int batch
 
 /*
  * Attention of new tokens over a paged cache, causal, heads grouped over kv heads (dtype 0 = bf16, 1 = f16; dim 64 or
- * 128; at most 128 heads per kv head). Sequence i has the n_i = cu_seqlens[i+1] - cu_seqlens[i] new tokens (n_i >= 0)
+ * 128; at most 128 heads per kv head, 2^31 - 2^17 - 1 sequences). Sequence i has the n_i = cu_seqlens[i+1] - cu_seqlens[i] new tokens (n_i >= 0)
  * in rows cu_seqlens[i].. of Q [tokens, heads, dim] (16-byte aligned rows, strides in elements), and its first
  * kv_lens[i] cached tokens are its keys, the new tokens' own keys the last n_i of them (append before attending). New
  * token t sees the keys at positions <= kv_lens[i] - n_i + t. The key at position p is in page
